@@ -19,6 +19,10 @@ summands (the fused layer's backward); ``check_errors`` raises if an earlier
 single-pass pre forward gave up one of its bounded waits (the pre backward
 and every later pre forward check that too).
 
+The operators between the two, with their own names, are in
+``FlagOS_mhc.sublayer``: layer norm, gated feed-forward block, dropout and the
+mHC feed-forward layer made of them.
+
 Importing the package also registers the operators as torch.ops.flagos_mhc.*
 (``FlagOS_mhc.library``) for torch.compile and HIP-graph capture.
 """
@@ -43,6 +47,7 @@ from .autograd import (
 )
 from .mhc_post_pre import mhc_post_pre_clamp_sinkhorn
 from ._lib import check_errors
+from . import sublayer  # layer norm, gated feed-forward block, dropout
 from . import library  # registers torch.ops.flagos_mhc.* (torch.compile / HIP graphs)
 
 __all__ = [

@@ -64,6 +64,17 @@ _SIGNATURES = {
     "mhc_pre_bwd": (_c.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                _f32, _f32, _f32, _i32, _vp, _vp, _vp, _vp, _vp, _sz,
                                _i64, _i32, _i32, _vp]),
+    "mhc_layer_norm_fwd": (_c.c_int, [_vp, _i32, _vp, _vp, _i32, _f32, _vp, _vp, _vp, _i64, _i32, _vp]),
+    "mhc_layer_norm_bwd_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "mhc_layer_norm_bwd": (_c.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                      _i64, _i32, _vp]),
+    "mhc_gated_ffn_fwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "mhc_gated_ffn_fwd": (_c.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _sz,
+                                     _i64, _i32, _i32, _i32, _vp]),
+    "mhc_gated_ffn_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "mhc_gated_ffn_bwd": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp,
+                                     _vp, _vp, _sz, _i64, _i32, _i32, _i32, _vp]),
+    "mhc_dropout": (_c.c_int, [_vp, _vp, _i64, _i32, _c.c_double, _c.c_uint64, _c.c_uint64, _vp, _vp]),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -308,6 +308,80 @@ int mhc_post_pre_fwd_ex(const void* x, const float* h_res, const void* h_out, co
                         float* pre, void* workspace, size_t workspace_bytes, int32_t* status, int64_t T,
                         int32_t N, int32_t D, void* stream);
 
+/*
+ * The operators of the sublayer between mhc_pre_fwd's y and mhc_post_fwd's
+ * h_out.  No counterpart in the reference, whose model code runs them in
+ * PyTorch.
+ *
+ * Layer norm of T rows of D elements:
+ *   mean = sum x / D, rstd = (sum (x - mean)^2 / D + eps)^-1/2,
+ *   y = (x - mean) * rstd * weight + bias
+ * x, y: (T,D) `x_dtype`, any element alignment; weight, bias: (D,) `w_dtype`
+ * (x_dtype or fp32), each may be NULL (1 and 0); mean, rstd: (T,) fp32 for
+ * the backward, both or neither.  Sums are fp32.  D >= 1; one block per row,
+ * so at most 4.19 M rows of the longest widths.
+ */
+int mhc_layer_norm_fwd(const void* x, int32_t x_dtype, const void* weight, const void* bias,
+                       int32_t w_dtype, float eps, void* y, float* mean, float* rstd, int64_t T,
+                       int32_t D, void* stream);
+
+/*
+ * Layer norm backward: grad_x (T,D) `x_dtype`; grad_weight, grad_bias (D,)
+ * fp32, each may be NULL (the workspace too, if both are).  Deterministic:
+ * sums over the rows are taken in a fixed order.  T == 0 writes nothing.
+ */
+size_t mhc_layer_norm_bwd_workspace_size(int64_t T, int32_t D, int32_t x_dtype);
+int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_dtype, const void* weight,
+                       int32_t w_dtype, const float* mean, const float* rstd, void* grad_x,
+                       float* grad_weight, float* grad_bias, void* workspace,
+                       size_t workspace_bytes, int64_t T, int32_t D, void* stream);
+
+/*
+ * Gated feed-forward block:
+ *   gate = x w_gate^T, up = x w_up^T, hidden = act(gate) * up,
+ *   out = hidden w_down^T
+ * x: (T,D), w_gate, w_up: (F,D), w_down: (O,F), out: (T,O), all `dtype`,
+ * 16-byte aligned.  Products accumulate in fp32; hidden is rounded to `dtype`
+ * between the two products.  For the backward, all or none of: gate, up (T,F)
+ * fp32 and hidden, (T, F) `dtype` in rows of stride F rounded up to 8
+ * elements (the rest of a row is written as zero).  With none, hidden lives in the workspace.
+ */
+#define MHC_ACT_SILU 0      /* g * sigmoid(g) */
+#define MHC_ACT_GELU 1      /* g * Phi(g) */
+#define MHC_ACT_GELU_TANH 2 /* 0.5 g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) */
+#define MHC_ACT_RELU 3      /* max(g, 0) */
+size_t mhc_gated_ffn_fwd_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype);
+int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down,
+                      int32_t dtype, int32_t activation, void* out, float* gate, float* up,
+                      void* hidden, void* workspace, size_t workspace_bytes, int64_t T, int32_t D,
+                      int32_t F, int32_t O, void* stream);
+
+/*
+ * Backward of the block from the forward's gate, up and hidden: grad_x (T,D),
+ * grad_w_gate, grad_w_up (F,D), grad_w_down (O,F), all `dtype`, 16-byte
+ * aligned.  The gradients of gate and up are rounded to `dtype` between the
+ * products.  Deterministic.  T == 0 writes nothing.
+ */
+size_t mhc_gated_ffn_bwd_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype);
+int mhc_gated_ffn_bwd(const void* grad_out, const void* x, const void* w_gate, const void* w_up,
+                      const void* w_down, const float* gate, const float* up, const void* hidden,
+                      int32_t dtype, int32_t activation, void* grad_x, void* grad_w_gate,
+                      void* grad_w_up, void* grad_w_down, void* workspace, size_t workspace_bytes,
+                      int64_t T, int32_t D, int32_t F, int32_t O, void* stream);
+
+/*
+ * Dropout with a mask that is a function of the element's index i:
+ * Philox4x32-10 with key = seed and counter = (i / 8, offset) gives 16 bits
+ * for each of 8 elements (element 2j of the group the low, 2j + 1 the high
+ * half of word j); y[i] = x[i] * 65536 / (65536 - t) where they are at least
+ * t = round(p * 65536), else 0.  x, y: n elements of `dtype`, any element
+ * alignment; y may be x.  state: device memory holding (seed, offset), read
+ * when the kernel runs, in place of the two arguments (for captured graphs),
+ * or NULL.  The backward is the same call on the gradient.
+ */
+int mhc_dropout(const void* x, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
+                uint64_t offset, const uint64_t* state, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
