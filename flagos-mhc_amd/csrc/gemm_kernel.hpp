@@ -1,0 +1,480 @@
+// The matrix products' kernels: what they compute, their epilogues, and the
+// tile kernel that runs every shape, type and layout.
+#pragma once
+
+#include "gemm_tile.hpp"
+
+namespace mhc {
+
+// ---- what a product is ----------------------------------------------------------
+
+// kEpiStore: out0 = C.  kEpiGated (two B operands, g = A B0^T, u = A B1^T):
+// out0 = act(g) u, and g and u where gate and up are given.  kEpiGatedGrad
+// (C is the gradient of act(g) u): out0 = C u act'(g), out1 = C act(g).
+enum { kEpiStore = 0, kEpiGated = 1, kEpiGatedGrad = 2 };
+enum { kActSilu = 0, kActGelu = 1, kActGeluTanh = 2, kActRelu = 3 };
+
+struct GemmArgs {
+  const void* A[2];  // second: the next segment of k, or of the next product of the batch
+  const void* B[2];  // second: the next segment of k, or the gated form's other operand
+  int64_t lda, ldb;  // elements between lines
+  int M, N, K;       // K of one segment
+  int segments;      // of k: C = A0 B0^T (+ A1 B1^T)
+  int batch;         // 2: also out1 = A1 B0^T
+  void* out0;
+  void* out1;
+  int64_t ldo;       // of out0 and out1; columns N .. ldo - 1 are written as zero
+  float* gate;       // (M, N)
+  float* up;
+  int act;
+  int splits;        // of the steps of k: partial sums go to `part`
+  float* part;       // [splits][batch or gated pair][M][ldp]
+  int64_t ldp;
+};
+
+// act(g) and act'(g) in fp32.
+__device__ __forceinline__ void act_both(int kind, float g, float* a, float* d) {
+  if (kind == kActSilu) {
+    const float s = 1.f / (1.f + expf(-g));
+    *a = g * s;
+    *d = s * (1.f + g * (1.f - s));
+  } else if (kind == kActGelu) {
+    const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    *a = g * p;
+    *d = p + g * 0.39894228040143268f * expf(-0.5f * g * g);
+  } else if (kind == kActGeluTanh) {
+    // 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v))
+    const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
+    const float s = 1.f / (1.f + expf(-2.f * v));
+    *a = g * s;
+    *d = s + g * 2.f * s * (1.f - s) * 0.79788456080286536f * (1.f + 0.134145f * fminf(g * g, 1e30f));
+  } else {
+    *a = g > 0.f ? g : (g != g ? g : 0.f);
+    *d = g > 0.f ? 1.f : 0.f;
+  }
+}
+
+// ---- epilogues -------------------------------------------------------------------
+
+typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+
+// Four consecutive elements of a row of `len`, the first at n.
+template <typename S>
+__device__ __forceinline__ void store4(S* row, int64_t n, int64_t len, const floatx4& c) {
+  if (n + 4 <= len) {
+    if constexpr (sizeof(S) == 4) {
+      *reinterpret_cast<floatx4_a4*>(row + n) = c;
+    } else {
+      const u32x2 v = {(uint32_t)Store<S>::from_f32(c[0]) | (uint32_t)Store<S>::from_f32(c[1]) << 16,
+                       (uint32_t)Store<S>::from_f32(c[2]) | (uint32_t)Store<S>::from_f32(c[3]) << 16};
+      *reinterpret_cast<u32x2_a2*>(row + n) = v;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < len) store_elem<S>(row, n + i, c[i]);
+  }
+}
+__device__ __forceinline__ floatx4 load4(const float* row, int64_t n, int64_t len) {
+  if (n + 4 <= len) return *reinterpret_cast<const floatx4_a4*>(row + n);
+  floatx4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < len) v[i] = row[n + i];
+  return v;
+}
+
+// Row m, columns n .. n + 3 of the product (c; gated: c0 = g, c1 = u); z is
+// the product of the batch.
+template <typename S, int EPI>
+__device__ __forceinline__ void epilogue(const GemmArgs& a, int z, int64_t m, int n, const floatx4& c0, const floatx4& c1) {
+  if (m >= a.M || n >= a.ldo) return;
+  S* o0 = static_cast<S*>(z ? a.out1 : a.out0) + m * a.ldo;
+  if constexpr (EPI == kEpiStore) {
+    store4<S>(o0, n, a.ldo, c0);
+  } else if constexpr (EPI == kEpiGated) {
+    floatx4 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v, d;
+      act_both(a.act, c0[i], &v, &d);
+      h[i] = v * c1[i];
+    }
+    store4<S>(o0, n, a.ldo, h);
+    if (a.gate) {
+      store4<float>(a.gate + m * a.N, n, a.N, c0);
+      store4<float>(a.up + m * a.N, n, a.N, c1);
+    }
+  } else {
+    const floatx4 g = load4(a.gate + m * a.N, n, a.N), u = load4(a.up + m * a.N, n, a.N);
+    floatx4 dg, du;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float v, d;
+      act_both(a.act, g[i], &v, &d);
+      dg[i] = c0[i] * u[i] * d;
+      du[i] = c0[i] * v;
+    }
+    store4<S>(o0, n, a.ldo, dg);
+    store4<S>(static_cast<S*>(a.out1) + m * a.ldo, n, a.ldo, du);
+  }
+}
+
+// A kernel's four columns of row m: through the epilogue, or to this split's partial sums.
+template <typename S, int EPI>
+__device__ __forceinline__ void finish(const GemmArgs& a, int z, int64_t m, int n, const floatx4& c0, const floatx4& c1) {
+  if (a.splits == 1) {
+    epilogue<S, EPI>(a, z, m, n, c0, c1);
+  } else if (m < a.M && n < a.ldp) {
+    constexpr int kParts = EPI == kEpiGated ? 2 : 1;
+    float* p = a.part + (((int64_t)blockIdx.y * a.batch + z) * kParts * a.M + m) * a.ldp + n;
+    *reinterpret_cast<floatx4*>(p) = c0;
+    if constexpr (kParts == 2) *reinterpret_cast<floatx4*>(p + (int64_t)a.M * a.ldp) = c1;
+  }
+}
+
+// ---- order of the tiles ------------------------------------------------------------
+
+// Tile (mt, nt) of the b-th block of tm x tn: each XCD walks a contiguous run
+// of the order, which goes down groups of 8 tile rows, so that the tiles an
+// XCD works on at one time share their operands in its L2.
+__device__ __forceinline__ void tile_of(int64_t b, int tm, int tn, int* mt, int* nt) {
+  constexpr int kGroup = 8;
+  const int t = (int)xcd_contig(b, (int64_t)tm * tn);
+  const int per = kGroup * tn, g = t / per, r = t % per;
+  const int rows = tm - g * kGroup < kGroup ? tm - g * kGroup : kGroup;
+  *mt = g * kGroup + r % rows;
+  *nt = r / rows;
+}
+
+// ---- the tile kernel -----------------------------------------------------------------
+// Four waves hold a BM x BN tile of C in registers (WM x WN waves); tiles of A
+// and B go through LDS in STAGES slots.  DMA: loads go straight to LDS,
+// STAGES - 1 tiles ahead; otherwise through registers, for operands whose rows
+// are not multiples of 16 bytes.  grid: (tiles, splits, batch).
+
+template <typename S_, int LA_, int LB_, int BM_, int BN_, int WAVES_M_, int STAGES_, int EPI_, bool DMA_>
+struct TileCfg {
+  using S = S_;
+  static constexpr int LA = LA_, LB = LB_, BM = BM_, BN = BN_, STAGES = STAGES_, EPI = EPI_;
+  static constexpr bool DMA = DMA_;
+  static constexpr int NW = 4, WAVES_M = WAVES_M_, WAVES_N = NW / WAVES_M_;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N;  // a wave's tile
+  static constexpr int NFA = WM / 16, NFB = WN / 16;
+  static constexpr int kNB = EPI == kEpiGated ? 2 : 1;         // B operands
+  static constexpr int kCols = BN / kNB;                       // columns of C
+  static constexpr int kSlot = (BM + BN) * 128;
+  static_assert(STAGES >= 2 && STAGES * kSlot <= 160 * 1024, "LDS");
+  static_assert(DMA || STAGES == 2, "register staging has two slots");
+  static_assert(EPI != kEpiGated || LB == kRow, "the gated form's weights are rows of k");
+};
+
+template <typename C>
+__global__ __launch_bounds__(256, 2) void gemm_tile_kernel(GemmArgs a) {
+  using S = typename C::S;
+  __shared__ __attribute__((aligned(1024))) char smem[C::STAGES * C::kSlot];
+  const uint32_t lds = lds_addr(smem);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % C::WAVES_M, wn = wave / C::WAVES_M;
+  const int z = blockIdx.z;
+  int mt, nt;
+  tile_of(blockIdx.x, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt);
+  const int m0 = mt * C::BM, n0 = nt * C::kCols;
+
+  // steps of k of this split
+  const int nk = (a.K + kStep<S> - 1) / kStep<S>, total = nk * a.segments;
+  const int s0 = (int)((int64_t)total * blockIdx.y / a.splits), s1 = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
+
+  using LdA = TileLoader<S, C::LA, C::BM, C::NW>;
+  using LdB = TileLoader<S, C::LB, C::BN, C::NW>;
+  const auto row_a = [](int l) { return l; };
+  // gated: each wave's columns are WN / 2 of the gate's, then the same of the other operand's
+  const auto row_b = [](int l) {
+    if constexpr (C::kNB == 2) return l / C::WN * (C::WN / 2) + l % (C::WN / 2);
+    return l;
+  };
+  const auto second_b = [](int l) { return C::kNB == 2 && l % C::WN >= C::WN / 2; };
+  // kCol operands: columns up to the line's end may be read (whole chunks)
+  const int rows_a = C::LA == kRow || !C::DMA ? a.M - m0 : (int)(a.lda - m0);
+  const int rows_b = C::LB == kRow || !C::DMA ? a.N - n0 : (int)(a.ldb - n0);
+  const auto corner = [&](const void* p, int layout, int64_t ld, int first, int kt) {
+    const int64_t k = (int64_t)kt * kStep<S>;
+    return static_cast<const S*>(p) + (layout == kRow ? first * ld + k : k * ld + first);
+  };
+
+  FragReader<S, C::LA, C::BM, C::NFA> ra;
+  FragReader<S, C::LB, C::BN, C::NFB> rb;
+  ra.init(wm * C::WM, lane);
+  rb.init(wn * C::WN, lane);
+  floatx4 acc[C::NFA][C::NFB];
+#pragma unroll
+  for (int i = 0; i < C::NFA; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NFB; ++j) acc[i][j] = {0.f, 0.f, 0.f, 0.f};
+
+  const auto multiply = [&](int slot) {
+    u32x4 fa[2][C::NFA], fb[2][C::NFB];
+    const uint32_t t = lds + slot * C::kSlot;
+    ra.read(fa, t);
+    rb.read(fb, t + C::BM * 128);
+    mma_frags<S>(acc, fa, fb);
+  };
+
+  if constexpr (C::DMA) {
+    LdA la;
+    LdB lb;
+    la.init(a.lda, rows_a, wave, lane, row_a);
+    lb.init(a.ldb, rows_b, wave, lane, row_b);
+    const auto issue = [&](int s, int slot) {
+      const int seg = s >= nk, kt = s - seg * nk;
+      const int left = s < s1 ? a.K - kt * kStep<S> : 0;
+      const uint32_t t = lds + slot * C::kSlot;
+      la.issue(corner(a.A[seg | z], C::LA, a.lda, m0, kt), left, t, wave);
+      if constexpr (C::kNB == 2) {
+        lb.issue_two(corner(a.B[0], C::LB, a.ldb, n0, kt), corner(a.B[1], C::LB, a.ldb, n0, kt), left, t + C::BM * 128,
+                     wave, second_b);
+      } else {
+        lb.issue(corner(a.B[seg], C::LB, a.ldb, n0, kt), left, t + C::BM * 128, wave);
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(s0 + i, i);
+    int slot = 0;
+    for (int s = s0; s < s1; ++s) {
+      wait_vmcnt<(C::STAGES - 2) * (LdA::kLoads + LdB::kLoads)>();
+      // every wave's part of slot s is there, and every wave has read slot s - 1
+      __builtin_amdgcn_s_barrier();
+      issue(s + C::STAGES - 1, slot == 0 ? C::STAGES - 1 : slot - 1);
+      multiply(slot);
+      slot = slot == C::STAGES - 1 ? 0 : slot + 1;
+    }
+    wait_vmcnt<0>();  // no load may still be on its way to LDS when the block ends
+  } else {
+    TileRegs<S, C::LA, C::BM, C::NW> va;
+    TileRegs<S, C::LB, C::BN, C::NW> vb;
+    const auto load = [&](int s) {
+      const int seg = s >= nk, kt = s - seg * nk;
+      const int left = s < s1 ? a.K - kt * kStep<S> : 0;
+      va.load(corner(a.A[seg | z], C::LA, a.lda, m0, kt), a.lda, rows_a, left, wave, lane, row_a);
+      if constexpr (C::kNB == 2)
+        vb.load_two(corner(a.B[0], C::LB, a.ldb, n0, kt), corner(a.B[1], C::LB, a.ldb, n0, kt), a.ldb, rows_b, left,
+                    wave, lane, row_b, second_b);
+      else
+        vb.load(corner(a.B[seg], C::LB, a.ldb, n0, kt), a.ldb, rows_b, left, wave, lane, row_b);
+    };
+    const auto store = [&](int slot) {
+      va.store(lds + slot * C::kSlot, wave, lane);
+      vb.store(lds + slot * C::kSlot + C::BM * 128, wave, lane);
+    };
+    load(s0);
+    store(0);
+    load(s0 + 1);
+    int slot = 0;
+    for (int s = s0; s < s1; ++s) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      if (s + 1 < s1) store(slot ^ 1);
+      if (s + 2 < s1) load(s + 2);
+      multiply(slot);
+      slot ^= 1;
+    }
+  }
+
+  // lane: row l % 16 of a fragment of A, columns 4 (l / 16) .. + 3 of one of B
+  const int64_t mw = m0 + wm * C::WM + (lane & 15);
+  constexpr int NC = C::NFB / C::kNB;
+  const int nw = n0 + wn * (C::WN / C::kNB) + (lane >> 4) * 4;
+#pragma unroll
+  for (int i = 0; i < C::NFA; ++i)
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int64_t m = mw + 16 * i;
+      const int n = nw + 16 * j;
+      const floatx4 c0 = acc[i][j], c1 = acc[i][C::kNB == 2 ? j + NC : j];
+      finish<S, C::EPI>(a, z, m, n, c0, c1);
+    }
+}
+
+// ---- the large tile's kernel -----------------------------------------------------------
+// 256 x 256 of C in the registers of eight waves (2 x 4), one block per CU.
+// The tile's rows and columns are two halves of 128 each (the gated form: B's
+// halves are its two operands), a wave has 64 rows and 32 columns of every
+// half, and multiplies quadrant by quadrant:
+//
+//   phase  LDS reads   products     loads started
+//     1    A0, B0      A0 x B0      A1 of step k + 1
+//     2    B1          A0 x B1      A0 of step k + 2
+//     3    A1          A1 x B1      B0 of step k + 2
+//     4                A1 x B0      B1 of step k + 2
+//
+// A half's slot is free as soon as the phase that reads it is over, so loads
+// run six quarters of a step ahead (five halves, 80 KB a CU, always on their
+// way) with two slots.  Every phase is reads, barrier, products, barrier, and
+// waves 4 .. 7 run one barrier behind waves 0 .. 3: of the two waves on a SIMD
+// one reads while the other multiplies.
+
+template <typename S_, int LA_, int LB_, int EPI_>
+struct WideCfg {
+  using S = S_;
+  static constexpr int LA = LA_, LB = LB_, EPI = EPI_, BM = 256;
+  static constexpr int kCols = EPI == kEpiGated ? 128 : 256;  // columns of C
+  static constexpr int kHalf = 128 * 128;                     // bytes of a half in LDS
+  static constexpr int kA0 = 0, kA1 = kHalf, kB0 = 2 * kHalf, kB1 = 3 * kHalf, kSlot = 4 * kHalf;
+};
+
+template <typename C>
+__global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
+  using S = typename C::S;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * C::kSlot];
+  const uint32_t lds = lds_addr(smem);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave >> 1) & 1, wn = (wave & 1) | ((wave >> 2) << 1);
+  const int z = blockIdx.z;
+  int mt, nt;
+  tile_of(blockIdx.x, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt);
+  const int m0 = mt * C::BM, n0 = nt * C::kCols;
+  const int nk = (a.K + kStep<S> - 1) / kStep<S>, total = nk * a.segments;
+  const int s0 = (int)((int64_t)total * blockIdx.y / a.splits), s1 = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
+
+  using LdA = TileLoader<S, C::LA, 128, 8>;
+  using LdB = TileLoader<S, C::LB, 128, 8>;
+  constexpr bool kPair = C::EPI == kEpiGated;
+  const int rows_a = C::LA == kRow ? a.M - m0 : (int)(a.lda - m0);
+  const int rows_b = C::LB == kRow ? a.N - n0 : (int)(a.ldb - n0);
+  const auto same = [](int l) { return l; };
+  LdA la0, la1;
+  LdB lb0, lb1;
+  la0.init(a.lda, rows_a, wave, lane, same);
+  la1.init(a.lda, rows_a - 128, wave, lane, same);
+  lb0.init(a.ldb, rows_b, wave, lane, same);
+  lb1.init(a.ldb, kPair ? rows_b : rows_b - 128, wave, lane, same);
+  const auto corner = [&](const void* p, int layout, int64_t ld, int64_t first, int kt) {
+    const int64_t k = (int64_t)kt * kStep<S>;
+    return static_cast<const S*>(p) + (layout == kRow ? first * ld + k : k * ld + first);
+  };
+  const auto issue_a = [&](int half, int s, uint32_t slot) {
+    const int seg = s >= nk, kt = s - seg * nk, left = s < s1 ? a.K - kt * kStep<S> : 0;
+    (half ? la1 : la0).issue(corner(a.A[seg | z], C::LA, a.lda, m0 + half * 128, kt), left, slot + (half ? C::kA1 : C::kA0), wave);
+  };
+  const auto issue_b = [&](int half, int s, uint32_t slot) {
+    const int seg = s >= nk, kt = s - seg * nk, left = s < s1 ? a.K - kt * kStep<S> : 0;
+    const void* p = a.B[kPair ? half : seg];
+    (half ? lb1 : lb0).issue(corner(p, C::LB, a.ldb, kPair ? n0 : n0 + half * 128, kt), left, slot + (half ? C::kB1 : C::kB0), wave);
+  };
+
+  FragReader<S, C::LA, 128, 4> ra;
+  FragReader<S, C::LB, 128, 2> rb;
+  ra.init(wm * 64, lane);
+  rb.init(wn * 32, lane);
+  floatx4 acc[2][2][4][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) acc[i][j][p][q] = {0.f, 0.f, 0.f, 0.f};
+
+  const auto barrier = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  u32x4 fa[2][4], fb0[2][2], fb1[2][2];
+  const auto products = [&](floatx4 (&c)[4][2], const u32x4 (&fb)[2][2]) {
+    barrier();
+    __builtin_amdgcn_s_setprio(1);
+    mma_frags<S>(c, fa, fb);
+    __builtin_amdgcn_s_setprio(0);
+    barrier();
+  };
+  // of the loads that may be on their way, how many are younger than those a phase waits for: five halves
+  constexpr int kYounger = 3 * LdA::kLoads + 2 * LdB::kLoads;
+  static_assert(LdA::kLoads == LdB::kLoads, "halves of equal size");
+
+  issue_a(0, s0, lds);
+  issue_b(0, s0, lds);
+  issue_b(1, s0, lds);
+  issue_a(1, s0, lds);
+  issue_a(0, s0 + 1, lds + C::kSlot);
+  issue_b(0, s0 + 1, lds + C::kSlot);
+  issue_b(1, s0 + 1, lds + C::kSlot);
+  wait_vmcnt<kYounger>();
+  barrier();
+  if (wave >= 4) barrier();
+  uint32_t t = lds, o = lds + C::kSlot;
+  for (int s = s0; s < s1; ++s) {
+    issue_a(1, s + 1, o);
+    ra.read(fa, t + C::kA0);
+    rb.read(fb0, t + C::kB0);
+    wait_vmcnt<kYounger>();  // B1 of this step, for the next phase
+    products(acc[0][0], fb0);
+
+    issue_a(0, s + 2, t);
+    rb.read(fb1, t + C::kB1);
+    wait_vmcnt<kYounger>();  // A1 of this step
+    products(acc[0][1], fb1);
+
+    issue_b(0, s + 2, t);
+    ra.read(fa, t + C::kA1);
+    products(acc[1][1], fb1);
+
+    issue_b(1, s + 2, t);
+    wait_vmcnt<kYounger>();  // A0 and B0 of the next step
+    products(acc[1][0], fb0);
+    const uint32_t n = t;
+    t = o;
+    o = n;
+  }
+  if (wave < 4) barrier();
+  wait_vmcnt<0>();  // no load may still be on its way to LDS when the block ends
+
+  // 128 rows of C at a time through LDS, so that a wave writes (and the gated
+  // gradient reads) whole rows; chunks are exclusive-ored with the row for the banks
+  floatx4* const cs = reinterpret_cast<floatx4*>(smem);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int r = wm * 64 + p * 16 + (lane & 15), c = j * 32 + wn * 8 + q * 4 + (lane >> 4);
+          cs[r * 64 + (c ^ (r & 15))] = acc[i][j][p][q];
+        }
+    __syncthreads();
+    constexpr int kRows = kPair ? 16 : 8;  // rows a turn
+#pragma unroll 2
+    for (int r0 = 0; r0 < 128; r0 += kRows) {
+      const int r = r0 + (kPair ? wave * 2 + (lane >> 5) : wave), c = kPair ? lane & 31 : lane;
+      const floatx4 c0 = cs[r * 64 + (c ^ (r & 15))];
+      const floatx4 c1 = kPair ? cs[r * 64 + ((c + 32) ^ (r & 15))] : c0;
+      finish<S, C::EPI>(a, z, (int64_t)m0 + i * 128 + r, n0 + c * 4, c0, c1);
+    }
+  }
+}
+
+// Adds the splits' partial sums in order and runs the epilogue; a thread has
+// four columns.
+template <typename S, int EPI>
+__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
+  constexpr int kParts = EPI == kEpiGated ? 2 : 1;
+  const int z = blockIdx.z;
+  const int64_t per_row = a.ldp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= per_row * a.M) return;
+  const int64_t m = i / per_row;
+  const int n = (int)(i % per_row) * 4;
+  floatx4 c[2] = {};
+  const int64_t plane = (int64_t)a.M * a.ldp;
+  const float* p = a.part + (int64_t)z * kParts * plane + m * a.ldp + n;
+  for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) c[k] += *reinterpret_cast<const floatx4*>(p + ((int64_t)s * a.batch * kParts + k) * plane);
+  epilogue<S, EPI>(a, z, m, n, c[0], c[1]);
+}
+
+}  // namespace mhc
