@@ -42,7 +42,7 @@ GemmPlan plan_gemm(const GemmShape& s, size_t es) {
   GemmPlan p;
   const int64_t line_a = s.lda * (int64_t)es, line_b = s.ldb * (int64_t)es;
   // 32-bit offsets within a tile's lines
-  p.dma = line_a % 16 == 0 && line_b % 16 == 0 && line_a < (1 << 24) && line_b < (1 << 24);
+  p.dma = line_a % 16 == 0 && line_b % 16 == 0 && line_a < (1 << 23) && line_b < (1 << 23);
   const int64_t steps = ((s.K * (int64_t)es + 127) / 128) * s.segments;
   const int64_t cus = device_cu_count();
   const auto tiles = [&](int64_t bm, int64_t bn) {

@@ -148,6 +148,39 @@ __device__ __forceinline__ void tile_of(int64_t b, int tm, int tn, int* mt, int*
   *nt = r / rows;
 }
 
+// Where a block's next tiles of A and B start, and how many k are left there
+// (0 past the block's steps).
+template <typename C>
+struct KCursor {
+  using S = typename C::S;
+  const S *pa, *pb, *pb2;  // pb2: the gated form's second operand
+  int s, left;
+
+  static __device__ __forceinline__ int64_t at(int layout, int64_t ld, int first, int kt) {
+    const int64_t k = (int64_t)kt * kStep<S>;
+    return layout == kRow ? first * ld + k : k * ld + first;
+  }
+  __device__ __forceinline__ void segment(const GemmArgs& a, int z, int m0, int n0, int seg, int kt) {
+    pa = static_cast<const S*>(seg | z ? a.A[1] : a.A[0]) + at(C::LA, a.lda, m0, kt);
+    pb = static_cast<const S*>(seg ? a.B[1] : a.B[0]) + at(C::LB, a.ldb, n0, kt);
+    if constexpr (C::EPI == kEpiGated) pb2 = static_cast<const S*>(a.B[1]) + at(C::LB, a.ldb, n0, kt);
+    left = a.K - kt * kStep<S>;
+  }
+  __device__ __forceinline__ KCursor(const GemmArgs& a, int z, int m0, int n0, int nk, int s0, int s1) : pb2(nullptr), s(s0) {
+    segment(a, z, m0, n0, s0 >= nk, s0 >= nk ? s0 - nk : s0);
+    if (s0 >= s1) left = 0;
+  }
+  __device__ __forceinline__ void advance(const GemmArgs& a, int z, int m0, int n0, int nk, int s1) {
+    ++s;
+    pa += C::LA == kRow ? (int64_t)kStep<S> : kStep<S> * a.lda;
+    pb += C::LB == kRow ? (int64_t)kStep<S> : kStep<S> * a.ldb;
+    if constexpr (C::EPI == kEpiGated) pb2 += C::LB == kRow ? (int64_t)kStep<S> : kStep<S> * a.ldb;
+    left -= kStep<S>;
+    if (a.segments == 2 && s == nk) segment(a, z, m0, n0, 1, 0);
+    if (s >= s1) left = 0;
+  }
+};
+
 // ---- the tile kernel -----------------------------------------------------------------
 // Four waves hold a BM x BN tile of C in registers (WM x WN waves); tiles of A
 // and B go through LDS in STAGES slots.  DMA: loads go straight to LDS,
@@ -224,28 +257,26 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(GemmArgs a) {
   if constexpr (C::DMA) {
     LdA la;
     LdB lb;
-    la.init(a.lda, rows_a, wave, lane, row_a);
-    lb.init(a.ldb, rows_b, wave, lane, row_b);
-    const auto issue = [&](int s, int slot) {
-      const int seg = s >= nk, kt = s - seg * nk;
-      const int left = s < s1 ? a.K - kt * kStep<S> : 0;
+    la.init(a.lda, 0, rows_a, wave, lane, row_a);
+    lb.init(a.ldb, 0, rows_b, wave, lane, row_b);
+    KCursor<C> cur(a, z, m0, n0, nk, s0, s1);
+    const auto issue = [&](int slot) {
       const uint32_t t = lds + slot * C::kSlot;
-      la.issue(corner(a.A[seg | z], C::LA, a.lda, m0, kt), left, t, wave);
-      if constexpr (C::kNB == 2) {
-        lb.issue_two(corner(a.B[0], C::LB, a.ldb, n0, kt), corner(a.B[1], C::LB, a.ldb, n0, kt), left, t + C::BM * 128,
-                     wave, second_b);
-      } else {
-        lb.issue(corner(a.B[seg], C::LB, a.ldb, n0, kt), left, t + C::BM * 128, wave);
-      }
+      la.issue(cur.pa, a.lda, cur.left, t, wave);
+      if constexpr (C::kNB == 2)
+        lb.issue_two(cur.pb, cur.pb2, a.ldb, cur.left, t + C::BM * 128, wave, second_b);
+      else
+        lb.issue(cur.pb, a.ldb, cur.left, t + C::BM * 128, wave);
+      cur.advance(a, z, m0, n0, nk, s1);
     };
 #pragma unroll
-    for (int i = 0; i < C::STAGES - 1; ++i) issue(s0 + i, i);
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(i);
     int slot = 0;
     for (int s = s0; s < s1; ++s) {
       wait_vmcnt<(C::STAGES - 2) * (LdA::kLoads + LdB::kLoads)>();
       // every wave's part of slot s is there, and every wave has read slot s - 1
       __builtin_amdgcn_s_barrier();
-      issue(s + C::STAGES - 1, slot == 0 ? C::STAGES - 1 : slot - 1);
+      issue(slot == 0 ? C::STAGES - 1 : slot - 1);
       multiply(slot);
       slot = slot == C::STAGES - 1 ? 0 : slot + 1;
     }
@@ -299,20 +330,18 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(GemmArgs a) {
 // ---- the large tile's kernel -----------------------------------------------------------
 // 256 x 256 of C in the registers of eight waves (2 x 4), one block per CU.
 // The tile's rows and columns are two halves of 128 each (the gated form: B's
-// halves are its two operands), a wave has 64 rows and 32 columns of every
-// half, and multiplies quadrant by quadrant:
+// halves are its two operands); a wave has 64 rows and 32 columns of every
+// half.  A step of k is two phases:
 //
-//   phase  LDS reads   products     loads started
-//     1    A0, B0      A0 x B0      A1 of step k + 1
-//     2    B1          A0 x B1      A0 of step k + 2
-//     3    A1          A1 x B1      B0 of step k + 2
-//     4                A1 x B0      B1 of step k + 2
+//   phase  LDS reads     products       loads started
+//     1    A0, B0, B1    A0 x B0, B1    A1 of step k + 1
+//     2    A1            A1 x B0, B1    A0, B0, B1 of step k + 2
 //
 // A half's slot is free as soon as the phase that reads it is over, so loads
-// run six quarters of a step ahead (five halves, 80 KB a CU, always on their
-// way) with two slots.  Every phase is reads, barrier, products, barrier, and
-// waves 4 .. 7 run one barrier behind waves 0 .. 3: of the two waves on a SIMD
-// one reads while the other multiplies.
+// run a whole step ahead (64 KB a CU on their way) with two slots.  Every
+// phase is reads, barrier, products, barrier, and waves 4 .. 7 run one barrier
+// behind waves 0 .. 3: of the two waves on a SIMD one reads while the other
+// multiplies.
 
 template <typename S_, int LA_, int LB_, int EPI_>
 struct WideCfg {
@@ -345,85 +374,66 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
   const auto same = [](int l) { return l; };
   LdA la0, la1;
   LdB lb0, lb1;
-  la0.init(a.lda, rows_a, wave, lane, same);
-  la1.init(a.lda, rows_a - 128, wave, lane, same);
-  lb0.init(a.ldb, rows_b, wave, lane, same);
-  lb1.init(a.ldb, kPair ? rows_b : rows_b - 128, wave, lane, same);
-  const auto corner = [&](const void* p, int layout, int64_t ld, int64_t first, int kt) {
-    const int64_t k = (int64_t)kt * kStep<S>;
-    return static_cast<const S*>(p) + (layout == kRow ? first * ld + k : k * ld + first);
+  la0.init(a.lda, 0, rows_a, wave, lane, same);
+  la1.init(a.lda, 128, rows_a - 128, wave, lane, same);
+  lb0.init(a.ldb, 0, rows_b, wave, lane, same);
+  if constexpr (!kPair) lb1.init(a.ldb, 128, rows_b - 128, wave, lane, same);
+  KCursor<C> cur(a, z, m0, n0, nk, s0, s1);
+  const auto issue_first = [&](uint32_t slot) {
+    la0.issue(cur.pa, a.lda, cur.left, slot + C::kA0, wave);
+    lb0.issue(cur.pb, a.ldb, cur.left, slot + C::kB0, wave);
+    (kPair ? lb0 : lb1).issue(kPair ? cur.pb2 : cur.pb, a.ldb, cur.left, slot + C::kB1, wave);
   };
-  const auto issue_a = [&](int half, int s, uint32_t slot) {
-    const int seg = s >= nk, kt = s - seg * nk, left = s < s1 ? a.K - kt * kStep<S> : 0;
-    (half ? la1 : la0).issue(corner(a.A[seg | z], C::LA, a.lda, m0 + half * 128, kt), left, slot + (half ? C::kA1 : C::kA0), wave);
-  };
-  const auto issue_b = [&](int half, int s, uint32_t slot) {
-    const int seg = s >= nk, kt = s - seg * nk, left = s < s1 ? a.K - kt * kStep<S> : 0;
-    const void* p = a.B[kPair ? half : seg];
-    (half ? lb1 : lb0).issue(corner(p, C::LB, a.ldb, kPair ? n0 : n0 + half * 128, kt), left, slot + (half ? C::kB1 : C::kB0), wave);
+  const auto issue_second = [&](uint32_t slot) {
+    la1.issue(cur.pa, a.lda, cur.left, slot + C::kA1, wave);
+    cur.advance(a, z, m0, n0, nk, s1);
   };
 
   FragReader<S, C::LA, 128, 4> ra;
   FragReader<S, C::LB, 128, 2> rb;
   ra.init(wm * 64, lane);
   rb.init(wn * 32, lane);
-  floatx4 acc[2][2][4][2];
+  floatx4 acc[2][4][4];  // [half of A][fragment][two of B0, two of B1]
 #pragma unroll
   for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int p = 0; p < 4; ++p)
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) acc[i][j][p][q] = {0.f, 0.f, 0.f, 0.f};
+      for (int q = 0; q < 4; ++q) acc[i][p][q] = {0.f, 0.f, 0.f, 0.f};
 
   const auto barrier = [] {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
   };
-  u32x4 fa[2][4], fb0[2][2], fb1[2][2];
-  const auto products = [&](floatx4 (&c)[4][2], const u32x4 (&fb)[2][2]) {
+  u32x4 fa[2][4], fb[2][4];
+  const auto products = [&](floatx4 (&c)[4][4]) {
     barrier();
     __builtin_amdgcn_s_setprio(1);
     mma_frags<S>(c, fa, fb);
     __builtin_amdgcn_s_setprio(0);
     barrier();
   };
-  // of the loads that may be on their way, how many are younger than those a phase waits for: five halves
-  constexpr int kYounger = 3 * LdA::kLoads + 2 * LdB::kLoads;
-  static_assert(LdA::kLoads == LdB::kLoads, "halves of equal size");
+  // the loads younger than those a phase waits for: four halves
+  constexpr int kYounger = 2 * LdA::kLoads + 2 * LdB::kLoads;
 
-  issue_a(0, s0, lds);
-  issue_b(0, s0, lds);
-  issue_b(1, s0, lds);
-  issue_a(1, s0, lds);
-  issue_a(0, s0 + 1, lds + C::kSlot);
-  issue_b(0, s0 + 1, lds + C::kSlot);
-  issue_b(1, s0 + 1, lds + C::kSlot);
+  issue_first(lds);
+  issue_second(lds);
+  issue_first(lds + C::kSlot);
   wait_vmcnt<kYounger>();
   barrier();
   if (wave >= 4) barrier();
   uint32_t t = lds, o = lds + C::kSlot;
   for (int s = s0; s < s1; ++s) {
-    issue_a(1, s + 1, o);
-    ra.read(fa, t + C::kA0);
-    rb.read(fb0, t + C::kB0);
-    wait_vmcnt<kYounger>();  // B1 of this step, for the next phase
-    products(acc[0][0], fb0);
+    issue_second(o);
+    read_all<S, C::LA, C::LB>(fa, fb, ra, rb, t + C::kA0, t + C::kB0);
+    wait_vmcnt<kYounger>();  // A1 of this step, for the next phase
+    products(acc[0]);
 
-    issue_a(0, s + 2, t);
-    rb.read(fb1, t + C::kB1);
-    wait_vmcnt<kYounger>();  // A1 of this step
-    products(acc[0][1], fb1);
-
-    issue_b(0, s + 2, t);
+    issue_first(t);
     ra.read(fa, t + C::kA1);
-    products(acc[1][1], fb1);
-
-    issue_b(1, s + 2, t);
-    wait_vmcnt<kYounger>();  // A0 and B0 of the next step
-    products(acc[1][0], fb0);
+    wait_vmcnt<kYounger>();  // A0, B0 and B1 of the next step
+    products(acc[1]);
     const uint32_t n = t;
     t = o;
     o = n;
@@ -438,17 +448,15 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
   for (int i = 0; i < 2; ++i) {
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int p = 0; p < 4; ++p)
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int r = wm * 64 + p * 16 + (lane & 15), c = j * 32 + wn * 8 + q * 4 + (lane >> 4);
-          cs[r * 64 + (c ^ (r & 15))] = acc[i][j][p][q];
-        }
+      for (int q = 0; q < 4; ++q) {
+        const int r = wm * 64 + p * 16 + (lane & 15), c = (q >> 1) * 32 + wn * 8 + (q & 1) * 4 + (lane >> 4);
+        cs[r * 64 + (c ^ (r & 15))] = acc[i][p][q];
+      }
     __syncthreads();
     constexpr int kRows = kPair ? 16 : 8;  // rows a turn
-#pragma unroll 2
+#pragma unroll 4
     for (int r0 = 0; r0 < 128; r0 += kRows) {
       const int r = r0 + (kPair ? wave * 2 + (lane >> 5) : wave), c = kPair ? lane & 31 : lane;
       const floatx4 c0 = cs[r * 64 + (c ^ (r & 15))];

@@ -110,7 +110,7 @@ struct TileLoader {
   static_assert(kLineChunks <= 64, "a unit holds whole lines");
 
   uint32_t off[kLoads];  // byte offset of a thread's chunk from the tile's corner, or out of range
-  int pos;          // kRow: the chunk's byte within the line; kCol: the first unit's line
+  int pos;               // kRow: the chunk's byte within the line
 
   static __device__ __forceinline__ int unit(int i, int wave) { return (wave + i * NW) % kUnits; }
   static __device__ __forceinline__ int line(int u, int lane) { return u * (64 / kLineChunks) + lane / kLineChunks; }
@@ -120,38 +120,42 @@ struct TileLoader {
     else return p ^ col_swizzle<S, R>(l);
   }
 
-  // rows: how many of the tile's rows exist; row_of(line) maps a kRow tile's
+  // first: the tile's first row from the corner; rows: how many of its rows
+  // exist; row_of(line) maps a kRow tile's
   // line to its row from the corner (identity but for interleaved operands).
   template <typename F>
-  __device__ __forceinline__ void init(int64_t ld, int rows, int wave, int lane, F row_of) {
+  __device__ __forceinline__ void init(int64_t ld, int first, int rows, int wave, int lane, F row_of) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int u = unit(i, wave), l = line(u, lane), c = chunk(u, lane);
       const bool ok = L == kRow ? row_of(l) < rows : c * kVec<S> < rows;
-      const int src = L == kRow ? row_of(l) : l;
-      off[i] = ok ? (uint32_t)(src * (int)ld * (int)sizeof(S) + c * 16) : kBufferOob;
+      const int line_bytes = (int)ld * (int)sizeof(S);
+      const int at = L == kRow ? (first + row_of(l)) * line_bytes + c * 16 : l * line_bytes + first * (int)sizeof(S) + c * 16;
+      off[i] = ok ? (uint32_t)at : kBufferOob;
     }
     // every unit of a wave has the same parity of 8 lines, so the same chunk
     static_assert(NW % 2 == 0, "units of a wave keep their parity");
-    pos = L == kRow ? chunk(unit(0, wave), lane) * 16 : line(0, lane);
+    pos = L == kRow ? chunk(unit(0, wave), lane) * 16 : 0;
   }
 
   // Starts the loads of the tile at `base` (its corner) into LDS at `dst`;
   // `left` k exist from there on (0 or less: zeros, no memory is read).
-  __device__ __forceinline__ void issue(const void* base, int left, uint32_t dst, int wave) const {
-    issue_two(base, base, left, dst, wave, [](int) { return false; });
+  __device__ __forceinline__ void issue(const void* base, int64_t ld, int left, uint32_t dst, int wave) const {
+    issue_two(base, base, ld, left, dst, wave, [](int) { return false; });
   }
   // Lines with second(line) come from the other corner (the same for a unit's lines).
   template <typename F>
-  __device__ __forceinline__ void issue_two(const void* base, const void* other, int left, uint32_t dst, int wave, F second) const {
+  __device__ __forceinline__ void issue_two(const void* base, const void* other, int64_t ld, int left, uint32_t dst,
+                                            int wave, F second) const {
+    // kCol: lines from `left` on are beyond the range
+    const int k = left < 0 ? 0 : (left < kStep<S> ? left : kStep<S>);
+    const int bytes = __builtin_amdgcn_readfirstlane(L == kCol ? k * (int)(ld * (int)sizeof(S)) : (k > 0 ? 0x7fffffff : 0));
+    const bool in = L == kCol || pos < left * (int)sizeof(S);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int u = unit(i, wave);
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<void*>(second(line(u, 0)) ? other : base), 0, 0x7fffffff, 0x00020000);
-      bool in;
-      if constexpr (L == kRow) in = pos < left * (int)sizeof(S);
-      else in = line(u, 0) + pos < left;
+      const __amdgpu_buffer_rsrc_t rs =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(second(line(u, 0)) ? other : base), 0, bytes, 0x00020000);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void_t*)(uintptr_t)(dst + u * 1024), 16, in ? off[i] : kBufferOob, 0, 0, 0);
     }
   }
@@ -321,5 +325,78 @@ struct FragReader {
     }
   }
 };
+
+// Four fragments of A and two of each half of B (16 KB apart) in one go, 16 bits.
+#define MHC_ROW4(v, a, o1, o2, o3)                                                                     \
+  "ds_read_b128 %[" v "0], %[" a "0]\n\tds_read_b128 %[" v "1], %[" a "0] offset:" o1 "\n\t"         \
+  "ds_read_b128 %[" v "2], %[" a "0] offset:" o2 "\n\tds_read_b128 %[" v "3], %[" a "0] offset:" o3 "\n\t" \
+  "ds_read_b128 %[" v "4], %[" a "1]\n\tds_read_b128 %[" v "5], %[" a "1] offset:" o1 "\n\t"         \
+  "ds_read_b128 %[" v "6], %[" a "1] offset:" o2 "\n\tds_read_b128 %[" v "7], %[" a "1] offset:" o3 "\n\t"
+#define MHC_COL2(v, w, a, o)                                                                          \
+  "ds_read_b64_tr_b16 %[" v "0" w "], %[" a "] offset:" o "\n\t"                                       \
+  "ds_read_b64_tr_b16 %[" v "1" w "], %[" a "] offset:" o "+1024\n\t"                                  \
+  "ds_read_b64_tr_b16 %[" v "2" w "], %[" a "] offset:" o "+8192\n\t"                                  \
+  "ds_read_b64_tr_b16 %[" v "3" w "], %[" a "] offset:" o "+9216\n\t"
+#define MHC_OUT8(v, r) \
+  [v##0] "=&v"(r[0]), [v##1] "=&v"(r[1]), [v##2] "=&v"(r[2]), [v##3] "=&v"(r[3]), [v##4] "=&v"(r[4]), \
+  [v##5] "=&v"(r[5]), [v##6] "=&v"(r[6]), [v##7] "=&v"(r[7])
+#define MHC_OUT4(v, w, r, i) \
+  [v##0##w] "=&v"(r[4 * i]), [v##1##w] "=&v"(r[4 * i + 1]), [v##2##w] "=&v"(r[4 * i + 2]), [v##3##w] "=&v"(r[4 * i + 3])
+
+// A: fragments of 128 lines at `ta`; B: those of the halves at `tb` and `tb` + 16 KB.
+template <typename S, int LA, int LB>
+__device__ __forceinline__ void read_all(u32x4 (&fa)[2][4], u32x4 (&fb)[2][4], const FragReader<S, LA, 128, 4>& ra,
+                                         const FragReader<S, LB, 128, 2>& rb, uint32_t ta, uint32_t tb) {
+  if constexpr (sizeof(S) == 4 && !(LA == kRow && LB == kRow)) {
+    u32x4 b0[2][2], b1[2][2];
+    ra.read(fa, ta);
+    rb.read(b0, tb);
+    rb.read(b1, tb + 16384);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fb[h][j] = b0[h][j], fb[h][2 + j] = b1[h][j];
+  } else if constexpr (LA == kRow && LB == kRow) {
+    u32x4 x[8], y[8];
+    asm volatile(MHC_ROW4("x", "a", "2048", "4096", "6144") MHC_ROW4("y", "b", "2048", "16384", "18432") "s_waitcnt lgkmcnt(0)"
+                 : MHC_OUT8(x, x), MHC_OUT8(y, y)
+                 : [a0] "v"(ta + ra.a[0]), [a1] "v"(ta + ra.a[1]), [b0] "v"(tb + rb.a[0]), [b1] "v"(tb + rb.a[1])
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fa[i / 4][i % 4] = x[i], fb[i / 4][i % 4] = y[i];
+  } else if constexpr (LA == kRow) {
+    u32x4 x[8];
+    u32x2 y[16];
+    asm volatile(MHC_ROW4("x", "a", "2048", "4096", "6144") MHC_COL2("y", "p", "b0", "0") MHC_COL2("y", "q", "b1", "0")
+                     MHC_COL2("y", "r", "b0", "16384") MHC_COL2("y", "s", "b1", "16384") "s_waitcnt lgkmcnt(0)"
+                 : MHC_OUT8(x, x), MHC_OUT4(y, p, y, 0), MHC_OUT4(y, q, y, 1), MHC_OUT4(y, r, y, 2), MHC_OUT4(y, s, y, 3)
+                 : [a0] "v"(ta + ra.a[0]), [a1] "v"(ta + ra.a[1]), [b0] "v"(tb + rb.a[0]), [b1] "v"(tb + rb.a[1])
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fa[i / 4][i % 4] = x[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fb[0][j] = join(y[4 * j], y[4 * j + 1]), fb[1][j] = join(y[4 * j + 2], y[4 * j + 3]);
+  } else {
+    static_assert(LB == kCol, "kCol A goes with kCol B");
+    u32x2 x[16], y[16];
+    asm volatile(MHC_COL2("x", "p", "a0", "0") MHC_COL2("x", "q", "a1", "0") MHC_COL2("x", "r", "a2", "0")
+                     MHC_COL2("x", "s", "a3", "0") MHC_COL2("y", "p", "b0", "0") MHC_COL2("y", "q", "b1", "0")
+                         MHC_COL2("y", "r", "b0", "16384") MHC_COL2("y", "s", "b1", "16384") "s_waitcnt lgkmcnt(0)"
+                 : MHC_OUT4(x, p, x, 0), MHC_OUT4(x, q, x, 1), MHC_OUT4(x, r, x, 2), MHC_OUT4(x, s, x, 3),
+                   MHC_OUT4(y, p, y, 0), MHC_OUT4(y, q, y, 1), MHC_OUT4(y, r, y, 2), MHC_OUT4(y, s, y, 3)
+                 : [a0] "v"(ta + ra.a[0]), [a1] "v"(ta + ra.a[1]), [a2] "v"(ta + ra.a[2]), [a3] "v"(ta + ra.a[3]),
+                   [b0] "v"(tb + rb.a[0]), [b1] "v"(tb + rb.a[1])
+                 : "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      fa[0][j] = join(x[4 * j], x[4 * j + 1]), fa[1][j] = join(x[4 * j + 2], x[4 * j + 3]);
+      fb[0][j] = join(y[4 * j], y[4 * j + 1]), fb[1][j] = join(y[4 * j + 2], y[4 * j + 3]);
+    }
+  }
+}
+#undef MHC_ROW4
+#undef MHC_COL2
+#undef MHC_OUT8
+#undef MHC_OUT4
 
 }  // namespace mhc
