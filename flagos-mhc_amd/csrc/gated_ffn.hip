@@ -3,7 +3,8 @@
 //   g = x Wg^T, u = x Wu^T, h = act(g) u, out = h Wd^T      (x (T,D), Wg, Wu (F,D), Wd (O,F))
 //   dh = dout Wd, du = dh act(g), dg = dh u act'(g)
 //   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dout^T h
-#include <math.h>
+#include <cmath>
+#include <initializer_list>
 
 #include "gemm_kernel.hpp"
 #include "mhc_launch.hpp"
@@ -21,13 +22,6 @@ int64_t hidden_ld(int64_t F) { return (F + 7) / 8 * 8; }
 
 // ---- which kernel runs a product ---------------------------------------------
 
-struct GemmPlan {
-  bool dma;    // operands' lines are whole 16-byte chunks
-  bool wide;   // the large tile's kernel
-  int bm;      // rows of a tile of the tile kernel
-  int splits;  // of k
-};
-
 // Operands as a product's plan sees them: the block's products differ in
 // which index of A and B is contiguous, in the epilogue and in the batch.
 struct GemmShape {
@@ -35,88 +29,177 @@ struct GemmShape {
   int64_t M, N, K, lda, ldb, ldo;
 };
 
-// Time of a 256 x 256 tile on a CU against two 128 x 128 tiles.
-constexpr int kWideWorth = 3;
+// The kernels: tile, blocks a CU, and microseconds for one step (128 bytes of
+// k) of one tile, for operands of 16 bits and 4 bytes: what a CU with all its
+// blocks takes, and what a block alone on its CU takes (measured; `reg`: through
+// registers).
+enum { kTile16, kTile64x128, kTile64, kTile128, kWide128, kWide256, kKinds };
+struct StepCost {
+  double full, alone;
+};
+struct KernelCost {
+  int bm, bn, per_cu;
+  StepCost dma16, dma32, reg16, reg32;
+};
+constexpr KernelCost kCosts[kKinds] = {
+    {16, 128, 2, {0.85, 0.7}, {0.85, 0.7}, {1.0, 1.2}, {1.0, 1.2}},
+    {64, 128, 2, {1.1, 0.9}, {1.6, 1.8}, {1.1, 1.2}, {1.8, 2.0}},
+    {64, 64, 4, {0.23, 0.6}, {0.6, 0.8}, {0.4, 0.76}, {0.65, 1.0}},
+    {128, 128, 2, {0.46, 0.8}, {2.3, 3.2}, {0.8, 1.28}, {2.5, 3.5}},
+    {128, 256, 1, {0.78, 0.78}, {4.4, 4.4}, {}, {}},
+    {256, 256, 1, {1.25, 1.25}, {8.5, 8.5}, {}, {}}};
+constexpr double kJoinUs = 5., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
 
-GemmPlan plan_gemm(const GemmShape& s, size_t es) {
-  GemmPlan p;
-  const int64_t line_a = s.lda * (int64_t)es, line_b = s.ldb * (int64_t)es;
-  // 32-bit offsets within a tile's lines
-  p.dma = line_a % 16 == 0 && line_b % 16 == 0 && line_a < (1 << 23) && line_b < (1 << 23);
-  const int64_t steps = ((s.K * (int64_t)es + 127) / 128) * s.segments;
-  const int64_t cus = device_cu_count();
-  const auto tiles = [&](int64_t bm, int64_t bn) {
-    const int64_t cols = s.epi == kEpiGated ? bn / 2 : bn;
-    return ((s.M + bm - 1) / bm) * ((s.ldo + cols - 1) / cols) * s.batch;
+struct GemmPlan {
+  bool dma;   // operands' lines are whole 16-byte chunks
+  int kind;
+  int whole_tiles, run_tiles, run_blocks;
+  double us;
+};
+
+int64_t tiles_of(const GemmShape& s, int64_t bm, int64_t bn) {
+  const int64_t cols = s.epi == kEpiGated ? bn / 2 : bn;
+  return ((s.M + bm - 1) / bm) * ((s.ldo + cols - 1) / cols) * s.batch;
+}
+
+// Whole tiles go out in rounds of all blocks that fit the card at once; the
+// last round's tiles are cut into equal runs of steps if that, with the
+// partial sums' way through memory, is less than the round.
+GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma) {
+  const KernelCost& c = kCosts[kind];
+  const StepCost& cost = dma ? (es == 4 ? c.dma32 : c.dma16) : (es == 4 ? c.reg32 : c.reg16);
+  const int64_t cus = device_cu_count(), slots = cus * c.per_cu;
+  const int64_t tiles = tiles_of(s, c.bm, c.bn), steps = (s.K * (int64_t)es + 127) / 128 * s.segments;
+  // `steps` steps of `blocks` blocks side by side
+  const auto side_by_side = [&](double blocks, double n) {
+    const double full = std::ceil(blocks / cus) * cost.full;
+    return n * (full > cost.alone ? full : cost.alone);
   };
-  const auto rounds = [](int64_t n, int64_t slots) { return (n + slots - 1) / slots; };
-  p.bm = s.la == kCol || s.M > 64 ? 128 : (s.M > 16 ? 64 : 16);
-  p.wide = p.dma && p.bm == 128 && kWideWorth * rounds(tiles(256, 256), cus) <= 2 * rounds(tiles(128, 128), 2 * cus);
-  // too few tiles to fill the card: split k, in pieces of eight steps or more
-  const int64_t n = p.wide ? tiles(256, 256) : tiles(p.bm, 128), slots = p.wide ? cus : 2 * cus;
-  int64_t splits = n >= slots ? 1 : slots / n;
-  if (splits > steps / 8) splits = steps / 8;
-  p.splits = (int)(splits < 1 ? 1 : (splits > 64 ? 64 : splits));
+  const int64_t rest = tiles % slots, rounds = tiles / slots;
+  const double rounds_us = kLaunchUs + rounds * side_by_side((double)slots, (double)steps);
+  GemmPlan p = {dma, kind, (int)tiles, 0, 0, rounds_us};
+  if (rest == 0) return p;
+  p.us += side_by_side((double)rest, (double)steps);
+  // Runs of six steps or more.  The large tiles' blocks that work side by side
+  // have to be at the same k of neighbouring tiles, or every one of them
+  // fetches its operands for itself: a tile is cut into as many equal runs as
+  // there is room for.
+  int64_t blocks = rest * steps / 6;
+  if (blocks > slots) blocks = slots;
+  if (kind >= kWide128) blocks = blocks / rest * rest;
+  if (blocks > rest) {
+    const double bytes = (double)(blocks + rest) * (s.M < c.bm ? s.M : c.bm) * c.bn * 4 * 2;
+    const double us = rounds_us + side_by_side((double)blocks, (double)rest * steps / blocks) + kJoinUs + bytes / kJoinBytesPerUs;
+    if (us < p.us) p = {dma, kind, (int)(tiles - rest), (int)rest, (int)blocks, us};
+  }
   return p;
 }
 
-int64_t part_ld(const GemmShape& s) { return (s.ldo + 3) / 4 * 4; }
-size_t part_bytes(const GemmShape& s, const GemmPlan& p) {
-  if (p.splits == 1) return 0;
-  return (size_t)p.splits * s.batch * (s.epi == kEpiGated ? 2 : 1) * s.M * part_ld(s) * sizeof(float);
+GemmPlan plan_rows(const GemmShape& s, size_t es) {
+  const int64_t line_a = s.lda * (int64_t)es, line_b = s.ldb * (int64_t)es;
+  // 32-bit offsets within a tile's lines
+  const bool dma = line_a % 16 == 0 && line_b % 16 == 0 && line_a < (1 << 23) && line_b < (1 << 23);
+  GemmPlan p = {};
+  for (int kind = 0; kind < kKinds; ++kind) {
+    if (kind >= kWide128 && !dma) break;
+    const bool few = kind <= kTile64x128;  // rows: the tile that holds them all; kCol tiles have 64 rows or more
+    if (few && (s.la == kCol || s.M > kCosts[kind].bm)) continue;
+    const GemmPlan q = deal_tiles(s, es, kind, dma);
+    if (p.us == 0. || q.us < p.us) p = q;
+    if (few) break;
+  }
+  return p;
+}
+
+// A product is one launch, or two: the rows past the last whole 256 go apart
+// where they are few and would take a row of large tiles.
+struct GemmPlans {
+  GemmPlan main, tail;
+  int64_t main_rows;  // M: no tail
+};
+GemmPlans plan_gemm(const GemmShape& s, size_t es) {
+  GemmPlans p = {plan_rows(s, es), {}, s.M};
+  const int64_t over = s.M % 256;
+  if (s.la == kRow && s.M > 256 && over > 0 && over <= 64) {
+    GemmShape m = s, t = s;
+    m.M = s.M - over;
+    t.M = over;
+    const GemmPlan a = plan_rows(m, es), b = plan_rows(t, es);
+    if (a.us + b.us < p.main.us) p = {a, b, m.M};
+  }
+  return p;
+}
+
+size_t part_bytes(const GemmPlans& p) {
+  size_t n = 0;
+  for (const GemmPlan* q : {&p.main, &p.tail}) {
+    const size_t b = (size_t)2 * q->run_blocks * kCosts[q->kind].bm * kCosts[q->kind].bn * sizeof(float);
+    n = b > n ? b : n;
+  }
+  return n;
+}
+
+template <typename C>
+int launch_join(const GemmArgs& a, hipStream_t st) {
+  if (a.run_tiles == 0) return MHC_OK;
+  const dim3 g((unsigned)a.run_tiles * (C::BM * (C::kCols / 4) / 256)), b(256);
+  if (const int rc = check_grid(g, b, "gated_ffn")) return rc;
+  hipLaunchKernelGGL((gemm_join_kernel<C>), g, b, 0, st, a);
+  return check_launch("gated_ffn");
 }
 
 template <typename C>
 int launch_tile(const GemmArgs& a, hipStream_t st) {
-  const int64_t tiles = (int64_t)((a.M + C::BM - 1) / C::BM) * ((a.ldo + C::kCols - 1) / C::kCols);
-  const dim3 g((unsigned)tiles, (unsigned)a.splits, (unsigned)a.batch), b(256);
-  if (tiles > 0x7fffffff) return set_error(MHC_ERR_UNSUPPORTED, "gated_ffn: %lld tiles", (long long)tiles);
+  const dim3 g((unsigned)a.whole_tiles + (unsigned)a.run_blocks), b(256);
   if (const int rc = check_grid(g, b, "gated_ffn")) return rc;
   hipLaunchKernelGGL((gemm_tile_kernel<C>), g, b, 0, st, a);
-  return check_launch("gated_ffn");
+  if (const int rc = check_launch("gated_ffn")) return rc;
+  return launch_join<C>(a, st);
 }
 
 template <typename C>
 int launch_wide(const GemmArgs& a, hipStream_t st) {
-  const int64_t tiles = (int64_t)((a.M + C::BM - 1) / C::BM) * ((a.ldo + C::kCols - 1) / C::kCols);
-  const dim3 g((unsigned)tiles, (unsigned)a.splits, (unsigned)a.batch), b(512);
-  if (tiles > 0x7fffffff) return set_error(MHC_ERR_UNSUPPORTED, "gated_ffn: %lld tiles", (long long)tiles);
+  const dim3 g((unsigned)a.whole_tiles + (unsigned)a.run_blocks), b(512);
   if (const int rc = check_grid(g, b, "gated_ffn")) return rc;
   hipLaunchKernelGGL((gemm_wide_kernel<C>), g, b, 0, st, a);
-  return check_launch("gated_ffn");
+  if (const int rc = check_launch("gated_ffn")) return rc;
+  return launch_join<C>(a, st);
 }
 
-template <typename S, int EPI>
-int launch_join(const GemmArgs& a, hipStream_t st) {
-  const int64_t n = a.ldp / 4 * a.M;
-  const dim3 g((unsigned)((n + 255) / 256), 1, (unsigned)a.batch), b(256);
-  if (const int rc = check_grid(g, b, "gated_ffn")) return rc;
-  hipLaunchKernelGGL((gemm_join_kernel<S, EPI>), g, b, 0, st, a);
-  return check_launch("gated_ffn");
+template <typename S, int LA, int LB, int EPI>
+int launch_plan(GemmArgs a, const GemmPlan& p, float* part, hipStream_t st) {
+  a.whole_tiles = p.whole_tiles, a.run_tiles = p.run_tiles, a.run_blocks = p.run_blocks;
+  a.part = part;
+  if (p.kind == kWide256) return launch_wide<WideCfg<S, LA, LB, 256, EPI>>(a, st);
+  if (p.kind == kWide128) return launch_wide<WideCfg<S, LA, LB, 128, EPI>>(a, st);
+  if constexpr (LA == kRow) {
+    if (p.kind == kTile64x128)
+      return p.dma ? launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 3, 2, EPI, true>>(a, st)
+                   : launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 2, 2, EPI, false>>(a, st);
+    if (p.kind == kTile16)
+      return p.dma ? launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 4, 2, EPI, true>>(a, st)
+                   : launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 2, 2, EPI, false>>(a, st);
+  }
+  if (p.kind == kTile64)
+    return p.dma ? launch_tile<TileCfg<S, LA, LB, 64, 64, 2, 2, 4, EPI, true>>(a, st)
+                 : launch_tile<TileCfg<S, LA, LB, 64, 64, 2, 2, 4, EPI, false>>(a, st);
+  return p.dma ? launch_tile<TileCfg<S, LA, LB, 128, 128, 2, 2, 2, EPI, true>>(a, st)
+               : launch_tile<TileCfg<S, LA, LB, 128, 128, 2, 2, 2, EPI, false>>(a, st);
 }
 
 template <typename S, int LA, int LB, int EPI>
 int launch_gemm(GemmArgs a, const GemmShape& s, float* part, hipStream_t st) {
-  const GemmPlan p = plan_gemm(s, sizeof(S));
-  a.splits = p.splits;
-  a.part = part;
-  a.ldp = part_ld(s);
-  int rc = MHC_OK;
-  if (p.wide) {
-    rc = launch_wide<WideCfg<S, LA, LB, EPI>>(a, st);
-  } else if (p.bm == 128) {
-    rc = p.dma ? launch_tile<TileCfg<S, LA, LB, 128, 128, 2, 2, EPI, true>>(a, st)
-               : launch_tile<TileCfg<S, LA, LB, 128, 128, 2, 2, EPI, false>>(a, st);
-  } else if constexpr (LA == kRow) {
-    if (p.bm == 64)
-      rc = p.dma ? launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 3, EPI, true>>(a, st)
-                 : launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 2, EPI, false>>(a, st);
-    else
-      rc = p.dma ? launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 4, EPI, true>>(a, st)
-                 : launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 2, EPI, false>>(a, st);
-  }
-  if (rc || p.splits == 1) return rc;
-  return launch_join<S, EPI>(a, st);
+  const GemmPlans p = plan_gemm(s, sizeof(S));
+  a.M = (int)p.main_rows;
+  if (const int rc = launch_plan<S, LA, LB, EPI>(a, p.main, part, st)) return rc;
+  if (p.main_rows == s.M) return MHC_OK;
+  const int64_t r = p.main_rows;
+  a.M = (int)(s.M - r);
+  for (const void*& q : a.A) q = static_cast<const S*>(q) + r * s.lda;
+  a.out0 = static_cast<S*>(a.out0) + r * s.ldo;
+  if (a.out1) a.out1 = static_cast<S*>(a.out1) + r * s.ldo;
+  if (a.gate) a.gate += r * s.N, a.up += r * s.N;
+  return launch_plan<S, LA, LB, EPI>(a, p.tail, part, st);
 }
 
 // ---- the block's products ------------------------------------------------------
@@ -133,12 +216,12 @@ size_t most(size_t a, size_t b) { return a > b ? a : b; }
 size_t hidden_bytes(const FfnDims& d, size_t es) { return round_up((size_t)d.T * hidden_ld(d.F) * es); }
 size_t fwd_part_bytes(const FfnDims& d, size_t es) {
   size_t n = 0;
-  for (const GemmShape& s : {fwd_hidden(d), fwd_out(d)}) n = most(n, part_bytes(s, plan_gemm(s, es)));
+  for (const GemmShape& s : {fwd_hidden(d), fwd_out(d)}) n = most(n, part_bytes(plan_gemm(s, es)));
   return n;
 }
 size_t bwd_part_bytes(const FfnDims& d, size_t es) {
   size_t n = 0;
-  for (const GemmShape& s : {bwd_hidden(d), bwd_x(d), bwd_down(d), bwd_gate_up(d)}) n = most(n, part_bytes(s, plan_gemm(s, es)));
+  for (const GemmShape& s : {bwd_hidden(d), bwd_x(d), bwd_down(d), bwd_gate_up(d)}) n = most(n, part_bytes(plan_gemm(s, es)));
   return n;
 }
 
@@ -181,6 +264,11 @@ int check_ffn(const char* who, const FfnDims& d, int32_t dtype, int32_t act) {
   if (d.T > kMaxTokens) return check_tokens(d.T, who);
   if (dtype != MHC_DTYPE_F32 && dtype != MHC_DTYPE_BF16 && dtype != MHC_DTYPE_F16)
     return set_error(MHC_ERR_UNSUPPORTED, "%s: dtype %d not supported", who, dtype);
+  // tiles are counted in 32 bits
+  if (((d.T + 15) / 16) * (((int64_t)(d.F > d.O ? d.F : d.O) + 63) / 64) > 0x3fffffff ||
+      (((int64_t)d.F + 63) / 64) * (((int64_t)(d.D > d.O ? d.D : d.O) + 63) / 64) > 0x3fffffff ||
+      ((d.T + 15) / 16) * (((int64_t)d.D + 63) / 64) > 0x3fffffff)
+    return set_error(MHC_ERR_UNSUPPORTED, "%s: T=%lld D=%d F=%d O=%d are too many tiles", who, (long long)d.T, d.D, d.F, d.O);
   if (act < 0 || act > kActRelu) return set_error(MHC_ERR_INVALID, "%s: activation %d", who, act);
   return MHC_OK;
 }

@@ -27,9 +27,11 @@ struct GemmArgs {
   float* gate;       // (M, N)
   float* up;
   int act;
-  int splits;        // of the steps of k: partial sums go to `part`
-  float* part;       // [splits][batch or gated pair][M][ldp]
-  int64_t ldp;
+  // How the tiles are dealt out: whole ones to the first blocks, one each; the
+  // steps of the others in equal runs to `run_blocks` more, whose parts of
+  // tiles go to `part` ([2 a block][tile]) and are added by the join kernel.
+  int whole_tiles, run_tiles, run_blocks;
+  float* part;
 };
 
 // act(g) and act'(g) in fp32.
@@ -121,31 +123,64 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, int64_t m, in
   }
 }
 
-// A kernel's four columns of row m: through the epilogue, or to this split's partial sums.
-template <typename S, int EPI>
-__device__ __forceinline__ void finish(const GemmArgs& a, int z, int64_t m, int n, const floatx4& c0, const floatx4& c1) {
-  if (a.splits == 1) {
-    epilogue<S, EPI>(a, z, m, n, c0, c1);
-  } else if (m < a.M && n < a.ldp) {
-    constexpr int kParts = EPI == kEpiGated ? 2 : 1;
-    float* p = a.part + (((int64_t)blockIdx.y * a.batch + z) * kParts * a.M + m) * a.ldp + n;
-    *reinterpret_cast<floatx4*>(p) = c0;
-    if constexpr (kParts == 2) *reinterpret_cast<floatx4*>(p + (int64_t)a.M * a.ldp) = c1;
-  }
-}
-
 // ---- order of the tiles ------------------------------------------------------------
 
-// Tile (mt, nt) of the b-th block of tm x tn: each XCD walks a contiguous run
-// of the order, which goes down groups of 8 tile rows, so that the tiles an
-// XCD works on at one time share their operands in its L2.
-__device__ __forceinline__ void tile_of(int64_t b, int tm, int tn, int* mt, int* nt) {
+// Tile (mt, nt) of product z for the t-th of batch x tm x tn: down groups of 8
+// tile rows, so that the tiles an XCD works on at one time (contiguous runs of
+// the order) share their operands in its L2.
+__device__ __forceinline__ void tile_of(int t, int tm, int tn, int* mt, int* nt, int* z) {
   constexpr int kGroup = 8;
-  const int t = (int)xcd_contig(b, (int64_t)tm * tn);
+  const int q = t / (tm * tn);
+  t -= q * tm * tn;
   const int per = kGroup * tn, g = t / per, r = t % per;
   const int rows = tm - g * kGroup < kGroup ? tm - g * kGroup : kGroup;
-  *mt = g * kGroup + r % rows;
-  *nt = r / rows;
+  // (the compiler divides in vector registers)
+  *z = __builtin_amdgcn_readfirstlane(q);
+  *mt = __builtin_amdgcn_readfirstlane(g * kGroup + r % rows);
+  *nt = __builtin_amdgcn_readfirstlane(r / rows);
+}
+
+// Where run block b's steps start: of `steps` steps a tile.
+__host__ __device__ __forceinline__ int64_t run_start(int64_t b, int tiles, int steps, int blocks) {
+  return b * tiles * steps / blocks;
+}
+
+// A block's i-th piece of work: steps s0 .. s1 - 1 of a tile, or none.
+// (A run is shorter than a tile, so it has one piece or two.)
+struct Piece {
+  int tile, s0, s1;
+  int slot;  // of the partial sums; -1: the whole tile
+};
+__device__ __forceinline__ bool piece_of(const GemmArgs& a, int steps, int i, Piece* p) {
+  const int bid = blockIdx.x;
+  p->slot = -1;
+  if (bid < a.whole_tiles) {
+    *p = {__builtin_amdgcn_readfirstlane((int)xcd_contig(bid, a.whole_tiles)), 0, steps, -1};
+    return i == 0;
+  }
+  const int64_t b = xcd_contig(bid - a.whole_tiles, a.run_blocks);
+  const int64_t lo = run_start(b, a.run_tiles, steps, a.run_blocks), hi = run_start(b + 1, a.run_tiles, steps, a.run_blocks);
+  const int64_t t = lo / steps + i;
+  const int64_t first = t * steps, s0 = lo > first ? lo - first : 0, s1 = hi - first < steps ? hi - first : steps;
+  if (s0 >= s1) return false;
+  const auto uniform = [](int64_t v) { return __builtin_amdgcn_readfirstlane((int)v); };
+  *p = {uniform(a.whole_tiles + t), uniform(s0), uniform(s1), uniform(s0 == 0 && s1 == steps ? -1 : 2 * b + i)};
+  return true;
+}
+
+// Row r, columns c .. c + 3 of the tile at (m0, n0): through the epilogue, or
+// to the piece's partial sums ([BM][columns, then those of the gated form's
+// second operand]).
+template <typename C>
+__device__ __forceinline__ void finish(const GemmArgs& a, const Piece& p, int z, int m0, int n0, int r, int c,
+                                       const floatx4& c0, const floatx4& c1) {
+  if (p.slot < 0) {
+    epilogue<typename C::S, C::EPI>(a, z, (int64_t)m0 + r, n0 + c, c0, c1);
+  } else if (m0 + r < a.M) {
+    float* q = a.part + ((int64_t)p.slot * C::BM + r) * C::BN + c;
+    *reinterpret_cast<floatx4*>(q) = c0;
+    if constexpr (C::EPI == kEpiGated) *reinterpret_cast<floatx4*>(q + C::kCols) = c1;
+  }
 }
 
 // Where a block's next tiles of A and B start, and how many k are left there
@@ -185,9 +220,9 @@ struct KCursor {
 // Four waves hold a BM x BN tile of C in registers (WM x WN waves); tiles of A
 // and B go through LDS in STAGES slots.  DMA: loads go straight to LDS,
 // STAGES - 1 tiles ahead; otherwise through registers, for operands whose rows
-// are not multiples of 16 bytes.  grid: (tiles, splits, batch).
+// are not multiples of 16 bytes.
 
-template <typename S_, int LA_, int LB_, int BM_, int BN_, int WAVES_M_, int STAGES_, int EPI_, bool DMA_>
+template <typename S_, int LA_, int LB_, int BM_, int BN_, int WAVES_M_, int STAGES_, int PER_CU_, int EPI_, bool DMA_>
 struct TileCfg {
   using S = S_;
   static constexpr int LA = LA_, LB = LB_, BM = BM_, BN = BN_, STAGES = STAGES_, EPI = EPI_;
@@ -198,27 +233,21 @@ struct TileCfg {
   static constexpr int kNB = EPI == kEpiGated ? 2 : 1;         // B operands
   static constexpr int kCols = BN / kNB;                       // columns of C
   static constexpr int kSlot = (BM + BN) * 128;
-  static_assert(STAGES >= 2 && STAGES * kSlot <= 160 * 1024, "LDS");
+  static constexpr int kPerCu = PER_CU_;  // blocks
+  static_assert(STAGES >= 2 && kPerCu * STAGES * kSlot <= 160 * 1024, "LDS");
   static_assert(DMA || STAGES == 2, "register staging has two slots");
   static_assert(EPI != kEpiGated || LB == kRow, "the gated form's weights are rows of k");
 };
 
 template <typename C>
-__global__ __launch_bounds__(256, 2) void gemm_tile_kernel(GemmArgs a) {
+__device__ __forceinline__ void gemm_tile_piece(const GemmArgs& a, const Piece& piece, int nk, char* smem) {
   using S = typename C::S;
-  __shared__ __attribute__((aligned(1024))) char smem[C::STAGES * C::kSlot];
   const uint32_t lds = lds_addr(smem);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave % C::WAVES_M, wn = wave / C::WAVES_M;
-  const int z = blockIdx.z;
-  int mt, nt;
-  tile_of(blockIdx.x, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt);
-  const int m0 = mt * C::BM, n0 = nt * C::kCols;
-
-  // steps of k of this split
-  const int nk = (a.K + kStep<S> - 1) / kStep<S>, total = nk * a.segments;
-  const int s0 = (int)((int64_t)total * blockIdx.y / a.splits), s1 = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
-
+  int mt, nt, z;
+  tile_of(piece.tile, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt, &z);
+  const int m0 = mt * C::BM, n0 = nt * C::kCols, s0 = piece.s0, s1 = piece.s1;
   using LdA = TileLoader<S, C::LA, C::BM, C::NW>;
   using LdB = TileLoader<S, C::LB, C::BN, C::NW>;
   const auto row_a = [](int l) { return l; };
@@ -313,59 +342,64 @@ __global__ __launch_bounds__(256, 2) void gemm_tile_kernel(GemmArgs a) {
   }
 
   // lane: row l % 16 of a fragment of A, columns 4 (l / 16) .. + 3 of one of B
-  const int64_t mw = m0 + wm * C::WM + (lane & 15);
   constexpr int NC = C::NFB / C::kNB;
-  const int nw = n0 + wn * (C::WN / C::kNB) + (lane >> 4) * 4;
 #pragma unroll
   for (int i = 0; i < C::NFA; ++i)
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const int64_t m = mw + 16 * i;
-      const int n = nw + 16 * j;
-      const floatx4 c0 = acc[i][j], c1 = acc[i][C::kNB == 2 ? j + NC : j];
-      finish<S, C::EPI>(a, z, m, n, c0, c1);
-    }
+    for (int j = 0; j < NC; ++j)
+      finish<C>(a, piece, z, m0, n0, wm * C::WM + 16 * i + (lane & 15), wn * (C::WN / C::kNB) + 16 * j + (lane >> 4) * 4,
+                acc[i][j], acc[i][C::kNB == 2 ? j + NC : j]);
 }
 
-// ---- the large tile's kernel -----------------------------------------------------------
-// 256 x 256 of C in the registers of eight waves (2 x 4), one block per CU.
-// The tile's rows and columns are two halves of 128 each (the gated form: B's
-// halves are its two operands); a wave has 64 rows and 32 columns of every
-// half.  A step of k is two phases:
+template <typename C>
+__global__ __launch_bounds__(256, C::kPerCu) void gemm_tile_kernel(GemmArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[C::STAGES * C::kSlot];
+  const int nk = (a.K + kStep<typename C::S> - 1) / kStep<typename C::S>;
+  Piece piece;
+  for (int i = 0; piece_of(a, nk * a.segments, i, &piece); ++i) {
+    if (i) __syncthreads();  // every wave is through with the last piece's LDS
+    gemm_tile_piece<C>(a, piece, nk, smem);
+  }
+}
+
+// ---- the large tiles' kernel ----------------------------------------------------------
+// BM x 256 of C in the registers of eight waves (2 x 4), one block per CU, BM
+// = 256 or 128.  The tile's rows are halves of 128 (one or two), its columns
+// two (the gated form: B's halves are its two operands); a wave has 64 rows
+// and 32 columns of every half.  A step of k is a phase for each half of A:
 //
-//   phase  LDS reads     products       loads started
+//   phase  LDS reads     products       loads started (BM = 256)
 //     1    A0, B0, B1    A0 x B0, B1    A1 of step k + 1
 //     2    A1            A1 x B0, B1    A0, B0, B1 of step k + 2
 //
-// A half's slot is free as soon as the phase that reads it is over, so loads
-// run a whole step ahead (64 KB a CU on their way) with two slots.  Every
+// With two slots a half's is free as soon as the phase that reads it is over,
+// so loads run a whole step ahead (64 KB a CU on their way).  BM = 128 has
+// three slots and starts the loads of step k + 2 in its only phase.  Every
 // phase is reads, barrier, products, barrier, and waves 4 .. 7 run one barrier
 // behind waves 0 .. 3: of the two waves on a SIMD one reads while the other
 // multiplies.
 
-template <typename S_, int LA_, int LB_, int EPI_>
+template <typename S_, int LA_, int LB_, int BM_, int EPI_>
 struct WideCfg {
   using S = S_;
-  static constexpr int LA = LA_, LB = LB_, EPI = EPI_, BM = 256;
+  static constexpr int LA = LA_, LB = LB_, EPI = EPI_, BM = BM_, BN = 256;
   static constexpr int kCols = EPI == kEpiGated ? 128 : 256;  // columns of C
   static constexpr int kHalf = 128 * 128;                     // bytes of a half in LDS
-  static constexpr int kA0 = 0, kA1 = kHalf, kB0 = 2 * kHalf, kB1 = 3 * kHalf, kSlot = 4 * kHalf;
+  static constexpr int kHalves = BM / 128;                    // of A
+  static constexpr int kA0 = 0, kA1 = kHalf, kB0 = kHalves * kHalf, kB1 = kB0 + kHalf, kSlot = kB1 + kHalf;
+  static constexpr int kSlots = kHalves == 2 ? 2 : 3;
+  static constexpr int kPerCu = 1;
 };
 
 template <typename C>
-__global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
+__device__ __forceinline__ void gemm_wide_piece(const GemmArgs& a, const Piece& piece, int nk, char* smem) {
   using S = typename C::S;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * C::kSlot];
   const uint32_t lds = lds_addr(smem);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave >> 1) & 1, wn = (wave & 1) | ((wave >> 2) << 1);
-  const int z = blockIdx.z;
-  int mt, nt;
-  tile_of(blockIdx.x, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt);
-  const int m0 = mt * C::BM, n0 = nt * C::kCols;
-  const int nk = (a.K + kStep<S> - 1) / kStep<S>, total = nk * a.segments;
-  const int s0 = (int)((int64_t)total * blockIdx.y / a.splits), s1 = (int)((int64_t)total * (blockIdx.y + 1) / a.splits);
-
+  int mt, nt, z;
+  tile_of(piece.tile, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt, &z);
+  const int m0 = mt * C::BM, n0 = nt * C::kCols, s0 = piece.s0, s1 = piece.s1;
   using LdA = TileLoader<S, C::LA, 128, 8>;
   using LdB = TileLoader<S, C::LB, 128, 8>;
   constexpr bool kPair = C::EPI == kEpiGated;
@@ -375,7 +409,7 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
   LdA la0, la1;
   LdB lb0, lb1;
   la0.init(a.lda, 0, rows_a, wave, lane, same);
-  la1.init(a.lda, 128, rows_a - 128, wave, lane, same);
+  if constexpr (C::kHalves == 2) la1.init(a.lda, 128, rows_a - 128, wave, lane, same);
   lb0.init(a.ldb, 0, rows_b, wave, lane, same);
   if constexpr (!kPair) lb1.init(a.ldb, 128, rows_b - 128, wave, lane, same);
   KCursor<C> cur(a, z, m0, n0, nk, s0, s1);
@@ -385,7 +419,7 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
     (kPair ? lb0 : lb1).issue(kPair ? cur.pb2 : cur.pb, a.ldb, cur.left, slot + C::kB1, wave);
   };
   const auto issue_second = [&](uint32_t slot) {
-    la1.issue(cur.pa, a.lda, cur.left, slot + C::kA1, wave);
+    if constexpr (C::kHalves == 2) la1.issue(cur.pa, a.lda, cur.left, slot + C::kA1, wave);
     cur.advance(a, z, m0, n0, nk, s1);
   };
 
@@ -393,9 +427,9 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
   FragReader<S, C::LB, 128, 2> rb;
   ra.init(wm * 64, lane);
   rb.init(wn * 32, lane);
-  floatx4 acc[2][4][4];  // [half of A][fragment][two of B0, two of B1]
+  floatx4 acc[C::kHalves][4][4];  // [half of A][fragment][two of B0, two of B1]
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < C::kHalves; ++i)
 #pragma unroll
     for (int p = 0; p < 4; ++p)
 #pragma unroll
@@ -414,29 +448,51 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
     __builtin_amdgcn_s_setprio(0);
     barrier();
   };
-  // the loads younger than those a phase waits for: four halves
-  constexpr int kYounger = 2 * LdA::kLoads + 2 * LdB::kLoads;
+  if constexpr (C::kHalves == 2) {
+    // the loads younger than those a phase waits for: four halves
+    constexpr int kYounger = 2 * LdA::kLoads + 2 * LdB::kLoads;
+    issue_first(lds);
+    issue_second(lds);
+    issue_first(lds + C::kSlot);
+    wait_vmcnt<kYounger>();
+    barrier();
+    if (wave >= 4) barrier();
+    uint32_t t = lds, o = lds + C::kSlot;
+    for (int s = s0; s < s1; ++s) {
+      issue_second(o);
+      read_all<S, C::LA, C::LB>(fa, fb, ra, rb, t + C::kA0, t + C::kB0);
+      wait_vmcnt<kYounger>();  // A1 of this step, for the next phase
+      products(acc[0]);
 
-  issue_first(lds);
-  issue_second(lds);
-  issue_first(lds + C::kSlot);
-  wait_vmcnt<kYounger>();
-  barrier();
-  if (wave >= 4) barrier();
-  uint32_t t = lds, o = lds + C::kSlot;
-  for (int s = s0; s < s1; ++s) {
-    issue_second(o);
-    read_all<S, C::LA, C::LB>(fa, fb, ra, rb, t + C::kA0, t + C::kB0);
-    wait_vmcnt<kYounger>();  // A1 of this step, for the next phase
-    products(acc[0]);
-
-    issue_first(t);
-    ra.read(fa, t + C::kA1);
-    wait_vmcnt<kYounger>();  // A0, B0 and B1 of the next step
-    products(acc[1]);
-    const uint32_t n = t;
-    t = o;
-    o = n;
+      issue_first(t);
+      ra.read(fa, t + C::kA1);
+      wait_vmcnt<kYounger>();  // A0, B0 and B1 of the next step
+      products(acc[1]);
+      const uint32_t n = t;
+      t = o;
+      o = n;
+    }
+  } else {
+    constexpr int kYounger = LdA::kLoads + 2 * LdB::kLoads;  // a step's
+    const auto issue = [&](uint32_t slot) {
+      issue_first(slot);
+      issue_second(slot);
+    };
+    issue(lds);
+    issue(lds + C::kSlot);
+    wait_vmcnt<kYounger>();
+    barrier();
+    if (wave >= 4) barrier();
+    // a step's slot, and that of the step before it, which nobody reads any more
+    uint32_t t = lds, free = lds + 2 * C::kSlot;
+    for (int s = s0; s < s1; ++s) {
+      issue(free);
+      read_all<S, C::LA, C::LB>(fa, fb, ra, rb, t + C::kA0, t + C::kB0);
+      wait_vmcnt<kYounger>();  // the next step
+      products(acc[0]);
+      free = t;
+      t = t == lds + 2 * C::kSlot ? lds : t + C::kSlot;
+    }
   }
   if (wave < 4) barrier();
   wait_vmcnt<0>();  // no load may still be on its way to LDS when the block ends
@@ -445,7 +501,7 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
   // gradient reads) whole rows; chunks are exclusive-ored with the row for the banks
   floatx4* const cs = reinterpret_cast<floatx4*>(smem);
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < C::kHalves; ++i) {
     __syncthreads();
 #pragma unroll
     for (int p = 0; p < 4; ++p)
@@ -461,28 +517,51 @@ __global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
       const int r = r0 + (kPair ? wave * 2 + (lane >> 5) : wave), c = kPair ? lane & 31 : lane;
       const floatx4 c0 = cs[r * 64 + (c ^ (r & 15))];
       const floatx4 c1 = kPair ? cs[r * 64 + ((c + 32) ^ (r & 15))] : c0;
-      finish<S, C::EPI>(a, z, (int64_t)m0 + i * 128 + r, n0 + c * 4, c0, c1);
+      finish<C>(a, piece, z, m0, n0, i * 128 + r, c * 4, c0, c1);
     }
   }
 }
 
-// Adds the splits' partial sums in order and runs the epilogue; a thread has
-// four columns.
-template <typename S, int EPI>
+template <typename C>
+__global__ __launch_bounds__(512, 2) void gemm_wide_kernel(GemmArgs a) {
+  __shared__ __attribute__((aligned(1024))) char smem[C::kSlots * C::kSlot];
+  const int nk = (a.K + kStep<typename C::S> - 1) / kStep<typename C::S>;
+  Piece piece;
+  for (int i = 0; piece_of(a, nk * a.segments, i, &piece); ++i) {
+    if (i) __syncthreads();  // every wave is through with the last piece's LDS
+    gemm_wide_piece<C>(a, piece, nk, smem);
+  }
+}
+
+// Adds the pieces of the tiles that several blocks have parts of, in order of
+// k, and runs the epilogue; a thread has four columns of a row.
+template <typename C>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
-  constexpr int kParts = EPI == kEpiGated ? 2 : 1;
-  const int z = blockIdx.z;
-  const int64_t per_row = a.ldp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= per_row * a.M) return;
-  const int64_t m = i / per_row;
-  const int n = (int)(i % per_row) * 4;
-  floatx4 c[2] = {};
-  const int64_t plane = (int64_t)a.M * a.ldp;
-  const float* p = a.part + (int64_t)z * kParts * plane + m * a.ldp + n;
-  for (int s = 0; s < a.splits; ++s)
-#pragma unroll
-    for (int k = 0; k < kParts; ++k) c[k] += *reinterpret_cast<const floatx4*>(p + ((int64_t)s * a.batch * kParts + k) * plane);
-  epilogue<S, EPI>(a, z, m, n, c[0], c[1]);
+  const int steps = (a.K + kStep<typename C::S> - 1) / kStep<typename C::S> * a.segments;
+  constexpr int kRowThreads = C::kCols / 4, kBlocks = C::BM * kRowThreads / 256;  // a tile's
+  static_assert(C::BM * kRowThreads % 256 == 0, "whole blocks");
+  const int t = blockIdx.x / kBlocks, i = blockIdx.x % kBlocks * 256 + threadIdx.x;
+  const int r = i / kRowThreads, c = i % kRowThreads * 4;
+  int mt, nt, z;
+  tile_of(a.whole_tiles + t, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt, &z);
+  const int64_t m = (int64_t)mt * C::BM + r;
+  if (m >= a.M) return;
+  // the run that holds the tile's first step
+  const int64_t first = (int64_t)t * steps, last = first + steps;
+  int64_t b = first * a.run_blocks / ((int64_t)a.run_tiles * steps);
+  while (b > 0 && run_start(b, a.run_tiles, steps, a.run_blocks) > first) --b;
+  while (run_start(b + 1, a.run_tiles, steps, a.run_blocks) <= first) ++b;
+  if (run_start(b, a.run_tiles, steps, a.run_blocks) <= first && run_start(b + 1, a.run_tiles, steps, a.run_blocks) >= last)
+    return;  // one block has the whole tile, and has finished it
+  floatx4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+  for (; b < a.run_blocks; ++b) {
+    const int64_t lo = run_start(b, a.run_tiles, steps, a.run_blocks);
+    if (lo >= last) break;
+    const float* q = a.part + ((2 * b + (lo < first ? 1 : 0)) * C::BM + r) * C::BN + c;
+    c0 += *reinterpret_cast<const floatx4*>(q);
+    if constexpr (C::EPI == kEpiGated) c1 += *reinterpret_cast<const floatx4*>(q + C::kCols);
+  }
+  epilogue<typename C::S, C::EPI>(a, z, m, nt * C::kCols + c, c0, c1);
 }
 
 }  // namespace mhc

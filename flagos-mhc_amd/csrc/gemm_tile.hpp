@@ -176,6 +176,15 @@ struct TileRegs {
   template <typename F, typename G>
   __device__ __forceinline__ void load_two(const S* corner, const S* other, int64_t ld, int rows, int left, int wave,
                                            int lane, F row_of, G second) {
+    if (rows >= R && left >= kStep<S>) {  // a whole tile: nothing to check
+#pragma unroll
+      for (int i = 0; i < T::kLoads; ++i) {
+        const int u = T::unit(i, wave), l = T::line(u, lane);
+        const S* p = (second(l) ? other : corner) + (int64_t)(L == kRow ? row_of(l) : l) * ld + T::chunk(u, lane) * kVec<S>;
+        v[i] = *reinterpret_cast<const u32x4_a2*>(p);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < T::kLoads; ++i) {
       const int u = T::unit(i, wave), l = T::line(u, lane), c = T::chunk(u, lane);
