@@ -48,6 +48,7 @@ constexpr KernelCost kCosts[kKinds] = {
     {128, 128, 2, {0.46, 0.8}, {2.3, 3.2}, {0.8, 1.28}, {2.5, 3.5}},
     {128, 256, 1, {0.78, 0.78}, {4.4, 4.4}, {}, {}},
     {256, 256, 1, {1.25, 1.25}, {8.5, 8.5}, {}, {}}};
+constexpr int kFewRows = 4;
 constexpr double kJoinUs = 5., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
 
 struct GemmPlan {
@@ -118,7 +119,9 @@ struct GemmPlans {
   int64_t main_rows;  // M: no tail
 };
 GemmPlans plan_gemm(const GemmShape& s, size_t es) {
-  GemmPlans p = {plan_rows(s, es), {}, s.M};
+  GemmPlans p = {};
+  if (s.la == kRow && s.lb == kRow && s.M <= kFewRows) return p;  // a kernel of its own
+  p = {plan_rows(s, es), {}, s.M};
   const int64_t over = s.M % 256;
   if (s.la == kRow && s.M > 256 && over > 0 && over <= 64) {
     GemmShape m = s, t = s;
@@ -187,8 +190,24 @@ int launch_plan(GemmArgs a, const GemmPlan& p, float* part, hipStream_t st) {
                : launch_tile<TileCfg<S, LA, LB, 128, 128, 2, 2, 2, EPI, false>>(a, st);
 }
 
+template <typename S, int EPI>
+int launch_few_rows(const GemmArgs& a, hipStream_t st) {
+  constexpr int kCols = EPI == kEpiGated ? 2 : 4;
+  const dim3 g((unsigned)((a.ldo + kCols - 1) / kCols)), b(256);
+  if (const int rc = check_grid(g, b, "gated_ffn")) return rc;
+  if (a.M == 1)
+    hipLaunchKernelGGL((few_rows_kernel<S, 1, EPI>), g, b, 0, st, a);
+  else if (a.M == 2)
+    hipLaunchKernelGGL((few_rows_kernel<S, 2, EPI>), g, b, 0, st, a);
+  else
+    hipLaunchKernelGGL((few_rows_kernel<S, 4, EPI>), g, b, 0, st, a);
+  return check_launch("gated_ffn");
+}
+
 template <typename S, int LA, int LB, int EPI>
 int launch_gemm(GemmArgs a, const GemmShape& s, float* part, hipStream_t st) {
+  if constexpr (LA == kRow && LB == kRow)
+    if (s.M <= kFewRows) return launch_few_rows<S, EPI>(a, st);
   const GemmPlans p = plan_gemm(s, sizeof(S));
   a.M = (int)p.main_rows;
   if (const int rc = launch_plan<S, LA, LB, EPI>(a, p.main, part, st)) return rc;

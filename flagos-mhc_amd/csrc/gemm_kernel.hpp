@@ -553,15 +553,138 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
   while (run_start(b + 1, a.run_tiles, steps, a.run_blocks) <= first) ++b;
   if (run_start(b, a.run_tiles, steps, a.run_blocks) <= first && run_start(b + 1, a.run_tiles, steps, a.run_blocks) >= last)
     return;  // one block has the whole tile, and has finished it
-  floatx4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
-  for (; b < a.run_blocks; ++b) {
-    const int64_t lo = run_start(b, a.run_tiles, steps, a.run_blocks);
-    if (lo >= last) break;
-    const float* q = a.part + ((2 * b + (lo < first ? 1 : 0)) * C::BM + r) * C::BN + c;
-    c0 += *reinterpret_cast<const floatx4*>(q);
-    if constexpr (C::EPI == kEpiGated) c1 += *reinterpret_cast<const floatx4*>(q + C::kCols);
-  }
+  // runs b .. e - 1; only the first may have started in the tile before
+  int64_t e = last * a.run_blocks / ((int64_t)a.run_tiles * steps);
+  while (e < a.run_blocks && run_start(e, a.run_tiles, steps, a.run_blocks) < last) ++e;
+  while (run_start(e - 1, a.run_tiles, steps, a.run_blocks) >= last) --e;
+  const int64_t stride = 2 * (int64_t)C::BM * C::BN;
+  const float* q = a.part + b * stride + (int64_t)r * C::BN + c;
+  if (run_start(b, a.run_tiles, steps, a.run_blocks) < first) q += stride / 2;
+  floatx4 c0 = *reinterpret_cast<const floatx4*>(q), c1 = c0;
+  if constexpr (C::EPI == kEpiGated) c1 = *reinterpret_cast<const floatx4*>(q + C::kCols);
+  q = a.part + (b + 1) * stride + (int64_t)r * C::BN + c;
+  const auto add = [&](int n) {  // n runs, their loads first
+    floatx4 u[8], v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) {
+        u[k] = *reinterpret_cast<const floatx4*>(q + k * stride);
+        if constexpr (C::EPI == kEpiGated) v[k] = *reinterpret_cast<const floatx4*>(q + k * stride + C::kCols);
+      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < n) {
+        c0 += u[k];
+        if constexpr (C::EPI == kEpiGated) c1 += v[k];
+      }
+    q += n * stride;
+  };
+  int64_t left = e - b - 1;
+  for (; left >= 8; left -= 8) add(8);
+  if (left > 0) add((int)left);
   epilogue<typename C::S, C::EPI>(a, z, m, nt * C::kCols + c, c0, c1);
+}
+
+// ---- few rows -------------------------------------------------------------------------
+// The forward's products for up to four rows of A (kRow operands): bound by
+// the reading of B's rows, once.  A block has the four rows B(n) .. B(n + 3)
+// (the gated form: two of each operand) and its four waves every fourth KB of
+// them, 1 KB a load; fp32 products and sums, the lanes' sums are added at the
+// end.  No LDS on the way, so that a CU holds up to 32 waves, each with eight
+// loads under way.
+template <typename S, int ROWS, int EPI>
+__global__ __launch_bounds__(256) void few_rows_kernel(GemmArgs a) {
+  constexpr int V = kVec<S>, kB = 4, kChunk = kWave * V;
+  constexpr int kCols = EPI == kEpiGated ? 2 : 4;  // columns of C
+  __shared__ float red[4][kB * ROWS];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * kCols;
+  const S* A = static_cast<const S*>(a.A[0]);
+  const S* row[kB];  // rows past the last one repeat it
+#pragma unroll
+  for (int j = 0; j < kB; ++j) {
+    const int64_t n = n0 + (EPI == kEpiGated ? j & 1 : j);
+    row[j] = static_cast<const S*>(EPI == kEpiGated && j >= 2 ? a.B[1] : a.B[0]) + (n < a.N ? n : a.N - 1) * a.ldb;
+  }
+  float acc[kB][ROWS] = {};
+  const auto dot = [&](const u32x4 (&w)[kB], const u32x4 (&x)[ROWS]) {
+    float fx[ROWS][V];
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) Store<S>::unpack(x[t], fx[t]);
+#pragma unroll
+    for (int j = 0; j < kB; ++j) {
+      float fw[V];
+      Store<S>::unpack(w[j], fw);
+#pragma unroll
+      for (int t = 0; t < ROWS; ++t)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[j][t] = fmaf(fw[i], fx[t][i], acc[j][t]);
+    }
+  };
+  const auto fetch = [&](int64_t k, u32x4 (&w)[kB], u32x4 (&x)[ROWS]) {
+#pragma unroll
+    for (int j = 0; j < kB; ++j) w[j] = ld16nt_u(row[j] + k);
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) x[t] = *reinterpret_cast<const u32x4_a2*>(A + (t < a.M ? t : 0) * a.lda + k);
+  };
+  const int64_t whole = a.K / kChunk;
+  int64_t c = wave;
+  for (; c + 4 < whole; c += 8) {
+    u32x4 w0[kB], w1[kB], x0[ROWS], x1[ROWS];
+    fetch(c * kChunk + lane * V, w0, x0);
+    fetch((c + 4) * kChunk + lane * V, w1, x1);
+    dot(w0, x0);
+    dot(w1, x1);
+  }
+  for (; c < whole; c += 4) {
+    u32x4 w0[kB], x0[ROWS];
+    fetch(c * kChunk + lane * V, w0, x0);
+    dot(w0, x0);
+  }
+  if (c == whole && whole * kChunk < a.K) {  // the last, shorter KB: one wave's, its lanes' chunks whole, cut or empty
+    const int64_t k = whole * kChunk + lane * V, have = a.K - k;
+    u32x4 w0[kB] = {}, x0[ROWS] = {};
+    if (have >= V) {
+      fetch(k, w0, x0);
+    } else if (have > 0) {
+#pragma unroll
+      for (int j = 0; j < kB; ++j) w0[j] = ld16_elems<S>(row[j] + k, (int)have);
+#pragma unroll
+      for (int t = 0; t < ROWS; ++t) x0[t] = ld16_elems<S>(A + (t < a.M ? t : 0) * a.lda + k, (int)have);
+    }
+    dot(w0, x0);
+  }
+#pragma unroll
+  for (int j = 0; j < kB; ++j)
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+      const float s = group_sum<63>(acc[j][t]);
+      if (lane == 0) red[wave][j * ROWS + t] = s;
+    }
+  __syncthreads();
+  // thread t: row t
+  const int t = threadIdx.x;
+  if (t >= ROWS || t >= a.M) return;
+  float s[kB];
+#pragma unroll
+  for (int j = 0; j < kB; ++j) s[j] = red[0][j * ROWS + t] + red[1][j * ROWS + t] + red[2][j * ROWS + t] + red[3][j * ROWS + t];
+  S* out = static_cast<S*>(a.out0) + t * a.ldo;
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    const int64_t n = n0 + j;
+    if (n >= a.ldo) continue;
+    if constexpr (EPI == kEpiGated) {
+      float v = 0.f, d;
+      if (n < a.N) {
+        act_both(a.act, s[j], &v, &d);
+        v *= s[j + 2];
+        if (a.gate) a.gate[t * (int64_t)a.N + n] = s[j], a.up[t * (int64_t)a.N + n] = s[j + 2];
+      }
+      store_elem<S>(out, n, v);
+    } else {
+      store_elem<S>(out, n, s[j]);
+    }
+  }
 }
 
 }  // namespace mhc
