@@ -42,12 +42,14 @@ struct KernelCost {
   StepCost dma16, dma32, reg16, reg32;
 };
 constexpr KernelCost kCosts[kKinds] = {
-    {16, 128, 2, {0.85, 0.7}, {0.85, 0.7}, {1.0, 1.2}, {1.0, 1.2}},
-    {64, 128, 2, {1.1, 0.9}, {1.6, 1.8}, {1.1, 1.2}, {1.8, 2.0}},
+    {16, 128, 1, {0.8, 0.8}, {0.8, 0.8}, {1.2, 1.2}, {1.2, 1.2}},
+    {64, 128, 1, {0.9, 0.9}, {1.8, 1.8}, {1.2, 1.2}, {2.0, 2.0}},
     {64, 64, 4, {0.23, 0.6}, {0.6, 0.8}, {0.4, 0.76}, {0.65, 1.0}},
-    {128, 128, 2, {0.46, 0.8}, {2.3, 3.2}, {0.8, 1.28}, {2.5, 3.5}},
-    {128, 256, 1, {0.78, 0.78}, {4.4, 4.4}, {}, {}},
-    {256, 256, 1, {1.25, 1.25}, {8.5, 8.5}, {}, {}}};
+    {128, 128, 2, {0.49, 0.8}, {2.3, 3.2}, {0.8, 1.28}, {2.5, 3.5}},
+    {128, 256, 1, {0.87, 0.75}, {4.4, 4.4}, {}, {}},
+    {256, 256, 1, {1.46, 1.25}, {8.5, 8.5}, {}, {}}};
+// both operands kCol: twice the LDS reads, which the large tiles feel
+constexpr double kColCol = 1.13;
 constexpr int kFewRows = 4;
 constexpr double kJoinUs = 5., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
 
@@ -71,10 +73,13 @@ GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma) {
   const StepCost& cost = dma ? (es == 4 ? c.dma32 : c.dma16) : (es == 4 ? c.reg32 : c.reg16);
   const int64_t cus = device_cu_count(), slots = cus * c.per_cu;
   const int64_t tiles = tiles_of(s, c.bm, c.bn), steps = (s.K * (int64_t)es + 127) / 128 * s.segments;
-  // `steps` steps of `blocks` blocks side by side
+  // n steps of `blocks` blocks side by side: on a part of the CUs each runs
+  // faster, as the card's power then allows a higher clock
   const auto side_by_side = [&](double blocks, double n) {
-    const double full = std::ceil(blocks / cus) * cost.full;
-    return n * (full > cost.alone ? full : cost.alone);
+    const double part = blocks < cus ? blocks / cus : 1.;
+    const double few = c.per_cu > 1 ? cost.alone : cost.alone + (cost.full - cost.alone) * part;
+    const double full = blocks < cus ? 0. : std::ceil(blocks / cus) * cost.full;
+    return n * (full > few ? full : few) * (s.la == kCol && kind >= kWide128 ? kColCol : 1.);
   };
   const int64_t rest = tiles % slots, rounds = tiles / slots;
   const double rounds_us = kLaunchUs + rounds * side_by_side((double)slots, (double)steps);
@@ -177,11 +182,11 @@ int launch_plan(GemmArgs a, const GemmPlan& p, float* part, hipStream_t st) {
   if (p.kind == kWide128) return launch_wide<WideCfg<S, LA, LB, 128, EPI>>(a, st);
   if constexpr (LA == kRow) {
     if (p.kind == kTile64x128)
-      return p.dma ? launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 3, 2, EPI, true>>(a, st)
-                   : launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 2, 2, EPI, false>>(a, st);
+      return p.dma ? launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 6, 1, EPI, true>>(a, st)
+                   : launch_tile<TileCfg<S, LA, LB, 64, 128, 1, 2, 1, EPI, false>>(a, st);
     if (p.kind == kTile16)
-      return p.dma ? launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 4, 2, EPI, true>>(a, st)
-                   : launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 2, 2, EPI, false>>(a, st);
+      return p.dma ? launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 8, 1, EPI, true>>(a, st)
+                   : launch_tile<TileCfg<S, LA, LB, 16, 128, 1, 2, 1, EPI, false>>(a, st);
   }
   if (p.kind == kTile64)
     return p.dma ? launch_tile<TileCfg<S, LA, LB, 64, 64, 2, 2, 4, EPI, true>>(a, st)

@@ -34,25 +34,55 @@ struct GemmArgs {
   float* part;
 };
 
+// 1 / (1 + exp(-z)).  16-bit results: by the hardware's exp2 and reciprocal,
+// whose errors (1 ulp each, and |z| half ulps of the exponent's rounding, where
+// the result is not yet 1) stay below 2^-17 while exp(-z) is finite; the
+// accurate functions cost four times the instructions, a tenth of a large
+// product with this epilogue.
+template <bool FAST>
+__device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+  return 1.f / (1.f + expf(-z));
+}
+
 // act(g) and act'(g) in fp32.
-__device__ __forceinline__ void act_both(int kind, float g, float* a, float* d) {
-  if (kind == kActSilu) {
-    const float s = 1.f / (1.f + expf(-g));
+template <int KIND, bool FAST>
+__device__ __forceinline__ void act_both(float g, float* a, float* d) {
+  if constexpr (KIND == kActSilu) {
+    const float s = sigmoid<FAST>(g);
     *a = g * s;
     *d = s * (1.f + g * (1.f - s));
-  } else if (kind == kActGelu) {
+  } else if constexpr (KIND == kActGelu) {
     const float p = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     *a = g * p;
     *d = p + g * 0.39894228040143268f * expf(-0.5f * g * g);
-  } else if (kind == kActGeluTanh) {
+  } else if constexpr (KIND == kActGeluTanh) {
     // 0.5 (1 + tanh v) = 1 / (1 + exp(-2 v))
     const float v = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-    const float s = 1.f / (1.f + expf(-2.f * v));
+    const float s = sigmoid<FAST>(2.f * v);
     *a = g * s;
     *d = s + g * 2.f * s * (1.f - s) * 0.79788456080286536f * (1.f + 0.134145f * fminf(g * g, 1e30f));
   } else {
     *a = g > 0.f ? g : (g != g ? g : 0.f);
     *d = g > 0.f ? 1.f : 0.f;
+  }
+}
+// The same for N gates and a kind known at run time; S: the results' type.
+template <typename S, int N>
+__device__ __forceinline__ void act_all(int kind, const float* g, float* a, float* d) {
+  constexpr bool kFast = sizeof(S) == 2;
+  if (kind == kActSilu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) act_both<kActSilu, kFast>(g[i], a + i, d + i);
+  } else if (kind == kActGelu) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) act_both<kActGelu, kFast>(g[i], a + i, d + i);
+  } else if (kind == kActGeluTanh) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) act_both<kActGeluTanh, kFast>(g[i], a + i, d + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) act_both<kActRelu, kFast>(g[i], a + i, d + i);
   }
 }
 
@@ -61,11 +91,16 @@ __device__ __forceinline__ void act_both(int kind, float g, float* a, float* d) 
 typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
 typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
 
-// Four consecutive elements of a row of `len`, the first at n.
-template <typename S>
+// Four consecutive elements of a row of `len`, the first at n.  STREAM: not
+// kept in the caches (gate and up are larger than they are and next read by
+// the backward: 1 to 3% of a forward and backward pass).
+template <typename S, bool STREAM = false>
 __device__ __forceinline__ void store4(S* row, int64_t n, int64_t len, const floatx4& c) {
   if (n + 4 <= len) {
-    if constexpr (sizeof(S) == 4) {
+    if constexpr (STREAM) {
+      static_assert(sizeof(S) == 4, "gate and up");
+      __builtin_nontemporal_store(c, reinterpret_cast<floatx4_a4*>(row + n));
+    } else if constexpr (sizeof(S) == 4) {
       *reinterpret_cast<floatx4_a4*>(row + n) = c;
     } else {
       const u32x2 v = {(uint32_t)Store<S>::from_f32(c[0]) | (uint32_t)Store<S>::from_f32(c[1]) << 16,
@@ -79,7 +114,7 @@ __device__ __forceinline__ void store4(S* row, int64_t n, int64_t len, const flo
   }
 }
 __device__ __forceinline__ floatx4 load4(const float* row, int64_t n, int64_t len) {
-  if (n + 4 <= len) return *reinterpret_cast<const floatx4_a4*>(row + n);
+  if (n + 4 <= len) return __builtin_nontemporal_load(reinterpret_cast<const floatx4_a4*>(row + n));
   floatx4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -96,27 +131,24 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, int64_t m, in
   if constexpr (EPI == kEpiStore) {
     store4<S>(o0, n, a.ldo, c0);
   } else if constexpr (EPI == kEpiGated) {
-    floatx4 h;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float v, d;
-      act_both(a.act, c0[i], &v, &d);
-      h[i] = v * c1[i];
-    }
-    store4<S>(o0, n, a.ldo, h);
+    const float g[4] = {c0[0], c0[1], c0[2], c0[3]};
+    float v[4], d[4];
+    act_all<S, 4>(a.act, g, v, d);
+    store4<S>(o0, n, a.ldo, floatx4{v[0] * c1[0], v[1] * c1[1], v[2] * c1[2], v[3] * c1[3]});
     if (a.gate) {
-      store4<float>(a.gate + m * a.N, n, a.N, c0);
-      store4<float>(a.up + m * a.N, n, a.N, c1);
+      store4<float, true>(a.gate + m * a.N, n, a.N, c0);
+      store4<float, true>(a.up + m * a.N, n, a.N, c1);
     }
   } else {
     const floatx4 g = load4(a.gate + m * a.N, n, a.N), u = load4(a.up + m * a.N, n, a.N);
+    const float ga[4] = {g[0], g[1], g[2], g[3]};
+    float v[4], d[4];
+    act_all<S, 4>(a.act, ga, v, d);
     floatx4 dg, du;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float v, d;
-      act_both(a.act, g[i], &v, &d);
-      dg[i] = c0[i] * u[i] * d;
-      du[i] = c0[i] * v;
+      dg[i] = c0[i] * u[i] * d[i];
+      du[i] = c0[i] * v[i];
     }
     store4<S>(o0, n, a.ldo, dg);
     store4<S>(static_cast<S*>(a.out1) + m * a.ldo, n, a.ldo, du);
@@ -676,7 +708,7 @@ __global__ __launch_bounds__(256) void few_rows_kernel(GemmArgs a) {
     if constexpr (EPI == kEpiGated) {
       float v = 0.f, d;
       if (n < a.N) {
-        act_both(a.act, s[j], &v, &d);
+        act_all<S, 1>(a.act, &s[j], &v, &d);
         v *= s[j + 2];
         if (a.gate) a.gate[t * (int64_t)a.N + n] = s[j], a.up[t * (int64_t)a.N + n] = s[j + 2];
       }
