@@ -86,9 +86,11 @@ def gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=False):
     return result
 
 
-def gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation="silu"):
+def gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation="silu",
+                       need_weights=True):
     """(grad_x, grad_w_gate, grad_w_up, grad_w_down) in the dtype of x, from the
-    forward's gate, up and hidden.  Deterministic."""
+    forward's gate, up and hidden; the last three are None with
+    ``need_weights=False``.  Deterministic."""
     what = "gated_ffn_backward"
     _lib.require_device(what, grad_out, x, w_gate, w_up, w_down, gate, up, hidden)
     T, D, F, O, code, act = _check(what, x, w_gate, w_up, w_down, activation)
@@ -102,8 +104,10 @@ def gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, acti
     dev = x.device
     gx = torch.empty(x.shape, dtype=x.dtype, device=dev)
     alloc = torch.empty if T > 0 else torch.zeros
-    gwg, gwu = (alloc((F, D), dtype=x.dtype, device=dev) for _ in range(2))
-    gwd = alloc((O, F), dtype=x.dtype, device=dev)
+    gwg = gwu = gwd = None
+    if need_weights:
+        gwg, gwu = (alloc((F, D), dtype=x.dtype, device=dev) for _ in range(2))
+        gwd = alloc((O, F), dtype=x.dtype, device=dev)
     if T > 0:
         xf, go = _aligned(x, (T, D), x.dtype), _aligned(grad_out, (T, O), x.dtype)
         wg, wu = _aligned(w_gate, (F, D), x.dtype), _aligned(w_up, (F, D), x.dtype)
@@ -115,7 +119,7 @@ def gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, acti
         with _lib.on_device(dev):
             rc = lib.mhc_gated_ffn_bwd(go.data_ptr(), xf.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
                                        g.data_ptr(), u.data_ptr(), h.data_ptr(), code, act, gx.data_ptr(),
-                                       gwg.data_ptr(), gwu.data_ptr(), gwd.data_ptr(), ws.data_ptr(), ws_bytes,
+                                       _lib.ptr(gwg), _lib.ptr(gwu), _lib.ptr(gwd), ws.data_ptr(), ws_bytes,
                                        T, D, F, O, _lib.stream_of(xf))
         _lib.check(rc, what)
     return gx, gwg, gwu, gwd
@@ -147,7 +151,8 @@ class GatedFfnFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_out):
-        return (*gated_ffn_backward(grad_out, *ctx.saved_tensors, activation=ctx.activation), None)
+        return (*gated_ffn_backward(grad_out, *ctx.saved_tensors, activation=ctx.activation,
+                                    need_weights=any(ctx.needs_input_grad[1:4])), None)
 
 
 def gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu"):

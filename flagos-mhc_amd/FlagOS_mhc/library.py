@@ -24,12 +24,26 @@ HIP-graph capture records their kernels on the current stream):
         phi, alpha, base, norm_eps, hc_eps, clamp_min, clamp_max, iter_times)
         -> (x_next, y, post_out, comb_frag, inv_rms, mixes, pre)
 
+and the operators between pre and post (``FlagOS_mhc.sublayer``):
+
+    torch.ops.flagos_mhc.layer_norm(x, weight, bias, eps) -> (y, mean, rstd)
+    torch.ops.flagos_mhc.layer_norm_backward(grad_y, x, weight, mean, rstd)
+        -> (grad_x, grad_weight, grad_bias)
+    torch.ops.flagos_mhc.gated_ffn(x, w_gate, w_up, w_down, activation, save)
+        -> (out, gate, up, hidden); the last three are empty with save=False
+    torch.ops.flagos_mhc.gated_ffn_backward(grad_out, x, w_gate, w_up, w_down,
+        gate, up, hidden, activation) -> (grad_x, grad_w_gate, grad_w_up, grad_w_down)
+    torch.ops.flagos_mhc.dropout(x, p, seed, offset, state) -> y, with seed and
+        offset as signed 64-bit integers; its backward is the op on the gradient
+
 The forward pre op also returns the fp32 inv_rms, mixes and pre its backward
 needs; they are marked non-differentiable (likewise for the fused op).
 ``mhc_post_op``, ``mhc_pre_clamp_sinkhorn_op`` and
 ``mhc_post_pre_clamp_sinkhorn_op`` are the autograd-aware entry points with
 the return conventions of ``mhc_post_fn`` / ``mhc_pre_clamp_sinkhorn_fn``
-(src/autograd.py:14-87) and ``mhc_post_pre_clamp_sinkhorn_fn``.  The kernels allocate nothing outside torch's
+(src/autograd.py:14-87) and ``mhc_post_pre_clamp_sinkhorn_fn``;
+``layer_norm_op``, ``gated_ffn_op``, ``dropout_op`` and ``mhc_ffn_layer_op``
+those of the same functions of ``FlagOS_mhc.sublayer``.  The kernels allocate nothing outside torch's
 allocator and call no host synchronisation, so they can be captured in a
 HIP graph (``torch.cuda.graph``) after one eager warm-up call.
 """
@@ -37,11 +51,14 @@ HIP graph (``torch.cuda.graph``) after one eager warm-up call.
 from __future__ import annotations
 
 import math
-from typing import Tuple
+from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
 
+from .dropout import dropout
+from .gated_ffn import gated_ffn, gated_ffn_backward, hidden_width
+from .layer_norm import layer_norm, layer_norm_backward
 from .mhc_post import mhc_post
 from .mhc_post_backward import mhc_post_backward, mhc_post_backward_sum, post_backward_sum_fused
 from .mhc_post_pre import mhc_post_pre_clamp_sinkhorn
@@ -243,6 +260,128 @@ def _post_pre_grad(ctx, grad_x_next, grad_y, grad_post_out, grad_comb_frag, _g_i
 _post_pre.register_autograd(_post_pre_grad, setup_context=_post_pre_setup)
 
 
+# ---- layer norm -----------------------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::layer_norm", mutates_args=())
+def _norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor],
+          eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    out = layer_norm(x, weight, bias, eps, need_backward=True)
+    return out["y"], out["mean"], out["rstd"]
+
+
+@_norm.register_fake
+def _norm_fake(x, weight, bias, eps):
+    rows = math.prod(x.shape[:-1])
+    return (x.new_empty(x.shape), x.new_empty((rows,), dtype=torch.float32),
+            x.new_empty((rows,), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::layer_norm_backward", mutates_args=())
+def _norm_bwd(grad_y: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor,
+              rstd: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    return layer_norm_backward(grad_y, x, weight, mean, rstd)
+
+
+@_norm_bwd.register_fake
+def _norm_bwd_fake(grad_y, x, weight, mean, rstd):
+    D = x.shape[-1]
+    return (x.new_empty(x.shape), x.new_empty((D,), dtype=torch.float32),
+            x.new_empty((D,), dtype=torch.float32))
+
+
+def _norm_setup(ctx, inputs, output):
+    x, weight, bias, _ = inputs
+    _, mean, rstd = output
+    ctx.mark_non_differentiable(mean, rstd)
+    ctx.save_for_backward(x, weight, mean, rstd)
+    ctx.params = tuple(None if p is None else (p.shape, p.dtype) for p in (weight, bias))
+
+
+def _norm_grad(ctx, grad_y, _g_mean, _g_rstd):
+    x, weight, mean, rstd = ctx.saved_tensors
+    gx, *gp = torch.ops.flagos_mhc.layer_norm_backward(grad_y.contiguous(), x, weight, mean, rstd)
+    gw, gb = (None if d is None else g.reshape(d[0]).to(d[1]) for g, d in zip(gp, ctx.params))
+    return gx, gw, gb, None
+
+
+_norm.register_autograd(_norm_grad, setup_context=_norm_setup)
+
+
+# ---- gated feed-forward block ------------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::gated_ffn", mutates_args=())
+def _ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, activation: str = "silu",
+         save: bool = True) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    f = gated_ffn(x, w_gate, w_up, w_down, activation, need_backward=save)
+    if save:
+        return f["out"], f["gate"], f["up"], f["hidden"]
+    return (f["out"], *(x.new_empty((0,), dtype=d) for d in (torch.float32, torch.float32, x.dtype)))
+
+
+@_ffn.register_fake
+def _ffn_fake(x, w_gate, w_up, w_down, activation="silu", save=True):
+    T, F = math.prod(x.shape[:-1]), w_gate.shape[0]
+    shapes = ((T, F), (T, F), (T, hidden_width(F))) if save else ((0,),) * 3
+    return (x.new_empty(tuple(x.shape[:-1]) + (w_down.shape[0],)),
+            *(x.new_empty(s, dtype=d) for s, d in zip(shapes, (torch.float32, torch.float32, x.dtype))))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::gated_ffn_backward", mutates_args=())
+def _ffn_bwd(grad_out: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, gate: Tensor,
+             up: Tensor, hidden: Tensor, activation: str = "silu") -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    return gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation)
+
+
+@_ffn_bwd.register_fake
+def _ffn_bwd_fake(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation="silu"):
+    return tuple(t.new_empty(t.shape) for t in (x, w_gate, w_up, w_down))
+
+
+def _ffn_setup(ctx, inputs, output):
+    x, w_gate, w_up, w_down, *opt = inputs
+    _, gate, up, hidden = output
+    ctx.mark_non_differentiable(gate, up, hidden)
+    ctx.save_for_backward(x, w_gate, w_up, w_down, gate, up, hidden)
+    ctx.activation = opt[0] if opt else "silu"
+    ctx.saved = opt[1] if len(opt) > 1 else True
+
+
+def _ffn_grad(ctx, grad_out, _g_gate, _g_up, _g_hidden):
+    if not ctx.saved:
+        raise RuntimeError("gated_ffn: the forward ran with save=False")
+    return (*torch.ops.flagos_mhc.gated_ffn_backward(grad_out.contiguous(), *ctx.saved_tensors, ctx.activation),
+            None, None)
+
+
+_ffn.register_autograd(_ffn_grad, setup_context=_ffn_setup)
+
+
+# ---- dropout ---------------------------------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::dropout", mutates_args=())
+def _drop(x: Tensor, p: float, seed: int, offset: int, state: Optional[Tensor] = None) -> Tensor:
+    return dropout(x, p, seed, offset, state)
+
+
+@_drop.register_fake
+def _drop_fake(x, p, seed, offset, state=None):
+    return x.new_empty(x.shape)
+
+
+def _drop_setup(ctx, inputs, output):
+    x, p, seed, offset, *state = inputs
+    ctx.args = (p, seed, offset)
+    # as it was at the forward: a program moves its own on before the backward
+    ctx.state = state[0].clone() if state and state[0] is not None else None
+
+
+def _drop_grad(ctx, grad_y):
+    return torch.ops.flagos_mhc.dropout(grad_y.contiguous(), *ctx.args, ctx.state), None, None, None, None
+
+
+_drop.register_autograd(_drop_grad, setup_context=_drop_setup)
+
+
 # ---- autograd-aware entry points ---------------------------------------------
 
 def mhc_post_op(x, h_res, h_out, h_post):
@@ -270,3 +409,33 @@ def mhc_post_pre_clamp_sinkhorn_op(x, h_res, h_out, h_post, phi, alpha, base, no
         x, h_res, h_out, h_post, phi, alpha, base, float(norm_eps), float(hc_eps), float(clamp_min),
         float(clamp_max), int(iter_times), bool(compensated))
     return x_next, y, post_out, comb
+
+
+def layer_norm_op(x, weight=None, bias=None, eps=1e-5):
+    """``layer_norm_fn`` through the registered op."""
+    return torch.ops.flagos_mhc.layer_norm(x, weight, bias, float(eps))[0]
+
+
+def gated_ffn_op(x, w_gate, w_up, w_down, activation="silu"):
+    """``gated_ffn_fn`` through the registered op."""
+    save = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down))
+    return torch.ops.flagos_mhc.gated_ffn(x, w_gate, w_up, w_down, activation, save)[0]
+
+
+def _signed64(v):
+    return (int(v) + (1 << 63)) % (1 << 64) - (1 << 63)
+
+
+def dropout_op(x, p, seed=0, offset=0, state=None):
+    """``dropout_fn`` through the registered op."""
+    return torch.ops.flagos_mhc.dropout(x, float(p), _signed64(seed), _signed64(offset), state)
+
+
+def mhc_ffn_layer_op(x, phi, alpha, base, norm_weight, norm_bias, w_gate, w_up, w_down, *, activation="silu",
+                     dropout_p=0.0, seed=0, offset=0, state=None, ln_eps=1e-5, **mhc):
+    """``mhc_ffn_layer_fn`` (``FlagOS_mhc.sublayer``) through the registered ops."""
+    y, post, comb = mhc_pre_clamp_sinkhorn_op(x, phi, alpha, base, **mhc)
+    h = gated_ffn_op(layer_norm_op(y, norm_weight, norm_bias, ln_eps), w_gate, w_up, w_down, activation)
+    if dropout_p > 0.0:
+        h = dropout_op(h, dropout_p, seed, offset, state)
+    return mhc_post_op(x, comb, h, post)

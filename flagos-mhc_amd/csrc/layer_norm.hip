@@ -5,14 +5,14 @@
 //   dx = rstd (g - sum(g) / D - xhat sum(g xhat) / D),  dw = sum_t dy xhat,  db = sum_t dy
 //
 // Both passes are bound by HBM.  A row is read once into the registers of G
-// lanes (a wave, or a block of 256 or 1024 threads, by the row's length), so
+// lanes (a wave, or a block of 256 to 1024 threads, by the row's length), so
 // the variance is the sum of squares about the mean that was just formed and
 // never a difference of two sums.  The backward's blocks walk rows with a
 // fixed stride; a thread keeps the same columns in every row and adds their
 // dw and db in fp32 registers, each block writes its sums once, and a second
 // kernel adds the blocks' sums in a fixed order: no atomics, the same bits in
-// every run.  Rows longer than 4096 16-byte vectors are read from memory
-// again for each sum (they come from the L2).
+// every run.  Rows longer than 4096 16-byte vectors (the backward: 2048) are
+// read from memory again for each sum (they come from the L2).
 #include "common.hpp"
 #include "mhc_launch.hpp"
 
@@ -277,8 +277,32 @@ __global__ __launch_bounds__(kBlockThreads<G>) void norm_bwd_kernel(NormBwdArgs 
       }
   }
   if (!a.part) return;
+  if constexpr (G == 64) {
+    // the block's four waves add theirs up in order: a quarter of the sums to write and read back
+    __shared__ float sums[R - 1][2 * NV * VEC][64];
+    if (r > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          sums[r - 1][i * VEC + j][t] = dw[i][j];
+          sums[r - 1][(NV + i) * VEC + j][t] = db[i][j];
+        }
+    }
+    __syncthreads();
+    if (r > 0) return;
+#pragma unroll
+    for (int k = 0; k < R - 1; ++k)
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          dw[i][j] += sums[k][i * VEC + j][t];
+          db[i][j] += sums[k][(NV + i) * VEC + j][t];
+        }
+  }
   // a repeated element of the last vector is the owner's to write: both hold the same sum
-  float* part = a.part + (int64_t)(blockIdx.x * R + r) * 2 * D;
+  float* part = a.part + (int64_t)blockIdx.x * 2 * D;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if (e[i] >= 0) {
@@ -355,14 +379,16 @@ __global__ __launch_bounds__(1024) void norm_bwd_sums_kernel(const float* part, 
 struct NormPlan {
   int G, NV;
 };
-NormPlan norm_plan(int64_t D, int vec) {
+NormPlan norm_plan(int64_t D, int vec, bool backward) {
   const int64_t nv = (D + vec - 1) / vec;
-  if (D < vec || nv > 4096) return {0, 0};
+  // the backward holds twice the row and its columns' sums: 2048 vectors fill 512 threads' registers
+  if (D < vec || nv > (backward ? 2048 : 4096)) return {0, 0};
   if (nv <= 64) return {64, 1};
   if (nv <= 128) return {64, 2};
   if (nv <= 256) return {256, 1};
   if (nv <= 512) return {256, 2};
   if (nv <= 1024) return {256, 4};
+  if (backward) return {512, 4};
   if (nv <= 2048) return {1024, 2};
   return {1024, 4};
 }
@@ -377,13 +403,10 @@ int norm_bwd_blocks(int64_t T, const NormPlan& p) {
   const int64_t want = (T + rows - 1) / rows;
   return (int)(want < most ? want : most);
 }
-int64_t norm_bwd_parts(int64_t T, const NormPlan& p) {
-  return (int64_t)norm_bwd_blocks(T, p) * (p.G == 64 ? 4 : 1);
-}
 
 template <typename S, typename W>
 int launch_norm_fwd(const NormFwdArgs& a, hipStream_t st) {
-  const NormPlan p = norm_plan(a.D, Store<S>::VEC);
+  const NormPlan p = norm_plan(a.D, Store<S>::VEC, false);
   const int rows = p.G == 64 ? 4 : 1, threads = p.G == 64 ? 256 : (p.G ? p.G : 1024);
   const dim3 g((unsigned)((a.T + rows - 1) / rows)), b(threads);
   if (const int rc = check_grid(g, b, "layer_norm")) return rc;
@@ -403,7 +426,7 @@ int launch_norm_fwd(const NormFwdArgs& a, hipStream_t st) {
 
 template <typename S, typename W>
 int launch_norm_bwd(const NormBwdArgs& a, float* gw, float* gb, hipStream_t st) {
-  const NormPlan p = norm_plan(a.D, Store<S>::VEC);
+  const NormPlan p = norm_plan(a.D, Store<S>::VEC, true);
   const int blocks = norm_bwd_blocks(a.T, p), threads = p.G == 64 ? 256 : (p.G ? p.G : 1024);
   const dim3 g(blocks), b(threads);
 #define MHC_NORM(GG, NN) \
@@ -413,14 +436,13 @@ int launch_norm_bwd(const NormBwdArgs& a, float* gw, float* gb, hipStream_t st) 
   MHC_NORM(256, 1);
   MHC_NORM(256, 2);
   MHC_NORM(256, 4);
-  MHC_NORM(1024, 2);
-  MHC_NORM(1024, 4);
+  MHC_NORM(512, 4);
 #undef MHC_NORM
   if (p.G == 0) hipLaunchKernelGGL((norm_bwd_loop_kernel<S, W>), g, b, 0, st, a);
   if (const int rc = check_launch("layer_norm_backward")) return rc;
   if (a.part) {
     const dim3 sg((unsigned)((a.D + 63) / 64), 2);
-    hipLaunchKernelGGL(norm_bwd_sums_kernel, sg, dim3(1024), 0, st, a.part, (int)norm_bwd_parts(a.T, p), a.D, gw, gb);
+    hipLaunchKernelGGL(norm_bwd_sums_kernel, sg, dim3(1024), 0, st, a.part, blocks, a.D, gw, gb);
     return check_launch("layer_norm_backward sums");
   }
   return MHC_OK;
@@ -460,7 +482,7 @@ extern "C" int mhc_layer_norm_fwd(const void* x, int32_t x_dtype, const void* we
 
 extern "C" size_t mhc_layer_norm_bwd_workspace_size(int64_t T, int32_t D, int32_t x_dtype) {
   if (T <= 0 || D < 1 || T > kMaxTokens || !known_dtype(x_dtype)) return 0;
-  return (size_t)norm_bwd_parts(T, norm_plan(D, vec_of(x_dtype))) * 2 * (size_t)D * sizeof(float);
+  return (size_t)norm_bwd_blocks(T, norm_plan(D, vec_of(x_dtype), true)) * 2 * (size_t)D * sizeof(float);
 }
 
 extern "C" int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_dtype, const void* weight,

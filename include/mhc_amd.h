@@ -342,7 +342,8 @@ int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_dtype, const
  *   out = hidden w_down^T
  * x: (T,D), w_gate, w_up: (F,D), w_down: (O,F), out: (T,O), all `dtype`,
  * 16-byte aligned.  Products accumulate in fp32; hidden is rounded to `dtype`
- * between the two products.  For the backward, all or none of: gate, up (T,F)
+ * between the two products.  The workspace holds hidden, padded copies of
+ * operands whose rows are no multiples of 16 bytes, and partial sums.  For the backward, all or none of: gate, up (T,F)
  * fp32 and hidden, (T, F) `dtype` in rows of stride F rounded up to 8
  * elements (the rest of a row is written as zero).  With none, hidden lives in the workspace.
  */
@@ -359,8 +360,9 @@ int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up, const
 /*
  * Backward of the block from the forward's gate, up and hidden: grad_x (T,D),
  * grad_w_gate, grad_w_up (F,D), grad_w_down (O,F), all `dtype`, 16-byte
- * aligned.  The gradients of gate and up are rounded to `dtype` between the
- * products.  Deterministic.  T == 0 writes nothing.
+ * aligned; all or none of the weights' three may be NULL.  The gradients of
+ * gate and up are rounded to `dtype` between the products.  Deterministic.
+ * T == 0 writes nothing.
  */
 size_t mhc_gated_ffn_bwd_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype);
 int mhc_gated_ffn_bwd(const void* grad_out, const void* x, const void* w_gate, const void* w_up,
