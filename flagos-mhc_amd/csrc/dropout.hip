@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(DropArgs a) {
     offset = a.state[1];
   }
   const int64_t full = a.n / 8, step = (int64_t)gridDim.x * 256;
-  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t first = xcd_contig(blockIdx.x, gridDim.x) * 256 + threadIdx.x;
   for (int64_t g = first; g < full; g += step) {
     u32x4 v[8 / VEC];
 #pragma unroll
