@@ -215,6 +215,25 @@ __device__ __forceinline__ void finish(const GemmArgs& a, const Piece& p, int z,
   }
 }
 
+// ROWS rows of a tile's sums, from its row `first` on, out of LDS: a wave has
+// whole rows, so that what it writes (and the gated gradient reads) are long
+// runs.  16-byte chunks are exclusive-ored with the row for the banks.
+template <typename C, int ROWS, int THREADS>
+__device__ __forceinline__ void stream_rows(const GemmArgs& a, const Piece& p, int z, int m0, int n0, int first,
+                                            const floatx4* cs) {
+  constexpr int kRow4 = C::BN / 4, kCols4 = C::kCols / 4, kTurn = THREADS / kCols4;  // rows a turn
+  static_assert(ROWS % kTurn == 0, "whole turns");
+  constexpr int kTurns = ROWS / kTurn, kUnroll = kTurns < 4 ? kTurns : 4;
+  const int r0 = threadIdx.x / kCols4, c = threadIdx.x % kCols4;
+#pragma unroll kUnroll
+  for (int i = 0; i < kTurns; ++i) {
+    const int r = i * kTurn + r0;
+    const floatx4 c0 = cs[r * kRow4 + (c ^ (r & 15))];
+    const floatx4 c1 = C::EPI == kEpiGated ? cs[r * kRow4 + ((kCols4 + c) ^ (r & 15))] : c0;
+    finish<C>(a, p, z, m0, n0, first + r, c * 4, c0, c1);
+  }
+}
+
 // Where a block's next tiles of A and B start, and how many k are left there
 // (0 past the block's steps).
 template <typename C>
@@ -373,14 +392,22 @@ __device__ __forceinline__ void gemm_tile_piece(const GemmArgs& a, const Piece& 
     }
   }
 
-  // lane: row l % 16 of a fragment of A, columns 4 (l / 16) .. + 3 of one of B
-  constexpr int NC = C::NFB / C::kNB;
+  // lane: row l % 16 of a fragment of A, columns 4 (l / 16) .. + 3 of one of B.
+  // Through LDS, as rows of [columns, those of the gated form's second operand].
+  constexpr int NC = C::NFB / C::kNB, kRow4 = C::BN / 4;
+  static_assert(C::BM * C::BN * 4 <= C::STAGES * C::kSlot, "the tile's sums fit the slots");
+  floatx4* const cs = reinterpret_cast<floatx4*>(smem);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < C::NFA; ++i)
 #pragma unroll
-    for (int j = 0; j < NC; ++j)
-      finish<C>(a, piece, z, m0, n0, wm * C::WM + 16 * i + (lane & 15), wn * (C::WN / C::kNB) + 16 * j + (lane >> 4) * 4,
-                acc[i][j], acc[i][C::kNB == 2 ? j + NC : j]);
+    for (int j = 0; j < C::NFB; ++j) {
+      const int r = wm * C::WM + 16 * i + (lane & 15);
+      const int c = j / NC * (C::kCols / 4) + wn * (C::WN / C::kNB / 4) + j % NC * 4 + (lane >> 4);
+      cs[r * kRow4 + (c ^ (r & 15))] = acc[i][j];
+    }
+  __syncthreads();
+  stream_rows<C, C::BM, 256>(a, piece, z, m0, n0, 0, cs);
 }
 
 template <typename C>
@@ -529,8 +556,7 @@ __device__ __forceinline__ void gemm_wide_piece(const GemmArgs& a, const Piece& 
   if (wave < 4) barrier();
   wait_vmcnt<0>();  // no load may still be on its way to LDS when the block ends
 
-  // 128 rows of C at a time through LDS, so that a wave writes (and the gated
-  // gradient reads) whole rows; chunks are exclusive-ored with the row for the banks
+  // 128 rows of C at a time through LDS
   floatx4* const cs = reinterpret_cast<floatx4*>(smem);
 #pragma unroll
   for (int i = 0; i < C::kHalves; ++i) {
@@ -543,14 +569,7 @@ __device__ __forceinline__ void gemm_wide_piece(const GemmArgs& a, const Piece& 
         cs[r * 64 + (c ^ (r & 15))] = acc[i][p][q];
       }
     __syncthreads();
-    constexpr int kRows = kPair ? 16 : 8;  // rows a turn
-#pragma unroll 4
-    for (int r0 = 0; r0 < 128; r0 += kRows) {
-      const int r = r0 + (kPair ? wave * 2 + (lane >> 5) : wave), c = kPair ? lane & 31 : lane;
-      const floatx4 c0 = cs[r * 64 + (c ^ (r & 15))];
-      const floatx4 c1 = kPair ? cs[r * 64 + ((c + 32) ^ (r & 15))] : c0;
-      finish<C>(a, piece, z, m0, n0, i * 128 + r, c * 4, c0, c1);
-    }
+    stream_rows<C, 128, 512>(a, piece, z, m0, n0, i * 128, cs);
   }
 }
 
