@@ -33,7 +33,7 @@ int check_ffn(const char* who, const FfnDims& d, int32_t dtype, int32_t act) {
       (((int64_t)d.F + 63) / 64) * (((int64_t)(d.D > d.O ? d.D : d.O) + 63) / 64) > 0x3fffffff ||
       ((d.T + 15) / 16) * (((int64_t)d.D + 63) / 64) > 0x3fffffff)
     return set_error(MHC_ERR_UNSUPPORTED, "%s: T=%lld D=%d F=%d O=%d are too many tiles", who, (long long)d.T, d.D, d.F, d.O);
-  if (act < 0 || act > kActRelu) return set_error(MHC_ERR_INVALID, "%s: activation %d", who, act);
+  if (act < 0 || act > MHC_ACT_RELU) return set_error(MHC_ERR_INVALID, "%s: activation %d", who, act);
   return MHC_OK;
 }
 
@@ -55,7 +55,7 @@ using namespace mhc;
 
 extern "C" size_t mhc_gated_ffn_fwd_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype) {
   if (check_ffn("", {T, D, F, O}, dtype, 0) || T == 0) return 0;
-  return FfnWorkspace({T, D, F, O}, elem_bytes(dtype), false).bytes(false);
+  return FfnWorkspace({T, D, F, O}, elem_bytes(dtype), false, device_cu_count()).bytes(false);
 }
 
 extern "C" int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down,
@@ -84,7 +84,7 @@ extern "C" int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* 
 
 extern "C" size_t mhc_gated_ffn_bwd_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype) {
   if (check_ffn("", {T, D, F, O}, dtype, 0) || T == 0) return 0;
-  return FfnWorkspace({T, D, F, O}, elem_bytes(dtype), true).bytes(true);
+  return FfnWorkspace({T, D, F, O}, elem_bytes(dtype), true, device_cu_count()).bytes(true);
 }
 
 extern "C" int mhc_gated_ffn_bwd(const void* grad_out, const void* x, const void* w_gate, const void* w_up,

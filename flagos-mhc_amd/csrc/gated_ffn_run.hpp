@@ -2,6 +2,7 @@
 #pragma once
 
 #include "gated_ffn.hpp"
+#include "gemm_kernel.hpp"
 
 namespace mhc {
 
@@ -128,7 +129,7 @@ template <typename S, int LA, int LB, int EPI>
 int launch_gemm(GemmArgs a, const GemmShape& s, float* part, hipStream_t st) {
   if constexpr (LA == kRow && LB == kRow)
     if (s.M <= kFewRows) return launch_few_rows<S, EPI>(a, st);
-  const GemmPlans p = plan_gemm(s, sizeof(S));
+  const GemmPlans p = plan_gemm(s, sizeof(S), device_cu_count());
   a.M = (int)p.main_rows;
   if (const int rc = launch_plan<S, LA, LB, EPI>(a, p.main, part, st)) return rc;
   if (p.main_rows == s.M) return MHC_OK;
@@ -157,7 +158,7 @@ inline GemmArgs gemm_args(const GemmShape& s, const void* a0, const void* a1, co
 template <typename S>
 int ffn_fwd(const FfnFwd& f, const FfnDims& d, char* ws, hipStream_t st) {
   const FfnLines l(d, sizeof(S));
-  const FfnWorkspace w(d, sizeof(S), false);
+  const FfnWorkspace w(d, sizeof(S), false, device_cu_count());
   void* h = f.hidden ? f.hidden : ws;
   Padder<S> pad(ws + w.hidden);
   const void *x = f.x, *wg = f.w_gate, *wu = f.w_up, *wd = f.w_down;
@@ -175,7 +176,7 @@ int ffn_fwd(const FfnFwd& f, const FfnDims& d, char* ws, hipStream_t st) {
 template <typename S>
 int ffn_bwd(const FfnBwd& f, const FfnDims& d, char* ws, hipStream_t st) {
   const FfnLines l(d, sizeof(S));
-  const FfnWorkspace w(d, sizeof(S), true);
+  const FfnWorkspace w(d, sizeof(S), true, device_cu_count());
   void *dg = ws, *du = ws + w.hidden;
   Padder<S> pad(ws + 2 * w.hidden);
   const void *go = f.grad_out, *x = f.x, *wg = f.w_gate, *wu = f.w_up, *wd = f.w_down;

@@ -2,6 +2,7 @@
 // tile kernel that runs every shape, type and layout.
 #pragma once
 
+#include "gemm_plan.hpp"
 #include "gemm_tile.hpp"
 
 namespace mhc {
@@ -11,7 +12,6 @@ namespace mhc {
 // kEpiStore: out0 = C.  kEpiGated (two B operands, g = A B0^T, u = A B1^T):
 // out0 = act(g) u, and g and u where gate and up are given.  kEpiGatedGrad
 // (C is the gradient of act(g) u): out0 = C u act'(g), out1 = C act(g).
-enum { kEpiStore = 0, kEpiGated = 1, kEpiGatedGrad = 2 };
 enum { kActSilu = 0, kActGelu = 1, kActGeluTanh = 2, kActRelu = 3 };
 
 struct GemmArgs {
@@ -172,31 +172,21 @@ __device__ __forceinline__ void tile_of(int t, int tm, int tn, int* mt, int* nt,
   *nt = __builtin_amdgcn_readfirstlane(r / rows);
 }
 
-// Where run block b's steps start: of `steps` steps a tile.
-__host__ __device__ __forceinline__ int64_t run_start(int64_t b, int tiles, int steps, int blocks) {
-  return b * tiles * steps / blocks;
-}
-
 // A block's i-th piece of work: steps s0 .. s1 - 1 of a tile, or none.
-// (A run is shorter than a tile, so it has one piece or two.)
 struct Piece {
   int tile, s0, s1;
   int slot;  // of the partial sums; -1: the whole tile
 };
 __device__ __forceinline__ bool piece_of(const GemmArgs& a, int steps, int i, Piece* p) {
   const int bid = blockIdx.x;
-  p->slot = -1;
+  const auto uniform = [](int64_t v) { return __builtin_amdgcn_readfirstlane((int)v); };
   if (bid < a.whole_tiles) {
-    *p = {__builtin_amdgcn_readfirstlane((int)xcd_contig(bid, a.whole_tiles)), 0, steps, -1};
+    *p = {uniform(xcd_contig(bid, a.whole_tiles)), 0, steps, -1};
     return i == 0;
   }
-  const int64_t b = xcd_contig(bid - a.whole_tiles, a.run_blocks);
-  const int64_t lo = run_start(b, a.run_tiles, steps, a.run_blocks), hi = run_start(b + 1, a.run_tiles, steps, a.run_blocks);
-  const int64_t t = lo / steps + i;
-  const int64_t first = t * steps, s0 = lo > first ? lo - first : 0, s1 = hi - first < steps ? hi - first : steps;
-  if (s0 >= s1) return false;
-  const auto uniform = [](int64_t v) { return __builtin_amdgcn_readfirstlane((int)v); };
-  *p = {uniform(a.whole_tiles + t), uniform(s0), uniform(s1), uniform(s0 == 0 && s1 == steps ? -1 : 2 * b + i)};
+  RunPiece r;
+  if (!run_piece(xcd_contig(bid - a.whole_tiles, a.run_blocks), i, a.run_tiles, steps, a.run_blocks, &r)) return false;
+  *p = {uniform(a.whole_tiles + r.tile), uniform(r.s0), uniform(r.s1), uniform(r.slot)};
   return true;
 }
 
@@ -597,23 +587,14 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
   tile_of(a.whole_tiles + t, (a.M + C::BM - 1) / C::BM, (int)((a.ldo + C::kCols - 1) / C::kCols), &mt, &nt, &z);
   const int64_t m = (int64_t)mt * C::BM + r;
   if (m >= a.M) return;
-  // the run that holds the tile's first step
-  const int64_t first = (int64_t)t * steps, last = first + steps;
-  int64_t b = first * a.run_blocks / ((int64_t)a.run_tiles * steps);
-  while (b > 0 && run_start(b, a.run_tiles, steps, a.run_blocks) > first) --b;
-  while (run_start(b + 1, a.run_tiles, steps, a.run_blocks) <= first) ++b;
-  if (run_start(b, a.run_tiles, steps, a.run_blocks) <= first && run_start(b + 1, a.run_tiles, steps, a.run_blocks) >= last)
-    return;  // one block has the whole tile, and has finished it
-  // runs b .. e - 1; only the first may have started in the tile before
-  int64_t e = last * a.run_blocks / ((int64_t)a.run_tiles * steps);
-  while (e < a.run_blocks && run_start(e, a.run_tiles, steps, a.run_blocks) < last) ++e;
-  while (run_start(e - 1, a.run_tiles, steps, a.run_blocks) >= last) --e;
+  const RunBlocks rb = run_blocks_of(t, a.run_tiles, steps, a.run_blocks);
+  if (rb.first == rb.last) return;  // one block has the whole tile, and has finished it
   const int64_t stride = 2 * (int64_t)C::BM * C::BN;
-  const float* q = a.part + b * stride + (int64_t)r * C::BN + c;
-  if (run_start(b, a.run_tiles, steps, a.run_blocks) < first) q += stride / 2;
+  const float* q = a.part + rb.first * stride + (int64_t)r * C::BN + c;
+  if (rb.begun_before) q += stride / 2;
   floatx4 c0 = *reinterpret_cast<const floatx4*>(q), c1 = c0;
   if constexpr (C::EPI == kEpiGated) c1 = *reinterpret_cast<const floatx4*>(q + C::kCols);
-  q = a.part + (b + 1) * stride + (int64_t)r * C::BN + c;
+  q = a.part + (rb.first + 1) * stride + (int64_t)r * C::BN + c;
   const auto add = [&](int n) {  // n runs, their loads first
     floatx4 u[8], v[8];
 #pragma unroll
@@ -630,7 +611,7 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
       }
     q += n * stride;
   };
-  int64_t left = e - b - 1;
+  int64_t left = rb.last - rb.first - 1;
   for (; left >= 8; left -= 8) add(8);
   if (left > 0) add((int)left);
   epilogue<typename C::S, C::EPI>(a, z, m, nt * C::kCols + c, c0, c1);

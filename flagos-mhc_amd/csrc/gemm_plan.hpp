@@ -1,13 +1,69 @@
 // Host side of the matrix products: which kernel runs one, and how its tiles
-// are dealt out.
+// are dealt out.  Plain C++ with no HIP in it: a test compiles it alone and
+// walks the plans of many shapes on the CPU.
 #pragma once
 
-#include <cmath>
+#include <math.h>
+#include <stddef.h>
+#include <stdint.h>
 
-#include "gemm_kernel.hpp"
-#include "mhc_launch.hpp"
+#ifdef __HIPCC__
+#define MHC_HOST_DEVICE __host__ __device__
+#else
+#define MHC_HOST_DEVICE
+#endif
 
 namespace mhc {
+
+enum { kRow = 0, kCol = 1 };  // an operand's contiguous index: k, or m or n
+
+// What becomes of a product C (gemm_kernel.hpp).
+enum { kEpiStore = 0, kEpiGated = 1, kEpiGatedGrad = 2 };
+
+// ---- runs of steps ------------------------------------------------------------
+// run_tiles tiles of `steps` steps each, dealt to run_blocks blocks in runs of
+// equal length (to one step).
+
+// Where block b's run starts, in steps from the first tile's first.
+MHC_HOST_DEVICE inline int64_t run_start(int64_t b, int tiles, int steps, int blocks) { return b * tiles * steps / blocks; }
+
+// The i-th piece of block b's run (a run is no longer than a tile, so it has
+// one or two): its tile, steps and slot of the partial sums (-1: the whole tile).
+struct RunPiece {
+  int64_t tile, s0, s1, slot;
+};
+MHC_HOST_DEVICE inline bool run_piece(int64_t b, int i, int tiles, int steps, int blocks, RunPiece* p) {
+  const int64_t lo = run_start(b, tiles, steps, blocks), hi = run_start(b + 1, tiles, steps, blocks);
+  const int64_t t = lo / steps + i, first = t * steps;
+  p->tile = t;
+  p->s0 = lo > first ? lo - first : 0;
+  p->s1 = hi - first < steps ? hi - first : steps;
+  p->slot = p->s0 == 0 && p->s1 == steps ? -1 : 2 * b + i;
+  return p->s0 < p->s1;
+}
+
+// The blocks with a piece of tile t: [first, last).  Only `first` can have
+// begun before the tile (its piece is then its second); none if one block has
+// the whole tile.
+struct RunBlocks {
+  int64_t first, last;
+  bool begun_before;
+};
+MHC_HOST_DEVICE inline RunBlocks run_blocks_of(int64_t t, int tiles, int steps, int blocks) {
+  const int64_t begin = t * steps, end = begin + steps, total = (int64_t)tiles * steps;
+  RunBlocks r;
+  r.first = begin * blocks / total;
+  while (r.first > 0 && run_start(r.first, tiles, steps, blocks) > begin) --r.first;
+  while (run_start(r.first + 1, tiles, steps, blocks) <= begin) ++r.first;
+  r.last = end * blocks / total;
+  while (r.last < blocks && run_start(r.last, tiles, steps, blocks) < end) ++r.last;
+  while (run_start(r.last - 1, tiles, steps, blocks) >= end) --r.last;
+  r.begun_before = run_start(r.first, tiles, steps, blocks) < begin;
+  if (r.last - r.first == 1 && !r.begun_before && run_start(r.last, tiles, steps, blocks) >= end) r.last = r.first;
+  return r;
+}
+
+// ---- plans ---------------------------------------------------------------------
 
 // Operands as a product's plan sees them: the block's products differ in
 // which index of A and B is contiguous, in the epilogue and in the batch.
@@ -55,17 +111,17 @@ inline int64_t tiles_of(const GemmShape& s, int64_t bm, int64_t bn) {
 // Whole tiles go out in rounds of all blocks that fit the card at once; the
 // last round's tiles are cut into equal runs of steps if that, with the
 // partial sums' way through memory, is less than the round.
-inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma) {
+inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma, int64_t cus) {
   const KernelCost& c = kCosts[kind];
   const StepCost& cost = dma ? (es == 4 ? c.dma32 : c.dma16) : (es == 4 ? c.reg32 : c.reg16);
-  const int64_t cus = device_cu_count(), slots = cus * c.per_cu;
+  const int64_t slots = cus * c.per_cu;
   const int64_t tiles = tiles_of(s, c.bm, c.bn), steps = (s.K * (int64_t)es + 127) / 128 * s.segments;
   // n steps of `blocks` blocks side by side: on a part of the CUs each runs
   // faster, as the card's power then allows a higher clock
   const auto side_by_side = [&](double blocks, double n) {
     const double part = blocks < cus ? blocks / cus : 1.;
     const double few = c.per_cu > 1 ? cost.alone : cost.alone + (cost.full - cost.alone) * part;
-    const double full = blocks < cus ? 0. : std::ceil(blocks / cus) * cost.full;
+    const double full = blocks < cus ? 0. : ceil(blocks / cus) * cost.full;
     return n * (full > few ? full : few) * (s.la == kCol && kind >= kWide128 ? kColCol : 1.);
   };
   const int64_t rest = tiles % slots, rounds = tiles / slots;
@@ -88,7 +144,7 @@ inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma) {
   return p;
 }
 
-inline GemmPlan plan_rows(const GemmShape& s, size_t es) {
+inline GemmPlan plan_rows(const GemmShape& s, size_t es, int64_t cus) {
   const int64_t line_a = s.lda * (int64_t)es, line_b = s.ldb * (int64_t)es;
   // 32-bit offsets within a tile's lines
   const bool dma = line_a % 16 == 0 && line_b % 16 == 0 && line_a < (1 << 23) && line_b < (1 << 23);
@@ -97,7 +153,7 @@ inline GemmPlan plan_rows(const GemmShape& s, size_t es) {
     if (kind >= kWide128 && !dma) break;
     const bool few = kind <= kTile64x128;  // rows: the tile that holds them all; kCol tiles have 64 rows or more
     if (few && (s.la == kCol || s.M > kCosts[kind].bm)) continue;
-    const GemmPlan q = deal_tiles(s, es, kind, dma);
+    const GemmPlan q = deal_tiles(s, es, kind, dma, cus);
     if (p.us == 0. || q.us < p.us) p = q;
     if (few) break;
   }
@@ -110,16 +166,16 @@ struct GemmPlans {
   GemmPlan main, tail;
   int64_t main_rows;  // M: no tail
 };
-inline GemmPlans plan_gemm(const GemmShape& s, size_t es) {
+inline GemmPlans plan_gemm(const GemmShape& s, size_t es, int64_t cus) {
   GemmPlans p = {};
   if (s.la == kRow && s.lb == kRow && s.M <= kFewRows) return p;  // a kernel of its own
-  p = {plan_rows(s, es), {}, s.M};
+  p = {plan_rows(s, es, cus), {}, s.M};
   const int64_t over = s.M % 256;
   if (s.la == kRow && s.M > 256 && over > 0 && over <= 64) {
     GemmShape m = s, t = s;
     m.M = s.M - over;
     t.M = over;
-    const GemmPlan a = plan_rows(m, es), b = plan_rows(t, es);
+    const GemmPlan a = plan_rows(m, es, cus), b = plan_rows(t, es, cus);
     if (a.us + b.us < p.main.us) p = {a, b, m.M};
   }
   return p;

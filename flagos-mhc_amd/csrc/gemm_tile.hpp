@@ -15,11 +15,10 @@
 #pragma once
 
 #include "common.hpp"
+#include "gemm_plan.hpp"
 #include "lds_dma.hpp"
 
 namespace mhc {
-
-enum { kRow = 0, kCol = 1 };
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 

@@ -116,7 +116,7 @@ def test_layer_matches_its_parts_and_pytorch():
     ref.backward(gh.float())
     # roundings to bf16 on the way: norm, hidden, out, dropped; the gradients of out, gate and up, norm, y
     eps = R.half_step(torch.bfloat16)
-    assert float((h.float() - ref).norm() / ref.norm()) <= 4 * eps
+    assert float((h.float() - ref.detach()).norm() / ref.detach().norm()) <= 4 * eps
     gx_y, _, _ = S.layer_norm_backward(gn, pre["y"], nw, n["mean"], n["rstd"])
     assert float((gx_y.float() - y.grad).norm() / y.grad.norm()) <= 8 * eps
 
