@@ -134,6 +134,18 @@ def on_device(dev: torch.device):
     return _no_guard if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def call(what: str, fn, dev_index: int, *args) -> None:
+    """fn(*args, current stream) on the device `dev_index`, checked.  (Host time
+    is what small calls cost: nothing is done here that they do not need.)"""
+    if torch._C._cuda_getDevice() == dev_index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev_index))
+    else:
+        with torch.cuda.device(dev_index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev_index))
+    if rc:
+        check(rc, what)
+
+
 def operand(t: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
     """t as a contiguous tensor of `dtype` with shape's elements in order (the
     kernels take its address only, so a tensor that already holds them is

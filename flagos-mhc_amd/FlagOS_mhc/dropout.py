@@ -32,13 +32,11 @@ def _apply(what, x, p, seed, offset, state):
                               or not state.is_contiguous()):
         raise ValueError(f"{what}: state must be a contiguous int64 tensor (seed, offset) on {x.device}")
     xf = x.contiguous()
-    y = torch.empty_like(xf, memory_format=torch.contiguous_format)
-    if xf.numel():
-        lib = _lib.load()
-        with _lib.on_device(xf.device):
-            rc = lib.mhc_dropout(xf.data_ptr(), y.data_ptr(), xf.numel(), code, p, int(seed) & _M64,
-                                 int(offset) & _M64, _lib.ptr(state), _lib.stream_of(xf))
-        _lib.check(rc, what)
+    y = torch.empty_like(xf)
+    n = xf.numel()
+    if n:
+        _lib.call(what, _lib.load().mhc_dropout, x.get_device(), xf.data_ptr(), y.data_ptr(), n, code, p,
+                  int(seed) & _M64, int(offset) & _M64, _lib.ptr(state))
     return y
 
 

@@ -50,7 +50,7 @@ def _check(what, x, w_gate, w_up, w_down, activation):
     for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         if w.dtype != x.dtype:
             raise ValueError(f"{what}: {name} is {w.dtype}, x {x.dtype}")
-        if w.device != x.device:
+        if w.get_device() != x.get_device():
             raise ValueError(f"{what}: {name} is on {w.device}, x on {x.device}")
     return math.prod(x.shape[:-1]), D, F, O, code, ACTIVATIONS[activation]
 
@@ -73,13 +73,10 @@ def gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=False):
         xf = _aligned(x, (T, D), x.dtype)
         wg, wu = _aligned(w_gate, (F, D), x.dtype), _aligned(w_up, (F, D), x.dtype)
         wd = _aligned(w_down, (O, F), x.dtype)
-        lib = _lib.load()
         ws, ws_bytes = _lib.workspace("mhc_gated_ffn_fwd_workspace_size", dev, T, D, F, O, code)
-        with _lib.on_device(dev):
-            rc = lib.mhc_gated_ffn_fwd(xf.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), code, act,
-                                       out.data_ptr(), _lib.ptr(gate), _lib.ptr(up), _lib.ptr(hidden),
-                                       ws.data_ptr(), ws_bytes, T, D, F, O, _lib.stream_of(xf))
-        _lib.check(rc, what)
+        _lib.call(what, _lib.load().mhc_gated_ffn_fwd, x.get_device(), xf.data_ptr(), wg.data_ptr(), wu.data_ptr(),
+                  wd.data_ptr(), code, act, out.data_ptr(), _lib.ptr(gate), _lib.ptr(up), _lib.ptr(hidden),
+                  ws.data_ptr(), ws_bytes, T, D, F, O)
     result = {"out": out}
     if need_backward:
         result.update(gate=gate, up=up, hidden=hidden)
@@ -114,14 +111,10 @@ def gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, acti
         wd = _aligned(w_down, (O, F), x.dtype)
         g, u = _aligned(gate, (T, F), torch.float32), _aligned(up, (T, F), torch.float32)
         h = _aligned(hidden, hidden.shape, x.dtype)
-        lib = _lib.load()
         ws, ws_bytes = _lib.workspace("mhc_gated_ffn_bwd_workspace_size", dev, T, D, F, O, code)
-        with _lib.on_device(dev):
-            rc = lib.mhc_gated_ffn_bwd(go.data_ptr(), xf.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(),
-                                       g.data_ptr(), u.data_ptr(), h.data_ptr(), code, act, gx.data_ptr(),
-                                       _lib.ptr(gwg), _lib.ptr(gwu), _lib.ptr(gwd), ws.data_ptr(), ws_bytes,
-                                       T, D, F, O, _lib.stream_of(xf))
-        _lib.check(rc, what)
+        _lib.call(what, _lib.load().mhc_gated_ffn_bwd, x.get_device(), go.data_ptr(), xf.data_ptr(), wg.data_ptr(),
+                  wu.data_ptr(), wd.data_ptr(), g.data_ptr(), u.data_ptr(), h.data_ptr(), code, act, gx.data_ptr(),
+                  _lib.ptr(gwg), _lib.ptr(gwu), _lib.ptr(gwd), ws.data_ptr(), ws_bytes, T, D, F, O)
     return gx, gwg, gwu, gwd
 
 

@@ -17,29 +17,39 @@ import torch
 from . import _lib
 
 
+_F32 = torch.float32
+
+
 def _rows(what, x):
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"{what}: x of shape {tuple(x.shape)} has no last dimension to normalise")
-    D = x.shape[-1]
-    return x.numel() // D, D
+    """(rows, their length, dtype code) of x."""
+    shape = x.shape
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"{what}: x of shape {tuple(shape)} has no last dimension to normalise")
+    D = shape[-1]
+    return x.numel() // D, D, _lib.dtype_code(what, x.dtype)
 
 
-def _param(what, name, p, x):
+def _param(what, name, p, x, D):
     """weight or bias as the kernel takes it: (D,), x's dtype or fp32."""
-    if p is None:
-        return None
-    if p.numel() != x.shape[-1]:
-        raise ValueError(f"{what}: {name} has {p.numel()} elements, x's rows {x.shape[-1]}")
-    if p.device != x.device:
+    if p.numel() != D:
+        raise ValueError(f"{what}: {name} has {p.numel()} elements, x's rows {D}")
+    if p.get_device() != x.get_device():
         raise ValueError(f"{what}: {name} is on {p.device}, x on {x.device}")
-    return _lib.operand(p, (p.numel(),), p.dtype if p.dtype == x.dtype else torch.float32)
+    dt = p.dtype
+    if (dt is _F32 or dt is x.dtype) and p.is_contiguous():
+        return p
+    return _lib.operand(p, (D,), dt if dt is x.dtype else _F32)
 
 
-def _params(what, x, weight, bias):
-    w, b = _param(what, "weight", weight, x), _param(what, "bias", bias, x)
-    if w is not None and b is not None and w.dtype != b.dtype:
-        w, b = w.float(), b.float()
-    dt = w.dtype if w is not None else b.dtype if b is not None else x.dtype
+def _params(what, x, D, weight, bias):
+    w = None if weight is None else _param(what, "weight", weight, x, D)
+    b = None if bias is None else _param(what, "bias", bias, x, D)
+    if w is None:
+        dt = x.dtype if b is None else b.dtype
+    else:
+        dt = w.dtype
+        if b is not None and b.dtype is not dt:
+            w, b, dt = w.float(), b.float(), _F32
     return w, b, _lib.DTYPE_CODE[dt]
 
 
@@ -48,22 +58,18 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, need_backward=False):
     dtype); with ``need_backward`` also mean and rstd (rows,) fp32."""
     what = "layer_norm"
     _lib.require_device(what, x, weight, bias)
-    code = _lib.dtype_code(what, x.dtype)
-    T, D = _rows(what, x)
-    w, b, wcode = _params(what, x, weight, bias)
+    T, D, code = _rows(what, x)
+    w, b, wcode = _params(what, x, D, weight, bias)
     xf = x.contiguous()
-    y = torch.empty_like(xf, memory_format=torch.contiguous_format)
+    y = torch.empty_like(xf)
     out = {"y": y}
     mean = rstd = None
     if need_backward:
-        mean, rstd = (torch.empty((T,), dtype=torch.float32, device=x.device) for _ in range(2))
-        out.update(mean=mean, rstd=rstd)
+        mean = out["mean"] = torch.empty(T, dtype=_F32, device=x.device)
+        rstd = out["rstd"] = torch.empty_like(mean)
     if T > 0:
-        lib = _lib.load()
-        with _lib.on_device(xf.device):
-            rc = lib.mhc_layer_norm_fwd(xf.data_ptr(), code, _lib.ptr(w), _lib.ptr(b), wcode, float(eps),
-                                        y.data_ptr(), _lib.ptr(mean), _lib.ptr(rstd), T, D, _lib.stream_of(xf))
-        _lib.check(rc, what)
+        _lib.call(what, _lib.load().mhc_layer_norm_fwd, x.get_device(), xf.data_ptr(), code, _lib.ptr(w), _lib.ptr(b),
+                  wcode, eps, y.data_ptr(), _lib.ptr(mean), _lib.ptr(rstd), T, D)
     return out
 
 
@@ -72,33 +78,27 @@ def layer_norm_backward(grad_y, x, weight, mean, rstd, need_params=True):
     other two (D,) fp32 (None with ``need_params=False``).  Deterministic."""
     what = "layer_norm_backward"
     _lib.require_device(what, grad_y, x, weight, mean, rstd)
-    code = _lib.dtype_code(what, x.dtype)
-    T, D = _rows(what, x)
+    T, D, code = _rows(what, x)
     if grad_y.shape != x.shape:
         raise ValueError(f"{what}: grad_y of shape {tuple(grad_y.shape)} for x of shape {tuple(x.shape)}")
     if mean.numel() != T or rstd.numel() != T:
         raise ValueError(f"{what}: {mean.numel()} means and {rstd.numel()} rstds for {T} rows")
-    w, _, wcode = _params(what, x, weight, None)
+    w, _, wcode = _params(what, x, D, weight, None)
     xf = x.contiguous()
     gy = _lib.operand(grad_y, x.shape, xf.dtype)
-    mu, rs = _lib.operand(mean, (T,), torch.float32), _lib.operand(rstd, (T,), torch.float32)
-    dev = xf.device
-    gx = torch.empty_like(xf, memory_format=torch.contiguous_format)
-    gw = gb = None
-    if T == 0:
-        if need_params:
-            gw, gb = (torch.zeros((D,), dtype=torch.float32, device=dev) for _ in range(2))
-        return gx, gw, gb
-    ws, ws_bytes = None, 0
+    mu, rs = _lib.operand(mean, (T,), _F32), _lib.operand(rstd, (T,), _F32)
+    gx = torch.empty_like(xf)
+    gw = gb = ws = None
+    ws_bytes = 0
     if need_params:
-        gw, gb = (torch.empty((D,), dtype=torch.float32, device=dev) for _ in range(2))
-        ws, ws_bytes = _lib.workspace("mhc_layer_norm_bwd_workspace_size", dev, T, D, code)
-    lib = _lib.load()
-    with _lib.on_device(dev):
-        rc = lib.mhc_layer_norm_bwd(gy.data_ptr(), xf.data_ptr(), code, _lib.ptr(w), wcode, mu.data_ptr(),
-                                    rs.data_ptr(), gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws),
-                                    ws_bytes, T, D, _lib.stream_of(xf))
-    _lib.check(rc, what)
+        gw = (torch.empty if T else torch.zeros)(D, dtype=_F32, device=x.device)
+        gb = torch.empty_like(gw) if T else torch.zeros_like(gw)
+    if T > 0:
+        if need_params:
+            ws, ws_bytes = _lib.workspace("mhc_layer_norm_bwd_workspace_size", x.device, T, D, code)
+        _lib.call(what, _lib.load().mhc_layer_norm_bwd, x.get_device(), gy.data_ptr(), xf.data_ptr(), code, _lib.ptr(w),
+                  wcode, mu.data_ptr(), rs.data_ptr(), gx.data_ptr(), _lib.ptr(gw), _lib.ptr(gb), _lib.ptr(ws),
+                  ws_bytes, T, D)
     return gx, gw, gb
 
 
