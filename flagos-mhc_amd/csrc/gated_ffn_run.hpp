@@ -157,7 +157,7 @@ inline GemmArgs gemm_args(const GemmShape& s, const void* a0, const void* a1, co
 
 template <typename S>
 int ffn_fwd(const FfnFwd& f, const FfnDims& d, char* ws, hipStream_t st) {
-  const FfnLines l(d, sizeof(S));
+  const FfnLines l(d, sizeof(S), false, device_cu_count());
   const FfnWorkspace w(d, sizeof(S), false, device_cu_count());
   void* h = f.hidden ? f.hidden : ws;
   Padder<S> pad(ws + w.hidden);
@@ -175,7 +175,7 @@ int ffn_fwd(const FfnFwd& f, const FfnDims& d, char* ws, hipStream_t st) {
 
 template <typename S>
 int ffn_bwd(const FfnBwd& f, const FfnDims& d, char* ws, hipStream_t st) {
-  const FfnLines l(d, sizeof(S));
+  const FfnLines l(d, sizeof(S), true, device_cu_count());
   const FfnWorkspace w(d, sizeof(S), true, device_cu_count());
   void *dg = ws, *du = ws + w.hidden;
   Padder<S> pad(ws + 2 * w.hidden);

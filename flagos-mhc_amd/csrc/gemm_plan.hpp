@@ -87,14 +87,16 @@ struct KernelCost {
 constexpr KernelCost kCosts[kKinds] = {
     {16, 128, 1, {0.8, 0.8}, {0.8, 0.8}, {1.2, 1.2}, {1.2, 1.2}},
     {64, 128, 1, {0.9, 0.9}, {1.8, 1.8}, {1.2, 1.2}, {2.0, 2.0}},
-    {64, 64, 4, {0.23, 0.6}, {0.6, 0.8}, {0.4, 0.76}, {0.65, 1.0}},
-    {128, 128, 2, {0.49, 0.8}, {2.3, 3.2}, {0.8, 1.28}, {2.5, 3.5}},
+    {64, 64, 4, {0.23, 0.6}, {0.6, 0.8}, {0.4, 1.2}, {0.65, 1.4}},
+    {128, 128, 2, {0.49, 0.8}, {2.3, 3.2}, {0.8, 1.5}, {2.5, 3.5}},
     {128, 256, 1, {0.87, 0.75}, {4.4, 4.4}, {}, {}},
     {256, 256, 1, {1.46, 1.25}, {8.5, 8.5}, {}, {}}};
-// both operands kCol: twice the LDS reads, which the large tiles feel
-constexpr double kColCol = 1.16;
+// both operands kCol: twice the LDS reads, which the large tiles feel; B's
+// lines of k through registers: a wait for memory every step
+constexpr double kColCol = 1.16, kColRegs = 1.7;
 constexpr int kFewRows = 4;
 constexpr double kJoinUs = 5., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
+constexpr double kCuBytesPerUs = 16e3;  // of a tile's results, with every CU at it
 
 struct GemmPlan {
   bool dma;   // operands' lines are whole 16-byte chunks
@@ -122,13 +124,17 @@ inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma, in
     const double part = blocks < cus ? blocks / cus : 1.;
     const double few = c.per_cu > 1 ? cost.alone : cost.alone + (cost.full - cost.alone) * part;
     const double full = blocks < cus ? 0. : ceil(blocks / cus) * cost.full;
-    return n * (full > few ? full : few) * (s.la == kCol && kind >= kWide128 ? kColCol : 1.);
+    return n * (full > few ? full : few) * (s.la == kCol && kind >= kWide128 ? kColCol : (s.lb == kCol && !dma ? kColRegs : 1.));
   };
   const int64_t rest = tiles % slots, rounds = tiles / slots;
-  const double rounds_us = kLaunchUs + rounds * side_by_side((double)slots, (double)steps);
+  // what a column of a tile's row reads and writes at the end, which only
+  // another block of the CU can overlap
+  const double ends = s.epi == kEpiStore ? es : (s.epi == kEpiGated ? (8. + es) / 2 : 8. + 2 * es);
+  const double end_us = c.bm * c.bn * ends / kCuBytesPerUs / (c.per_cu > 1 ? 2 : 1);
+  const double rounds_us = kLaunchUs + rounds * (side_by_side((double)slots, (double)steps) + c.per_cu * end_us);
   GemmPlan p = {dma, kind, (int)tiles, 0, 0, rounds_us};
   if (rest == 0) return p;
-  p.us += side_by_side((double)rest, (double)steps);
+  p.us += side_by_side((double)rest, (double)steps) + ceil((double)rest / cus) * end_us;
   // Runs of six steps or more.  The large tiles' blocks that work side by side
   // have to be at the same k of neighbouring tiles, or every one of them
   // fetches its operands for itself: a tile is cut into as many equal runs as
@@ -138,7 +144,7 @@ inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma, in
   if (kind >= kWide128) blocks = blocks / rest * rest;
   if (blocks > rest) {
     const double bytes = (double)(blocks + rest) * (s.M < c.bm ? s.M : c.bm) * c.bn * 4 * 2;
-    const double us = rounds_us + side_by_side((double)blocks, (double)rest * steps / blocks) + kJoinUs + bytes / kJoinBytesPerUs;
+    const double us = rounds_us + end_us + side_by_side((double)blocks, (double)rest * steps / blocks) + kJoinUs + bytes / kJoinBytesPerUs;
     if (us < p.us) p = {dma, kind, (int)(tiles - rest), (int)rest, (int)blocks, us};
   }
   return p;

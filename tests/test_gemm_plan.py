@@ -88,19 +88,28 @@ static void product(const GemmShape& s, size_t es, int cus, size_t part) {
   if (p.main_rows < s.M) ++tails, walk(s, s.M - p.main_rows, p.tail, es, cus, part);
 }
 
-static void block(const FfnDims& d, size_t es, int cus) {
-  const FfnLines l(d, es);
-  const FfnWorkspace f(d, es, false, cus), b(d, es, true, cus);
-  for (const GemmShape& s : {fwd_hidden(d, l), fwd_out(d, l)}) product(s, es, cus, f.part);
-  for (const GemmShape& s : {bwd_hidden(d, l), bwd_x(d, l), bwd_down(d, l), bwd_gate_up(d, l)}) product(s, es, cus, b.part);
-  // copies: whole 16-byte lines that hold the rows
+static long copies = 0;
+
+static void pass(const FfnDims& d, size_t es, int cus, bool back) {
+  const FfnLines l(d, es, back, cus);
+  const FfnWorkspace w(d, es, back, cus);
+  const FfnShapes f(d, l, back);
+  for (int i = 0; i < f.n; ++i) product(f.s[i], es, cus, w.part);
+  copies += l.copy_D || l.copy_F || l.copy_O;
+  // copies: whole 16-byte lines that hold the rows, in regions that hold them
   for (auto [copied, n, ld] : {std::tuple<bool, int64_t, int64_t>{l.copy_D, d.D, l.D}, {l.copy_F, d.F, l.F}, {l.copy_O, d.O, l.O}})
-    if (copied ? ld < n || ld * es % 16 != 0 : ld != n) fail("a copy's lines", fwd_hidden(d, l), es, cus);
-  if (l.copy_D && (f.x < (size_t)d.T * l.D * es || f.w < (size_t)d.F * l.D * es)) fail("copies of x, w", fwd_hidden(d, l), es, cus);
-  if (l.copy_F && f.w_down < (size_t)d.O * l.F * es) fail("copy of w_down", fwd_hidden(d, l), es, cus);
-  if (l.copy_O && b.grad_out < (size_t)d.T * l.O * es) fail("copy of grad_out", fwd_hidden(d, l), es, cus);
-  for (size_t n : {f.hidden, f.x, f.w, f.w_down, b.grad_out})
-    if (n % 256 != 0) fail("a region's alignment", fwd_hidden(d, l), es, cus);
+    if (copied ? ld < n || ld * es % 16 != 0 : ld != n) fail("a copy's lines", f.s[0], es, cus);
+  if (l.copy_D && (w.x < (size_t)d.T * l.D * es || w.w < (size_t)d.F * l.D * es)) fail("copies of x, w", f.s[0], es, cus);
+  if (l.copy_F && w.w_down < (size_t)d.O * l.F * es) fail("copy of w_down", f.s[0], es, cus);
+  if (l.copy_O && w.grad_out < (size_t)d.T * l.O * es) fail("copy of grad_out", f.s[0], es, cus);
+  if (w.hidden < (size_t)d.T * hidden_ld(d.F) * es) fail("hidden", f.s[0], es, cus);
+  for (size_t n : {w.hidden, w.x, w.w, w.w_down, w.grad_out})
+    if (n % 256 != 0) fail("a region's alignment", f.s[0], es, cus);
+  if (w.bytes(back) != (back ? 2 : 1) * w.hidden + w.x + 2 * w.w + w.w_down + w.grad_out + w.part) fail("the sum", f.s[0], es, cus);
+}
+
+static void block(const FfnDims& d, size_t es, int cus) {
+  for (int back = 0; back < 2; ++back) pass(d, es, cus, back);
 }
 
 int main() {
@@ -117,10 +126,10 @@ int main() {
     block(d, rng() % 3 ? 2 : 4, rng() % 8 ? 256 : (int)logu(1, 304));
   }
   for (int k = 0; k < kKinds; ++k) printf("%s%ld", k ? " " : "", kinds[k]);
-  printf(" of each kernel, %ld few rows, %ld in runs, %ld tails, %ld faults\n", few, runs, tails, bad);
+  printf(" of each kernel, %ld few rows, %ld in runs, %ld tails, %ld copies, %ld faults\n", few, runs, tails, copies, bad);
   for (long n : kinds)
     if (n < 50) return 1;
-  return bad || runs < 500 || tails < 50 || few < 100;
+  return bad || runs < 500 || tails < 50 || few < 100 || copies < 500;
 }
 """
 
