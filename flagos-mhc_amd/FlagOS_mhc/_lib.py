@@ -165,7 +165,7 @@ def workspace_size(name: str, dev_index: int, *args) -> int:
 def workspace(name: str, dev: torch.device, *args):
     """(tensor, bytes) of scratch for a call on `dev`."""
     n = workspace_size(name, dev.index, *args)
-    return torch.empty((max(n, 1),), dtype=torch.uint8, device=dev), n
+    return torch.empty(n or 1, dtype=torch.uint8, device=dev), n
 
 
 def pre_fwd_size_code(x_code: int, phi_code: int, addresses: int) -> int:

@@ -85,8 +85,9 @@ def layer_norm_backward(grad_y, x, weight, mean, rstd, need_params=True):
         raise ValueError(f"{what}: {mean.numel()} means and {rstd.numel()} rstds for {T} rows")
     w, _, wcode = _params(what, x, D, weight, None)
     xf = x.contiguous()
-    gy = _lib.operand(grad_y, x.shape, xf.dtype)
-    mu, rs = _lib.operand(mean, (T,), _F32), _lib.operand(rstd, (T,), _F32)
+    gy = grad_y if grad_y.dtype is x.dtype and grad_y.is_contiguous() else _lib.operand(grad_y, x.shape, x.dtype)
+    mu = mean if mean.dtype is _F32 and mean.is_contiguous() else _lib.operand(mean, (T,), _F32)
+    rs = rstd if rstd.dtype is _F32 and rstd.is_contiguous() else _lib.operand(rstd, (T,), _F32)
     gx = torch.empty_like(xf)
     gw = gb = ws = None
     ws_bytes = 0

@@ -277,19 +277,27 @@ __device__ __forceinline__ void read_col16_frags4(u32x4 (&f)[2][4], const uint32
   }
 }
 
-// kCol, fp32: one fragment at a, both halves of k.
-template <int LINE>
-__device__ __forceinline__ void read_col32_frag(u32x4& f0, u32x4& f1, uint32_t a) {
-  uint32_t r[8];
+// kCol, fp32: two fragments, at a and b, both halves of k.
+template <int LINE, int NF>
+__device__ __forceinline__ void read_col32_frags(u32x4 (&f)[2][NF], int i, uint32_t a, uint32_t b) {
+  uint32_t r[16];
   asm volatile(
-      "ds_read_b32 %0, %8\n\tds_read_b32 %1, %8 offset:%9\n\tds_read_b32 %2, %8 offset:%10\n\t"
-      "ds_read_b32 %3, %8 offset:%11\n\tds_read_b32 %4, %8 offset:%12\n\tds_read_b32 %5, %8 offset:%13\n\t"
-      "ds_read_b32 %6, %8 offset:%14\n\tds_read_b32 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7])
-      : "v"(a), "i"(LINE), "i"(2 * LINE), "i"(3 * LINE), "i"(16 * LINE), "i"(17 * LINE), "i"(18 * LINE),
-        "i"(19 * LINE) : "memory");
-  f0 = {r[0], r[1], r[2], r[3]};
-  f1 = {r[4], r[5], r[6], r[7]};
+      "ds_read_b32 %0, %16\n\tds_read_b32 %1, %16 offset:%18\n\tds_read_b32 %2, %16 offset:%19\n\t"
+      "ds_read_b32 %3, %16 offset:%20\n\tds_read_b32 %4, %16 offset:%21\n\tds_read_b32 %5, %16 offset:%22\n\t"
+      "ds_read_b32 %6, %16 offset:%23\n\tds_read_b32 %7, %16 offset:%24\n\t"
+      "ds_read_b32 %8, %17\n\tds_read_b32 %9, %17 offset:%18\n\tds_read_b32 %10, %17 offset:%19\n\t"
+      "ds_read_b32 %11, %17 offset:%20\n\tds_read_b32 %12, %17 offset:%21\n\tds_read_b32 %13, %17 offset:%22\n\t"
+      "ds_read_b32 %14, %17 offset:%23\n\tds_read_b32 %15, %17 offset:%24\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3]), "=&v"(r[4]), "=&v"(r[5]), "=&v"(r[6]), "=&v"(r[7]),
+        "=&v"(r[8]), "=&v"(r[9]), "=&v"(r[10]), "=&v"(r[11]), "=&v"(r[12]), "=&v"(r[13]), "=&v"(r[14]), "=&v"(r[15])
+      : "v"(a), "v"(b), "i"(LINE), "i"(2 * LINE), "i"(3 * LINE), "i"(16 * LINE), "i"(17 * LINE), "i"(18 * LINE),
+        "i"(19 * LINE)
+      : "memory");
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    f[0][i + k] = {r[8 * k], r[8 * k + 1], r[8 * k + 2], r[8 * k + 3]};
+    f[1][i + k] = {r[8 * k + 4], r[8 * k + 5], r[8 * k + 6], r[8 * k + 7]};
+  }
 }
 
 // The NF fragments of a wave, from row `first` (a multiple of 16 NF) of a tile of R rows.
@@ -321,8 +329,9 @@ struct FragReader {
     if constexpr (L == kRow) {
       read_row_frags<NF>(f, tile + a[0], tile + a[1]);
     } else if constexpr (sizeof(S) == 4) {
+      static_assert(NF % 2 == 0, "pairs of fragments");
 #pragma unroll
-      for (int j = 0; j < NF; ++j) read_col32_frag<kLine>(f[0][j], f[1][j], tile + a[j]);
+      for (int j = 0; j < NF; j += 2) read_col32_frags<kLine, NF>(f, j, tile + a[j], tile + a[j + 1]);
     } else if constexpr (NF == 4) {
       const uint32_t t[4] = {tile + a[0], tile + a[1], tile + a[2], tile + a[3]};
       read_col16_frags4<kLine>(f, t);

@@ -197,6 +197,9 @@ __global__ __launch_bounds__(1024) void norm_fwd_loop_kernel(NormFwdArgs a) {
 }
 
 struct NormBwdArgs {
+  float* gw;  // where one launch does all: the weights' gradients (null: not wanted), its row blocks
+  float* gb;
+  int row_blocks;
   const void* gy;
   const void* x;
   const void* w;
@@ -209,7 +212,7 @@ struct NormBwdArgs {
 };
 
 template <typename S, typename W, int G, int NV>
-__global__ __launch_bounds__(kBlockThreads<G>) void norm_bwd_kernel(NormBwdArgs a) {
+__device__ __forceinline__ void norm_bwd_rows(const NormBwdArgs& a, int blocks) {
   constexpr int VEC = Store<S>::VEC, R = kRowsPerBlock<G>;
   __shared__ float red[2][2][16];
   const int r = G == 64 ? threadIdx.x >> 6 : 0, t = G == 64 ? threadIdx.x & 63 : threadIdx.x;
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(kBlockThreads<G>) void norm_bwd_kernel(NormBwdArgs 
     for (int j = 0; j < VEC; ++j) w[i][j] = 1.f, dw[i][j] = 0.f, db[i][j] = 0.f;
     if (e[i] >= 0 && a.w) load_f32<W, VEC>(static_cast<const W*>(a.w), e[i], w[i]);
   }
-  const int64_t step = (int64_t)gridDim.x * R;
+  const int64_t step = (int64_t)blocks * R;
   int64_t row = (int64_t)blockIdx.x * R + r;
   u32x4 xr[NV], gr[NV];
   float mean = 0.f, rstd = 0.f;
@@ -334,6 +337,83 @@ __global__ __launch_bounds__(kBlockThreads<G>) void norm_bwd_kernel(NormBwdArgs 
         part[D + e[i] + j] = db[i][j];
       }
     }
+}
+
+template <typename S, typename W, int G, int NV>
+__global__ __launch_bounds__(kBlockThreads<G>) void norm_bwd_kernel(NormBwdArgs a) {
+  norm_bwd_rows<S, W, G, NV>(a, gridDim.x);
+}
+
+// Few rows: one launch.  dw and db need nothing of the row sums that dx does
+// (mean and rstd are there), so the blocks past the rows' add up a slab of
+// four vectors' columns each: lane l of a wave has vector l % 4 of row l / 4 of
+// its 16; x and grad_y come from the L2 the second time.  Saves the launch of
+// the sums kernel, which is as long as the work here (T = 1024, D = 256 fp32,
+// forward + backward of an eager program: 27 -> 20 us).
+constexpr int kSlab = 4;
+template <typename S, typename W, int G, int NV>
+__global__ __launch_bounds__(kBlockThreads<G>) void norm_bwd_one_kernel(NormBwdArgs a) {
+  if ((int)blockIdx.x < a.row_blocks) {
+    norm_bwd_rows<S, W, G, NV>(a, a.row_blocks);
+    return;
+  }
+  constexpr int VEC = Store<S>::VEC, kWaves = kBlockThreads<G> / 64, kRows = 64 / kSlab, kStep = kRows * kWaves, kUnroll = 8;
+  __shared__ float sums[kWaves][2 * VEC][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int D = a.D, nv = (D + VEC - 1) / VEC, v = (blockIdx.x - a.row_blocks) * kSlab + lane % kSlab;
+  int skip;
+  const int e = v < nv ? vec_start<VEC>(v, D, &skip) : -1;
+  const S* x = static_cast<const S*>(a.x);
+  const S* gy = static_cast<const S*>(a.gy);
+  float dw[VEC] = {}, db[VEC] = {};
+  for (int64_t r0 = wave * kRows + lane / kSlab; r0 < a.T; r0 += kUnroll * kStep) {
+    u32x4 xr[kUnroll], gr[kUnroll];
+    float mean[kUnroll], rstd[kUnroll];
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int64_t r = r0 + k * kStep;
+      xr[k] = gr[k] = {0u, 0u, 0u, 0u};
+      mean[k] = rstd[k] = 0.f;
+      if (e >= 0 && r < a.T) {
+        xr[k] = *reinterpret_cast<const u32x4_a2*>(x + r * D + e);
+        gr[k] = *reinterpret_cast<const u32x4_a2*>(gy + r * D + e);
+        mean[k] = a.mean[r];
+        rstd[k] = a.rstd[r];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {  // rows past the last one add zeros
+      float f[VEC], g[VEC];
+      Store<S>::unpack(xr[k], f);
+      Store<S>::unpack(gr[k], g);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        db[j] += g[j];
+        dw[j] += g[j] * ((f[j] - mean[k]) * rstd[k]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    sums[wave][j][lane] = dw[j];
+    sums[wave][VEC + j][lane] = db[j];
+  }
+  __syncthreads();
+  // thread: one of the slab's 2 x VEC x kSlab sums, over waves and rows in order
+  for (int t = threadIdx.x; t < 2 * VEC * kSlab; t += kBlockThreads<G>) {
+    const int j = t / kSlab, q = t % kSlab;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) s += sums[w][j][r * kSlab + q];
+    const int vq = (blockIdx.x - a.row_blocks) * kSlab + q;
+    if (vq >= nv) continue;
+    int unused;
+    float* o = j < VEC ? a.gw : a.gb;
+    // a column that two vectors hold has the same sum in both
+    if (o) o[vec_start<VEC>(vq, D, &unused) + j % VEC] = s;
+  }
 }
 
 template <typename S, typename W>
@@ -458,9 +538,34 @@ int launch_norm_fwd(const NormFwdArgs& a, hipStream_t st) {
   return check_launch("layer_norm");
 }
 
+// The one-launch form: rows that the second reading finds in the L2, few
+// enough that a slab's walk over them is no longer than a launch or two.
+bool norm_bwd_in_one(int64_t T, int64_t D, size_t es, const NormPlan& p) {
+  return p.G > 0 && T <= 1536 && 2 * T * D * (int64_t)es <= (8 << 20);
+}
+
 template <typename S, typename W>
-int launch_norm_bwd(const NormBwdArgs& a, float* gw, float* gb, hipStream_t st) {
+int launch_norm_bwd(NormBwdArgs a, float* gw, float* gb, hipStream_t st) {
   const NormPlan p = norm_plan(a.D, Store<S>::VEC, true);
+  if (a.part && norm_bwd_in_one(a.T, a.D, sizeof(S), p)) {
+    a.part = nullptr;
+    a.gw = gw, a.gb = gb;
+    const int rows = p.G == 64 ? 4 : 1;
+    const int64_t want = (a.T + rows - 1) / rows, most = (int64_t)device_cu_count() * 8;
+    a.row_blocks = (int)(want < most ? want : most);
+    const int slabs = (a.D + kSlab * Store<S>::VEC - 1) / (kSlab * Store<S>::VEC);
+    const dim3 g(a.row_blocks + slabs), b(p.G == 64 ? 256 : p.G);
+#define MHC_NORM(GG, NN) \
+  if (p.G == GG && p.NV == NN) hipLaunchKernelGGL((norm_bwd_one_kernel<S, W, GG, NN>), g, b, 0, st, a)
+    MHC_NORM(64, 1);
+    MHC_NORM(64, 2);
+    MHC_NORM(256, 1);
+    MHC_NORM(256, 2);
+    MHC_NORM(256, 4);
+    MHC_NORM(512, 4);
+#undef MHC_NORM
+    return check_launch("layer_norm_backward");
+  }
   const int blocks = norm_bwd_blocks(a.T, p), threads = p.G == 64 ? 256 : (p.G ? p.G : 1024);
   const dim3 g(blocks), b(threads);
 #define MHC_NORM(GG, NN) \
@@ -533,7 +638,7 @@ extern "C" int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_d
   if (sums && (!workspace || workspace_bytes < need))
     return set_error(MHC_ERR_INVALID, "layer_norm_backward: workspace too small (%zu < %zu bytes)",
                      workspace ? workspace_bytes : (size_t)0, need);
-  const NormBwdArgs a = {grad_y, x, weight, mean, rstd, grad_x, sums ? static_cast<float*>(workspace) : nullptr, T, D};
+  const NormBwdArgs a = {nullptr, nullptr, 0, grad_y, x, weight, mean, rstd, grad_x, sums ? static_cast<float*>(workspace) : nullptr, T, D};
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (x_dtype == MHC_DTYPE_F32) return launch_norm_bwd<float, float>(a, grad_weight, grad_bias, st);
   if (x_dtype == MHC_DTYPE_BF16)
