@@ -85,8 +85,8 @@ struct KernelCost {
   StepCost dma16, dma32, reg16, reg32;
 };
 constexpr KernelCost kCosts[kKinds] = {
-    {16, 128, 1, {0.8, 0.8}, {0.8, 0.8}, {1.2, 1.2}, {1.2, 1.2}},
-    {64, 128, 1, {0.9, 0.9}, {1.8, 1.8}, {1.2, 1.2}, {2.0, 2.0}},
+    {16, 128, 1, {0.72, 0.4}, {0.72, 0.4}, {1.2, 1.2}, {1.2, 1.2}},
+    {64, 128, 1, {0.72, 0.4}, {1.8, 1.8}, {1.2, 1.2}, {2.0, 2.0}},
     {64, 64, 4, {0.23, 0.6}, {0.6, 0.8}, {0.4, 1.2}, {0.65, 1.4}},
     {128, 128, 2, {0.49, 0.8}, {2.3, 3.2}, {0.8, 1.5}, {2.5, 3.5}},
     {128, 256, 1, {0.87, 0.75}, {4.4, 4.4}, {}, {}},
@@ -95,7 +95,7 @@ constexpr KernelCost kCosts[kKinds] = {
 // lines of k through registers: a wait for memory every step
 constexpr double kColCol = 1.16, kColRegs = 1.7;
 constexpr int kFewRows = 4;
-constexpr double kJoinUs = 5., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
+constexpr double kJoinUs = 8., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
 constexpr double kCuBytesPerUs = 16e3;  // of a tile's results, with every CU at it
 
 struct GemmPlan {
@@ -119,7 +119,9 @@ inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma, in
   const int64_t slots = cus * c.per_cu;
   const int64_t tiles = tiles_of(s, c.bm, c.bn), steps = (s.K * (int64_t)es + 127) / 128 * s.segments;
   // n steps of `blocks` blocks side by side: on a part of the CUs each runs
-  // faster, as the card's power then allows a higher clock
+  // faster, as the card's power then allows a higher clock, and each has more
+  // of the memory's rate (T = 64, D = 4096, F = 11008: 172 whole tiles take 35
+  // us, cut into 256 runs 32 and 5 more for the join)
   const auto side_by_side = [&](double blocks, double n) {
     const double part = blocks < cus ? blocks / cus : 1.;
     const double few = c.per_cu > 1 ? cost.alone : cost.alone + (cost.full - cost.alone) * part;
