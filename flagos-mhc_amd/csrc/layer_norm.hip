@@ -587,10 +587,16 @@ int launch_norm_bwd(NormBwdArgs a, float* gw, float* gb, hipStream_t st) {
   return MHC_OK;
 }
 
+// The loop kernels count a row's elements, and the backward's two sums of
+// each, in 32 bits and steps of 1024.
+constexpr int32_t kMaxRow = (1 << 30) - 512;
+
 bool known_dtype(int32_t d) { return d == MHC_DTYPE_F32 || d == MHC_DTYPE_BF16 || d == MHC_DTYPE_F16; }
 
 int check_norm(const char* who, int64_t T, int64_t D, int32_t x_dtype, int32_t w_dtype) {
   if (T < 0 || D < 1) return set_error(MHC_ERR_INVALID, "%s: T=%lld D=%lld", who, (long long)T, (long long)D);
+  if (D > kMaxRow)
+    return set_error(MHC_ERR_UNSUPPORTED, "%s: rows of %lld elements, above the supported %d", who, (long long)D, kMaxRow);
   if (const int rc = check_tokens(T, who)) return rc;
   if (!known_dtype(x_dtype)) return set_error(MHC_ERR_UNSUPPORTED, "%s: dtype %d not supported", who, x_dtype);
   if (w_dtype != x_dtype && w_dtype != MHC_DTYPE_F32)
@@ -620,7 +626,7 @@ extern "C" int mhc_layer_norm_fwd(const void* x, int32_t x_dtype, const void* we
 }
 
 extern "C" size_t mhc_layer_norm_bwd_workspace_size(int64_t T, int32_t D, int32_t x_dtype) {
-  if (T <= 0 || D < 1 || T > kMaxTokens || !known_dtype(x_dtype)) return 0;
+  if (T <= 0 || D < 1 || D > kMaxRow || T > kMaxTokens || !known_dtype(x_dtype)) return 0;
   return (size_t)norm_bwd_blocks(T, norm_plan(D, vec_of(x_dtype), true)) * 2 * (size_t)D * sizeof(float);
 }
 

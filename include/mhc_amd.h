@@ -318,8 +318,9 @@ int mhc_post_pre_fwd_ex(const void* x, const float* h_res, const void* h_out, co
  *   y = (x - mean) * rstd * weight + bias
  * x, y: (T,D) `x_dtype`, any element alignment; weight, bias: (D,) `w_dtype`
  * (x_dtype or fp32), each may be NULL (1 and 0); mean, rstd: (T,) fp32 for
- * the backward, both or neither.  Sums are fp32.  D >= 1; widths below one
- * 16-byte vector or above 4096 take one block a row, at most 4.19 M rows.
+ * the backward, both or neither.  Sums are fp32.  1 <= D <= 2^30 - 512 (the
+ * loops' 32-bit counts); widths below one 16-byte vector or above 4096 take
+ * one block a row, at most 4.19 M rows.
  */
 int mhc_layer_norm_fwd(const void* x, int32_t x_dtype, const void* weight, const void* bias,
                        int32_t w_dtype, float eps, void* y, float* mean, float* rstd, int64_t T,
