@@ -20,14 +20,19 @@ extern template int ffn_bwd<f16_t>(const FfnBwd&, const FfnDims&, char*, hipStre
 
 namespace {
 
+// The kernels round a size up to a tile's rows, or a step's k, in 32 bits.
+constexpr int64_t kMaxSize = (1ll << 31) - 256;
+
 size_t elem_bytes(int32_t dtype) { return dtype == MHC_DTYPE_F32 ? 4 : 2; }
 
 int check_ffn(const char* who, const FfnDims& d, int32_t dtype, int32_t act) {
   if (d.T < 0 || d.D < 1 || d.F < 1 || d.O < 1)
     return set_error(MHC_ERR_INVALID, "%s: T=%lld D=%d F=%d O=%d", who, (long long)d.T, d.D, d.F, d.O);
-  if (d.T > kMaxTokens) return check_tokens(d.T, who);
   if (dtype != MHC_DTYPE_F32 && dtype != MHC_DTYPE_BF16 && dtype != MHC_DTYPE_F16)
     return set_error(MHC_ERR_UNSUPPORTED, "%s: dtype %d not supported", who, dtype);
+  if (d.T > kMaxSize || d.D > kMaxSize || d.F > kMaxSize || d.O > kMaxSize)
+    return set_error(MHC_ERR_UNSUPPORTED, "%s: T=%lld D=%d F=%d O=%d, above the supported %lld", who, (long long)d.T, d.D,
+                     d.F, d.O, (long long)kMaxSize);
   // tiles are counted in 32 bits
   if (((d.T + 15) / 16) * (((int64_t)(d.F > d.O ? d.F : d.O) + 63) / 64) > 0x3fffffff ||
       (((int64_t)d.F + 63) / 64) * (((int64_t)(d.D > d.O ? d.D : d.O) + 63) / 64) > 0x3fffffff ||

@@ -342,7 +342,7 @@ int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_dtype, const
  *   gate = x w_gate^T, up = x w_up^T, hidden = act(gate) * up,
  *   out = hidden w_down^T
  * x: (T,D), w_gate, w_up: (F,D), w_down: (O,F), out: (T,O), all `dtype`,
- * 16-byte aligned.  Products accumulate in fp32; hidden is rounded to `dtype`
+ * 16-byte aligned; every size at most 2^31 - 256.  Products accumulate in fp32; hidden is rounded to `dtype`
  * between the two products.  The workspace holds hidden, padded copies of
  * operands whose rows are no multiples of 16 bytes, and partial sums.  For the backward, all or none of: gate, up (T,F)
  * fp32 and hidden, (T, F) `dtype` in rows of stride F rounded up to 8

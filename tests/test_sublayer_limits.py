@@ -31,3 +31,27 @@ def test_layer_norm_longest_rows_are_taken():
     # past the size checks: the workspace is what is missed
     assert lib.mhc_layer_norm_bwd(P, P, 1, P, 0, P, P, P, P, P, None, 0, 1, MAX_ROW, None) == -1
     assert b"workspace" in lib.mhc_last_error()
+
+
+@pytest.mark.parametrize("which", ["T", "D", "F", "O"])
+@pytest.mark.parametrize("size", [(1 << 31) - 255, (1 << 31) - 1])
+def test_gated_ffn_sizes_that_wrap_are_refused(which, size):
+    """A size is rounded up to a tile's 256 rows in 32 bits."""
+    assert size + 255 > (1 << 31) - 1
+    lib = _lib.load()
+    n = {"T": 1, "D": 1, "F": 1, "O": 1, which: size}
+    dims = [n[k] for k in "TDFO"]
+    assert lib.mhc_gated_ffn_fwd(P, P, P, P, 1, 0, P, None, None, None, P, 1 << 60, *dims, None) == -2
+    assert b"above the supported" in lib.mhc_last_error()
+    assert lib.mhc_gated_ffn_bwd(P, P, P, P, P, P, P, P, 1, 0, P, P, P, P, P, 1 << 60, *dims, None) == -2
+    assert b"above the supported" in lib.mhc_last_error()
+    assert lib.mhc_gated_ffn_fwd_workspace_size(*dims, 1) == lib.mhc_gated_ffn_bwd_workspace_size(*dims, 1) == 0
+
+
+def test_gated_ffn_largest_sizes_are_taken():
+    lib = _lib.load()
+    size = (1 << 31) - 256
+    assert size + 255 == (1 << 31) - 1
+    # past the size checks: the workspace is what is missed
+    assert lib.mhc_gated_ffn_fwd(P, P, P, P, 1, 0, P, None, None, None, None, 0, 1, size, 1, 1, None) == -1
+    assert b"workspace" in lib.mhc_last_error()
