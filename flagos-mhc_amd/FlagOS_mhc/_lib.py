@@ -177,11 +177,21 @@ def pre_fwd_size_code(x_code: int, phi_code: int, addresses: int) -> int:
 
 
 def require_device(what: str, *tensors) -> None:
+    """Every tensor given is on one HIP device (kernels take addresses: one of
+    another GPU would be read there)."""
+    first = -1
     for t in tensors:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        if not t.is_cuda:
             raise RuntimeError(
                 f"{what}: expected tensors on a HIP (cuda) device, got {t.device}; "
                 "the MI355X operators have no CPU path (use the *_ref functions on CPU)")
+        index = t.get_device()
+        if index != first:
+            if first >= 0:
+                raise ValueError(f"{what}: tensors on cuda:{first} and {t.device}, expected one device")
+            first = index
 
 
 def dtype_code(what: str, dt: torch.dtype) -> int:

@@ -28,8 +28,7 @@ def _apply(what, x, p, seed, offset, state):
     p = float(p)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"{what}: p={p} is no probability")
-    if state is not None and (state.dtype != torch.int64 or state.numel() != 2 or state.device != x.device
-                              or not state.is_contiguous()):
+    if state is not None and (state.dtype != torch.int64 or state.numel() != 2 or not state.is_contiguous()):
         raise ValueError(f"{what}: state must be a contiguous int64 tensor (seed, offset) on {x.device}")
     xf = x.contiguous()
     y = torch.empty_like(xf)

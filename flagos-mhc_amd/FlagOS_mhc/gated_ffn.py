@@ -50,8 +50,6 @@ def _check(what, x, w_gate, w_up, w_down, activation):
     for name, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         if w.dtype != x.dtype:
             raise ValueError(f"{what}: {name} is {w.dtype}, x {x.dtype}")
-        if w.get_device() != x.get_device():
-            raise ValueError(f"{what}: {name} is on {w.device}, x on {x.device}")
     return math.prod(x.shape[:-1]), D, F, O, code, ACTIVATIONS[activation]
 
 

@@ -33,8 +33,6 @@ def _param(what, name, p, x, D):
     """weight or bias as the kernel takes it: (D,), x's dtype or fp32."""
     if p.numel() != D:
         raise ValueError(f"{what}: {name} has {p.numel()} elements, x's rows {D}")
-    if p.get_device() != x.get_device():
-        raise ValueError(f"{what}: {name} is on {p.device}, x on {x.device}")
     dt = p.dtype
     if (dt is _F32 or dt is x.dtype) and p.is_contiguous():
         return p
