@@ -122,8 +122,21 @@ __device__ __forceinline__ floatx4 load4(const float* row, int64_t n, int64_t le
   return v;
 }
 
+// c with zeros from column `len` on; c[0] is column n.
+__device__ __forceinline__ floatx4 zero_past(floatx4 c, int64_t n, int64_t len) {
+  if (n + 4 > len) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i >= len) c[i] = 0.f;
+  }
+  return c;
+}
+
 // Row m, columns n .. n + 3 of the product (c; gated: c0 = g, c1 = u); z is
-// the product of the batch.
+// the product of the batch.  The gated forms' results are operands of the next
+// product, which reads whole chunks of k: their columns from N on are set to
+// zero, as the sums there are NaN in rows with a NaN or an infinity (times the
+// zeros that stand for operands out of range).
 template <typename S, int EPI>
 __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, int64_t m, int n, const floatx4& c0, const floatx4& c1) {
   if (m >= a.M || n >= a.ldo) return;
@@ -134,7 +147,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, int64_t m, in
     const float g[4] = {c0[0], c0[1], c0[2], c0[3]};
     float v[4], d[4];
     act_all<S, 4>(a.act, g, v, d);
-    store4<S>(o0, n, a.ldo, floatx4{v[0] * c1[0], v[1] * c1[1], v[2] * c1[2], v[3] * c1[3]});
+    store4<S>(o0, n, a.ldo, zero_past(floatx4{v[0] * c1[0], v[1] * c1[1], v[2] * c1[2], v[3] * c1[3]}, n, a.N));
     if (a.gate) {
       store4<float, true>(a.gate + m * a.N, n, a.N, c0);
       store4<float, true>(a.up + m * a.N, n, a.N, c1);
@@ -150,8 +163,8 @@ __device__ __forceinline__ void epilogue(const GemmArgs& a, int z, int64_t m, in
       dg[i] = c0[i] * u[i] * d[i];
       du[i] = c0[i] * v[i];
     }
-    store4<S>(o0, n, a.ldo, dg);
-    store4<S>(static_cast<S*>(a.out1) + m * a.ldo, n, a.ldo, du);
+    store4<S>(o0, n, a.ldo, zero_past(dg, n, a.N));
+    store4<S>(static_cast<S*>(a.out1) + m * a.ldo, n, a.ldo, zero_past(du, n, a.N));
   }
 }
 
