@@ -16,6 +16,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_NAME = "libmhc_amd.so"
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), _LIB_NAME)
@@ -192,6 +193,20 @@ def require_device(what: str, *tensors) -> None:
             if first >= 0:
                 raise ValueError(f"{what}: tensors on cuda:{first} and {t.device}, expected one device")
             first = index
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether a tensor carries a forward-mode derivative (which requires_grad
+    does not tell; the level is looked at first, as no program that runs none
+    should pay for asking)."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def needs_autograd(*tensors) -> bool:
+    """Whether an operator has to go through its autograd.Function: a gradient
+    may be taken, or there is a tangent, which the Function refuses."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or has_tangent(*tensors)
 
 
 def dtype_code(what: str, dt: torch.dtype) -> int:

@@ -149,6 +149,6 @@ class GatedFfnFn(torch.autograd.Function):
 def gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu"):
     """Autograd-aware gated_ffn: out.  Without gradients to take, nothing is
     saved."""
-    if not (torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down))):
+    if not _lib.needs_autograd(x, w_gate, w_up, w_down):
         return gated_ffn(x, w_gate, w_up, w_down, activation)["out"]
     return GatedFfnFn.apply(x, w_gate, w_up, w_down, activation)

@@ -133,6 +133,6 @@ class LayerNormFn(torch.autograd.Function):
 def layer_norm_fn(x, weight=None, bias=None, eps=1e-5):
     """Autograd-aware layer_norm: y.  Without gradients to take, nothing is
     saved."""
-    if not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias))):
+    if not _lib.needs_autograd(x, weight, bias):
         return layer_norm(x, weight, bias, eps)["y"]
     return LayerNormFn.apply(x, weight, bias, eps)

@@ -43,9 +43,11 @@ needs; they are marked non-differentiable (likewise for the fused op).
 the return conventions of ``mhc_post_fn`` / ``mhc_pre_clamp_sinkhorn_fn``
 (src/autograd.py:14-87) and ``mhc_post_pre_clamp_sinkhorn_fn``;
 ``layer_norm_op``, ``gated_ffn_op``, ``dropout_op`` and ``mhc_ffn_layer_op``
-those of the same functions of ``FlagOS_mhc.sublayer``.  The kernels allocate nothing outside torch's
-allocator and call no host synchronisation, so they can be captured in a
-HIP graph (``torch.cuda.graph``) after one eager warm-up call.
+those of the same functions of ``FlagOS_mhc.sublayer``.  They refuse inputs
+with forward-mode derivatives, which the bare ops would drop without a word
+where no input requires a gradient.  The kernels allocate nothing outside
+torch's allocator and call no host synchronisation, so they can be captured in
+a HIP graph (``torch.cuda.graph``) after one eager warm-up call.
 """
 
 from __future__ import annotations
@@ -56,6 +58,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
+from . import _lib
 from .dropout import dropout
 from .gated_ffn import gated_ffn, gated_ffn_backward, hidden_width
 from .layer_norm import layer_norm, layer_norm_backward
@@ -384,8 +387,15 @@ _drop.register_autograd(_drop_grad, setup_context=_drop_setup)
 
 # ---- autograd-aware entry points ---------------------------------------------
 
+def _refuse_tangents(what, *tensors):
+    # (a traced call has no tangents to look at)
+    if not torch.compiler.is_compiling() and _lib.has_tangent(*tensors):
+        raise NotImplementedError(f"{what}: forward-mode derivatives are not implemented")
+
+
 def mhc_post_op(x, h_res, h_out, h_post):
     """``mhc_post`` through the registered op (differentiable, compilable)."""
+    _refuse_tangents("mhc_post", x, h_res, h_out, h_post)
     return torch.ops.flagos_mhc.mhc_post(x, h_res, h_out, h_post)
 
 
@@ -394,6 +404,7 @@ def mhc_pre_clamp_sinkhorn_op(x, phi, alpha, base, norm_eps=1e-6, hc_eps=1e-6, c
     """``mhc_pre_clamp_sinkhorn`` through the registered op: (y, post_out,
     comb_frag), differentiable in x, phi, alpha and base; ``compensated``
     selects the backward's compensated T-reductions."""
+    _refuse_tangents("mhc_pre_clamp_sinkhorn", x, phi, alpha, base)
     y, post_out, comb, _, _, _ = torch.ops.flagos_mhc.mhc_pre_clamp_sinkhorn(
         x, phi, alpha, base, float(norm_eps), float(hc_eps), float(clamp_min), float(clamp_max),
         int(iter_times), bool(compensated))
@@ -405,6 +416,7 @@ def mhc_post_pre_clamp_sinkhorn_op(x, h_res, h_out, h_post, phi, alpha, base, no
                                    compensated=False):
     """The fused mhc_post + mhc_pre_clamp_sinkhorn through the registered op:
     (x_next, y, post_out, comb_frag), differentiable in every tensor input."""
+    _refuse_tangents("mhc_post_pre_clamp_sinkhorn", x, h_res, h_out, h_post, phi, alpha, base)
     x_next, y, post_out, comb, _, _, _ = torch.ops.flagos_mhc.mhc_post_pre_clamp_sinkhorn(
         x, h_res, h_out, h_post, phi, alpha, base, float(norm_eps), float(hc_eps), float(clamp_min),
         float(clamp_max), int(iter_times), bool(compensated))
@@ -413,11 +425,13 @@ def mhc_post_pre_clamp_sinkhorn_op(x, h_res, h_out, h_post, phi, alpha, base, no
 
 def layer_norm_op(x, weight=None, bias=None, eps=1e-5):
     """``layer_norm_fn`` through the registered op."""
+    _refuse_tangents("layer_norm", x, weight, bias)
     return torch.ops.flagos_mhc.layer_norm(x, weight, bias, float(eps))[0]
 
 
 def gated_ffn_op(x, w_gate, w_up, w_down, activation="silu"):
     """``gated_ffn_fn`` through the registered op."""
+    _refuse_tangents("gated_ffn", x, w_gate, w_up, w_down)
     save = torch.is_grad_enabled() and any(t.requires_grad for t in (x, w_gate, w_up, w_down))
     return torch.ops.flagos_mhc.gated_ffn(x, w_gate, w_up, w_down, activation, save)[0]
 
@@ -428,6 +442,7 @@ def _signed64(v):
 
 def dropout_op(x, p, seed=0, offset=0, state=None):
     """``dropout_fn`` through the registered op."""
+    _refuse_tangents("dropout", x)
     return torch.ops.flagos_mhc.dropout(x, float(p), _signed64(seed), _signed64(offset), state)
 
 

@@ -1,0 +1,75 @@
+"""What the autograd-aware functions do with derivatives that they do not
+have: forward-mode ones are refused, never dropped.  No GPU: the kernel calls
+are replaced by ones that compute nothing."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from FlagOS_mhc import _lib, library as L, sublayer as S
+
+
+class _NoKernels:
+    def __getattr__(self, name):
+        return lambda *a: 0
+
+
+@pytest.fixture(autouse=True)
+def no_kernels(monkeypatch):
+    monkeypatch.setattr(_lib, "require_device", lambda *a: None)
+    monkeypatch.setattr(_lib, "call", lambda *a: None)
+    monkeypatch.setattr(_lib, "load", lambda: _NoKernels())
+    monkeypatch.setattr(_lib, "workspace", lambda *a: (torch.zeros(1, dtype=torch.uint8), 1))
+
+
+X, W, V = torch.ones(4, 8), torch.ones(6, 8), torch.ones(8, 6)
+VECTOR = torch.ones(8)
+
+# the operator as a function of one input, and that input
+INPUTS = {
+    "layer_norm_fn x": (lambda t: S.layer_norm_fn(t), X),
+    "layer_norm_fn weight": (lambda t: S.layer_norm_fn(X, t), VECTOR),
+    "layer_norm_fn bias": (lambda t: S.layer_norm_fn(X, None, t), VECTOR),
+    "gated_ffn_fn x": (lambda t: S.gated_ffn_fn(t, W, W, V), X),
+    "gated_ffn_fn w_gate": (lambda t: S.gated_ffn_fn(X, t, W, V), W),
+    "gated_ffn_fn w_up": (lambda t: S.gated_ffn_fn(X, W, t, V), W),
+    "gated_ffn_fn w_down": (lambda t: S.gated_ffn_fn(X, W, W, t), V),
+    "dropout_fn": (lambda t: S.dropout_fn(t, 0.5), X),
+    "layer_norm_op x": (lambda t: L.layer_norm_op(t), X),
+    "layer_norm_op bias": (lambda t: L.layer_norm_op(X, None, t), VECTOR),
+    "gated_ffn_op x": (lambda t: L.gated_ffn_op(t, W, W, V), X),
+    "gated_ffn_op w_down": (lambda t: L.gated_ffn_op(X, W, W, t), V),
+    "dropout_op": (lambda t: L.dropout_op(t, 0.5), X),
+    "mhc_post_op": (lambda t: L.mhc_post_op(t, X, X, X), X),
+    "mhc_pre_clamp_sinkhorn_op": (lambda t: L.mhc_pre_clamp_sinkhorn_op(X, t, X, X), X),
+    "mhc_post_pre_clamp_sinkhorn_op": (lambda t: L.mhc_post_pre_clamp_sinkhorn_op(X, X, X, t, X, X, X), X),
+}
+
+
+@pytest.mark.parametrize("name", INPUTS)
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused(name, grad_mode):
+    fn, t = INPUTS[name]
+    with torch.set_grad_enabled(grad_mode), fwAD.dual_level():
+        dual = fwAD.make_dual(t, torch.ones_like(t))
+        with pytest.raises(NotImplementedError, match="forward"):
+            fn(dual)
+
+
+@pytest.mark.parametrize("name", INPUTS)
+def test_jvp_transform_is_refused(name):
+    fn, t = INPUTS[name]
+    with pytest.raises((NotImplementedError, RuntimeError)):
+        torch.func.jvp(fn, (t,), (torch.ones_like(t),))
+
+
+@pytest.mark.parametrize("fn", [lambda t: S.layer_norm_fn(t), lambda t: S.gated_ffn_fn(t, W, W, V),
+                                lambda t: L.layer_norm_op(t), lambda t: L.gated_ffn_op(t, W, W, V),
+                                lambda t: L.dropout_op(t, 0.5)])
+def test_tensors_without_a_tangent_pass(fn):
+    """.. at a level where others have one."""
+    with fwAD.dual_level():
+        fwAD.make_dual(X, X)
+        assert fn(X).shape == X.shape and not fn(X).requires_grad
