@@ -209,6 +209,31 @@ def needs_autograd(*tensors) -> bool:
     return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or has_tangent(*tensors)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Hands on the first n of its tensors; its own backward is an error."""
+
+    @staticmethod
+    def forward(ctx, what, n, *tensors):
+        ctx.what = what
+        return tuple(t.view_as(t) for t in tensors[:n])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what}: second derivatives are not implemented")
+
+
+def first_order(what: str, grads, *inputs):
+    """grads (None among them), computed from `inputs` by kernels: where a graph
+    of the backward is asked for (create_graph), one that fails when it is
+    differentiated, instead of none.  (torch's once_differentiable leaves it out
+    where the output's gradient needs none, though the saved inputs do.)"""
+    if not torch.is_grad_enabled():
+        return grads
+    have = [g for g in grads if g is not None]
+    wrapped = iter(_NoSecondDerivative.apply(what, len(have), *have, *inputs))
+    return tuple(None if g is None else next(wrapped) for g in grads)
+
+
 def dtype_code(what: str, dt: torch.dtype) -> int:
     try:
         return DTYPE_CODE[dt]

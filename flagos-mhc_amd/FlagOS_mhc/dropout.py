@@ -81,7 +81,9 @@ class DropoutFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_y):
-        return dropout_backward(grad_y, *ctx.args, ctx.state), None, None, None, None
+        # linear: where a graph of the backward is asked for, the gradient is dropout_fn of grad_y
+        fn = dropout_fn if torch.is_grad_enabled() else dropout_backward
+        return fn(grad_y, *ctx.args, ctx.state), None, None, None, None
 
 
 def dropout_fn(x, p, seed=0, offset=0, state=None):

@@ -142,8 +142,9 @@ class GatedFfnFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_out):
-        return (*gated_ffn_backward(grad_out, *ctx.saved_tensors, activation=ctx.activation,
-                                    need_weights=any(ctx.needs_input_grad[1:4])), None)
+        grads = gated_ffn_backward(grad_out, *ctx.saved_tensors, activation=ctx.activation,
+                                   need_weights=any(ctx.needs_input_grad[1:4]))
+        return (*_lib.first_order("gated_ffn", grads, grad_out, *ctx.saved_tensors[:4]), None)
 
 
 def gated_ffn_fn(x, w_gate, w_up, w_down, activation="silu"):

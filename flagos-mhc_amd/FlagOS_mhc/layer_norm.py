@@ -127,7 +127,7 @@ class LayerNormFn(torch.autograd.Function):
         need = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         gx, gw, gb = layer_norm_backward(grad_y, x, weight, mean, rstd, need_params=need)
         gw, gb = (g.reshape(d[0]).to(d[1]) if d is not None and need else None for g, d in zip((gw, gb), ctx.dtypes))
-        return gx, gw, gb, None
+        return (*_lib.first_order("layer_norm", (gx, gw, gb), grad_y, x, weight), None)
 
 
 def layer_norm_fn(x, weight=None, bias=None, eps=1e-5):

@@ -1,8 +1,10 @@
 """What the autograd-aware functions do with derivatives that they do not
-have: forward-mode ones are refused, never dropped.  No GPU: the kernel calls
-are replaced by ones that compute nothing."""
+have: forward-mode ones and second ones are refused, never dropped.  No GPU:
+the kernel calls are replaced by ones that compute nothing."""
 
 from __future__ import annotations
+
+import sys
 
 import pytest
 import torch
@@ -73,3 +75,40 @@ def test_tensors_without_a_tangent_pass(fn):
     with fwAD.dual_level():
         fwAD.make_dual(X, X)
         assert fn(X).shape == X.shape and not fn(X).requires_grad
+
+
+# each differentiable input of the operators whose second derivative depends on it
+SECOND = [n for n in INPUTS if n.startswith(("layer_norm", "gated_ffn")) and "bias" not in n]
+
+
+@pytest.mark.parametrize("name", SECOND)
+def test_second_derivatives_are_refused(name):
+    """.. also where the output's gradient is a constant, as after sum(), and
+    beside another term of the loss."""
+    fn, t = INPUTS[name]
+    t = t.clone().requires_grad_(True)
+    for grad_out in (None, torch.ones_like(fn(t)).requires_grad_(True)):
+        y = fn(t)
+        g, = torch.autograd.grad(y.sum() if grad_out is None else y, t, grad_out, create_graph=True)
+        assert g.shape == t.shape and g.requires_grad
+        with pytest.raises(RuntimeError, match="second derivatives|no autograd formula|autograd formula"):
+            (g.sum() + t.sum()).backward()
+    # first derivatives, with a graph of the backward or without
+    for create in (True, False):
+        assert torch.autograd.grad(fn(t).sum(), t, create_graph=create)[0].requires_grad == create
+
+
+@pytest.mark.parametrize("fn", [S.dropout_fn, L.dropout_op])
+def test_dropout_is_differentiable_twice(fn, monkeypatch):
+    """Linear in x: the gradient of its gradient with respect to grad_y is the mask and factor again."""
+    # (as the kernel: no graph of its own)
+    apply = torch.no_grad()(lambda x, p, seed=0, offset=0, state=None: S.dropout_ref(x, p, seed, offset))
+    for module in ("dropout", "library"):
+        monkeypatch.setattr(sys.modules[f"FlagOS_mhc.{module}"], "dropout", apply)
+    monkeypatch.setattr(sys.modules["FlagOS_mhc.dropout"], "dropout_backward", apply)
+    x, c = torch.ones(5, 9, requires_grad=True), torch.full((5, 9), 2.0, requires_grad=True)
+    g, = torch.autograd.grad((fn(x, 0.5, 3, 4) * c).sum(), x, create_graph=True)
+    mask = S.dropout_ref(torch.ones(5, 9), 0.5, 3, 4)
+    assert torch.equal(g.detach(), 2 * mask)
+    gc, = torch.autograd.grad(g.sum(), c)
+    assert torch.equal(gc, mask) and 0 < int((mask == 0).sum()) < mask.numel()
