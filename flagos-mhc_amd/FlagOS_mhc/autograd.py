@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib
 from .mhc_post import mhc_post
 from .mhc_post_backward import mhc_post_backward, mhc_post_backward_sum, post_backward_sum_fused
 from .mhc_post_pre import mhc_post_pre_clamp_sinkhorn
@@ -22,7 +23,8 @@ class MhcPostFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_y):
         x, h_res, h_out, h_post = ctx.saved_tensors
-        return mhc_post_backward(grad_y.contiguous(), x, h_res, h_out, h_post)
+        grads = mhc_post_backward(grad_y.contiguous(), x, h_res, h_out, h_post)
+        return _lib.first_order("mhc_post", grads, grad_y, x, h_res, h_out, h_post)
 
 
 def mhc_post_fn(x, h_res, h_out, h_post):
@@ -65,8 +67,10 @@ class MhcPreClampSinkhornFn(torch.autograd.Function):
             grad_y.contiguous(), grad_post_out.contiguous(), grad_comb_frag.contiguous(),
             norm_eps=ctx.norm_eps, hc_eps=ctx.hc_eps, clamp_min=ctx.clamp_min,
             clamp_max=ctx.clamp_max, iter_times=ctx.iter_times, compensated=ctx.compensated)
+        grads = _lib.first_order("mhc_pre_clamp_sinkhorn", (gx, gphi, galpha, gbase), grad_y, grad_post_out,
+                                 grad_comb_frag, x, phi, alpha, base)
         # (x, phi, alpha, base, norm_eps, hc_eps, clamp_min, clamp_max, iter_times, compensated)
-        return gx, gphi, galpha, gbase, None, None, None, None, None, None
+        return (*grads, None, None, None, None, None, None)
 
 
 def mhc_pre_clamp_sinkhorn_fn(
@@ -127,7 +131,10 @@ class MhcPostPreClampSinkhornFn(torch.autograd.Function):
             gx, ghres, ghout, ghpost = mhc_post_backward_sum(grad_x_next, g, x, h_res, h_out, h_post)
         else:
             gx, ghres, ghout, ghpost = mhc_post_backward(g, x, h_res, h_out, h_post)
-        return gx, ghres, ghout, ghpost, gphi, galpha, gbase, None, None, None, None, None, None
+        grads = _lib.first_order("mhc_post_pre_clamp_sinkhorn", (gx, ghres, ghout, ghpost, gphi, galpha, gbase),
+                                 grad_x_next, grad_y, grad_post_out, grad_comb_frag, x, h_res, h_out, h_post, phi,
+                                 alpha, base)
+        return (*grads, None, None, None, None, None, None)
 
 
 def mhc_post_pre_clamp_sinkhorn_fn(

@@ -112,3 +112,42 @@ def test_dropout_is_differentiable_twice(fn, monkeypatch):
     assert torch.equal(g.detach(), 2 * mask)
     gc, = torch.autograd.grad(g.sum(), c)
     assert torch.equal(gc, mask) and 0 < int((mask == 0).sum()) < mask.numel()
+
+
+# ---- the mHC functions: N = 2 streams of width 4 ---------------------------------
+
+T, N, D = 3, 2, 4
+M = N * (N + 2)
+STREAMS, H_RES, H_OUT, H_POST = torch.ones(T, N, D), torch.ones(T, N, N), torch.ones(T, D), torch.ones(T, N)
+PHI, ALPHA, BASE = torch.ones(M, N * D), torch.ones(3), torch.ones(M)
+PRE = {"y": H_OUT, "post_out": H_POST, "comb_frag": H_RES, "inv_rms": torch.ones(T), "mixes": torch.ones(T, M),
+       "pre": torch.ones(T, N)}
+
+
+@pytest.mark.parametrize("fn,inputs", [
+    ("mhc_post_fn", (STREAMS, H_RES, H_OUT, H_POST)),
+    ("mhc_pre_clamp_sinkhorn_fn", (STREAMS, PHI, ALPHA, BASE)),
+    ("mhc_post_pre_clamp_sinkhorn_fn", (STREAMS, H_RES, H_OUT, H_POST, PHI, ALPHA, BASE))])
+@pytest.mark.parametrize("summed", [True, False])
+def test_mhc_second_derivatives_are_refused(fn, inputs, summed, monkeypatch):
+    """.. with respect to every input; the operators are replaced by ones that
+    return tensors of their results' shapes."""
+    a = sys.modules["FlagOS_mhc.autograd"]
+    like = lambda *ts: tuple(torch.zeros_like(t) for t in ts)
+    out = lambda: {k: v.clone() for k, v in PRE.items()}
+    monkeypatch.setattr(a, "mhc_post", lambda x, *r: torch.zeros_like(x))
+    monkeypatch.setattr(a, "mhc_post_backward", lambda g, x, *r: like(x, *r))
+    monkeypatch.setattr(a, "mhc_post_backward_sum", lambda g, g2, x, *r: like(x, *r))
+    monkeypatch.setattr(a, "post_backward_sum_fused", lambda *s: summed)
+    monkeypatch.setattr(a, "_pre_forward", lambda *r, **k: out())
+    monkeypatch.setattr(a, "_pre_backward", lambda x, phi, alpha, base, *r, **k: like(x, phi, alpha, base))
+    monkeypatch.setattr(a, "mhc_pre_clamp_sinkhorn_backward", lambda x, phi, alpha, base, *r, **k: like(x, phi, alpha, base))
+    monkeypatch.setattr(a, "mhc_post_pre_clamp_sinkhorn", lambda x, *r, **k: (torch.zeros_like(x), out()))
+    leaves = [t.clone().requires_grad_(True) for t in inputs]
+    run = lambda: (lambda y: y if isinstance(y, torch.Tensor) else sum(t.sum() for t in y))(getattr(a, fn)(*leaves))
+    for i, t in enumerate(leaves):
+        g, = torch.autograd.grad(run().sum(), t, create_graph=True)
+        assert g.shape == t.shape and g.requires_grad
+        with pytest.raises(RuntimeError, match="second derivatives"):
+            (g.sum() + t.sum()).backward()
+        assert not torch.autograd.grad(run().sum(), t)[0].requires_grad
