@@ -27,12 +27,13 @@ HIP-graph capture records their kernels on the current stream):
 and the operators between pre and post (``FlagOS_mhc.sublayer``):
 
     torch.ops.flagos_mhc.layer_norm(x, weight, bias, eps) -> (y, mean, rstd)
-    torch.ops.flagos_mhc.layer_norm_backward(grad_y, x, weight, mean, rstd)
-        -> (grad_x, grad_weight, grad_bias)
+    torch.ops.flagos_mhc.layer_norm_backward(grad_y, x, weight, mean, rstd, need_params)
+        -> (grad_x, grad_weight, grad_bias); the last two are empty with need_params=False
     torch.ops.flagos_mhc.gated_ffn(x, w_gate, w_up, w_down, activation, save)
         -> (out, gate, up, hidden); the last three are empty with save=False
     torch.ops.flagos_mhc.gated_ffn_backward(grad_out, x, w_gate, w_up, w_down,
-        gate, up, hidden, activation) -> (grad_x, grad_w_gate, grad_w_up, grad_w_down)
+        gate, up, hidden, activation, need_weights)
+        -> (grad_x, grad_w_gate, grad_w_up, grad_w_down); the last three are empty with need_weights=False
     torch.ops.flagos_mhc.dropout(x, p, seed, offset, state) -> y, with seed and
         offset as signed 64-bit integers; its backward is the op on the gradient
 
@@ -280,14 +281,17 @@ def _norm_fake(x, weight, bias, eps):
 
 
 @torch.library.custom_op(f"{NAMESPACE}::layer_norm_backward", mutates_args=())
-def _norm_bwd(grad_y: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor,
-              rstd: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
-    return layer_norm_backward(grad_y, x, weight, mean, rstd)
+def _norm_bwd(grad_y: Tensor, x: Tensor, weight: Optional[Tensor], mean: Tensor, rstd: Tensor,
+              need_params: bool = True) -> Tuple[Tensor, Tensor, Tensor]:
+    gx, gw, gb = layer_norm_backward(grad_y, x, weight, mean, rstd, need_params)
+    if not need_params:
+        gw, gb = (x.new_empty((0,), dtype=torch.float32) for _ in range(2))
+    return gx, gw, gb
 
 
 @_norm_bwd.register_fake
-def _norm_bwd_fake(grad_y, x, weight, mean, rstd):
-    D = x.shape[-1]
+def _norm_bwd_fake(grad_y, x, weight, mean, rstd, need_params=True):
+    D = x.shape[-1] if need_params else 0
     return (x.new_empty(x.shape), x.new_empty((D,), dtype=torch.float32),
             x.new_empty((D,), dtype=torch.float32))
 
@@ -302,8 +306,9 @@ def _norm_setup(ctx, inputs, output):
 
 def _norm_grad(ctx, grad_y, _g_mean, _g_rstd):
     x, weight, mean, rstd = ctx.saved_tensors
-    gx, *gp = torch.ops.flagos_mhc.layer_norm_backward(grad_y.contiguous(), x, weight, mean, rstd)
-    gw, gb = (None if d is None else g.reshape(d[0]).to(d[1]) for g, d in zip(gp, ctx.params))
+    need = any(ctx.needs_input_grad[1:3])
+    gx, *gp = torch.ops.flagos_mhc.layer_norm_backward(grad_y.contiguous(), x, weight, mean, rstd, need)
+    gw, gb = (g.reshape(d[0]).to(d[1]) if need and d is not None else None for g, d in zip(gp, ctx.params))
     return gx, gw, gb, None
 
 
@@ -331,13 +336,15 @@ def _ffn_fake(x, w_gate, w_up, w_down, activation="silu", save=True):
 
 @torch.library.custom_op(f"{NAMESPACE}::gated_ffn_backward", mutates_args=())
 def _ffn_bwd(grad_out: Tensor, x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, gate: Tensor,
-             up: Tensor, hidden: Tensor, activation: str = "silu") -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    return gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation)
+             up: Tensor, hidden: Tensor, activation: str = "silu",
+             need_weights: bool = True) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    grads = gated_ffn_backward(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation, need_weights)
+    return grads if need_weights else (grads[0], *(x.new_empty((0,)) for _ in range(3)))
 
 
 @_ffn_bwd.register_fake
-def _ffn_bwd_fake(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation="silu"):
-    return tuple(t.new_empty(t.shape) for t in (x, w_gate, w_up, w_down))
+def _ffn_bwd_fake(grad_out, x, w_gate, w_up, w_down, gate, up, hidden, activation="silu", need_weights=True):
+    return (x.new_empty(x.shape), *(t.new_empty(t.shape if need_weights else (0,)) for t in (w_gate, w_up, w_down)))
 
 
 def _ffn_setup(ctx, inputs, output):
@@ -352,8 +359,9 @@ def _ffn_setup(ctx, inputs, output):
 def _ffn_grad(ctx, grad_out, _g_gate, _g_up, _g_hidden):
     if not ctx.saved:
         raise RuntimeError("gated_ffn: the forward ran with save=False")
-    return (*torch.ops.flagos_mhc.gated_ffn_backward(grad_out.contiguous(), *ctx.saved_tensors, ctx.activation),
-            None, None)
+    need = any(ctx.needs_input_grad[1:4])
+    gx, *gw = torch.ops.flagos_mhc.gated_ffn_backward(grad_out.contiguous(), *ctx.saved_tensors, ctx.activation, need)
+    return (gx, *(gw if need else (None,) * 3), None, None)
 
 
 _ffn.register_autograd(_ffn_grad, setup_context=_ffn_setup)
