@@ -459,6 +459,6 @@ def mhc_ffn_layer_op(x, phi, alpha, base, norm_weight, norm_bias, w_gate, w_up, 
     """``mhc_ffn_layer_fn`` (``FlagOS_mhc.sublayer``) through the registered ops."""
     y, post, comb = mhc_pre_clamp_sinkhorn_op(x, phi, alpha, base, **mhc)
     h = gated_ffn_op(layer_norm_op(y, norm_weight, norm_bias, ln_eps), w_gate, w_up, w_down, activation)
-    if dropout_p > 0.0:
+    if dropout_p != 0.0:
         h = dropout_op(h, dropout_p, seed, offset, state)
     return mhc_post_op(x, comb, h, post)

@@ -35,6 +35,6 @@ def mhc_ffn_layer_fn(x, phi, alpha, base, norm_weight, norm_bias, w_gate, w_up, 
     y, post, comb = mhc_pre_clamp_sinkhorn_fn(x, phi, alpha, base, **mhc)
     h = layer_norm_fn(y, norm_weight, norm_bias, ln_eps)
     h = gated_ffn_fn(h, w_gate, w_up, w_down, activation)
-    if dropout_p > 0.0:
+    if dropout_p != 0.0:
         h = dropout_fn(h, dropout_p, seed, offset, state)
     return mhc_post_fn(x, comb, h, post)
