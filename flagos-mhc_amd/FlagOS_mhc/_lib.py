@@ -70,6 +70,7 @@ _SIGNATURES = {
     "mhc_layer_norm_bwd": (_c.c_int, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                       _i64, _i32, _vp]),
     "mhc_gated_ffn_fwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "mhc_gated_ffn_fwd_save_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "mhc_gated_ffn_fwd": (_c.c_int, [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _sz,
                                      _i64, _i32, _i32, _i32, _vp]),
     "mhc_gated_ffn_bwd_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),

@@ -71,7 +71,8 @@ def gated_ffn(x, w_gate, w_up, w_down, activation="silu", need_backward=False):
         xf = _aligned(x, (T, D), x.dtype)
         wg, wu = _aligned(w_gate, (F, D), x.dtype), _aligned(w_up, (F, D), x.dtype)
         wd = _aligned(w_down, (O, F), x.dtype)
-        ws, ws_bytes = _lib.workspace("mhc_gated_ffn_fwd_workspace_size", dev, T, D, F, O, code)
+        query = "mhc_gated_ffn_fwd_save_workspace_size" if need_backward else "mhc_gated_ffn_fwd_workspace_size"
+        ws, ws_bytes = _lib.workspace(query, dev, T, D, F, O, code)
         _lib.call(what, _lib.load().mhc_gated_ffn_fwd, x.get_device(), xf.data_ptr(), wg.data_ptr(), wu.data_ptr(),
                   wd.data_ptr(), code, act, out.data_ptr(), _lib.ptr(gate), _lib.ptr(up), _lib.ptr(hidden),
                   ws.data_ptr(), ws_bytes, T, D, F, O)

@@ -63,6 +63,11 @@ extern "C" size_t mhc_gated_ffn_fwd_workspace_size(int64_t T, int32_t D, int32_t
   return FfnWorkspace({T, D, F, O}, elem_bytes(dtype), false, device_cu_count()).bytes(false);
 }
 
+extern "C" size_t mhc_gated_ffn_fwd_save_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype) {
+  if (check_ffn("", {T, D, F, O}, dtype, 0) || T == 0) return 0;
+  return FfnWorkspace({T, D, F, O}, elem_bytes(dtype), false, device_cu_count()).bytes_saving();
+}
+
 extern "C" int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down,
                                  int32_t dtype, int32_t activation, void* out, float* gate, float* up, void* hidden,
                                  void* workspace, size_t workspace_bytes, int64_t T, int32_t D, int32_t F, int32_t O,
@@ -75,7 +80,8 @@ extern "C" int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* 
     return set_error(MHC_ERR_INVALID, "gated_ffn: gate, up and hidden go together");
   const void* bufs[] = {x, w_gate, w_up, w_down, out};
   if (const int rc = check_buffers("gated_ffn", bufs, 5, workspace, workspace_bytes,
-                                   mhc_gated_ffn_fwd_workspace_size(T, D, F, O, dtype)))
+                                   hidden ? mhc_gated_ffn_fwd_save_workspace_size(T, D, F, O, dtype)
+                                          : mhc_gated_ffn_fwd_workspace_size(T, D, F, O, dtype)))
     return rc;
   if (gate && !(aligned16(gate) && aligned16(up) && aligned16(hidden)))
     return set_error(MHC_ERR_INVALID, "gated_ffn: gate, up or hidden is not 16-byte aligned");

@@ -99,6 +99,8 @@ struct FfnWorkspace {
     }
   }
   size_t bytes(bool backward) const { return (backward ? 2 : 1) * hidden + x + 2 * w + w_down + grad_out + part; }
+  // of a forward whose hidden is the caller's
+  size_t bytes_saving() const { return bytes(false) - hidden; }
 };
 
 }  // namespace mhc

@@ -160,7 +160,7 @@ int ffn_fwd(const FfnFwd& f, const FfnDims& d, char* ws, hipStream_t st) {
   const FfnLines l(d, sizeof(S), false, device_cu_count());
   const FfnWorkspace w(d, sizeof(S), false, device_cu_count());
   void* h = f.hidden ? f.hidden : ws;
-  Padder<S> pad(ws + w.hidden);
+  Padder<S> pad(f.hidden ? ws : ws + w.hidden);
   const void *x = f.x, *wg = f.w_gate, *wu = f.w_up, *wd = f.w_down;
   if (l.copy_D) x = pad.copy(x, d.T, d.D, l.D), wg = pad.copy(wg, d.F, d.D, l.D), wu = pad.copy(wu, d.F, d.D, l.D);
   if (l.copy_F) wd = pad.copy(wd, d.O, d.F, l.F);

@@ -344,15 +344,18 @@ int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_dtype, const
  * x: (T,D), w_gate, w_up: (F,D), w_down: (O,F), out: (T,O), all `dtype`,
  * 16-byte aligned; every size at most 2^31 - 256.  Products accumulate in fp32; hidden is rounded to `dtype`
  * between the two products.  The workspace holds hidden, padded copies of
- * operands whose rows are no multiples of 16 bytes, and partial sums.  For the backward, all or none of: gate, up (T,F)
- * fp32 and hidden, (T, F) `dtype` in rows of stride F rounded up to 8
- * elements (the rest of a row is written as zero).  With none, hidden lives in the workspace.
+ * operands whose rows are no multiples of 16 bytes, and partial sums.  For the
+ * backward, all or none of: gate, up (T,F) fp32 and hidden, (T, F) `dtype` in rows of stride F rounded up to 8
+ * elements (the rest of a row is written as zero).  With none, hidden lives in
+ * the workspace, of mhc_gated_ffn_fwd_workspace_size bytes; with all, that of
+ * mhc_gated_ffn_fwd_save_workspace_size (less by hidden) is enough.
  */
 #define MHC_ACT_SILU 0      /* g * sigmoid(g) */
 #define MHC_ACT_GELU 1      /* g * Phi(g) */
 #define MHC_ACT_GELU_TANH 2 /* 0.5 g (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) */
 #define MHC_ACT_RELU 3      /* max(g, 0) */
 size_t mhc_gated_ffn_fwd_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype);
+size_t mhc_gated_ffn_fwd_save_workspace_size(int64_t T, int32_t D, int32_t F, int32_t O, int32_t dtype);
 int mhc_gated_ffn_fwd(const void* x, const void* w_gate, const void* w_up, const void* w_down,
                       int32_t dtype, int32_t activation, void* out, float* gate, float* up,
                       void* hidden, void* workspace, size_t workspace_bytes, int64_t T, int32_t D,
