@@ -36,9 +36,10 @@ struct GemmArgs {
 
 // 1 / (1 + exp(-z)).  16-bit results: by the hardware's exp2 and reciprocal,
 // whose errors (1 ulp each, and |z| half ulps of the exponent's rounding, where
-// the result is not yet 1) stay below 2^-17 while exp(-z) is finite; the
-// accurate functions cost four times the instructions, a tenth of a large
-// product with this epilogue.
+// the result is not yet 1) stay below 2^-17 for z >= -87.3.  Below, 1 + exp(-z)
+// is above 2^126, whose reciprocal is subnormal and comes out as 0: off by less
+// than 2^-126, z times it by 1.1e-36.  The accurate functions cost four times
+// the instructions, a tenth of a large product with this epilogue.
 template <bool FAST>
 __device__ __forceinline__ float sigmoid(float z) {
   if constexpr (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
