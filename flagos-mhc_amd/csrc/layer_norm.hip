@@ -23,20 +23,16 @@ namespace mhc {
 namespace {
 
 // VEC elements from element `e` of a row of D >= VEC elements, as fp32; rows
-// start at any element, so accesses are unaligned 16-byte ones.
+// start at any element, so accesses are unaligned 16-byte ones.  W is the
+// activations' type or fp32, so VEC is one or two of its vectors.
 template <typename W, int VEC>
 __device__ __forceinline__ void load_f32(const W* row, int64_t e, float* o) {
   constexpr int V = Store<W>::VEC;
-  static_assert(VEC % V == 0 || V % VEC == 0, "vector widths");
-  if constexpr (VEC >= V) {
+  static_assert(VEC % V == 0, "whole vectors");
 #pragma unroll
-    for (int i = 0; i < VEC / V; ++i) {
-      const u32x4 v = *reinterpret_cast<const u32x4_a2*>(row + e + i * V);
-      Store<W>::unpack(v, o + i * V);
-    }
-  } else {  // fp32 activations with 16-bit weights: 4 elements in 8 bytes
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = load_elem<W>(row, e + i);
+  for (int i = 0; i < VEC / V; ++i) {
+    const u32x4 v = *reinterpret_cast<const u32x4_a2*>(row + e + i * V);
+    Store<W>::unpack(v, o + i * V);
   }
 }
 
