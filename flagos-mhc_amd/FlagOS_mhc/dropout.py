@@ -8,7 +8,9 @@ they are at least t = round(p * 65536) and then multiplied by
 tensor's elements in row-major order, whatever its strides.  The backward is
 the same call on the gradient.  A program gives every call of a step its own
 offset (or seed); with ``state``, an int64 tensor (seed, offset) on the
-device, a captured graph reads them when it is replayed.
+device, a captured graph reads them when it is replayed; seed and offset are
+then not looked at, so calls that share a state share their mask: give each
+layer a state of its own.
 """
 
 from __future__ import annotations

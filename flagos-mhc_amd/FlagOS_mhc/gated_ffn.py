@@ -5,7 +5,10 @@
 x is (..., D), w_gate and w_up (F, D), w_down (O, F) as torch.nn.Linear keeps
 its weights; out is (..., O).  All have one dtype (fp32, bf16 or fp16);
 products accumulate in fp32 and hidden is rounded to that dtype between
-them.  In an mHC layer x is the norm of ``mhc_pre_clamp_sinkhorn``'s y and
+them, as the gradients of gate and up are in the backward: results carry one
+rounding more than with fp32 between the products, and in fp16 a hidden above
+65504 is infinite.  Operands that are not contiguous, or whose address is no
+multiple of 16 bytes, are copied in every call.  In an mHC layer x is the norm of ``mhc_pre_clamp_sinkhorn``'s y and
 out the h_out of ``mhc_post``.  The reference has no such operator: its
 model code runs PyTorch's.
 """

@@ -10,7 +10,7 @@
 // expectation is exact for the probability in use.  16 bits an element
 // instead of 32 halve the generator's work (10 rounds of two 32x32 products
 // a group), which at 32 bits would exceed the time of reading and writing
-// bf16 rows.  65536 x 7168 bf16: 350 us, 5.4 TB/s, bound by HBM; blocks in runs
+// bf16 rows.  65536 x 7168 bf16: 358 us, 5.2 TB/s, bound by HBM; blocks in runs
 // of one XCD (400 us interleaved over all eight).
 #include "common.hpp"
 #include "mhc_launch.hpp"

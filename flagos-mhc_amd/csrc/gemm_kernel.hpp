@@ -277,10 +277,11 @@ struct KCursor {
 // STAGES - 1 tiles ahead; otherwise through registers, for operands whose rows
 // are not multiples of 16 bytes.  128 x 128 (the waves 2 x 2) and 64 x 64 run
 // two and four blocks a CU, so that one's products cover another's waits and
-// its results' way to memory: two 5632 x 2048 x 4099 bf16 products 177 us (1.07
-// PFLOP/s); fp32, bound by its matrix instructions, 125 - 135 TFLOP/s at 2048
-// tokens.  16 and 64 rows x 128 are bound by B's bytes: one block a CU with 80
-// KB or more on their way (T = 64, 180 MB of weights in 35 us).
+// its results' way to memory: two 5632 x 2048 x 4099 bf16 products 193 us (0.98
+// PFLOP/s; 179 at best); fp32, bound by its matrix instructions, 126 and 135
+// TFLOP/s at 2048 and 4096 tokens.  16 and 64 rows x 128 are bound by B's bytes:
+// one block a CU with 80 KB or more on their way (T = 64, 180 MB of weights in 41
+// us, 4.4 TB/s).
 
 template <typename S_, int LA_, int LB_, int BM_, int BN_, int WAVES_M_, int STAGES_, int PER_CU_, int EPI_, bool DMA_>
 struct TileCfg {
@@ -445,11 +446,11 @@ __global__ __launch_bounds__(256, C::kPerCu) void gemm_tile_kernel(GemmArgs a) {
 // three slots and starts the loads of step k + 2 in its only phase.  Every
 // phase is reads, barrier, products, barrier, and waves 4 .. 7 run one barrier
 // behind waves 0 .. 3: of the two waves on a SIMD one reads while the other
-// multiplies.  16384 x 7168 x 18432 bf16: 2.92 ms, 1.48 PFLOP/s, the matrix
+// multiplies.  16384 x 7168 x 18432 bf16: 2.94 ms, 1.47 PFLOP/s, the matrix
 // instructions busy 82% of the cycles at the 1.57 GHz that the card's power
-// leaves them; a phase for each quadrant, with twice the barriers, reached
-// 1.16.  BM = 128 is a seventh slower for its products and leaves fewer CUs
-// without a tile.
+// leaves them; with a phase for each quadrant, and twice the barriers, a forward
+// and backward at this size took 36.3 ms instead of 29.3.  BM = 128 is a seventh
+// slower for its products and leaves fewer CUs without a tile.
 
 template <typename S_, int LA_, int LB_, int BM_, int EPI_>
 struct WideCfg {

@@ -95,7 +95,8 @@ constexpr KernelCost kCosts[kKinds] = {
 // lines of k through registers: a wait for memory every step
 constexpr double kColCol = 1.16, kColRegs = 1.7;
 constexpr int kFewRows = 4;
-constexpr double kJoinUs = 8., kJoinBytesPerUs = 3.5e6, kLaunchUs = 3.;
+// a launch, and the join's (the kernel takes 5 us for few bytes)
+constexpr double kLaunchUs = 3., kJoinUs = kLaunchUs + 5., kJoinBytesPerUs = 3.5e6;
 constexpr double kCuBytesPerUs = 16e3;  // of a tile's results, with every CU at it
 
 struct GemmPlan {
@@ -120,8 +121,10 @@ inline GemmPlan deal_tiles(const GemmShape& s, size_t es, int kind, bool dma, in
   const int64_t tiles = tiles_of(s, c.bm, c.bn), steps = (s.K * (int64_t)es + 127) / 128 * s.segments;
   // n steps of `blocks` blocks side by side: on a part of the CUs each runs
   // faster, as the card's power then allows a higher clock, and each has more
-  // of the memory's rate (T = 64, D = 4096, F = 11008: 172 whole tiles take 35
-  // us, cut into 256 runs 32 and 5 more for the join)
+  // of the memory's rate (forwards with the gated product in whole tiles, and in
+  // 256 runs with a join, weights out of HBM: T = 64, D = 4096, F = 11008 bf16,
+  // 172 tiles, 75 and 77 us; D = 1024, F = 2816, 44 tiles, 28 and 31; D = 7168, F =
+  // 18432, 288 tiles, whose last round is nearly empty, 207 and 174)
   const auto side_by_side = [&](double blocks, double n) {
     const double part = blocks < cus ? blocks / cus : 1.;
     const double few = c.per_cu > 1 ? cost.alone : cost.alone + (cost.full - cost.alone) * part;

@@ -12,10 +12,11 @@
 // columns in every row and keeps their weight and bias.  The backward adds its
 // columns' dw and db in fp32 registers, each block writes its sums once, and a
 // second kernel adds the blocks' sums in a fixed order: no atomics, the same
-// bits in every run.  T = 65536, D = 7168 bf16: forward 337 us (5.6 TB/s),
-// backward 525 us (5.4 TB/s).  Rows longer than 4096 16-byte vectors (the
+// bits in every run.  T = 65536, D = 7168 bf16: forward 336 us (5.6 TB/s),
+// backward 527 us (5.3 TB/s).  Rows longer than 4096 16-byte vectors (the
 // backward: 2048) are read from memory again for each sum (they come from the
-// L2).
+// L2), element by element, and the backward's dw and db are added in memory: T =
+// 4096, D = 12288 fp32 467 us, a quarter of the rate (forward, in registers, 70).
 #include "common.hpp"
 #include "mhc_launch.hpp"
 
@@ -420,7 +421,7 @@ __global__ __launch_bounds__(1024) void norm_bwd_loop_kernel(NormBwdArgs a) {
   const S* x = static_cast<const S*>(a.x);
   const S* gy = static_cast<const S*>(a.gy);
   float* part = a.part ? a.part + (int64_t)blockIdx.x * 2 * D : nullptr;
-  if (part)  // each element of the block's sums belongs to one thread
+  if (part)  // zeroed before the barrier; from then on column i of both sums is thread i % 1024's
     for (int i = threadIdx.x; i < 2 * D; i += 1024) part[i] = 0.f;
   __syncthreads();
   int buf = 0;
@@ -535,7 +536,12 @@ int launch_norm_fwd(const NormFwdArgs& a, hipStream_t st) {
 }
 
 // The one-launch form: rows that the second reading finds in the L2, few
-// enough that a slab's walk over them is no longer than a launch or two.
+// enough that a slab's walk over them is no longer than a launch or two.  One
+// launch and two, us in a replayed graph: fp32 D = 256 T = 1024 4.3, 5.6, T = 2048
+// 6.5, 6.9, T = 4096 11.1, 10.3; bf16 D = 256 T = 1536 6.7, 6.7, T = 2048 8.5, 7.3;
+// fp16 D = 1003 T = 1536 10.8, 11.0, T = 2048 16.5, 12.4.  By bytes of x and grad_y:
+// bf16 D = 4096 8 MB 5.5, 24.8, 16 MB 14.6, 25.5; fp32 D = 2048 16 MB 13.8, 14.4, 24 MB
+// 24.4, 16.4 (the limit leaves what one launch would gain up to 16 MB).
 bool norm_bwd_in_one(int64_t T, int64_t D, size_t es, const NormPlan& p) {
   return p.G > 0 && T <= 1536 && 2 * T * D * (int64_t)es <= (8 << 20);
 }

@@ -342,8 +342,9 @@ int mhc_layer_norm_bwd(const void* grad_y, const void* x, int32_t x_dtype, const
  *   gate = x w_gate^T, up = x w_up^T, hidden = act(gate) * up,
  *   out = hidden w_down^T
  * x: (T,D), w_gate, w_up: (F,D), w_down: (O,F), out: (T,O), all `dtype`,
- * 16-byte aligned; every size at most 2^31 - 256.  Products accumulate in fp32; hidden is rounded to `dtype`
- * between the two products.  The workspace holds hidden, padded copies of
+ * 16-byte aligned; every size at most 2^31 - 256.  Products accumulate in
+ * fp32; hidden is rounded to `dtype` between the two products (fp16: above
+ * 65504 it is infinite).  The workspace holds hidden, padded copies of
  * operands whose rows are no multiples of 16 bytes, and partial sums.  For the
  * backward, all or none of: gate, up (T,F) fp32 and hidden, (T, F) `dtype` in rows of stride F rounded up to 8
  * elements (the rest of a row is written as zero).  With none, hidden lives in
@@ -382,8 +383,8 @@ int mhc_gated_ffn_bwd(const void* grad_out, const void* x, const void* w_gate, c
  * half of word j); y[i] = x[i] * 65536 / (65536 - t) where they are at least
  * t = round(p * 65536), else 0.  x, y: n elements of `dtype`, any element
  * alignment; y may be x.  state: device memory holding (seed, offset), read
- * when the kernel runs, in place of the two arguments (for captured graphs),
- * or NULL.  The backward is the same call on the gradient.
+ * when the kernel runs, in place of the two arguments (for captured graphs;
+ * calls with the same state have the same mask), or NULL.  The backward is the same call on the gradient.
  */
 int mhc_dropout(const void* x, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
                 uint64_t offset, const uint64_t* state, void* stream);
