@@ -106,6 +106,8 @@ def draw(rng):
         return _rot(None, max(1, min(T, 65536 * 64 * 128 // (2 * (H + Hk) * d))), H, Hk, d, r, dtype, rng.choice(["half", "interleaved"]),
                     rng.choice([None, "linear", "ntk", "yarn"]), rng.choice([0, _log_int(rng, 1, 500000)]),
                     1, rng.random() < 0.5)
+    if dtype == "f32":
+        d = min(d, 128)
     if op == "decode":
         B = _log_int(rng, 1, 64)
         # at most the cache of the largest listed case
