@@ -1,0 +1,211 @@
+"""Rotary positions of an attention sublayer's queries and keys, forward and
+backward.
+
+    (a, b) -> amplitude (a cos w - b sin w, a sin w + b cos w),  w = position * freqs[i]
+
+for the pairs of a head's first r = 2 len(freqs) elements: (i, i + r/2) in the
+"half" layout, (2i, 2i + 1) in the "interleaved" one; elements past r are
+copied.  ``rotary_frequencies`` gives freqs, and the amplitude, of the usual
+ways to stretch positions.  Angles are reduced in 64 bits, products are fp32.
+The reference has no such operator: its model code runs PyTorch's.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+#: layouts and their codes (include/mhc_amd.h)
+LAYOUTS = {"half": 0, "interleaved": 1}
+SCALINGS = (None, "linear", "ntk", "yarn")
+
+
+def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, original_length=None, turns=(1.0, 32.0),
+                       device="cuda"):
+    """(freqs, amplitude) for ``rotary``: freqs (rotary_dim / 2,) float64 on
+    `device`, radians a position, base^(-2i / rotary_dim).  ``scaling``, by
+    ``factor`` > 0:
+      None      as they are
+      "linear"  positions divided by factor
+      "ntk"     base * factor^(r / (r - 2)): the slowest pair is stretched by factor, the fastest stays
+      "yarn"    pairs that turn less than turns[0] times over original_length positions are stretched by
+                factor, those above turns[1] stay, in between by a linear share of their turns;
+                amplitude 0.1 ln(factor) + 1 (factor > 1)
+    """
+    what = "rotary_frequencies"
+    r = int(rotary_dim)
+    if r < 2 or r % 2:
+        raise ValueError(f"{what}: rotary_dim {rotary_dim}, expected an even number of at least 2")
+    if scaling not in SCALINGS:
+        raise ValueError(f"{what}: scaling {scaling!r}, expected one of {SCALINGS}")
+    if not (base > 0 and math.isfinite(base)) or not (factor > 0 and math.isfinite(factor)):
+        raise ValueError(f"{what}: base {base} and factor {factor}, expected positive numbers")
+    if scaling == "ntk" and r > 2:
+        base = base * factor ** (r / (r - 2))
+    f = [base ** (-2.0 * i / r) for i in range(r // 2)]
+    amplitude = 1.0
+    if scaling == "linear":
+        f = [v / factor for v in f]
+    elif scaling == "yarn":
+        low, high = turns
+        if not original_length or original_length < 1 or not 0 <= low < high:
+            raise ValueError(f"{what}: original_length {original_length} and turns {turns} for yarn")
+        keep = [min(1.0, max(0.0, (original_length * v / (2 * math.pi) - low) / (high - low))) for v in f]
+        f = [v * s + v / factor * (1 - s) for v, s in zip(f, keep)]
+        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    return torch.tensor(f, dtype=torch.float64, device=device), amplitude
+
+
+def _strided(t):
+    """(t, row stride, head stride): t (..., H, d) with its rows one stride apart
+    and a head's elements side by side; a copy where it is not so."""
+    if t.is_contiguous():
+        return t, t.shape[-2] * t.shape[-1], t.shape[-1]
+    shape, st = t.shape, t.stride()
+    if st[-1] == 1 or shape[-1] == 1:
+        row = 0
+        rows = 1  # of the dimensions seen so far
+        for n, s in zip(reversed(shape[:-2]), reversed(st[:-2])):
+            if n == 1:
+                continue
+            if rows == 1:
+                row = s
+            elif s != row * rows:
+                break
+            rows *= n
+        else:
+            return t, row, st[-2]
+    t = t.contiguous()
+    return t, shape[-2] * shape[-1], shape[-1]
+
+
+def _run(what, q, k, freqs, positions, cu_seqlens, layout, amplitude, inverse):
+    _lib.require_device(what, q, k, freqs, positions, cu_seqlens)
+    code = _lib.dtype_code(what, q.dtype)
+    if layout not in LAYOUTS:
+        raise ValueError(f"{what}: layout {layout!r}, expected one of {tuple(LAYOUTS)}")
+    if q.dim() < 3:
+        raise ValueError(f"{what}: q of shape {tuple(q.shape)}, expected (..., heads, d) with a dimension of tokens")
+    lead, (H, d) = q.shape[:-2], q.shape[-2:]
+    T = math.prod(lead)
+    Hk = 0
+    if k is not None:
+        if k.dim() != q.dim() or k.shape[:-2] != lead or k.shape[-1] != d or k.dtype is not q.dtype:
+            raise ValueError(f"{what}: k of shape {tuple(k.shape)} and {k.dtype} for q of {tuple(q.shape)} and {q.dtype}")
+        Hk = k.shape[-2]
+    if H < 1 or d < 1 or (k is not None and Hk < 1):
+        raise ValueError(f"{what}: q of shape {tuple(q.shape)} has no heads" if H < 1 or d < 1 else f"{what}: k has no heads")
+    r = 2 * freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or r > d:
+        raise ValueError(f"{what}: freqs of shape {tuple(freqs.shape)} and {freqs.dtype}, expected float64 and at most {d // 2}")
+    if not freqs.is_contiguous():
+        freqs = freqs.contiguous()
+    if positions is not None:
+        if cu_seqlens is not None:
+            raise ValueError(f"{what}: positions and cu_seqlens")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.numel() != T:
+            raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} and {positions.dtype}, expected "
+                             f"{T} of int32 or int64")
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+    if cu_seqlens is not None:
+        if q.dim() != 3:
+            raise ValueError(f"{what}: cu_seqlens goes with packed rows (T, heads, d), q is {tuple(q.shape)}")
+        cu_seqlens = _lib.cu_operand(what, "cu_seqlens", cu_seqlens)
+    qs, q_row, q_head = _strided(q)
+    ks, k_row, k_head = (None, 0, 0) if k is None else _strided(k)
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if T > 0:
+        _lib.call(what, _lib.load().mhc_rotary, q.get_device(), qs.data_ptr(), _lib.ptr(ks), code, q_row, q_head, k_row,
+                  k_head, freqs.data_ptr(), _lib.ptr(positions),
+                  0 if positions is None else int(positions.dtype is torch.int64), _lib.ptr(cu_seqlens),
+                  0 if cu_seqlens is None else cu_seqlens.numel() - 1, lead[-1], LAYOUTS[layout], amplitude, inverse,
+                  qo.data_ptr(), _lib.ptr(ko), T, H, Hk, d, r)
+    return qo, ko
+
+
+def rotary(q, k, freqs, positions=None, *, cu_seqlens=None, layout="half", amplitude=1.0):
+    """Rotary positions on the HIP device, for q (..., H, d) and k (..., Hk, d)
+    (or None) of one call: new tensors (q, k), k's None if it is.
+
+    A row's position is positions[t] (int32 or int64, one a row; any sign),
+    else, with cu_seqlens (B + 1,) of packed rows (T, H, d), its place in its
+    sequence, else its place along the dimension before the heads."""
+    return _run("rotary", q, k, freqs, positions, cu_seqlens, layout, amplitude, 0)
+
+
+def rotary_backward(grad_q, grad_k, freqs, positions=None, *, cu_seqlens=None, layout="half", amplitude=1.0):
+    """Gradients of q and k: the gradients rotated back."""
+    return _run("rotary_backward", grad_q, grad_k, freqs, positions, cu_seqlens, layout, amplitude, 1)
+
+
+def rotary_ref(x, freqs, positions, layout="half", amplitude=1.0):
+    """The same in PyTorch for one tensor (..., H, d) and positions of its
+    leading dimensions: angles in 64 bits, products fp32, cast to x's dtype."""
+    w = positions.double()[..., None] * freqs.double()
+    cos, sin = ((f(w) * amplitude).float()[..., None, :] for f in (torch.cos, torch.sin))
+    r = 2 * freqs.numel()
+    xf = x.float()
+    half = layout == "half"
+    a, b = (xf[..., :r // 2], xf[..., r // 2:r]) if half else (xf[..., 0:r:2], xf[..., 1:r:2])
+    pair = (a * cos - b * sin, a * sin + b * cos)
+    turned = torch.cat(pair, -1) if half else torch.stack(pair, -1).flatten(-2)
+    return torch.cat((turned, xf[..., r:]), -1).to(x.dtype)
+
+
+class RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, freqs, positions, cu_seqlens, layout, amplitude):
+        ctx.save_for_backward(freqs, positions, cu_seqlens)
+        ctx.args = (layout, amplitude)
+        ctx.set_materialize_grads(False)
+        qo, ko = rotary(q, k, freqs, positions, cu_seqlens=cu_seqlens, layout=layout, amplitude=amplitude)
+        return qo if k is None else (qo, ko)
+
+    @staticmethod
+    def backward(ctx, grad_q, grad_k=None):
+        freqs, positions, cu = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        gq, gk = (g if n else None for g, n in zip((grad_q, grad_k), need))
+        # (linear: the backward of the backward is the same rotation again, forward)
+        out = _back(gq, gk, freqs, positions, cu, *ctx.args)
+        return (*out, None, None, None, None, None)
+
+
+class _RotaryBackFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gq, gk, freqs, positions, cu_seqlens, layout, amplitude):
+        ctx.save_for_backward(freqs, positions, cu_seqlens)
+        ctx.args = (layout, amplitude)
+        q, k = rotary_backward(gq, gk, freqs, positions, cu_seqlens=cu_seqlens, layout=layout, amplitude=amplitude)
+        return q if gk is None else (q, k)
+
+    @staticmethod
+    def backward(ctx, q, k=None):
+        freqs, positions, cu = ctx.saved_tensors
+        return (*_pair(RotaryFn.apply, q, k, freqs, positions, cu, *ctx.args), None, None, None, None, None)
+
+
+def _pair(fn, q, k, *args):
+    """fn of either or both of q and k: (q', k'), None for what is None."""
+    if q is None and k is None:
+        return None, None
+    if q is None:
+        return None, fn(k, None, *args)
+    return (fn(q, None, *args), None) if k is None else fn(q, k, *args)
+
+
+def _back(gq, gk, *args):
+    return _pair(_RotaryBackFn.apply, gq, gk, *args)
+
+
+def rotary_fn(q, k, freqs, positions=None, *, cu_seqlens=None, layout="half", amplitude=1.0):
+    """Autograd-aware rotary: (q, k)."""
+    if not _lib.needs_autograd(q, k):
+        return rotary(q, k, freqs, positions, cu_seqlens=cu_seqlens, layout=layout, amplitude=amplitude)
+    out = RotaryFn.apply(q, k, freqs, positions, cu_seqlens, layout, amplitude)
+    return (out, None) if k is None else out

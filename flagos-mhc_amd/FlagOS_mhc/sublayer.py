@@ -11,15 +11,19 @@ registered as torch.ops.flagos_mhc.* (``FlagOS_mhc.library``).
 
 from __future__ import annotations
 
+from .attention import AttentionFn, attention, attention_backward, attention_fn, attention_ref
 from .autograd import mhc_post_fn, mhc_pre_clamp_sinkhorn_fn
 from .dropout import DropoutFn, dropout, dropout_backward, dropout_fn, dropout_ref
 from .gated_ffn import GatedFfnFn, gated_ffn, gated_ffn_backward, gated_ffn_fn, gated_ffn_ref
 from .layer_norm import LayerNormFn, layer_norm, layer_norm_backward, layer_norm_fn, layer_norm_ref
+from .rotary import RotaryFn, rotary, rotary_backward, rotary_fn, rotary_frequencies, rotary_ref
 
 __all__ = [
     "layer_norm", "layer_norm_backward", "layer_norm_ref", "LayerNormFn", "layer_norm_fn",
     "gated_ffn", "gated_ffn_backward", "gated_ffn_ref", "GatedFfnFn", "gated_ffn_fn",
     "dropout", "dropout_backward", "dropout_ref", "DropoutFn", "dropout_fn",
+    "rotary", "rotary_backward", "rotary_frequencies", "rotary_ref", "RotaryFn", "rotary_fn",
+    "attention", "attention_backward", "attention_ref", "AttentionFn", "attention_fn",
     "mhc_ffn_layer_fn",
 ]
 

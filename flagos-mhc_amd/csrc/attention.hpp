@@ -1,0 +1,446 @@
+// Attention over sequences of different lengths: arguments, the map from
+// blocks to sequences, tiles in LDS and the matrix operands read from them.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i . k_j - lse_i),  lse_i = ln sum_j exp(scale q_i . k_j)
+//
+// over the keys j that query i sees: j < Lk and, if causal, j <= i + Lk - Lq
+// (the queries are the last Lq of the Lk positions).
+//
+// Every product keeps the index that is summed last in a lane's own
+// registers: with 32x32 products, S^T = K Q^T leaves lane l with query l % 32
+// and keys 8 (i / 4) + 4 (l / 32) + i % 4, i = 0..15, which is, packed, the
+// second operand of O^T = V^T P^T with its k order permuted; the first operand
+// is read in that order.  Maxima and sums over keys are then a lane's own but
+// for one exchange with lane l ^ 32, factors of a query are one register, and
+// P never goes through LDS.
+#pragma once
+
+#include "attention_plan.hpp"
+#include "common.hpp"
+#include "lds_dma.hpp"
+
+namespace mhc {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8_att __attribute__((ext_vector_type(8)));
+typedef short s16x4_att __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Two scaled products per exp2: a new row maximum moves the reference point
+// only where it exceeds the old one by more than this (in powers of two), so
+// that sums are rescaled a few times a row and not once a tile.  p is then at
+// most 2^8, exact in every type's range, and the result does not depend on it.
+constexpr float kLazyMax = 8.0f;
+
+// One of q, k, v or a gradient: element (sequence's row t, head h, i) at
+// p[b * bs + t * ts + h * hs + i]; packed sequences have bs = 0 and rows
+// counted from the first sequence's start.
+struct AttRows {
+  const void* p;
+  int64_t bs, ts, hs;  // elements
+};
+
+struct AttArgs {
+  AttRows q, k, v, go, o;  // go, o: backward; o contiguous
+  void* out;               // (rows of q, H, d), forward: o, backward: dq
+  void *dk, *dv;           // (rows of k, Hk, d)
+  float* lse;              // (H, rows of q)
+  float* delta;            // (H, rows of q): sum_d go o, backward
+  float* part;             // partial results of splits
+  AttDims n;
+  float scale, scale2;     // scale, scale * log2(e)
+};
+
+// ---- sequences ---------------------------------------------------------------
+
+struct AttSeq {
+  int64_t row0;    // first row in the outputs' and lse's order
+  int64_t q0, k0;  // element offsets of row 0 of q and k: add AttRows.p
+  int lq, lk;      // rows; lq counts output rows of the sequence behind the last one too
+  int b;
+  bool none;       // rows behind the last sequence: zeros are written
+};
+
+__device__ __forceinline__ int64_t cu_at(const int32_t* cu, int b, int64_t T) {
+  const int64_t c = b == 0 ? 0 : (int64_t)cu[b];
+  return c < 0 ? 0 : (c > T ? T : c);
+}
+
+// First slot of sequence b, where tiles of R rows are dealt to slots: sequence
+// b's tiles begin at slot cu[b] / R + b, which leaves each the ceil(L / R) it
+// needs without a sum over the sequences before it.
+__device__ __forceinline__ int64_t slot_start(const int32_t* cu, int b, int64_t T, int R) { return cu_at(cu, b, T) / R + b; }
+
+// The sequence whose slots hold `slot`, of B + 1 (the last: rows behind the
+// sequences): 64 candidates a step, one a lane.
+__device__ __forceinline__ int slot_sequence(const int32_t* cu, int B, int64_t T, int R, int64_t slot) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = B + 1;
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int c = lane * step;
+    const bool in = c < n && slot_start(cu, lo + c, T, R) <= slot;
+    int hit = __popcll(__ballot(in));
+    hit = hit < 1 ? 1 : hit;
+    const int skip = (hit - 1) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// The rows of sequence b, and where its keys are.
+__device__ __forceinline__ AttSeq att_seq(const AttDims& n, int b) {
+  AttSeq s;
+  s.b = b;
+  s.none = b >= n.B;
+  if (n.cu_q) {
+    s.row0 = cu_at(n.cu_q, b, n.Tq);
+    const int64_t e = s.none ? n.Tq : cu_at(n.cu_q, b + 1, n.Tq);
+    s.lq = e > s.row0 ? (int)(e - s.row0) : 0;
+  } else {
+    s.row0 = (int64_t)b * n.Sq;
+    s.lq = n.Sq;
+  }
+  s.lk = 0;
+  s.k0 = 0;
+  if (!s.none) {
+    if (n.cu_k) {
+      s.k0 = cu_at(n.cu_k, b, n.Tk);
+      const int64_t e = cu_at(n.cu_k, b + 1, n.Tk);
+      s.lk = e > s.k0 ? (int)(e - s.k0) : 0;
+    } else {
+      s.lk = n.Sk;
+      if (n.len_k) {
+        const int l = n.len_k[b];
+        s.lk = l < 0 ? 0 : (l < n.Sk ? l : n.Sk);
+      }
+    }
+  }
+  return s;
+}
+
+// Tile of `R` query rows that slot `slot` stands for: its sequence and first
+// row (lq or more: nothing to do).
+__device__ __forceinline__ AttSeq q_tile(const AttDims& n, int64_t slot, int R, int& first) {
+  if (!n.cu_q) {
+    const int per = (n.Sq + R - 1) / R;
+    const int b = (int)(slot / per);
+    first = (int)(slot % per) * R;
+    return att_seq(n, b);
+  }
+  const int b = slot_sequence(n.cu_q, n.B, n.Tq, R, slot);
+  const int64_t t = slot - slot_start(n.cu_q, b, n.Tq, R);
+  AttSeq s = att_seq(n, b);
+  first = t * R < s.lq ? (int)(t * R) : s.lq;
+  return s;
+}
+
+// The same for key rows; rows is how many of dk and dv the sequence has
+// (those past lk are zero).
+__device__ __forceinline__ AttSeq k_tile(const AttDims& n, int64_t slot, int R, int& first, int& rows, int64_t& row0) {
+  if (!n.cu_k) {
+    const int per = (n.Sk + R - 1) / R;
+    const int b = (int)(slot / per);
+    first = (int)(slot % per) * R;
+    rows = n.Sk;
+    row0 = (int64_t)b * n.Sk;
+    return att_seq(n, b);
+  }
+  const int b = slot_sequence(n.cu_k, n.B, n.Tk, R, slot);
+  const int64_t t = slot - slot_start(n.cu_k, b, n.Tk, R);
+  AttSeq s = att_seq(n, b);
+  row0 = cu_at(n.cu_k, b, n.Tk);
+  const int64_t e = s.none ? n.Tk : cu_at(n.cu_k, b + 1, n.Tk);
+  rows = e > row0 ? (int)(e - row0) : 0;
+  first = t * R < rows ? (int)(t * R) : rows;
+  return s;
+}
+
+// Address of row `t` of sequence s for head h.  (Packed rows are counted from
+// the buffer's first.)
+__device__ __forceinline__ const char* row_ptr(const AttRows& r, const int32_t* cu, int64_t start, int b, int64_t t, int h, int es) {
+  const int64_t at = (cu ? start + t : t) * r.ts + (cu ? 0 : (int64_t)b * r.bs) + (int64_t)h * r.hs;
+  return static_cast<const char*>(r.p) + at * es;
+}
+
+// ---- operands -----------------------------------------------------------------
+// A fragment is 16 bytes a lane: E elements of the summed index for one of 32
+// rows.  Two lane halves make a step of 2 E: 16 (16-bit types, one 32x32x16
+// product) or 8 (fp32, four 32x32x2 products, element j of both halves each).
+
+template <typename S> struct Mma32;
+template <> struct Mma32<bf16_t> {
+  static constexpr int E = 8;
+  __device__ static floatx16 fma(const u32x4& a, const u32x4& b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  __device__ static uint32_t pack2(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  __device__ static bool nonfinite(uint32_t w) {
+    return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+  }
+};
+template <> struct Mma32<f16_t> {
+  static constexpr int E = 8;
+  __device__ static floatx16 fma(const u32x4& a, const u32x4& b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_att, a), __builtin_bit_cast(f16x8_att, b), c, 0, 0, 0);
+  }
+  __device__ static uint32_t pack2(float lo, float hi) { return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16); }
+  __device__ static bool nonfinite(uint32_t w) {
+    return (w & 0x7c000000u) == 0x7c000000u || (w & 0x7c00u) == 0x7c00u;
+  }
+};
+template <> struct Mma32<float> {
+  static constexpr int E = 4;
+  __device__ static floatx16 fma(const u32x4& a, const u32x4& b, floatx16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+    return c;
+  }
+  __device__ static bool nonfinite(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+};
+
+// The fragment of elements E t .. E t + E - 1 of the 16 that a product left a
+// lane: step t of that block of 32.
+template <typename S>
+__device__ __forceinline__ u32x4 acc_frag(const floatx16& s, int t) {
+  u32x4 f;
+  if constexpr (sizeof(S) == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = Mma32<S>::pack2(s[8 * t + 2 * i], s[8 * t + 2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __float_as_uint(s[4 * t + i]);
+  }
+  return f;
+}
+
+// ---- tiles ----------------------------------------------------------------------
+// R rows of a head as they lie in memory, in chunks of 16 bytes whose position
+// within the row is exclusive-ored with a function of the row.  Two kinds of
+// reads have to meet all 64 banks: 16 rows of one chunk (row fragments), and
+// 4 rows of 4 chunks (16-bit columns, one transposing read of 32 lanes) or
+// rows j and j + 4 of 8 chunks (fp32 columns).  Rows of 256 bytes start at
+// the same bank, those of 128 at alternating halves.
+template <typename S, int DB>
+struct Tile {
+  static constexpr int kEs = (int)sizeof(S);
+  static constexpr int kE = Mma32<S>::E;
+  static constexpr int kD = 32 * DB;                                   // columns held
+  static constexpr int kWide = DB <= 2 ? 64 : (DB <= 4 ? 128 : 256);   // columns of a row's place
+  static constexpr int kPitch = kWide * kEs;                           // bytes
+  static constexpr int kChunks = kPitch / 16;
+  static constexpr int kUsed = kD * kEs / 16;    // chunks that are loaded
+  static constexpr int kSteps = kUsed / 2;       // row fragments
+  static constexpr int kColSteps = 16 / kE;      // column fragments of 32 rows
+
+  static __device__ __forceinline__ int swizzle(int r) {
+    if constexpr (kEs == 4) return ((r & 4) << 1) | ((r & 8) >> 1) | (r & 3);
+    if constexpr (kChunks == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+    return ((r & 3) << 2) | ((r >> 2) & 3);
+  }
+  static __device__ __forceinline__ uint32_t at(int r, int c) { return (uint32_t)(r * kPitch + ((c ^ swizzle(r)) * 16)); }
+
+  // Row fragment: row 32 blk + l % 32, chunk 2 step + l / 32.
+  static __device__ __forceinline__ u32x4 row_frag(const char* tile, int blk, int step, int lane) {
+    const int r = lane & 31, h = lane >> 5;
+    const uint32_t a = (uint32_t)(r * kPitch) + (uint32_t)((h ^ swizzle(r)) * 16);
+    // (chunks are exclusive-ored in their low bits only)
+    constexpr int kLow = kChunks >= 16 ? 16 : 8;
+    const int c = 2 * step;
+    return *reinterpret_cast<const u32x4*>(tile + blk * 32 * kPitch + ((a ^ (uint32_t)((c % kLow) * 16)) + (c / kLow) * kLow * 16));
+  }
+
+  // Column fragment: column 32 db + l % 32; rows of step t of block blk in the
+  // order of acc_frag.
+  static __device__ __forceinline__ u32x4 col_frag(const char* tile, int blk, int t, int db, int lane) {
+    const int h = lane >> 5;
+    if constexpr (kEs == 2) {
+      const int i = lane & 15, g = (lane >> 4) & 1;
+      u32x4 f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = 8 * u + 4 * h + (i >> 2);
+        const int c = 2 * g + ((i & 3) >> 1);
+        const uint32_t a = (uint32_t)(r * kPitch) + (uint32_t)((c ^ swizzle(r)) * 16) + (i & 1) * 8;
+        constexpr int kLow = kChunks >= 16 ? 4 : 2;  // blocks of 32 columns within the exclusive-ored bits
+        const char* p = tile + (blk * 32 + t * 16) * kPitch + ((a ^ (uint32_t)((db % kLow) * 64)) + (db / kLow) * kLow * 64);
+        const s16x4_att v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4_att*)reinterpret_cast<const s16x4_att*>(p));
+        const u32x2 w = __builtin_bit_cast(u32x2, v);
+        f[2 * u] = w[0];
+        f[2 * u + 1] = w[1];
+      }
+      return f;
+    } else {
+      const int col = lane & 31;
+      u32x4 f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 8 * t + 4 * h + j;
+        const uint32_t a = at(r, 8 * db + (col >> 2)) + (col & 3) * 4;
+        f[j] = *reinterpret_cast<const uint32_t*>(tile + blk * 32 * kPitch + a);
+      }
+      return f;
+    }
+  }
+};
+
+// Rows of a head on their way from memory to a tile, through registers: NT
+// threads hold the next tile while this one is computed with.  `left` rows
+// exist (others read zero without touching memory), chunks past `d` too.
+template <typename S, int DB, int R, int NT>
+struct TileStage {
+  using T = Tile<S, DB>;
+  static constexpr int kAll = R * T::kUsed;
+  static constexpr int kLoads = (kAll + NT - 1) / NT;
+  u32x4 v[kLoads];
+
+  __device__ __forceinline__ void load(const char* base, int ts_bytes, int left, int d_chunks, int tid) {
+    const int rows = left < 0 ? 0 : (left < R ? left : R);
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows * ts_bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int id = tid + i * NT, r = id / T::kUsed, c = id % T::kUsed;
+      const bool in = c < d_chunks && (kAll % NT == 0 || id < kAll);
+      const uint32_t off = in ? (uint32_t)(r * ts_bytes + c * 16) : kBufferOob;
+      v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int id = tid + i * NT, r = id / T::kUsed, c = id % T::kUsed;
+      if (kAll % NT == 0 || id < kAll) *reinterpret_cast<u32x4*>(tile + T::at(r, c)) = v[i];
+    }
+  }
+};
+
+// A wave's own 32 rows as fragments (row l % 32), from memory; rows from `left`
+// on and chunks from d_chunks on are zero.
+template <typename S, int DB>
+__device__ __forceinline__ void load_rows(const char* base, int ts_bytes, int left, int d_chunks, int lane,
+                                          u32x4 (&f)[Tile<S, DB>::kSteps]) {
+  const int rows = left < 0 ? 0 : (left < 32 ? left : 32);
+  const __amdgpu_buffer_rsrc_t rs =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows * ts_bytes, 0x00020000);
+#pragma unroll
+  for (int s = 0; s < Tile<S, DB>::kSteps; ++s) {
+    const int c = 2 * s + (lane >> 5);
+    f[s] = __builtin_bit_cast(
+        u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c < d_chunks ? (uint32_t)((lane & 31) * ts_bytes + c * 16) : kBufferOob, 0, 0));
+  }
+}
+
+// The transposed 32 x 32 DB result of a wave (lane: row l % 32 of the output,
+// its columns 32 db + 8 (i / 4) + 4 (l / 32) + i % 4) to rows of `ts` elements.
+template <typename S, int DB>
+__device__ __forceinline__ void store_rows(const floatx16 (&acc)[DB], float f, S* row, bool live, int d, int lane) {
+  const int h = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < DB; ++db) {
+    if constexpr (sizeof(S) == 2) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 8) {
+        // lanes l and l + 32 hold columns 0..3 | 4..7 and 8..11 | 12..15: exchanged, 0..7 and 8..15
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = Mma32<S>::pack2(acc[db][i + 2 * j] * f, acc[db][i + 2 * j + 1] * f);
+        const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+        const int col = 32 * db + 2 * i + 8 * h;
+        if (live && col < d) *reinterpret_cast<u32x4*>(row + col) = u32x4{a[0], b[0], a[1], b[1]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int col = 32 * db + 2 * i + 4 * h;
+        if (live && col < d)
+          *reinterpret_cast<u32x4*>(row + col) = u32x4{__float_as_uint(acc[db][i] * f), __float_as_uint(acc[db][i + 1] * f),
+                                                       __float_as_uint(acc[db][i + 2] * f), __float_as_uint(acc[db][i + 3] * f)};
+      }
+    }
+  }
+}
+
+// acc[db] += (columns of the tile's rows)^T p over NB blocks of 32 rows; p: what
+// the lane's own row weighs the tile's rows with.  Where some of the tile's
+// rows are not seen (check), a row that is not, but holds an infinity or NaN,
+// must not reach the result through 0 * inf: such a tile goes row by row, and
+// only rows that the lane sees are added.  seen(r): row r of the tile.
+template <typename S, int DB, int NB, typename F>
+__device__ __forceinline__ void add_columns(floatx16 (&acc)[DB], const char* tile, const u32x4 (&p)[NB][Tile<S, DB>::kColSteps],
+                                            bool check, int lane, F seen) {
+  using T = Tile<S, DB>;
+  if (check) {
+    bool bad = false;
+#pragma unroll
+    for (int blk = 0; blk < NB; ++blk)
+#pragma unroll 1
+      for (int t = 0; t < T::kColSteps; ++t)
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+          const u32x4 a = T::col_frag(tile, blk, t, db, lane);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bad |= Mma32<S>::nonfinite(a[j]);
+        }
+    if (__any(bad)) {
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+        for (int t = 0; t < T::kColSteps; ++t)
+#pragma unroll
+          for (int db = 0; db < DB; ++db) {
+            const u32x4 a = T::col_frag(tile, blk, t, db, lane);
+#pragma unroll 1
+            for (int e = 0; e < 2 * T::kE; ++e) {  // element e % E of lane half e / E
+              const int j = e % T::kE, half = e / T::kE;
+              u32x4 one = {0u, 0u, 0u, 0u};
+              if ((lane >> 5) == half) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                  if constexpr (sizeof(S) == 2) one[w] = w == (j >> 1) ? a[w] & (j & 1 ? 0xffff0000u : 0xffffu) : 0u;
+                  else one[w] = w == j ? a[w] : 0u;
+                }
+              }
+              floatx16 z;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) z[i] = 0.f;
+              z = Mma32<S>::fma(one, p[blk][t], z);
+              // the rows of acc_frag's order
+              const int r = 32 * blk + (sizeof(S) == 2 ? 16 * t + 8 * (j >> 2) + 4 * half + (j & 3) : 8 * t + 4 * half + j);
+              const bool s = seen(r);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[db][i] += s ? z[i] : 0.f;
+            }
+          }
+      return;
+    }
+  }
+#pragma unroll
+  for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+    for (int t = 0; t < T::kColSteps; ++t)
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = Mma32<S>::fma(T::col_frag(tile, blk, t, db, lane), p[blk][t], acc[db]);
+}
+
+// s = rows of block blk of the tile times the wave's own rows.
+template <typename S, int DB>
+__device__ __forceinline__ floatx16 row_products(const char* tile, int blk, const u32x4 (&own)[Tile<S, DB>::kSteps], int lane) {
+  floatx16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+  for (int t = 0; t < Tile<S, DB>::kSteps; ++t) s = Mma32<S>::fma(Tile<S, DB>::row_frag(tile, blk, t, lane), own[t], s);
+  return s;
+}
+
+__device__ __forceinline__ float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Row of a block of 32 that element i of a product is, for the lane's half.
+__device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+}  // namespace mhc

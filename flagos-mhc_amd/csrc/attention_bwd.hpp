@@ -1,0 +1,264 @@
+// Attention backward, from the forward's lse.
+//
+//   D_i = go_i . o_i,  P = exp(scale q k - lse),  dS = P (go v^T - D)
+//   dq = scale dS k,  dk = scale dS^T q,  dv = P^T go
+//
+// Two kernels, each of which recomputes P: one whose waves own 32 queries and
+// walk the keys (dq; it computes D first, for itself and the other), one
+// whose waves own 32 keys and walk the queries of every head that shares them
+// (dk, dv).  That is seven products instead of the five of one kernel, but no
+// sum is taken by atomics or in memory: results do not depend on an order,
+// and nothing but the gradients is written.
+//
+// P and dS are rounded to the operands' type for the products that sum them,
+// in fp16 with its limits: P below 2^-14 and dS outside 2^-14 .. 65504 lose
+// bits, as values of that type do.
+#pragma once
+
+#include "attention.hpp"
+#include "attention_fwd.hpp"
+
+namespace mhc {
+
+// dq, and D.
+template <typename S, int DB, int NW, int NB, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t slots) {
+  using T = Tile<S, DB>;
+  constexpr int BN = 32 * NB, BM = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
+  constexpr int kTileBytes = BN * T::kPitch;
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 x (K, V)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t slot;
+  int h, first;
+  att_item(slots, slot, h);
+  const AttSeq s = q_tile(a.n, slot, BM, first);
+  if (first >= s.lq) return;
+  const int hk = h / (a.n.H / a.n.Hk), d = a.n.d, dc = d * ES / 16;
+  const int row = first + 32 * wave + (lane & 31);
+  const bool live = row < s.lq;
+  S* out = static_cast<S*>(a.out) + ((s.row0 + row) * a.n.H + h) * (int64_t)d;
+  const int64_t stat = (int64_t)h * a.n.Tq + s.row0 + row;
+  const int shift = s.lk - s.lq;
+  const int block_last = (first + BM < s.lq ? first + BM : s.lq) - 1;
+  const int keys = s.none ? 0 : (a.n.causal ? min(s.lk, block_last + shift + 1) : s.lk);
+  if (keys <= 0) {
+    store_none<S, DB>(out, live, d, lane);
+    if (live && lane < 32) a.delta[stat] = 0.f;
+    return;
+  }
+  const int lim = a.n.causal ? min(s.lk - 1, row + shift) : s.lk - 1;
+  const int wave_first = first + 32 * wave;
+  const int wave_lo = a.n.causal ? min(s.lk - 1, wave_first + shift) : s.lk - 1;
+  const int wave_hi = a.n.causal ? min(s.lk - 1, wave_first + 31 + shift) : s.lk - 1;
+
+  const int q_ts = (int)(a.q.ts * ES), k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES), go_ts = (int)(a.go.ts * ES);
+  const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
+  TileStage<S, DB, BN, NT> sk, sv;
+  sk.load(kp, k_ts, s.lk, dc, tid);
+  sv.load(vp, v_ts, s.lk, dc, tid);
+
+  u32x4 q[T::kSteps], go[T::kSteps];
+  const int left = s.lq - wave_first;
+  load_rows<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, wave_first, h, ES), q_ts, left, dc, lane, q);
+  load_rows<S, DB>(row_ptr(a.go, a.n.cu_q, s.row0, s.b, wave_first, h, ES), go_ts, left, dc, lane, go);
+  float delta = 0.f;
+  {
+    u32x4 o[T::kSteps];
+    load_rows<S, DB>(row_ptr(a.o, a.n.cu_q, s.row0, s.b, wave_first, h, ES), (int)(a.o.ts * ES), left, dc, lane, o);
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      float x[Store<S>::VEC], y[Store<S>::VEC];
+      Store<S>::unpack(o[t], x);
+      Store<S>::unpack(go[t], y);
+#pragma unroll
+      for (int j = 0; j < Store<S>::VEC; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
+    }
+    delta = add_xor32(delta);
+    if (live && lane < 32) a.delta[stat] = delta;
+  }
+  const float lse = live ? a.lse[stat] : -__builtin_inff();
+  const float lse2 = lse == -__builtin_inff() ? __builtin_inff() : lse * kLog2e;  // an empty row: P = 0
+
+  sk.store(smem, tid);
+  sv.store(smem + kTileBytes, tid);
+  __syncthreads();
+
+  floatx16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+  const float c = a.scale2;
+  const int tiles = (keys + BN - 1) / BN, half = lane >> 5;
+  for (int t = 0; t < tiles; ++t) {
+    const char* tk = smem + (t & 1) * 2 * kTileBytes;
+    const char* tv = tk + kTileBytes;
+    const int k0 = t * BN;
+    if (t + 1 < tiles) {
+      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, dc, tid);
+      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, dc, tid);
+    }
+    if (k0 <= wave_hi) {
+      const bool masked = k0 + BN - 1 > wave_lo;
+      u32x4 p[NB][T::kColSteps];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        floatx16 sc = row_products<S, DB>(tk, b, q, lane);
+        floatx16 dp = row_products<S, DB>(tv, b, go, lane);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dp[i] = hw_exp2(__builtin_fmaf(sc[i], c, -lse2)) * (dp[i] - delta);
+        if (masked) {
+          const int left = lim - k0 - 4 * half;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[i] = 32 * b + acc_row(i, 0) <= left ? dp[i] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < T::kColSteps; ++u) p[b][u] = acc_frag<S>(dp, u);
+      }
+      add_columns<S, DB, NB>(acc, tk, p, masked, lane, [&](int r) { return k0 + r <= lim; });
+    }
+    if (t + 1 < tiles) {
+      char* nk = smem + ((t + 1) & 1) * 2 * kTileBytes;
+      sk.store(nk, tid);
+      sv.store(nk + kTileBytes, tid);
+      __syncthreads();
+    }
+  }
+  store_rows<S, DB>(acc, a.scale, out, live, d, lane);
+}
+
+// dk and dv.
+template <typename S, int DB, int NW, int NB, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_t slots) {
+  using T = Tile<S, DB>;
+  constexpr int BQ = 32 * NB, BK = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
+  constexpr int kTileBytes = BQ * T::kPitch, kStage = 2 * kTileBytes + 2 * BQ * 4;
+  static_assert(BQ <= NT, "a thread a row's lse and D");
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 x (Q, dO, lse, D)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t slot, row0;
+  int hk, first, rows;
+  const int64_t item = xcd_contig(blockIdx.x, gridDim.x);
+  hk = (int)(item / slots);
+  slot = item % slots;  // a head's first keys are seen by the most queries
+  const AttSeq s = k_tile(a.n, slot, BK, first, rows, row0);
+  if (first >= rows) return;
+  const int G = a.n.H / a.n.Hk, d = a.n.d, dc = d * ES / 16;
+  const int key = first + 32 * wave + (lane & 31);
+  const bool live = key < rows;
+  const int64_t at = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
+  S* dk = static_cast<S*>(a.dk) + at;
+  S* dv = static_cast<S*>(a.dv) + at;
+  const int shift = s.lk - s.lq;
+  // the first query that sees the block's first key
+  const int q_first = a.n.causal ? max(0, first - shift) : 0;
+  const int t0 = q_first / BQ, tiles = s.none || first >= s.lk || q_first >= s.lq ? 0 : (s.lq + BQ - 1) / BQ - t0;
+  if (tiles <= 0) {
+    store_none<S, DB>(dk, live, d, lane);
+    store_none<S, DB>(dv, live, d, lane);
+    return;
+  }
+  const int wave_first = first + 32 * wave;
+  const int q_ts = (int)(a.q.ts * ES), go_ts = (int)(a.go.ts * ES);
+  u32x4 k[T::kSteps], v[T::kSteps];
+  load_rows<S, DB>(row_ptr(a.k, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.k.ts * ES), s.lk - wave_first, dc, lane, k);
+  load_rows<S, DB>(row_ptr(a.v, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.v.ts * ES), s.lk - wave_first, dc, lane, v);
+
+  TileStage<S, DB, BQ, NT> sq, sg;
+  float st_lse = 0.f, st_delta = 0.f;
+  auto load = [&](int it) {
+    const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ;
+    sq.load(row_ptr(a.q, a.n.cu_q, s.row0, s.b, q0, h, ES), q_ts, s.lq - q0, dc, tid);
+    sg.load(row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, s.lq - q0, dc, tid);
+    if (tid < BQ) {
+      const bool in = q0 + tid < s.lq;
+      const int64_t i = (int64_t)h * a.n.Tq + s.row0 + q0 + tid;
+      const float l = in ? a.lse[i] : -__builtin_inff();
+      st_lse = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;  // no such row, or an empty one: P = 0
+      st_delta = in ? a.delta[i] : 0.f;
+    }
+  };
+  auto store = [&](char* to) {
+    sq.store(to, tid);
+    sg.store(to + kTileBytes, tid);
+    if (tid < BQ) {
+      reinterpret_cast<float*>(to + 2 * kTileBytes)[tid] = st_lse;
+      reinterpret_cast<float*>(to + 2 * kTileBytes)[BQ + tid] = st_delta;
+    }
+  };
+  load(0);
+  store(smem);
+  __syncthreads();
+
+  floatx16 ak[DB], av[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
+  const float c = a.scale2;
+  const int half = lane >> 5, items = tiles * G;
+  for (int it = 0; it < items; ++it) {
+    const char* tq = smem + (it & 1) * kStage;
+    const char* tg = tq + kTileBytes;
+    const float* stats = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
+    const int q0 = (t0 + it % tiles) * BQ;
+    if (it + 1 < items) load(it + 1);
+    // queries from here on see the lane's key; all of the wave's keys are seen by the tile or none
+    const int lim = a.n.causal ? key - shift : 0;
+    const bool any = wave_first < s.lk && (!a.n.causal || q0 + BQ - 1 >= wave_first - shift);
+    if (any) {
+      const bool masked = a.n.causal && q0 < wave_first + 31 - shift;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        floatx16 sc = row_products<S, DB>(tq, b, k, lane);
+        floatx16 dp = row_products<S, DB>(tg, b, v, lane);
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const floatx4 lse = *reinterpret_cast<const floatx4*>(stats + 32 * b + acc_row(i, half));
+          const floatx4 del = *reinterpret_cast<const floatx4*>(stats + BQ + 32 * b + acc_row(i, half));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            sc[i + j] = hw_exp2(__builtin_fmaf(sc[i + j], c, -lse[j]));
+            dp[i + j] = sc[i + j] * (dp[i + j] - del[j]);
+          }
+        }
+        if (masked) {
+          const int from = lim - q0 - 4 * half;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const bool in = 32 * b + acc_row(i, 0) >= from;
+            sc[i] = in ? sc[i] : 0.f;
+            dp[i] = in ? dp[i] : 0.f;
+          }
+        }
+        u32x4 p[1][T::kColSteps], ds[1][T::kColSteps];
+#pragma unroll
+        for (int u = 0; u < T::kColSteps; ++u) {
+          p[0][u] = acc_frag<S>(sc, u);
+          ds[0][u] = acc_frag<S>(dp, u);
+        }
+        const auto seen = [&](int r) { return q0 + 32 * b + r >= lim; };
+        add_columns<S, DB, 1>(av, tg + b * 32 * T::kPitch, p, masked, lane, seen);
+        add_columns<S, DB, 1>(ak, tq + b * 32 * T::kPitch, ds, masked, lane, seen);
+      }
+    }
+    if (it + 1 < items) {
+      store(smem + ((it + 1) & 1) * kStage);
+      __syncthreads();
+    }
+  }
+  // keys past the sequence's are zero rows of k, but no zero rows of dk
+  const bool has = key < s.lk;
+  if (!has) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
+  }
+  store_rows<S, DB>(ak, a.scale, dk, live, d, lane);
+  store_rows<S, DB>(av, 1.f, dv, live, d, lane);
+}
+
+}  // namespace mhc

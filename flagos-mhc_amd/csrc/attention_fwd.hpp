@@ -1,0 +1,148 @@
+// Attention forward: a block takes 32 NW queries of one head, a wave 32 of
+// them, and walks the keys they see in tiles of 32 NB, one pass with a running
+// maximum and sum.
+#pragma once
+
+#include "attention.hpp"
+
+namespace mhc {
+
+// Items (tile of queries, head): an XCD walks a contiguous run of heads, so
+// that the blocks it runs at a time read the same keys and values from its L2;
+// a head's tiles go from its last to its first, since under a causal mask the
+// last ones are the longest.
+__device__ __forceinline__ void att_item(int64_t slots, int64_t& slot, int& h) {
+  const int64_t item = xcd_contig(blockIdx.x, gridDim.x);
+  h = (int)(item / slots);
+  slot = slots - 1 - item % slots;
+}
+
+template <typename S, int DB>
+__device__ __forceinline__ void store_none(S* row, bool live, int d, int lane) {
+  floatx16 z[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[db][i] = 0.f;
+  store_rows<S, DB>(z, 0.f, row, live, d, lane);
+}
+
+template <typename S, int DB, int NW, int NB, int WPE>
+__global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_t slots) {
+  using T = Tile<S, DB>;
+  constexpr int BN = 32 * NB, BM = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
+  constexpr int kTileBytes = BN * T::kPitch;
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 x (K, V)
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int64_t slot;
+  int h, first;
+  att_item(slots, slot, h);
+  const AttSeq s = q_tile(a.n, slot, BM, first);
+  if (first >= s.lq) return;
+  const int hk = h / (a.n.H / a.n.Hk), d = a.n.d, dc = d * ES / 16;
+  const int row = first + 32 * wave + (lane & 31);  // the lane's query
+  const bool live = row < s.lq;
+  S* out = static_cast<S*>(a.out) + ((s.row0 + row) * a.n.H + h) * (int64_t)d;
+  const int shift = s.lk - s.lq;
+  // keys that the block's last query sees, and this lane's
+  const int block_last = (first + BM < s.lq ? first + BM : s.lq) - 1;
+  const int keys = s.none ? 0 : (a.n.causal ? min(s.lk, block_last + shift + 1) : s.lk);
+  if (keys <= 0) {
+    store_none<S, DB>(out, live, d, lane);
+    if (a.lse && live && lane < 32) a.lse[(int64_t)h * a.n.Tq + s.row0 + row] = -__builtin_inff();
+    return;
+  }
+  const int lim = a.n.causal ? min(s.lk - 1, row + shift) : s.lk - 1;  // last key the lane sees
+  const int wave_first = first + 32 * wave;
+  const int wave_lo = a.n.causal ? min(s.lk - 1, wave_first + shift) : s.lk - 1;       // seen by all of the wave
+  const int wave_hi = a.n.causal ? min(s.lk - 1, wave_first + 31 + shift) : s.lk - 1;  // by any
+
+  const int q_ts = (int)(a.q.ts * ES), k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES);
+  u32x4 q[T::kSteps];
+  load_rows<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, wave_first, h, ES), q_ts, s.lq - wave_first, dc, lane, q);
+  const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
+
+  TileStage<S, DB, BN, NT> sk, sv;
+  sk.load(kp, k_ts, s.lk, dc, tid);
+  sv.load(vp, v_ts, s.lk, dc, tid);
+  sk.store(smem, tid);
+  sv.store(smem + kTileBytes, tid);
+  __syncthreads();
+
+  floatx16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;  // reference point (powers of two) and the lane's share of the sum
+  const float c = a.scale2;
+  const int tiles = (keys + BN - 1) / BN, half = lane >> 5;
+  for (int t = 0; t < tiles; ++t) {
+    const char* tk = smem + (t & 1) * 2 * kTileBytes;
+    const char* tv = tk + kTileBytes;
+    const int k0 = t * BN;
+    if (t + 1 < tiles) {
+      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, dc, tid);
+      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, dc, tid);
+    }
+    if (k0 <= wave_hi) {
+      floatx16 sc[NB];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) sc[b] = row_products<S, DB>(tk, b, q, lane);
+      const bool masked = k0 + BN - 1 > wave_lo;
+      if (masked) {
+        const int left = lim - k0 - 4 * half;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[b][i] = 32 * b + acc_row(i, 0) <= left ? sc[b][i] : -__builtin_inff();
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[b][i]);
+      top = max_xor32(top) * c;
+      if (__any(top > m + kLazyMax || m == -__builtin_inff())) {
+        const float mn = fmaxf(m, top);
+        const float f = mn == -__builtin_inff() ? 1.f : hw_exp2(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+      }
+      const float ref = m == -__builtin_inff() ? 0.f : m;
+      u32x4 p[NB][T::kColSteps];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[b][i] = hw_exp2(__builtin_fmaf(sc[b][i], c, -ref));
+          l += sc[b][i];
+        }
+        // p is rounded to the type of v, the sum is of the unrounded values
+#pragma unroll
+        for (int u = 0; u < T::kColSteps; ++u) p[b][u] = acc_frag<S>(sc[b], u);
+      }
+      add_columns<S, DB, NB>(acc, tv, p, masked, lane, [&](int r) { return k0 + r <= lim; });
+    }
+    if (t + 1 < tiles) {
+      char* nk = smem + ((t + 1) & 1) * 2 * kTileBytes;
+      sk.store(nk, tid);
+      sv.store(nk + kTileBytes, tid);
+      __syncthreads();
+    }
+  }
+  l = add_xor32(l);
+  // (a NaN among the scores leaves l NaN: not the empty row's zero)
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  store_rows<S, DB>(acc, inv, out, live, d, lane);
+  if (a.lse && live && lane < 32)
+    a.lse[(int64_t)h * a.n.Tq + s.row0 + row] = l == 0.f ? -__builtin_inff() : m * kLn2 + __logf(l);
+}
+
+}  // namespace mhc

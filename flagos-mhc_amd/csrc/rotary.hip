@@ -1,0 +1,177 @@
+// Rotary positions of the queries and keys, forward and inverse.
+//
+//   (a, b) -> amplitude (a cos w - b sin w, a sin w + b cos w),  w = position * freq_i
+//
+// for the r / 2 pairs of a head's first r elements: (i, i + r / 2) or
+// (2 i, 2 i + 1); elements past r are copied.  The backward is the rotation by
+// -w.  A position's angles are the same for every head: a block takes a few
+// tokens, computes their sines and cosines once, into LDS, and rotates every
+// head of both tensors with them, so that nothing but q and k is read and
+// written.  Angles are reduced in 64 bits (turns = position * freq / 2 pi, less
+// their nearest integer): in 32 a position of 10^6 would be off by 0.06.
+#include "attention.hpp"
+#include "mhc_launch.hpp"
+
+namespace mhc {
+namespace {
+
+struct RotArgs {
+  const void* x[2];         // q, k
+  void* y[2];               // contiguous
+  int64_t ts[2], hs[2];     // elements
+  int heads[2];
+  const double* freqs;      // radians a position
+  const void* positions;    // (T,) int32 or int64, or null: from cu or t % S
+  const int32_t* cu;
+  int64_t T, S;
+  int wide, B;              // wide: positions are int64
+  int d, r;
+  float amplitude;
+  int sign;
+};
+
+// Tokens before t of t's own sequence: 64 candidates a step, one a lane.
+__device__ __forceinline__ int64_t packed_position(const int32_t* cu, int B, int64_t T, int64_t t) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, n = B + 1;
+  while (n > 1) {
+    const int step = (n + 63) / 64, c = lane * step;
+    int hit = __popcll(__ballot(c < n && cu_at(cu, lo + c, T) <= t));
+    hit = hit < 1 ? 1 : hit;
+    const int skip = (hit - 1) * step;
+    lo += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  return t - cu_at(cu, lo, T);
+}
+
+constexpr int kThreads = 256, kTrig = 2048;  // float2 of LDS: tokens * r / 2 at most
+
+// VEC: elements of an access; 1: any layout and alignment.
+template <typename S, int VEC, bool HALF>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(RotArgs a, int tokens) {
+  __shared__ float2 trig[kTrig];
+  const int64_t t0 = xcd_contig(blockIdx.x, gridDim.x) * tokens;
+  const int n = (int)(a.T - t0 < tokens ? a.T - t0 : tokens), half = a.r / 2, wave = threadIdx.x >> 6;
+  for (int i = wave; i < n; i += kThreads / 64) {
+    const int64_t t = t0 + i;
+    int64_t p;
+    if (a.positions) p = a.wide ? static_cast<const int64_t*>(a.positions)[t] : static_cast<const int32_t*>(a.positions)[t];
+    else if (a.cu) p = packed_position(a.cu, a.B, a.T, t);
+    else p = t % a.S;
+    for (int j = threadIdx.x & 63; j < half; j += 64) {
+      const double turns = (double)p * (a.freqs[j] * 0.15915494309189533577);
+      const float f = (float)(turns - rint(turns));
+      float sn, cs;
+      sincospif(2.f * f, &sn, &cs);
+      trig[i * half + j] = make_float2(cs * a.amplitude, a.sign < 0 ? -sn * a.amplitude : sn * a.amplitude);
+    }
+  }
+  __syncthreads();
+  // a head's items: pairs of vectors (HALF) or vectors of pairs, then what is copied
+  const int rot = HALF ? half / VEC : (VEC == 1 ? half : a.r / VEC), copies = (a.d - a.r) / VEC, per = rot + copies;
+  const int heads = a.heads[0] + a.heads[1], all = n * heads * per;
+  for (int id = threadIdx.x; id < all; id += kThreads) {
+    const int item = id % per, th = id / per;
+    int h = th % heads;
+    const int i = th / heads;
+    const int64_t t = t0 + i;
+    const int w = h >= a.heads[0];
+    h -= w ? a.heads[0] : 0;
+    const S* x = static_cast<const S*>(a.x[w]) + t * a.ts[w] + (int64_t)h * a.hs[w];
+    S* y = static_cast<S*>(a.y[w]) + (t * a.heads[w] + h) * (int64_t)a.d;
+    const float2* cs = trig + i * half;
+    if (item >= rot) {
+      const int e = a.r + (item - rot) * VEC;
+      if constexpr (VEC == 1) store_elem<S>(y, e, load_elem<S>(x, e));
+      else st16nt(y + e, ld16nt(x + e));
+    } else if constexpr (VEC == 1) {
+      const int i0 = HALF ? item : 2 * item, i1 = HALF ? item + half : i0 + 1;
+      const float u = load_elem<S>(x, i0), v = load_elem<S>(x, i1);
+      const float2 q = cs[item];
+      store_elem<S>(y, i0, u * q.x - v * q.y);
+      store_elem<S>(y, i1, u * q.y + v * q.x);
+    } else if constexpr (HALF) {
+      const int e = item * VEC;
+      float u[VEC], v[VEC];
+      Store<S>::unpack(ld16nt(x + e), u);
+      Store<S>::unpack(ld16nt(x + half + e), v);
+      float p[VEC], q[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const float2 z = cs[e + j];
+        p[j] = u[j] * z.x - v[j] * z.y;
+        q[j] = u[j] * z.y + v[j] * z.x;
+      }
+      st16nt(y + e, Store<S>::pack(p));
+      st16nt(y + half + e, Store<S>::pack(q));
+    } else {
+      const int e = item * VEC;
+      float u[VEC];
+      Store<S>::unpack(ld16nt(x + e), u);
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        const float2 z = cs[(e + j) / 2];
+        const float p = u[j] * z.x - u[j + 1] * z.y;
+        u[j + 1] = u[j] * z.y + u[j + 1] * z.x;
+        u[j] = p;
+      }
+      st16nt(y + e, Store<S>::pack(u));
+    }
+  }
+}
+
+template <typename S>
+int rotary_run(const RotArgs& a, bool half_layout, hipStream_t st) {
+  constexpr int VEC = Store<S>::VEC;
+  const int half = a.r / 2;
+  bool vec = a.d % VEC == 0 && a.r % VEC == 0 && (!half_layout || half % VEC == 0);
+  for (int w = 0; w < 2; ++w)
+    if (a.heads[w])
+      vec = vec && aligned16(a.x[w]) && aligned16(a.y[w]) && a.ts[w] % VEC == 0 && a.hs[w] % VEC == 0;
+  // four tokens a block (a wave a token's angles) where there are blocks enough
+  int tokens = a.T >= (int64_t)device_cu_count() * 16 ? 4 : 1;
+  while (tokens > 1 && tokens * half > kTrig) tokens /= 2;
+  const int64_t blocks = (a.T + tokens - 1) / tokens;
+  if (blocks > 0xffffffffll / kThreads)
+    return set_error(MHC_ERR_UNSUPPORTED, "rotary: %lld rows exceed a dispatch", (long long)a.T);
+  const dim3 g((unsigned)blocks), b(kThreads);
+  if (vec && half_layout) hipLaunchKernelGGL((rotary_kernel<S, VEC, true>), g, b, 0, st, a, tokens);
+  else if (vec) hipLaunchKernelGGL((rotary_kernel<S, VEC, false>), g, b, 0, st, a, tokens);
+  else if (half_layout) hipLaunchKernelGGL((rotary_kernel<S, 1, true>), g, b, 0, st, a, tokens);
+  else hipLaunchKernelGGL((rotary_kernel<S, 1, false>), g, b, 0, st, a, tokens);
+  return check_launch("rotary");
+}
+
+}  // namespace
+}  // namespace mhc
+
+using namespace mhc;
+
+extern "C" int mhc_rotary(const void* q, const void* k, int32_t dtype, int64_t q_row, int64_t q_head, int64_t k_row,
+                          int64_t k_head, const double* freqs, const void* positions, int32_t positions_wide,
+                          const int32_t* cu_seqlens, int32_t sequences, int64_t length, int32_t layout, float amplitude,
+                          int32_t inverse, void* q_out, void* k_out, int64_t T, int32_t heads, int32_t heads_k, int32_t d,
+                          int32_t r, void* stream) {
+  clear_error();
+  if (T < 0 || heads < 1 || heads_k < 0 || d < 1 || r < 0 || r > d || r % 2 || (layout != 0 && layout != 1))
+    return set_error(MHC_ERR_INVALID, "rotary: T=%lld heads=%d heads_k=%d d=%d r=%d layout=%d", (long long)T, heads, heads_k,
+                     d, r, layout);
+  if (dtype != MHC_DTYPE_F32 && dtype != MHC_DTYPE_BF16 && dtype != MHC_DTYPE_F16)
+    return set_error(MHC_ERR_UNSUPPORTED, "rotary: dtype %d not supported", dtype);
+  if (r > 2 * kTrig) return set_error(MHC_ERR_UNSUPPORTED, "rotary: r=%d above the supported %d", r, 2 * kTrig);
+  // a block's items are counted in 32 bits
+  if (((int64_t)heads + heads_k) * d > (1 << 28))
+    return set_error(MHC_ERR_UNSUPPORTED, "rotary: heads=%d heads_k=%d d=%d above the supported sizes", heads, heads_k, d);
+  if (q_row < 0 || q_head < 0 || k_row < 0 || k_head < 0) return set_error(MHC_ERR_INVALID, "rotary: negative stride");
+  if (!positions && !cu_seqlens && length < 1) return set_error(MHC_ERR_INVALID, "rotary: length %lld", (long long)length);
+  if (cu_seqlens && sequences < 0) return set_error(MHC_ERR_INVALID, "rotary: sequences %d", sequences);
+  if (T == 0) return MHC_OK;
+  if (!q || !q_out || (heads_k && (!k || !k_out)) || (r && !freqs)) return set_error(MHC_ERR_INVALID, "rotary: null pointer");
+  const RotArgs a = {{q, k}, {q_out, k_out}, {q_row, k_row}, {q_head, k_head}, {heads, heads_k}, freqs, positions, cu_seqlens,
+                     T, length, positions_wide, sequences, d, r, amplitude, inverse ? -1 : 1};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == MHC_DTYPE_F32) return rotary_run<float>(a, layout == 0, st);
+  if (dtype == MHC_DTYPE_BF16) return rotary_run<bf16_t>(a, layout == 0, st);
+  return rotary_run<f16_t>(a, layout == 0, st);
+}

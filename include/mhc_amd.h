@@ -389,6 +389,78 @@ int mhc_gated_ffn_bwd(const void* grad_out, const void* x, const void* w_gate, c
 int mhc_dropout(const void* x, void* y, int64_t n, int32_t dtype, double p, uint64_t seed,
                 uint64_t offset, const uint64_t* state, void* stream);
 
+/*
+ * Rotary positions of q (T, heads, d) and k (T, heads_k, d; heads_k == 0:
+ * none), all `dtype`, any element alignment; rows and heads `*_row` and
+ * `*_head` elements apart, a head's elements side by side:
+ *   (a, b) -> amplitude (a cos w - b sin w, a sin w + b cos w), w = position * freqs[i]
+ * for the r / 2 pairs (i, i + r / 2) (layout 0) or (2 i, 2 i + 1) (layout 1)
+ * of the first r elements; the others are copied.  inverse: by -w (the
+ * backward).  freqs: (r / 2,) device doubles, radians a position; angles are
+ * reduced in 64 bits.  A row's position: positions[t] (int32, or int64 with
+ * positions_wide), else its place in its packed sequence (cu_seqlens:
+ * (sequences + 1,) first rows, the first one 0; rows behind the last sequence
+ * count from its end), else t % length.  q_out, k_out: contiguous, not q or k.
+ * r <= 4096, (heads + heads_k) * d <= 2^28.
+ */
+#define MHC_ROTARY_HALF 0
+#define MHC_ROTARY_INTERLEAVED 1
+int mhc_rotary(const void* q, const void* k, int32_t dtype, int64_t q_row, int64_t q_head, int64_t k_row,
+               int64_t k_head, const double* freqs, const void* positions, int32_t positions_wide,
+               const int32_t* cu_seqlens, int32_t sequences, int64_t length, int32_t layout, float amplitude,
+               int32_t inverse, void* q_out, void* k_out, int64_t T, int32_t heads, int32_t heads_k, int32_t d,
+               int32_t r, void* stream);
+
+/*
+ * Attention of `heads` query heads over `heads_k` key heads (a divisor; head h
+ * goes with key head h / (heads / heads_k)):
+ *   out_i = sum_j exp(scale q_i . k_j - lse_i) v_j, lse_i = ln sum_j exp(scale q_i . k_j)
+ * over the keys j < Lk of i's sequence and, if causal, j <= i + Lk - Lq: the
+ * Lq queries are the last of the Lk positions.  A query that sees no key has
+ * out 0 and lse -infinity.
+ *
+ * Element (sequence b, row t, head h, i) of q is q[b * q_stride[0] + t *
+ * q_stride[1] + h * q_stride[2] + i], strides in elements; k and v likewise.
+ * Addresses and strides are whole 16 bytes, d whole 16 bytes and at most 512,
+ * a row stride at least d and at most 2^24 bytes.
+ * With cu_seqlens_q ((sequences + 1,) device int32, the first one taken as 0)
+ * sequence b has the rows cu_seqlens_q[b] up to cu_seqlens_q[b + 1] of rows_q
+ * (q_stride[0] unused); without, rows_q / sequences rows.  The keys likewise
+ * by cu_seqlens_k, or rows_k / sequences, of which lengths_k[b] (device int32,
+ * or NULL: all) count; rows past them are not read.  Both are kept within the
+ * buffers: wrong entries give wrong results, but no access outside.  Rows
+ * behind the last packed sequence get out 0, lse -infinity and gradients 0.
+ */
+typedef struct {
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* sequence, row, head */
+  const int32_t *cu_seqlens_q, *cu_seqlens_k, *lengths_k;
+  int64_t rows_q, rows_k;
+  int32_t sequences, heads, heads_k, d, dtype, causal;
+  float scale; /* > 0 */
+  int32_t reserved; /* 0 */
+} mhc_attention_args;
+
+/*
+ * out: (rows_q, heads, d) `dtype`, 16-byte aligned; lse: (heads, rows_q) fp32
+ * or NULL.  Sums and statistics are fp32; exp(..) is rounded to `dtype` for
+ * the product with v.
+ */
+size_t mhc_attention_fwd_workspace_size(const mhc_attention_args* args);
+int mhc_attention_fwd(const mhc_attention_args* args, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
+ * Backward from the forward's out and lse: grad_q (rows_q, heads, d), grad_k
+ * and grad_v (rows_k, heads_k, d), `dtype`, 16-byte aligned; grad_out has
+ * strides grad_stride[3] as q.  Deterministic.  The gradients of the scores
+ * and the weights are rounded to `dtype` between the products.
+ */
+size_t mhc_attention_bwd_workspace_size(const mhc_attention_args* args);
+int mhc_attention_bwd(const mhc_attention_args* args, const void* grad_out, const int64_t* grad_stride, const void* out,
+                      const float* lse, void* grad_q, void* grad_k, void* grad_v, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
