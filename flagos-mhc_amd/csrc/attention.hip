@@ -4,14 +4,14 @@
 
 namespace mhc {
 
-template <typename S> int att_fwd(const AttArgs&, void* ws, hipStream_t);
-template <typename S> int att_bwd(const AttArgs&, void* ws, hipStream_t);
-extern template int att_fwd<float>(const AttArgs&, void*, hipStream_t);
-extern template int att_fwd<bf16_t>(const AttArgs&, void*, hipStream_t);
-extern template int att_fwd<f16_t>(const AttArgs&, void*, hipStream_t);
-extern template int att_bwd<float>(const AttArgs&, void*, hipStream_t);
-extern template int att_bwd<bf16_t>(const AttArgs&, void*, hipStream_t);
-extern template int att_bwd<f16_t>(const AttArgs&, void*, hipStream_t);
+template <typename S> int att_fwd(const AttArgs&, hipStream_t);
+template <typename S> int att_bwd(const AttArgs&, hipStream_t);
+extern template int att_fwd<float>(const AttArgs&, hipStream_t);
+extern template int att_fwd<bf16_t>(const AttArgs&, hipStream_t);
+extern template int att_fwd<f16_t>(const AttArgs&, hipStream_t);
+extern template int att_bwd<float>(const AttArgs&, hipStream_t);
+extern template int att_bwd<bf16_t>(const AttArgs&, hipStream_t);
+extern template int att_bwd<f16_t>(const AttArgs&, hipStream_t);
 
 namespace {
 
@@ -70,7 +70,11 @@ int check_att(const char* who, const mhc_attention_args* c, AttArgs& a) {
 
 using namespace mhc;
 
-extern "C" size_t mhc_attention_fwd_workspace_size(const mhc_attention_args* c) { return 0; }
+extern "C" size_t mhc_attention_fwd_workspace_size(const mhc_attention_args* c) {
+  AttArgs a;
+  if (check_att("", c, a)) return 0;
+  return att_split(a.n, device_cu_count()).bytes(a.n);
+}
 
 extern "C" int mhc_attention_fwd(const mhc_attention_args* c, void* out, float* lse, void* workspace, size_t workspace_bytes,
                                  void* stream) {
@@ -79,12 +83,17 @@ extern "C" int mhc_attention_fwd(const mhc_attention_args* c, void* out, float* 
   if (const int rc = check_att("attention", c, a)) return rc;
   if (c->rows_q == 0) return MHC_OK;
   if (!out || !aligned16(out)) return set_error(MHC_ERR_INVALID, "attention: out is null or not 16-byte aligned");
+  const size_t need = att_split(a.n, device_cu_count()).bytes(a.n);
+  if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+    return set_error(MHC_ERR_INVALID, "attention: workspace too small or not 16-byte aligned (%zu < %zu bytes)",
+                     workspace ? workspace_bytes : (size_t)0, need);
   a.out = out;
   a.lse = lse;
+  a.part = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (c->dtype == MHC_DTYPE_F32) return att_fwd<float>(a, workspace, st);
-  if (c->dtype == MHC_DTYPE_BF16) return att_fwd<bf16_t>(a, workspace, st);
-  return att_fwd<f16_t>(a, workspace, st);
+  if (c->dtype == MHC_DTYPE_F32) return att_fwd<float>(a, st);
+  if (c->dtype == MHC_DTYPE_BF16) return att_fwd<bf16_t>(a, st);
+  return att_fwd<f16_t>(a, st);
 }
 
 extern "C" size_t mhc_attention_bwd_workspace_size(const mhc_attention_args* c) {
@@ -119,7 +128,7 @@ extern "C" int mhc_attention_bwd(const mhc_attention_args* c, const void* grad_o
   a.lse = const_cast<float*>(lse);
   a.delta = static_cast<float*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (c->dtype == MHC_DTYPE_F32) return att_bwd<float>(a, workspace, st);
-  if (c->dtype == MHC_DTYPE_BF16) return att_bwd<bf16_t>(a, workspace, st);
-  return att_bwd<f16_t>(a, workspace, st);
+  if (c->dtype == MHC_DTYPE_F32) return att_bwd<float>(a, st);
+  if (c->dtype == MHC_DTYPE_BF16) return att_bwd<bf16_t>(a, st);
+  return att_bwd<f16_t>(a, st);
 }

@@ -176,8 +176,10 @@ template <> struct Mma32<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
   __device__ static uint32_t pack2(float lo, float hi) { return pack_bf16x2(lo, hi); }
-  __device__ static bool nonfinite(uint32_t w) {
-    return (w & 0x7f800000u) == 0x7f800000u || (w & 0x7f80u) == 0x7f80u;
+  // w with infinities and NaNs as zero
+  __device__ static uint32_t finite(uint32_t w) {
+    w = (w & 0x7f800000u) == 0x7f800000u ? w & 0xffffu : w;
+    return (w & 0x7f80u) == 0x7f80u ? w & 0xffff0000u : w;
   }
 };
 template <> struct Mma32<f16_t> {
@@ -186,8 +188,9 @@ template <> struct Mma32<f16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_att, a), __builtin_bit_cast(f16x8_att, b), c, 0, 0, 0);
   }
   __device__ static uint32_t pack2(float lo, float hi) { return f32_to_f16_bits(lo) | (f32_to_f16_bits(hi) << 16); }
-  __device__ static bool nonfinite(uint32_t w) {
-    return (w & 0x7c000000u) == 0x7c000000u || (w & 0x7c00u) == 0x7c00u;
+  __device__ static uint32_t finite(uint32_t w) {
+    w = (w & 0x7c000000u) == 0x7c000000u ? w & 0xffffu : w;
+    return (w & 0x7c00u) == 0x7c00u ? w & 0xffff0000u : w;
   }
 };
 template <> struct Mma32<float> {
@@ -198,7 +201,7 @@ template <> struct Mma32<float> {
       c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
     return c;
   }
-  __device__ static bool nonfinite(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u; }
+  __device__ static uint32_t finite(uint32_t w) { return (w & 0x7f800000u) == 0x7f800000u ? 0u : w; }
 };
 
 // The fragment of elements E t .. E t + E - 1 of the 16 that a product left a
@@ -216,6 +219,9 @@ __device__ __forceinline__ u32x4 acc_frag(const floatx16& s, int t) {
   return f;
 }
 
+// Row of a block of 32 that element i of a product is, for the lane's half.
+__device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
 // ---- tiles ----------------------------------------------------------------------
 // R rows of a head as they lie in memory, in chunks of 16 bytes whose position
 // within the row is exclusive-ored with a function of the row.  Two kinds of
@@ -223,6 +229,15 @@ __device__ __forceinline__ u32x4 acc_frag(const floatx16& s, int t) {
 // 4 rows of 4 chunks (16-bit columns, one transposing read of 32 lanes) or
 // rows j and j + 4 of 8 chunks (fp32 columns).  Rows of 256 bytes start at
 // the same bank, those of 128 at alternating halves.
+//
+// Addresses are a lane's two base registers, exclusive-ored with constants and
+// added to a tile's place: kept as they are they cost one instruction a read,
+// whereas all of them hoisted out of a loop would cost a register each.
+
+typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) const uint32_t lds_u32;
+typedef __attribute__((address_space(3))) s16x4_att lds_s16x4;
+
 template <typename S, int DB>
 struct Tile {
   static constexpr int kEs = (int)sizeof(S);
@@ -234,6 +249,7 @@ struct Tile {
   static constexpr int kUsed = kD * kEs / 16;    // chunks that are loaded
   static constexpr int kSteps = kUsed / 2;       // row fragments
   static constexpr int kColSteps = 16 / kE;      // column fragments of 32 rows
+  static constexpr int kLow = kChunks >= 16 ? 16 : 8;  // chunks whose position is exclusive-ored
 
   static __device__ __forceinline__ int swizzle(int r) {
     if constexpr (kEs == 4) return ((r & 4) << 1) | ((r & 8) >> 1) | (r & 3);
@@ -242,79 +258,90 @@ struct Tile {
   }
   static __device__ __forceinline__ uint32_t at(int r, int c) { return (uint32_t)(r * kPitch + ((c ^ swizzle(r)) * 16)); }
 
+  uint32_t row, col;  // a lane's base addresses
+
+  __device__ __forceinline__ explicit Tile(int lane) {
+    const int h = lane >> 5, i = lane & 15, g = (lane >> 4) & 1;
+    row = at(lane & 31, h);
+    if constexpr (kEs == 2) col = at(4 * h + (i >> 2), 2 * g + ((i & 3) >> 1)) + (i & 1) * 8;
+    else col = at(4 * h, (lane & 31) >> 2) + (lane & 3) * 4;
+  }
+  // What follows is not to be computed before a loop that this stands in.
+  __device__ __forceinline__ void keep() { asm volatile("" : "+v"(row), "+v"(col)); }
+
   // Row fragment: row 32 blk + l % 32, chunk 2 step + l / 32.
-  static __device__ __forceinline__ u32x4 row_frag(const char* tile, int blk, int step, int lane) {
-    const int r = lane & 31, h = lane >> 5;
-    const uint32_t a = (uint32_t)(r * kPitch) + (uint32_t)((h ^ swizzle(r)) * 16);
-    // (chunks are exclusive-ored in their low bits only)
-    constexpr int kLow = kChunks >= 16 ? 16 : 8;
+  __device__ __forceinline__ u32x4 row_frag(uint32_t tile, int blk, int step) const {
     const int c = 2 * step;
-    return *reinterpret_cast<const u32x4*>(tile + blk * 32 * kPitch + ((a ^ (uint32_t)((c % kLow) * 16)) + (c / kLow) * kLow * 16));
+    return *(lds_u32x4*)(uintptr_t)((row ^ (uint32_t)((c % kLow) * 16)) + tile + blk * 32 * kPitch + (c / kLow) * kLow * 16);
   }
 
   // Column fragment: column 32 db + l % 32; rows of step t of block blk in the
   // order of acc_frag.
-  static __device__ __forceinline__ u32x4 col_frag(const char* tile, int blk, int t, int db, int lane) {
-    const int h = lane >> 5;
+  __device__ __forceinline__ u32x4 col_frag(uint32_t tile, int blk, int t, int db) const {
+    u32x4 f;
     if constexpr (kEs == 2) {
-      const int i = lane & 15, g = (lane >> 4) & 1;
-      u32x4 f;
+      constexpr int kDbs = kLow / 4;  // blocks of 32 columns within the exclusive-ored bits
+      const uint32_t at = tile + (blk * 32 + t * 16) * kPitch + (db / kDbs) * kLow * 16;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int r = 8 * u + 4 * h + (i >> 2);
-        const int c = 2 * g + ((i & 3) >> 1);
-        const uint32_t a = (uint32_t)(r * kPitch) + (uint32_t)((c ^ swizzle(r)) * 16) + (i & 1) * 8;
-        constexpr int kLow = kChunks >= 16 ? 4 : 2;  // blocks of 32 columns within the exclusive-ored bits
-        const char* p = tile + (blk * 32 + t * 16) * kPitch + ((a ^ (uint32_t)((db % kLow) * 64)) + (db / kLow) * kLow * 64);
         const s16x4_att v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4_att*)reinterpret_cast<const s16x4_att*>(p));
+            (lds_s16x4*)(uintptr_t)((col ^ (uint32_t)((db % kDbs) * 64 + 32 * u)) + at + 8 * u * kPitch));
         const u32x2 w = __builtin_bit_cast(u32x2, v);
         f[2 * u] = w[0];
         f[2 * u + 1] = w[1];
       }
-      return f;
     } else {
-      const int col = lane & 31;
-      u32x4 f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 8 * t + 4 * h + j;
-        const uint32_t a = at(r, 8 * db + (col >> 2)) + (col & 3) * 4;
-        f[j] = *reinterpret_cast<const uint32_t*>(tile + blk * 32 * kPitch + a);
-      }
-      return f;
+      for (int j = 0; j < 4; ++j)
+        f[j] = *(lds_u32*)(uintptr_t)((col ^ (uint32_t)(((db & 1) * 8 + (t & 1) * 4 + j) * 16)) + tile +
+                                      (blk * 32 + 8 * t + j) * kPitch + (db >> 1) * 256);
     }
+    return f;
   }
 };
 
 // Rows of a head on their way from memory to a tile, through registers: NT
 // threads hold the next tile while this one is computed with.  `left` rows
-// exist (others read zero without touching memory), chunks past `d` too.
+// exist (others read zero without touching memory), chunks past `d` too.  A
+// thread's loads differ in the resource's base alone.
 template <typename S, int DB, int R, int NT>
 struct TileStage {
   using T = Tile<S, DB>;
-  static constexpr int kAll = R * T::kUsed;
-  static constexpr int kLoads = (kAll + NT - 1) / NT;
+  static_assert(NT % T::kUsed == 0 && R * T::kUsed % NT == 0, "a thread keeps its chunk");
+  static constexpr int kRows = NT / T::kUsed;  // of a load
+  static constexpr int kLoads = R / kRows;
   u32x4 v[kLoads];
 
-  __device__ __forceinline__ void load(const char* base, int ts_bytes, int left, int d_chunks, int tid) {
-    const int rows = left < 0 ? 0 : (left < R ? left : R);
-    const __amdgpu_buffer_rsrc_t rs =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows * ts_bytes, 0x00020000);
+  static __device__ __forceinline__ uint32_t offset(int ts_bytes, int d_chunks, int tid) {
+    const int c = tid % T::kUsed;
+    return c < d_chunks ? (uint32_t)(tid / T::kUsed * ts_bytes + c * 16) : kBufferOob;
+  }
+  __device__ __forceinline__ void load(const char* base, int ts_bytes, int left, uint32_t off) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int id = tid + i * NT, r = id / T::kUsed, c = id % T::kUsed;
-      const bool in = c < d_chunks && (kAll % NT == 0 || id < kAll);
-      const uint32_t off = in ? (uint32_t)(r * ts_bytes + c * 16) : kBufferOob;
+      const int rows = min(max(left - i * kRows, 0), kRows);
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<char*>(base + (int64_t)(i * kRows) * ts_bytes), 0, rows * ts_bytes, 0x00020000);
       v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
     }
   }
-  __device__ __forceinline__ void store(char* tile, int tid) const {
+  // Infinities and NaNs become zero; whether the thread had any.
+  __device__ __forceinline__ bool clean() {
+    bool any = false;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int id = tid + i * NT, r = id / T::kUsed, c = id % T::kUsed;
-      if (kAll % NT == 0 || id < kAll) *reinterpret_cast<u32x4*>(tile + T::at(r, c)) = v[i];
-    }
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t w = Mma32<S>::finite(v[i][j]);
+        any |= w != v[i][j];
+        v[i][j] = w;
+      }
+    return any;
+  }
+  __device__ __forceinline__ void store(uint32_t tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(tile + T::at(tid / T::kUsed + i * kRows, tid % T::kUsed)) = v[i];
   }
 };
 
@@ -323,14 +350,20 @@ struct TileStage {
 template <typename S, int DB>
 __device__ __forceinline__ void load_rows(const char* base, int ts_bytes, int left, int d_chunks, int lane,
                                           u32x4 (&f)[Tile<S, DB>::kSteps]) {
-  const int rows = left < 0 ? 0 : (left < 32 ? left : 32);
+  const int rows = min(max(left, 0), 32);
   const __amdgpu_buffer_rsrc_t rs =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows * ts_bytes, 0x00020000);
+  const uint32_t off = (uint32_t)((lane & 31) * ts_bytes + (lane >> 5) * 16);
+  if (d_chunks == Tile<S, DB>::kUsed) {
 #pragma unroll
-  for (int s = 0; s < Tile<S, DB>::kSteps; ++s) {
-    const int c = 2 * s + (lane >> 5);
-    f[s] = __builtin_bit_cast(
-        u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, c < d_chunks ? (uint32_t)((lane & 31) * ts_bytes + c * 16) : kBufferOob, 0, 0));
+    for (int s = 0; s < Tile<S, DB>::kSteps; ++s)
+      f[s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off + s * 32, 0, 0));
+  } else {
+    asm volatile("" : "+s"(d_chunks));  // the offsets are not to be kept over a loop
+#pragma unroll
+    for (int s = 0; s < Tile<S, DB>::kSteps; ++s)
+      f[s] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, 2 * s + (lane >> 5) < d_chunks ? off + s * 32 : kBufferOob, 0, 0));
   }
 }
 
@@ -366,81 +399,71 @@ __device__ __forceinline__ void store_rows(const floatx16 (&acc)[DB], float f, S
 }
 
 // acc[db] += (columns of the tile's rows)^T p over NB blocks of 32 rows; p: what
-// the lane's own row weighs the tile's rows with.  Where some of the tile's
-// rows are not seen (check), a row that is not, but holds an infinity or NaN,
-// must not reach the result through 0 * inf: such a tile goes row by row, and
-// only rows that the lane sees are added.  seen(r): row r of the tile.
-template <typename S, int DB, int NB, typename F>
-__device__ __forceinline__ void add_columns(floatx16 (&acc)[DB], const char* tile, const u32x4 (&p)[NB][Tile<S, DB>::kColSteps],
-                                            bool check, int lane, F seen) {
-  using T = Tile<S, DB>;
-  if (check) {
-    bool bad = false;
-#pragma unroll
-    for (int blk = 0; blk < NB; ++blk)
-#pragma unroll 1
-      for (int t = 0; t < T::kColSteps; ++t)
-#pragma unroll
-        for (int db = 0; db < DB; ++db) {
-          const u32x4 a = T::col_frag(tile, blk, t, db, lane);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) bad |= Mma32<S>::nonfinite(a[j]);
-        }
-    if (__any(bad)) {
-#pragma unroll
-      for (int blk = 0; blk < NB; ++blk)
-#pragma unroll
-        for (int t = 0; t < T::kColSteps; ++t)
-#pragma unroll
-          for (int db = 0; db < DB; ++db) {
-            const u32x4 a = T::col_frag(tile, blk, t, db, lane);
-#pragma unroll 1
-            for (int e = 0; e < 2 * T::kE; ++e) {  // element e % E of lane half e / E
-              const int j = e % T::kE, half = e / T::kE;
-              u32x4 one = {0u, 0u, 0u, 0u};
-              if ((lane >> 5) == half) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  if constexpr (sizeof(S) == 2) one[w] = w == (j >> 1) ? a[w] & (j & 1 ? 0xffff0000u : 0xffffu) : 0u;
-                  else one[w] = w == j ? a[w] : 0u;
-                }
-              }
-              floatx16 z;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) z[i] = 0.f;
-              z = Mma32<S>::fma(one, p[blk][t], z);
-              // the rows of acc_frag's order
-              const int r = 32 * blk + (sizeof(S) == 2 ? 16 * t + 8 * (j >> 2) + 4 * half + (j & 3) : 8 * t + 4 * half + j);
-              const bool s = seen(r);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[db][i] += s ? z[i] : 0.f;
-            }
-          }
-      return;
-    }
-  }
+// the lane's own row weighs the tile's rows with.
+template <typename S, int DB, int NB>
+__device__ __forceinline__ void add_columns(floatx16 (&acc)[DB], const Tile<S, DB>& at, uint32_t tile,
+                                            const u32x4 (&p)[NB][Tile<S, DB>::kColSteps]) {
 #pragma unroll
   for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
-    for (int t = 0; t < T::kColSteps; ++t)
+    for (int t = 0; t < Tile<S, DB>::kColSteps; ++t)
 #pragma unroll
-      for (int db = 0; db < DB; ++db) acc[db] = Mma32<S>::fma(T::col_frag(tile, blk, t, db, lane), p[blk][t], acc[db]);
+      for (int db = 0; db < DB; ++db) acc[db] = Mma32<S>::fma(at.col_frag(tile, blk, t, db), p[blk][t], acc[db]);
+}
+
+// A row that a causal mask hides from some of the tile's queries, but that
+// holds an infinity or NaN, must not reach them through 0 * inf.  Where a tile
+// has hidden rows its infinities and NaNs are zero in LDS (TileStage::clean);
+// if there were any, this adds them after the last tile, from memory, with
+// weight 1 where they are seen (an infinity's weight is positive, and a NaN's
+// does not matter).
+// base: row 0 of the tile; seen(r): the lane sees row r.  WHOLE: rows that were
+// operands of the scores too (k, q): all of the result becomes NaN, as the
+// scores' weights are not those of the zeroed row.
+template <typename S, int DB, bool WHOLE, typename F>
+__device__ __forceinline__ void add_nonfinite(floatx16 (&acc)[DB], const char* base, int64_t ts_bytes, int rows, int d,
+                                              int lane, F seen) {
+  const int half = lane >> 5;
+  const auto value = [&](int r, int col) {
+    const float v = col + 4 * half < d ? load_elem<S>(reinterpret_cast<const S*>(base + r * ts_bytes) + 4 * half, col) : 0.f;
+    return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.f;
+  };
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r) {
+    if constexpr (WHOLE) {
+      float any = 0.f;
+#pragma unroll 1
+      for (int i = 0; i < 16 * DB; ++i) any = value(r, 8 * (i >> 2) + (i & 3)) != 0.f ? 1.f : any;
+      if (max_xor32(any) != 0.f && seen(r)) {
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[db][i] = __builtin_nanf("");
+      }
+    } else if (seen(r)) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          acc[db][i] += value(r, 32 * db + acc_row(i, 0));
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // rare: not to cost the kernel registers
+        }
+    }
+  }
 }
 
 // s = rows of block blk of the tile times the wave's own rows.
 template <typename S, int DB>
-__device__ __forceinline__ floatx16 row_products(const char* tile, int blk, const u32x4 (&own)[Tile<S, DB>::kSteps], int lane) {
+__device__ __forceinline__ floatx16 row_products(const Tile<S, DB>& at, uint32_t tile, int blk,
+                                                 const u32x4 (&own)[Tile<S, DB>::kSteps]) {
   floatx16 s;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-  for (int t = 0; t < Tile<S, DB>::kSteps; ++t) s = Mma32<S>::fma(Tile<S, DB>::row_frag(tile, blk, t, lane), own[t], s);
+  for (int t = 0; t < Tile<S, DB>::kSteps; ++t) s = Mma32<S>::fma(at.row_frag(tile, blk, t), own[t], s);
   return s;
 }
 
 __device__ __forceinline__ float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Row of a block of 32 that element i of a product is, for the lane's half.
-__device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 }  // namespace mhc

@@ -56,8 +56,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES);
   const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
   TileStage<S, DB, BN, NT> sk, sv;
-  sk.load(kp, k_ts, s.lk, dc, tid);
-  sv.load(vp, v_ts, s.lk, dc, tid);
+  const uint32_t k_off = sk.offset(k_ts, dc, tid), v_off = sv.offset(v_ts, dc, tid), lds = lds_addr(smem);
+  sk.load(kp, k_ts, s.lk, k_off);
+  sv.load(vp, v_ts, s.lk, v_off);
 
   u32x4 q[T::kSteps], go[T::kSteps];
   const int left = s.lq - wave_first;
@@ -81,9 +82,17 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const float lse = live ? a.lse[stat] : -__builtin_inff();
   const float lse2 = lse == -__builtin_inff() ? __builtin_inff() : lse * kLog2e;  // an empty row: P = 0
 
-  sk.store(smem, tid);
-  sv.store(smem + kTileBytes, tid);
+  const int zone = a.n.causal ? max(0, first + shift + 1) : 0x7fffffff;  // as in the forward, for the keys
+  bool bad = false;
+  auto stage = [&](int t) {
+    if ((t + 1) * BN > zone) bad |= sk.clean();
+    const uint32_t to = lds + (t & 1) * 2 * kTileBytes;
+    sk.store(to, tid);
+    sv.store(to + kTileBytes, tid);
+  };
+  stage(0);
   __syncthreads();
+  T at(lane);
 
   floatx16 acc[DB];
 #pragma unroll
@@ -93,20 +102,20 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const float c = a.scale2;
   const int tiles = (keys + BN - 1) / BN, half = lane >> 5;
   for (int t = 0; t < tiles; ++t) {
-    const char* tk = smem + (t & 1) * 2 * kTileBytes;
-    const char* tv = tk + kTileBytes;
+    const uint32_t tk = lds + (t & 1) * 2 * kTileBytes, tv = tk + kTileBytes;
+    at.keep();
     const int k0 = t * BN;
     if (t + 1 < tiles) {
-      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, dc, tid);
-      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, dc, tid);
+      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, k_off);
+      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, v_off);
     }
     if (k0 <= wave_hi) {
       const bool masked = k0 + BN - 1 > wave_lo;
       u32x4 p[NB][T::kColSteps];
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        floatx16 sc = row_products<S, DB>(tk, b, q, lane);
-        floatx16 dp = row_products<S, DB>(tv, b, go, lane);
+        floatx16 sc = row_products<S, DB>(at, tk, b, q);
+        floatx16 dp = row_products<S, DB>(at, tv, b, go);
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] = hw_exp2(__builtin_fmaf(sc[i], c, -lse2)) * (dp[i] - delta);
         if (masked) {
@@ -117,14 +126,16 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
 #pragma unroll
         for (int u = 0; u < T::kColSteps; ++u) p[b][u] = acc_frag<S>(dp, u);
       }
-      add_columns<S, DB, NB>(acc, tk, p, masked, lane, [&](int r) { return k0 + r <= lim; });
+      add_columns<S, DB, NB>(acc, at, tk, p);
     }
     if (t + 1 < tiles) {
-      char* nk = smem + ((t + 1) & 1) * 2 * kTileBytes;
-      sk.store(nk, tid);
-      sv.store(nk + kTileBytes, tid);
+      stage(t + 1);
       __syncthreads();
     }
+  }
+  if (__syncthreads_or(bad)) {
+    const int z = zone / BN;
+    add_nonfinite<S, DB, true>(acc, kp + z * k_step, k_ts, keys - z * BN, d, lane, [&](int r) { return z * BN + r <= lim; });
   }
   store_rows<S, DB>(acc, a.scale, out, live, d, lane);
 }
@@ -148,9 +159,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   const int G = a.n.H / a.n.Hk, d = a.n.d, dc = d * ES / 16;
   const int key = first + 32 * wave + (lane & 31);
   const bool live = key < rows;
-  const int64_t at = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
-  S* dk = static_cast<S*>(a.dk) + at;
-  S* dv = static_cast<S*>(a.dv) + at;
+  const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
+  S* dk = static_cast<S*>(a.dk) + place;
+  S* dv = static_cast<S*>(a.dv) + place;
   const int shift = s.lk - s.lq;
   // the first query that sees the block's first key
   const int q_first = a.n.causal ? max(0, first - shift) : 0;
@@ -167,11 +178,12 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   load_rows<S, DB>(row_ptr(a.v, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.v.ts * ES), s.lk - wave_first, dc, lane, v);
 
   TileStage<S, DB, BQ, NT> sq, sg;
+  const uint32_t q_off = sq.offset(q_ts, dc, tid), go_off = sg.offset(go_ts, dc, tid), lds = lds_addr(smem);
   float st_lse = 0.f, st_delta = 0.f;
   auto load = [&](int it) {
     const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ;
-    sq.load(row_ptr(a.q, a.n.cu_q, s.row0, s.b, q0, h, ES), q_ts, s.lq - q0, dc, tid);
-    sg.load(row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, s.lq - q0, dc, tid);
+    sq.load(row_ptr(a.q, a.n.cu_q, s.row0, s.b, q0, h, ES), q_ts, s.lq - q0, q_off);
+    sg.load(row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, s.lq - q0, go_off);
     if (tid < BQ) {
       const bool in = q0 + tid < s.lq;
       const int64_t i = (int64_t)h * a.n.Tq + s.row0 + q0 + tid;
@@ -180,17 +192,28 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
       st_delta = in ? a.delta[i] : 0.f;
     }
   };
-  auto store = [&](char* to) {
-    sq.store(to, tid);
-    sg.store(to + kTileBytes, tid);
+  // queries before `zone` see not all of the block's keys: as in the forward,
+  // for q and the output's gradient
+  const int zone = a.n.causal ? first + BK - 1 - shift : 0;
+  bool bad = false;
+  auto store = [&](int it) {
+    const int buf = it & 1;
+    if ((t0 + it % tiles) * BQ < zone) {
+      bad |= sq.clean();
+      bad |= sg.clean();
+    }
+    sq.store(lds + buf * kStage, tid);
+    sg.store(lds + buf * kStage + kTileBytes, tid);
     if (tid < BQ) {
-      reinterpret_cast<float*>(to + 2 * kTileBytes)[tid] = st_lse;
-      reinterpret_cast<float*>(to + 2 * kTileBytes)[BQ + tid] = st_delta;
+      float* to = reinterpret_cast<float*>(smem + buf * kStage + 2 * kTileBytes);
+      to[tid] = st_lse;
+      to[BQ + tid] = st_delta;
     }
   };
   load(0);
-  store(smem);
+  store(0);
   __syncthreads();
+  T at(lane);
 
   floatx16 ak[DB], av[DB];
 #pragma unroll
@@ -200,9 +223,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   const float c = a.scale2;
   const int half = lane >> 5, items = tiles * G;
   for (int it = 0; it < items; ++it) {
-    const char* tq = smem + (it & 1) * kStage;
-    const char* tg = tq + kTileBytes;
-    const float* stats = reinterpret_cast<const float*>(tq + 2 * kTileBytes);
+    const uint32_t tq = lds + (it & 1) * kStage, tg = tq + kTileBytes;
+    const float* stats = reinterpret_cast<const float*>(smem + (it & 1) * kStage + 2 * kTileBytes);
+    at.keep();
     const int q0 = (t0 + it % tiles) * BQ;
     if (it + 1 < items) load(it + 1);
     // queries from here on see the lane's key; all of the wave's keys are seen by the tile or none
@@ -212,8 +235,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
       const bool masked = a.n.causal && q0 < wave_first + 31 - shift;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        floatx16 sc = row_products<S, DB>(tq, b, k, lane);
-        floatx16 dp = row_products<S, DB>(tg, b, v, lane);
+        floatx16 sc = row_products<S, DB>(at, tq, b, k);
+        floatx16 dp = row_products<S, DB>(at, tg, b, v);
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const floatx4 lse = *reinterpret_cast<const floatx4*>(stats + 32 * b + acc_row(i, half));
@@ -239,14 +262,21 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
           p[0][u] = acc_frag<S>(sc, u);
           ds[0][u] = acc_frag<S>(dp, u);
         }
-        const auto seen = [&](int r) { return q0 + 32 * b + r >= lim; };
-        add_columns<S, DB, 1>(av, tg + b * 32 * T::kPitch, p, masked, lane, seen);
-        add_columns<S, DB, 1>(ak, tq + b * 32 * T::kPitch, ds, masked, lane, seen);
+        add_columns<S, DB, 1>(av, at, tg + b * 32 * T::kPitch, p);
+        add_columns<S, DB, 1>(ak, at, tq + b * 32 * T::kPitch, ds);
       }
     }
     if (it + 1 < items) {
-      store(smem + ((it + 1) & 1) * kStage);
+      store(it + 1);
       __syncthreads();
+    }
+  }
+  if (__syncthreads_or(bad)) {
+    const int q0 = t0 * BQ, n = min((zone + BQ - 1) / BQ * BQ, s.lq) - q0;
+    const auto seen = [&](int r) { return q0 + r >= key - shift; };
+    for (int h = hk * G; h < hk * G + G; ++h) {
+      add_nonfinite<S, DB, false>(av, row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, n, d, lane, seen);
+      add_nonfinite<S, DB, true>(ak, row_ptr(a.q, a.n.cu_q, s.row0, s.b, q0, h, ES), q_ts, n, d, lane, seen);
     }
   }
   // keys past the sequence's are zero rows of k, but no zero rows of dk

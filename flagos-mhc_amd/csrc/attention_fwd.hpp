@@ -65,11 +65,22 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
 
   TileStage<S, DB, BN, NT> sk, sv;
-  sk.load(kp, k_ts, s.lk, dc, tid);
-  sv.load(vp, v_ts, s.lk, dc, tid);
-  sk.store(smem, tid);
-  sv.store(smem + kTileBytes, tid);
+  uint32_t k_off = sk.offset(k_ts, dc, tid), v_off = sv.offset(v_ts, dc, tid);
+  const uint32_t lds = lds_addr(smem);
+  sk.load(kp, k_ts, s.lk, k_off);
+  sv.load(vp, v_ts, s.lk, v_off);
+  // tiles with keys from here on are hidden from some of the block's queries
+  const int zone = a.n.causal ? max(0, first + shift + 1) : 0x7fffffff;
+  bool bad = false;
+  auto stage = [&](int t) {
+    if ((t + 1) * BN > zone) bad |= sv.clean();
+    const uint32_t to = lds + (t & 1) * 2 * kTileBytes;
+    sk.store(to, tid);
+    sv.store(to + kTileBytes, tid);
+  };
+  stage(0);
   __syncthreads();
+  T at(lane);
 
   floatx16 acc[DB];
 #pragma unroll
@@ -80,17 +91,17 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   const float c = a.scale2;
   const int tiles = (keys + BN - 1) / BN, half = lane >> 5;
   for (int t = 0; t < tiles; ++t) {
-    const char* tk = smem + (t & 1) * 2 * kTileBytes;
-    const char* tv = tk + kTileBytes;
+    const uint32_t tk = lds + (t & 1) * 2 * kTileBytes, tv = tk + kTileBytes;
+    at.keep();
     const int k0 = t * BN;
     if (t + 1 < tiles) {
-      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, dc, tid);
-      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, dc, tid);
+      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, k_off);
+      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, v_off);
     }
     if (k0 <= wave_hi) {
       floatx16 sc[NB];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) sc[b] = row_products<S, DB>(tk, b, q, lane);
+      for (int b = 0; b < NB; ++b) sc[b] = row_products<S, DB>(at, tk, b, q);
       const bool masked = k0 + BN - 1 > wave_lo;
       if (masked) {
         const int left = lim - k0 - 4 * half;
@@ -128,14 +139,16 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
 #pragma unroll
         for (int u = 0; u < T::kColSteps; ++u) p[b][u] = acc_frag<S>(sc[b], u);
       }
-      add_columns<S, DB, NB>(acc, tv, p, masked, lane, [&](int r) { return k0 + r <= lim; });
+      add_columns<S, DB, NB>(acc, at, tv, p);
     }
     if (t + 1 < tiles) {
-      char* nk = smem + ((t + 1) & 1) * 2 * kTileBytes;
-      sk.store(nk, tid);
-      sv.store(nk + kTileBytes, tid);
+      stage(t + 1);
       __syncthreads();
     }
+  }
+  if (__syncthreads_or(bad)) {
+    const int z = zone / BN;
+    add_nonfinite<S, DB, false>(acc, vp + z * v_step, v_ts, keys - z * BN, d, lane, [&](int r) { return z * BN + r <= lim; });
   }
   l = add_xor32(l);
   // (a NaN among the scores leaves l NaN: not the empty row's zero)

@@ -3,6 +3,7 @@
 
 #include "attention_bwd.hpp"
 #include "attention_fwd.hpp"
+#include "attention_split.hpp"
 #include "mhc_launch.hpp"
 
 namespace mhc {
@@ -28,8 +29,24 @@ template <typename S, int DB> struct AttShape {
 };
 
 template <typename S, int DB>
+int att_split_width(const AttArgs& a, const AttSplit& p, hipStream_t st) {
+  const int64_t blocks = p.slots * a.n.Hk * p.splits, rows = a.n.Tq * a.n.H;
+  if (blocks > 0xffffffffll / 256 || rows > 0xffffffffll / 64)
+    return set_error(MHC_ERR_UNSUPPORTED, "attention: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
+  constexpr int WPE = AttShape<S, DB>::kBytes <= 256 ? 2 : 1;
+  hipLaunchKernelGGL((att_split_kernel<S, DB, WPE>), dim3((unsigned)blocks), dim3(64 * kSplitWaves), (split_lds<S, DB>()), st, a,
+                     p.slots, p.splits);
+  if (const int rc = check_launch("attention")) return rc;
+  if (p.splits == 1) return MHC_OK;
+  hipLaunchKernelGGL(att_join_kernel<S>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows, p.splits);
+  return check_launch("attention");
+}
+
+template <typename S, int DB>
 int att_fwd_width(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
+  const AttSplit p = att_split(a.n, device_cu_count());
+  if (p.use) return att_split_width<S, DB>(a, p, st);
   constexpr size_t lds = 4 * 32 * A::kFwdNB * Tile<S, DB>::kPitch;
   const int64_t slots = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 32 * A::kFwdNW);
   return att_launch(att_fwd_kernel<S, DB, A::kFwdNW, A::kFwdNB, A::kFwdWPE>, a, slots, a.n.H, 64 * A::kFwdNW, lds, st,
@@ -50,14 +67,14 @@ int att_bwd_width(const AttArgs& a, hipStream_t st) {
 }
 
 template <typename S>
-int att_fwd(const AttArgs& a, void* ws, hipStream_t st) {
+int att_fwd(const AttArgs& a, hipStream_t st) {
   if (a.n.d <= 64) return att_fwd_width<S, 2>(a, st);
   if (a.n.d <= 128) return att_fwd_width<S, 4>(a, st);
   if constexpr (sizeof(S) == 2) return att_fwd_width<S, 8>(a, st);
   return MHC_ERR_UNSUPPORTED;  // (refused before)
 }
 template <typename S>
-int att_bwd(const AttArgs& a, void* ws, hipStream_t st) {
+int att_bwd(const AttArgs& a, hipStream_t st) {
   if (a.n.d <= 64) return att_bwd_width<S, 2>(a, st);
   if (a.n.d <= 128) return att_bwd_width<S, 4>(a, st);
   if constexpr (sizeof(S) == 2) return att_bwd_width<S, 8>(a, st);

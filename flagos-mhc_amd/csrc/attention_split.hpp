@@ -1,0 +1,246 @@
+// Attention forward for few queries: single tokens over a cache, short chunks
+// over long contexts.
+//
+// Rows are (query, head of the group) pairs, so that a key head's keys and
+// values are read once for every head that shares them.  A block takes 32
+// rows and one part of their keys, its four waves every fourth tile of 32
+// keys of that part; their sums meet in LDS at the end.  Where there are too
+// few rows for the GPU the keys are split further over blocks, and a second
+// kernel joins the parts, in their order.  A wave keeps its tile of keys in
+// registers, loaded as the operand it is, and turns the values through 8 KB
+// of LDS of its own: no wave waits for another, and 16 KB a wave are in
+// flight while it computes.
+#pragma once
+
+#include "attention.hpp"
+#include "attention_fwd.hpp"
+
+namespace mhc {
+
+constexpr int kSplitWaves = 4;
+
+// Bytes of LDS: a wave's tile of values, later its sums.
+template <typename S, int DB>
+constexpr size_t split_lds() {
+  constexpr size_t tile = 32 * Tile<S, DB>::kPitch, sums = DB * 4096;
+  return kSplitWaves * ((tile > sums ? tile : sums) + 32 * 2 * 4);
+}
+
+template <typename S, int DB, int WPE>
+__global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_split_kernel(AttArgs a, int64_t slots, int splits) {
+  using T = Tile<S, DB>;
+  constexpr int ES = (int)sizeof(S);
+  constexpr size_t kRegion = split_lds<S, DB>() / kSplitWaves - 256;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  // the parts of one tile of rows lie side by side: they read neighbouring keys
+  const int64_t item = blockIdx.x;
+  const int part = (int)(item % splits);
+  const int hk = (int)(item / splits % a.n.Hk);
+  const int64_t slot = item / splits / a.n.Hk;
+  const int G = a.n.H / a.n.Hk, d = a.n.d, dc = d * ES / 16;
+  AttSeq s;
+  int64_t first;  // first row (query * G + head)
+  if (a.n.cu_q) {
+    // rows are G a query: the slots of tiles of 32 of them
+    int lo = 0, n = a.n.B + 1;
+    while (n > 1) {
+      const int step = (n + 63) / 64, c = lane * step;
+      int hit = __popcll(__ballot(c < n && cu_at(a.n.cu_q, lo + c, a.n.Tq) * G / 32 + lo + c <= slot));
+      hit = hit < 1 ? 1 : hit;
+      const int skip = (hit - 1) * step;
+      lo += skip;
+      n = n - skip < step ? n - skip : step;
+    }
+    const int b = __builtin_amdgcn_readfirstlane(lo);
+    s = att_seq(a.n, b);
+    first = (slot - (s.row0 * G / 32 + b)) * 32;
+  } else {
+    const int64_t per = ((int64_t)a.n.Sq * G + 31) / 32;
+    s = att_seq(a.n, (int)(slot / per));
+    first = slot % per * 32;
+  }
+  if (first >= (int64_t)s.lq * G) return;
+  const int64_t r = first + (lane & 31);
+  const int i = (int)(r / G), g = (int)(r % G), h = hk * G + g;
+  const bool live = i < s.lq;
+  const int64_t orow = (s.row0 + i) * a.n.H + h;
+  const int shift = s.lk - s.lq;
+  const int lim = s.none || !live ? -1 : (a.n.causal ? min(s.lk - 1, i + shift) : s.lk - 1);
+  // the block's part of the keys that its last row sees
+  const int last = (int)min((int64_t)s.lq - 1, (first + 31) / G);
+  const int keys = s.none ? 0 : max(0, a.n.causal ? min(s.lk, last + shift + 1) : s.lk);
+  const int chunk = ((keys + splits - 1) / splits + 31) / 32 * 32;
+  const int from = (int)min((int64_t)keys, (int64_t)part * chunk), to = min(keys, from + chunk);
+  const int tiles = (to - from + 31) / 32;
+
+  u32x4 q[T::kSteps];
+  {
+    const char* p = row_ptr(a.q, a.n.cu_q, s.row0, s.b, live ? i : 0, h, ES);
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      const int c = 2 * t + half;
+      q[t] = u32x4{0u, 0u, 0u, 0u};
+      if (live && !s.none && c < dc) q[t] = ld16(p + c * 16);
+    }
+  }
+  const int k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES);
+  const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, from, hk, ES);
+  const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, from, hk, ES);
+  char* mine = smem + wave * kRegion;
+  const uint32_t tile = lds_addr(mine);
+
+  floatx16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[db][j] = 0.f;
+  float m = -__builtin_inff(), l = 0.f;
+  const float c = a.scale2;
+  u32x4 k[T::kSteps];
+  TileStage<S, DB, 32, 64> sv;
+  const uint32_t v_off = sv.offset(v_ts, dc, lane);
+  T at(lane);
+  const int have = to - from;
+  // tiles from here on are hidden from some of the rows
+  const int zone = a.n.causal ? max(0, (int)(first / G) + shift + 1) : 0x7fffffff;
+  bool bad = false;
+  if (wave < tiles) {
+    load_rows<S, DB>(kp + (int64_t)wave * 32 * k_ts, k_ts, have - wave * 32, dc, lane, k);
+    sv.load(vp + (int64_t)wave * 32 * v_ts, v_ts, have - wave * 32, v_off);
+  }
+  for (int t = wave; t < tiles; t += kSplitWaves) {
+    const int next = t + kSplitWaves, k0 = from + t * 32;
+    at.keep();
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    floatx16 sc;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) sc[j] = 0.f;
+#pragma unroll
+    for (int u = 0; u < T::kSteps; ++u) sc = Mma32<S>::fma(k[u], q[u], sc);
+    if (next < tiles) load_rows<S, DB>(kp + (int64_t)next * 32 * k_ts, k_ts, have - next * 32, dc, lane, k);
+    const int left = min(lim, to - 1) - k0 - 4 * half;
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      sc[j] = acc_row(j, 0) <= left ? sc[j] : -__builtin_inff();
+      top = fmaxf(top, sc[j]);
+    }
+    top = max_xor32(top) * c;
+    if (__any(top > m + kLazyMax || m == -__builtin_inff())) {
+      const float mn = fmaxf(m, top);
+      const float f = mn == -__builtin_inff() ? 1.f : hw_exp2(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[db][j] *= f;
+    }
+    const float ref = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      sc[j] = hw_exp2(__builtin_fmaf(sc[j], c, -ref));
+      l += sc[j];
+    }
+    u32x4 p[1][T::kColSteps];
+#pragma unroll
+    for (int u = 0; u < T::kColSteps; ++u) p[0][u] = acc_frag<S>(sc, u);
+    if (k0 + 32 > zone) bad |= sv.clean();
+    sv.store(tile, ln & 63);
+    if (next < tiles) sv.load(vp + (int64_t)next * 32 * v_ts, v_ts, have - next * 32, v_off);
+    add_columns<S, DB, 1>(acc, at, tile, p);
+  }
+
+  // the four waves' sums, each from its own reference point to the largest
+  float* stats = reinterpret_cast<float*>(smem + kSplitWaves * kRegion);
+  l = add_xor32(l);
+  if (lane < 32) {
+    stats[wave * 64 + lane] = m;
+    stats[wave * 64 + 32 + lane] = l;
+  }
+  bad = __syncthreads_or(bad);
+  float top = m, sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSplitWaves; ++w) top = fmaxf(top, stats[w * 64 + (lane & 31)]);
+  const float ref = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < kSplitWaves; ++w) sum += stats[w * 64 + 32 + (lane & 31)] * hw_exp2(stats[w * 64 + (lane & 31)] - ref);
+  const float f = hw_exp2(m - ref);
+  float* region = reinterpret_cast<float*>(mine);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) region[(db * 16 + j) * 64 + lane] = acc[db][j] * f;
+  __syncthreads();
+  const float inv = splits > 1 ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+  if (splits > 1) {
+    float* ml = a.part + (int64_t)splits * a.n.Tq * a.n.H * d;
+    const int64_t to_ml = (int64_t)part * a.n.Tq * a.n.H + orow;
+    if (wave == 0 && live && lane < 32) {
+      ml[2 * to_ml] = top;
+      ml[2 * to_ml + 1] = sum;
+    }
+  } else if (a.lse && wave == 0 && live && lane < 32) {
+    a.lse[(int64_t)h * a.n.Tq + s.row0 + i] = sum == 0.f ? -__builtin_inff() : top * kLn2 + logf(sum);
+  }
+  for (int db = wave; db < DB; db += kSplitWaves) {
+    floatx16 z[1];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float v = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSplitWaves; ++w) v += reinterpret_cast<const float*>(smem + w * kRegion)[(db * 16 + j) * 64 + lane];
+      z[0][j] = v;
+    }
+    if (bad) {
+      // the parts' tiles of 32 begin at `from`
+      const int z0 = from + max(0, zone - from) / 32 * 32;
+      add_nonfinite<S, 1, false>(z, vp + (int64_t)(z0 - from) * v_ts + 32 * db * ES, v_ts, to - z0, d - 32 * db, lane,
+                                 [&](int row) { return z0 + row <= lim; });
+    }
+    if (splits > 1)
+      store_rows<float, 1>(z, 1.f, a.part + ((int64_t)part * a.n.Tq * a.n.H + orow) * d + 32 * db, live, d - 32 * db, lane);
+    else
+      store_rows<S, 1>(z, inv, static_cast<S*>(a.out) + orow * d + 32 * db, live, d - 32 * db, lane);
+  }
+}
+
+// out = sum over parts of 2^(m - M) O / sum of 2^(m - M) l: a wave a row and head.
+template <typename S>
+__global__ __launch_bounds__(256) void att_join_kernel(AttArgs a, int64_t rows, int splits) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);  // (row of q, head)
+  if (row >= rows) return;
+  const int d = a.n.d;
+  const float* ml = a.part + (int64_t)splits * rows * d;
+  float top = -__builtin_inff();
+  for (int p = lane; p < splits; p += 64) top = fmaxf(top, ml[2 * ((int64_t)p * rows + row)]);
+  top = group_max<63>(top);
+  const float ref = top == -__builtin_inff() ? 0.f : top;
+  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int e = lane * 4;  // the lane's elements
+  for (int p = 0; p < splits; ++p) {
+    const int64_t at = (int64_t)p * rows + row;
+    const float l = ml[2 * at + 1];
+    if (l == 0.f) continue;  // no keys in this part
+    const float f = hw_exp2(ml[2 * at] - ref);
+    sum += l * f;
+    if (e < d) {
+      const floatx4 o = *reinterpret_cast<const floatx4*>(a.part + at * d + e);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += o[j] * f;
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  S* out = static_cast<S*>(a.out) + row * d + e;
+  if (e < d) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) store_elem<S>(out, j, v[j] * inv);
+  }
+  if (a.lse && lane == 0)
+    a.lse[row % a.n.H * a.n.Tq + row / a.n.H] = sum == 0.f ? -__builtin_inff() : top * kLn2 + logf(sum);
+}
+
+}  // namespace mhc
