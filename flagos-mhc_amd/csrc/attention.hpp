@@ -230,9 +230,10 @@ __device__ __forceinline__ int acc_row(int i, int h) { return 8 * (i >> 2) + 4 *
 // rows j and j + 4 of 8 chunks (fp32 columns).  Rows of 256 bytes start at
 // the same bank, those of 128 at alternating halves.
 //
-// Addresses are a lane's two base registers, exclusive-ored with constants and
-// added to a tile's place: kept as they are they cost one instruction a read,
-// whereas all of them hoisted out of a loop would cost a register each.
+// Addresses are a lane's two base registers and the tile's place (whole 256
+// bytes), exclusive-ored with constants, plus constants that the instructions
+// hold: one instruction for every few reads, computed where they are read (all
+// of them hoisted out of a loop would cost a register each).
 
 typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) const uint32_t lds_u32;
@@ -272,7 +273,7 @@ struct Tile {
   // Row fragment: row 32 blk + l % 32, chunk 2 step + l / 32.
   __device__ __forceinline__ u32x4 row_frag(uint32_t tile, int blk, int step) const {
     const int c = 2 * step;
-    return *(lds_u32x4*)(uintptr_t)((row ^ (uint32_t)((c % kLow) * 16)) + tile + blk * 32 * kPitch + (c / kLow) * kLow * 16);
+    return *(lds_u32x4*)(uintptr_t)(((row + tile) ^ (uint32_t)((c % kLow) * 16)) + blk * 32 * kPitch + (c / kLow) * kLow * 16);
   }
 
   // Column fragment: column 32 db + l % 32; rows of step t of block blk in the
@@ -281,11 +282,11 @@ struct Tile {
     u32x4 f;
     if constexpr (kEs == 2) {
       constexpr int kDbs = kLow / 4;  // blocks of 32 columns within the exclusive-ored bits
-      const uint32_t at = tile + (blk * 32 + t * 16) * kPitch + (db / kDbs) * kLow * 16;
+      const uint32_t at = (blk * 32 + t * 16) * kPitch + (db / kDbs) * kLow * 16;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const s16x4_att v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (lds_s16x4*)(uintptr_t)((col ^ (uint32_t)((db % kDbs) * 64 + 32 * u)) + at + 8 * u * kPitch));
+            (lds_s16x4*)(uintptr_t)(((col + tile) ^ (uint32_t)((db % kDbs) * 64 + 32 * u)) + at + 8 * u * kPitch));
         const u32x2 w = __builtin_bit_cast(u32x2, v);
         f[2 * u] = w[0];
         f[2 * u + 1] = w[1];
@@ -293,7 +294,7 @@ struct Tile {
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        f[j] = *(lds_u32*)(uintptr_t)((col ^ (uint32_t)(((db & 1) * 8 + (t & 1) * 4 + j) * 16)) + tile +
+        f[j] = *(lds_u32*)(uintptr_t)(((col + tile) ^ (uint32_t)(((db & 1) * 8 + (t & 1) * 4 + j) * 16)) +
                                       (blk * 32 + 8 * t + j) * kPitch + (db >> 1) * 256);
     }
     return f;
@@ -463,6 +464,10 @@ __device__ __forceinline__ floatx16 row_products(const Tile<S, DB>& at, uint32_t
   for (int t = 0; t < Tile<S, DB>::kSteps; ++t) s = Mma32<S>::fma(at.row_frag(tile, blk, t), own[t], s);
   return s;
 }
+
+// What follows stays behind the branch it stands in (selects over a whole tile
+// are otherwise taken for every tile).
+__device__ __forceinline__ void stay() { asm volatile(""); }
 
 __device__ __forceinline__ float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 

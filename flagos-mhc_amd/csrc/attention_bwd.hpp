@@ -26,7 +26,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   using T = Tile<S, DB>;
   constexpr int BN = 32 * NB, BM = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
   constexpr int kTileBytes = BN * T::kPitch;
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 x (K, V)
+  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (K, V)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot;
   int h, first;
@@ -119,7 +119,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
 #pragma unroll
         for (int i = 0; i < 16; ++i) dp[i] = hw_exp2(__builtin_fmaf(sc[i], c, -lse2)) * (dp[i] - delta);
         if (masked) {
-          const int left = lim - k0 - 4 * half;
+          stay();
+        const int left = lim - k0 - 4 * half;
 #pragma unroll
           for (int i = 0; i < 16; ++i) dp[i] = 32 * b + acc_row(i, 0) <= left ? dp[i] : 0.f;
         }
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   constexpr int BQ = 32 * NB, BK = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
   constexpr int kTileBytes = BQ * T::kPitch, kStage = 2 * kTileBytes + 2 * BQ * 4;
   static_assert(BQ <= NT, "a thread a row's lse and D");
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 x (Q, dO, lse, D)
+  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (Q, dO, lse, D)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot, row0;
   int hk, first, rows;
@@ -248,6 +249,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
           }
         }
         if (masked) {
+          stay();
           const int from = lim - q0 - 4 * half;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {

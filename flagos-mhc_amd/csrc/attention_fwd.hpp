@@ -32,7 +32,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   using T = Tile<S, DB>;
   constexpr int BN = 32 * NB, BM = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
   constexpr int kTileBytes = BN * T::kPitch;
-  extern __shared__ __attribute__((aligned(16))) char smem[];  // 2 x (K, V)
+  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (K, V)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot;
   int h, first;
@@ -104,6 +104,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
       for (int b = 0; b < NB; ++b) sc[b] = row_products<S, DB>(at, tk, b, q);
       const bool masked = k0 + BN - 1 > wave_lo;
       if (masked) {
+        stay();
         const int left = lim - k0 - 4 * half;
 #pragma unroll
         for (int b = 0; b < NB; ++b)

@@ -31,14 +31,14 @@ template <typename S, int DB> struct AttShape {
 template <typename S, int DB>
 int att_split_width(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   const int64_t blocks = p.slots * a.n.Hk * p.splits, rows = a.n.Tq * a.n.H;
-  if (blocks > 0xffffffffll / 256 || rows > 0xffffffffll / 64)
+  if (blocks > 0xffffffffll / 256 || rows > 0xffffffffll / 256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
   constexpr int WPE = AttShape<S, DB>::kBytes <= 256 ? 2 : 1;
   hipLaunchKernelGGL((att_split_kernel<S, DB, WPE>), dim3((unsigned)blocks), dim3(64 * kSplitWaves), (split_lds<S, DB>()), st, a,
                      p.slots, p.splits);
   if (const int rc = check_launch("attention")) return rc;
   if (p.splits == 1) return MHC_OK;
-  hipLaunchKernelGGL(att_join_kernel<S>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, rows, p.splits);
+  hipLaunchKernelGGL(att_join_kernel<S>, dim3((unsigned)rows), dim3(256), 0, st, a, rows, p.splits);
   return check_launch("attention");
 }
 
