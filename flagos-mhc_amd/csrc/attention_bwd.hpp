@@ -141,14 +141,16 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   store_rows<S, DB>(acc, a.scale, out, live, d, lane);
 }
 
-// dk and dv.
-template <typename S, int DB, int NW, int NB, int WPE>
+// dk and dv.  VLDS: the block's own rows of v are in LDS, and read as they are
+// needed, instead of in registers: with those two waves fit a SIMD unit.
+template <typename S, int DB, int NW, int NB, int WPE, bool VLDS>
 __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_t slots) {
   using T = Tile<S, DB>;
   constexpr int BQ = 32 * NB, BK = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
-  constexpr int kTileBytes = BQ * T::kPitch, kStage = 2 * kTileBytes + 2 * BQ * 4;
+  constexpr int kTileBytes = BQ * T::kPitch, kStage = 2 * kTileBytes + (2 * BQ * 4 + 255) / 256 * 256;
   static_assert(BQ <= NT, "a thread a row's lse and D");
-  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (Q, dO, lse, D)
+  constexpr int kOwn = VLDS ? BK * T::kPitch : 0;
+  extern __shared__ __attribute__((aligned(256))) char smem[];  // own V, 2 x (Q, dO, lse, D)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot, row0;
   int hk, first, rows;
@@ -160,26 +162,32 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   const int G = a.n.H / a.n.Hk, d = a.n.d, dc = d * ES / 16;
   const int key = first + 32 * wave + (lane & 31);
   const bool live = key < rows;
-  const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
-  S* dk = static_cast<S*>(a.dk) + place;
-  S* dv = static_cast<S*>(a.dv) + place;
   const int shift = s.lk - s.lq;
   // the first query that sees the block's first key
   const int q_first = a.n.causal ? max(0, first - shift) : 0;
   const int t0 = q_first / BQ, tiles = s.none || first >= s.lk || q_first >= s.lq ? 0 : (s.lq + BQ - 1) / BQ - t0;
   if (tiles <= 0) {
-    store_none<S, DB>(dk, live, d, lane);
-    store_none<S, DB>(dv, live, d, lane);
+    const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
+    store_none<S, DB>(static_cast<S*>(a.dk) + place, live, d, lane);
+    store_none<S, DB>(static_cast<S*>(a.dv) + place, live, d, lane);
     return;
   }
-  const int wave_first = first + 32 * wave;
+  int wave_first = first + 32 * wave;
   const int q_ts = (int)(a.q.ts * ES), go_ts = (int)(a.go.ts * ES);
-  u32x4 k[T::kSteps], v[T::kSteps];
+  u32x4 k[T::kSteps], v[VLDS ? 1 : T::kSteps];
   load_rows<S, DB>(row_ptr(a.k, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.k.ts * ES), s.lk - wave_first, dc, lane, k);
-  load_rows<S, DB>(row_ptr(a.v, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.v.ts * ES), s.lk - wave_first, dc, lane, v);
+  if constexpr (VLDS) {
+    // (a wave reads back its own rows alone)
+    TileStage<S, DB, 32, 64> own;
+    own.load(row_ptr(a.v, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.v.ts * ES), s.lk - wave_first,
+             own.offset((int)(a.v.ts * ES), dc, lane));
+    own.store(lds_addr(smem) + wave * 32 * T::kPitch, lane);
+  } else {
+    load_rows<S, DB>(row_ptr(a.v, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.v.ts * ES), s.lk - wave_first, dc, lane, v);
+  }
 
   TileStage<S, DB, BQ, NT> sq, sg;
-  const uint32_t q_off = sq.offset(q_ts, dc, tid), go_off = sg.offset(go_ts, dc, tid), lds = lds_addr(smem);
+  const uint32_t q_off = sq.offset(q_ts, dc, tid), go_off = sg.offset(go_ts, dc, tid), lds = lds_addr(smem) + kOwn;
   float st_lse = 0.f, st_delta = 0.f;
   auto load = [&](int it) {
     const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ;
@@ -206,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
     sq.store(lds + buf * kStage, tid);
     sg.store(lds + buf * kStage + kTileBytes, tid);
     if (tid < BQ) {
-      float* to = reinterpret_cast<float*>(smem + buf * kStage + 2 * kTileBytes);
+      float* to = reinterpret_cast<float*>(smem + kOwn + buf * kStage + 2 * kTileBytes);
       to[tid] = st_lse;
       to[BQ + tid] = st_delta;
     }
@@ -223,9 +231,10 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
     for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
   const float c = a.scale2;
   const int half = lane >> 5, items = tiles * G;
+  const uint32_t own_v = lds_addr(smem) + wave * 32 * T::kPitch;
   for (int it = 0; it < items; ++it) {
     const uint32_t tq = lds + (it & 1) * kStage, tg = tq + kTileBytes;
-    const float* stats = reinterpret_cast<const float*>(smem + (it & 1) * kStage + 2 * kTileBytes);
+    const float* stats = reinterpret_cast<const float*>(smem + kOwn + (it & 1) * kStage + 2 * kTileBytes);
     at.keep();
     const int q0 = (t0 + it % tiles) * BQ;
     if (it + 1 < items) load(it + 1);
@@ -237,7 +246,15 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         floatx16 sc = row_products<S, DB>(at, tq, b, k);
-        floatx16 dp = row_products<S, DB>(at, tg, b, v);
+        floatx16 dp;
+        if constexpr (VLDS) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dp[i] = 0.f;
+#pragma unroll
+          for (int u = 0; u < T::kSteps; ++u) dp = Mma32<S>::fma(at.row_frag(tg, b, u), at.row_frag(own_v, 0, u), dp);
+        } else {
+          dp = row_products<S, DB>(at, tg, b, v);
+        }
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const floatx4 lse = *reinterpret_cast<const floatx4*>(stats + 32 * b + acc_row(i, half));
@@ -289,8 +306,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
   }
-  store_rows<S, DB>(ak, a.scale, dk, live, d, lane);
-  store_rows<S, DB>(av, 1.f, dv, live, d, lane);
+  const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
+  store_rows<S, DB>(ak, a.scale, static_cast<S*>(a.dk) + place, live, d, lane);
+  store_rows<S, DB>(av, 1.f, static_cast<S*>(a.dv) + place, live, d, lane);
 }
 
 }  // namespace mhc

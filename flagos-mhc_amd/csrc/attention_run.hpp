@@ -25,7 +25,8 @@ template <typename S, int DB> struct AttShape {
   static constexpr int kBytes = 32 * DB * (int)sizeof(S);
   static constexpr int kFwdNW = kBytes == 256 && sizeof(S) == 2 ? 8 : 4, kFwdNB = sizeof(S) == 2 && DB <= 4 ? 2 : 1, kFwdWPE = kBytes <= 256 ? 2 : 1;
   static constexpr int kDqNW = kBytes == 256 && sizeof(S) == 2 ? 8 : 4, kDqNB = 1, kDqWPE = kBytes <= 256 ? 2 : 1;
-  static constexpr int kDkvNW = 4, kDkvNB = 1, kDkvWPE = kBytes <= 128 ? 2 : 1;
+  static constexpr int kDkvNW = 4, kDkvNB = 1, kDkvWPE = kBytes <= 256 ? 2 : 1;
+  static constexpr bool kDkvLds = kBytes >= 256;
 };
 
 template <typename S, int DB>
@@ -56,13 +57,14 @@ template <typename S, int DB>
 int att_bwd_width(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
   constexpr size_t lds = 4 * 32 * A::kDqNB * Tile<S, DB>::kPitch;
-  constexpr size_t lds2 = 4 * 32 * A::kDkvNB * (Tile<S, DB>::kPitch + 4);
+  constexpr size_t lds2 = 2 * (2 * 32 * A::kDkvNB * Tile<S, DB>::kPitch + (2 * 32 * A::kDkvNB * 4 + 255) / 256 * 256) +
+                          (A::kDkvLds ? 32 * A::kDkvNW * Tile<S, DB>::kPitch : 0);
   const int64_t slots = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 32 * A::kDqNW);
   if (const int rc = att_launch(att_dq_kernel<S, DB, A::kDqNW, A::kDqNB, A::kDqWPE>, a, slots, a.n.H, 64 * A::kDqNW, lds, st,
                                 "attention_backward"))
     return rc;
   const int64_t slots_k = att_slots(a.n.cu_k != nullptr, a.n.Tk, a.n.B, a.n.Sk, 32 * A::kDkvNW);
-  return att_launch(att_dkv_kernel<S, DB, A::kDkvNW, A::kDkvNB, A::kDkvWPE>, a, slots_k, a.n.Hk, 64 * A::kDkvNW, lds2, st,
+  return att_launch(att_dkv_kernel<S, DB, A::kDkvNW, A::kDkvNB, A::kDkvWPE, A::kDkvLds>, a, slots_k, a.n.Hk, 64 * A::kDkvNW, lds2, st,
                     "attention_backward");
 }
 
