@@ -141,10 +141,11 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   store_rows<S, DB>(acc, a.scale, out, live, d, lane);
 }
 
-// dk and dv.  VLDS: the block's own rows of v are in LDS, and read as they are
+// dk and dv, or, of `splits` parts of the queries, a part's share of them in
+// fp32, for att_dkv_join_kernel.  VLDS: the block's own rows of v are in LDS, and read as they are
 // needed, instead of in registers: with those two waves fit a SIMD unit.
 template <typename S, int DB, int NW, int NB, int WPE, bool VLDS>
-__global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_t slots) {
+__global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_t slots, int splits) {
   using T = Tile<S, DB>;
   constexpr int BQ = 32 * NB, BK = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
   constexpr int kTileBytes = BQ * T::kPitch, kStage = 2 * kTileBytes + (2 * BQ * 4 + 255) / 256 * 256;
@@ -154,7 +155,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot, row0;
   int hk, first, rows;
-  const int64_t item = xcd_contig(blockIdx.x, gridDim.x);
+  const int64_t item = xcd_contig(blockIdx.x, gridDim.x) / splits;
+  const int part = (int)(xcd_contig(blockIdx.x, gridDim.x) % splits);
   hk = (int)(item / slots);
   slot = item % slots;  // a head's first keys are seen by the most queries
   const AttSeq s = k_tile(a.n, slot, BK, first, rows, row0);
@@ -167,9 +169,14 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   const int q_first = a.n.causal ? max(0, first - shift) : 0;
   const int t0 = q_first / BQ, tiles = s.none || first >= s.lk || q_first >= s.lq ? 0 : (s.lq + BQ - 1) / BQ - t0;
   if (tiles <= 0) {
-    const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
-    store_none<S, DB>(static_cast<S*>(a.dk) + place, live, d, lane);
-    store_none<S, DB>(static_cast<S*>(a.dv) + place, live, d, lane);
+    const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d, all = a.n.Tk * a.n.Hk * d;
+    if (splits > 1) {
+      store_none<float, DB>(a.part + 2 * part * all + place, live, d, lane);
+      store_none<float, DB>(a.part + (2 * part + 1) * all + place, live, d, lane);
+    } else {
+      store_none<S, DB>(static_cast<S*>(a.dk) + place, live, d, lane);
+      store_none<S, DB>(static_cast<S*>(a.dv) + place, live, d, lane);
+    }
     return;
   }
   int wave_first = first + 32 * wave;
@@ -219,8 +226,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
       to[BQ + tid] = st_delta;
     }
   };
-  load(0);
-  store(0);
+  const int items = tiles * G, it0 = (int)((int64_t)items * part / splits), it1 = (int)((int64_t)items * (part + 1) / splits);
+  load(it0);
+  store(it0);
   __syncthreads();
   T at(lane);
 
@@ -230,14 +238,14 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
 #pragma unroll
     for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
   const float c = a.scale2;
-  const int half = lane >> 5, items = tiles * G;
+  const int half = lane >> 5;
   const uint32_t own_v = lds_addr(smem) + wave * 32 * T::kPitch;
-  for (int it = 0; it < items; ++it) {
+  for (int it = it0; it < it1; ++it) {
     const uint32_t tq = lds + (it & 1) * kStage, tg = tq + kTileBytes;
     const float* stats = reinterpret_cast<const float*>(smem + kOwn + (it & 1) * kStage + 2 * kTileBytes);
     at.keep();
     const int q0 = (t0 + it % tiles) * BQ;
-    if (it + 1 < items) load(it + 1);
+    if (it + 1 < it1) load(it + 1);
     // queries from here on see the lane's key; all of the wave's keys are seen by the tile or none
     const int lim = a.n.causal ? key - shift : 0;
     const bool any = wave_first < s.lk && (!a.n.causal || q0 + BQ - 1 >= wave_first - shift);
@@ -285,15 +293,16 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
         add_columns<S, DB, 1>(ak, at, tq + b * 32 * T::kPitch, ds);
       }
     }
-    if (it + 1 < items) {
+    if (it + 1 < it1) {
       store(it + 1);
       __syncthreads();
     }
   }
   if (__syncthreads_or(bad)) {
-    const int q0 = t0 * BQ, n = min((zone + BQ - 1) / BQ * BQ, s.lq) - q0;
-    const auto seen = [&](int r) { return q0 + r >= key - shift; };
-    for (int h = hk * G; h < hk * G + G; ++h) {
+    for (int it = it0; it < it1; ++it) {
+      const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ, n = min(BQ, s.lq - q0);
+      if (q0 >= zone) continue;
+      const auto seen = [&](int r) { return q0 + r >= key - shift; };
       add_nonfinite<S, DB, false>(av, row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, n, d, lane, seen);
       add_nonfinite<S, DB, true>(ak, row_ptr(a.q, a.n.cu_q, s.row0, s.b, q0, h, ES), q_ts, n, d, lane, seen);
     }
@@ -306,9 +315,28 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
   }
-  const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d;
-  store_rows<S, DB>(ak, a.scale, static_cast<S*>(a.dk) + place, live, d, lane);
-  store_rows<S, DB>(av, 1.f, static_cast<S*>(a.dv) + place, live, d, lane);
+  const int64_t place = ((row0 + key) * a.n.Hk + hk) * (int64_t)d, all = a.n.Tk * a.n.Hk * d;
+  if (splits > 1) {
+    store_rows<float, DB>(ak, a.scale, a.part + 2 * part * all + place, live, d, lane);
+    store_rows<float, DB>(av, 1.f, a.part + (2 * part + 1) * all + place, live, d, lane);
+  } else {
+    store_rows<S, DB>(ak, a.scale, static_cast<S*>(a.dk) + place, live, d, lane);
+    store_rows<S, DB>(av, 1.f, static_cast<S*>(a.dv) + place, live, d, lane);
+  }
+}
+
+// dk, dv: the parts' shares added in their order, four elements a thread.
+template <typename S>
+__global__ __launch_bounds__(256) void att_dkv_join_kernel(AttArgs a, int64_t all, int splits) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // of 2 `all`: dk, then dv
+  if (e >= 2 * all) return;
+  floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < splits; ++p) sum += *reinterpret_cast<const floatx4*>(a.part + 2 * p * all + e);
+  S* out = e < all ? static_cast<S*>(a.dk) + e : static_cast<S*>(a.dv) + (e - all);
+  if constexpr (sizeof(S) == 2)
+    *reinterpret_cast<u32x2*>(out) = u32x2{Mma32<S>::pack2(sum[0], sum[1]), Mma32<S>::pack2(sum[2], sum[3])};
+  else
+    *reinterpret_cast<floatx4*>(out) = sum;
 }
 
 }  // namespace mhc

@@ -9,24 +9,25 @@
 namespace mhc {
 
 // A launch of `blocks` blocks; a size that the grid does not hold is refused.
-template <typename K>
-int att_launch(K kernel, const AttArgs& a, int64_t slots, int64_t heads, int threads, size_t lds, hipStream_t st, const char* what) {
-  const int64_t blocks = slots * heads;
+template <typename K, typename... X>
+int att_launch(K kernel, const AttArgs& a, int64_t slots, int64_t per_slot, int threads, size_t lds, hipStream_t st,
+               const char* what, X... x) {
+  const int64_t blocks = slots * per_slot;
   if (blocks > 0xffffffffll / threads)
     return set_error(MHC_ERR_UNSUPPORTED, "%s: %lld blocks exceed the 2^32 work-items of a dispatch", what, (long long)blocks);
   if (blocks == 0) return MHC_OK;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, a, slots);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, a, slots, x...);
   return check_launch(what);
 }
 
-// Waves of a block, tile height / 32 and waves a SIMD unit holds of each
-// kernel, by the bytes of a head: registers hold a wave's own rows and its sums.
+// What a head's bytes leave of the registers: two waves a SIMD unit, or one;
+// tiles of 64 keys, or 32; the block's own values in LDS in the dk, dv kernel.
 template <typename S, int DB> struct AttShape {
   static constexpr int kBytes = 32 * DB * (int)sizeof(S);
-  static constexpr int kFwdNW = kBytes == 256 && sizeof(S) == 2 ? 8 : 4, kFwdNB = sizeof(S) == 2 && DB <= 4 ? 2 : 1, kFwdWPE = kBytes <= 256 ? 2 : 1;
-  static constexpr int kDqNW = kBytes == 256 && sizeof(S) == 2 ? 8 : 4, kDqNB = 1, kDqWPE = kBytes <= 256 ? 2 : 1;
-  static constexpr int kDkvNW = 4, kDkvNB = 1, kDkvWPE = kBytes <= 256 ? 2 : 1;
+  static constexpr int kWPE = kBytes <= 256 ? 2 : 1;
+  static constexpr int kFwdNB = sizeof(S) == 2 && DB <= 4 ? 2 : 1;
   static constexpr bool kDkvLds = kBytes >= 256;
+  static constexpr bool kBig = kBytes == 256 && sizeof(S) == 2;  // 256 queries a block are a choice
 };
 
 template <typename S, int DB>
@@ -34,7 +35,7 @@ int att_split_width(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   const int64_t blocks = p.slots * a.n.Hk * p.splits, rows = a.n.Tq * a.n.H;
   if (blocks > 0xffffffffll / 256 || rows > 0xffffffffll / 256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
-  constexpr int WPE = AttShape<S, DB>::kBytes <= 256 ? 2 : 1;
+  constexpr int WPE = AttShape<S, DB>::kWPE;
   hipLaunchKernelGGL((att_split_kernel<S, DB, WPE>), dim3((unsigned)blocks), dim3(64 * kSplitWaves), (split_lds<S, DB>()), st, a,
                      p.slots, p.splits);
   if (const int rc = check_launch("attention")) return rc;
@@ -43,29 +44,56 @@ int att_split_width(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   return check_launch("attention");
 }
 
+template <typename S, int DB, int NW>
+int att_fwd_run(const AttArgs& a, int64_t slots, hipStream_t st) {
+  using A = AttShape<S, DB>;
+  return att_launch(att_fwd_kernel<S, DB, NW, A::kFwdNB, A::kWPE>, a, slots, a.n.H, 64 * NW,
+                    (size_t)4 * 32 * A::kFwdNB * Tile<S, DB>::kPitch, st, "attention");
+}
+template <typename S, int DB, int NW>
+int att_dq_run(const AttArgs& a, int64_t slots, hipStream_t st) {
+  return att_launch(att_dq_kernel<S, DB, NW, 1, AttShape<S, DB>::kWPE>, a, slots, a.n.H, 64 * NW,
+                    (size_t)4 * 32 * Tile<S, DB>::kPitch, st, "attention_backward");
+}
+
 template <typename S, int DB>
 int att_fwd_width(const AttArgs& a, hipStream_t st) {
-  using A = AttShape<S, DB>;
-  const AttSplit p = att_split(a.n, device_cu_count());
+  const int cus = device_cu_count();
+  const AttSplit p = att_split(a.n, cus);
   if (p.use) return att_split_width<S, DB>(a, p, st);
-  constexpr size_t lds = 4 * 32 * A::kFwdNB * Tile<S, DB>::kPitch;
-  const int64_t slots = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 32 * A::kFwdNW);
-  return att_launch(att_fwd_kernel<S, DB, A::kFwdNW, A::kFwdNB, A::kFwdWPE>, a, slots, a.n.H, 64 * A::kFwdNW, lds, st,
-                    "attention");
+  if constexpr (AttShape<S, DB>::kBig) {
+    const int64_t big = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 256);
+    if (att_big(a.n, big, cus)) return att_fwd_run<S, DB, 8>(a, big, st);
+  }
+  return att_fwd_run<S, DB, 4>(a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 128), st);
 }
+
+template <typename S, int DB>
+int att_dq_width(const AttArgs& a, hipStream_t st) {
+  if constexpr (AttShape<S, DB>::kBig) {
+    const int64_t big = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 256);
+    if (att_big(a.n, big, device_cu_count())) return att_dq_run<S, DB, 8>(a, big, st);
+  }
+  return att_dq_run<S, DB, 4>(a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 128), st);
+}
+
 template <typename S, int DB>
 int att_bwd_width(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
-  constexpr size_t lds = 4 * 32 * A::kDqNB * Tile<S, DB>::kPitch;
-  constexpr size_t lds2 = 2 * (2 * 32 * A::kDkvNB * Tile<S, DB>::kPitch + (2 * 32 * A::kDkvNB * 4 + 255) / 256 * 256) +
-                          (A::kDkvLds ? 32 * A::kDkvNW * Tile<S, DB>::kPitch : 0);
-  const int64_t slots = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 32 * A::kDqNW);
-  if (const int rc = att_launch(att_dq_kernel<S, DB, A::kDqNW, A::kDqNB, A::kDqWPE>, a, slots, a.n.H, 64 * A::kDqNW, lds, st,
-                                "attention_backward"))
+  constexpr int kPitch = Tile<S, DB>::kPitch;
+  if (const int rc = att_dq_width<S, DB>(a, st)) return rc;
+  const AttBwdPlan p = att_bwd_plan(a.n, device_cu_count());
+  const int64_t slots = att_slots(a.n.cu_k != nullptr, a.n.Tk, a.n.B, a.n.Sk, 128);
+  constexpr size_t lds = 2 * (2 * 32 * kPitch + 256) + (A::kDkvLds ? 128 * kPitch : 0);
+  if (const int rc = att_launch(att_dkv_kernel<S, DB, 4, 1, A::kWPE, A::kDkvLds>, a, slots, (int64_t)a.n.Hk * p.splits, 256,
+                                lds, st, "attention_backward", p.splits))
     return rc;
-  const int64_t slots_k = att_slots(a.n.cu_k != nullptr, a.n.Tk, a.n.B, a.n.Sk, 32 * A::kDkvNW);
-  return att_launch(att_dkv_kernel<S, DB, A::kDkvNW, A::kDkvNB, A::kDkvWPE, A::kDkvLds>, a, slots_k, a.n.Hk, 64 * A::kDkvNW, lds2, st,
-                    "attention_backward");
+  if (p.splits == 1) return MHC_OK;
+  const int64_t all = a.n.Tk * a.n.Hk * a.n.d, blocks = (2 * all + 1023) / 1024;
+  if (blocks > 0xffffffffll / 256)
+    return set_error(MHC_ERR_UNSUPPORTED, "attention_backward: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
+  hipLaunchKernelGGL(att_dkv_join_kernel<S>, dim3((unsigned)blocks), dim3(256), 0, st, a, all, p.splits);
+  return check_launch("attention_backward");
 }
 
 template <typename S>
