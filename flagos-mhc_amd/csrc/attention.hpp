@@ -247,7 +247,7 @@ struct Tile {
   static constexpr int kWide = DB <= 2 ? 64 : (DB <= 4 ? 128 : 256);   // columns of a row's place
   static constexpr int kPitch = kWide * kEs;                           // bytes
   static constexpr int kChunks = kPitch / 16;
-  static constexpr int kUsed = kD * kEs / 16;    // chunks that are loaded
+  static constexpr int kUsed = kD * kEs / 16;    // chunks that are read
   static constexpr int kSteps = kUsed / 2;       // row fragments
   static constexpr int kColSteps = 16 / kE;      // column fragments of 32 rows
   static constexpr int kLow = kChunks >= 16 ? 16 : 8;  // chunks whose position is exclusive-ored
@@ -308,14 +308,14 @@ struct Tile {
 template <typename S, int DB, int R, int NT>
 struct TileStage {
   using T = Tile<S, DB>;
-  static_assert(NT % T::kUsed == 0 && R * T::kUsed % NT == 0, "a thread keeps its chunk");
-  static constexpr int kRows = NT / T::kUsed;  // of a load
+  static_assert(NT % T::kChunks == 0 && R * T::kChunks % NT == 0, "a thread keeps its chunk");
+  static constexpr int kRows = NT / T::kChunks;  // of a load
   static constexpr int kLoads = R / kRows;
   u32x4 v[kLoads];
 
   static __device__ __forceinline__ uint32_t offset(int ts_bytes, int d_chunks, int tid) {
-    const int c = tid % T::kUsed;
-    return c < d_chunks ? (uint32_t)(tid / T::kUsed * ts_bytes + c * 16) : kBufferOob;
+    const int c = tid % T::kChunks;
+    return c < d_chunks ? (uint32_t)(tid / T::kChunks * ts_bytes + c * 16) : kBufferOob;
   }
   __device__ __forceinline__ void load(const char* base, int ts_bytes, int left, uint32_t off) {
 #pragma unroll
@@ -342,7 +342,7 @@ struct TileStage {
   __device__ __forceinline__ void store(uint32_t tile, int tid) const {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
-      *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(tile + T::at(tid / T::kUsed + i * kRows, tid % T::kUsed)) = v[i];
+      *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(tile + T::at(tid / T::kChunks + i * kRows, tid % T::kChunks)) = v[i];
   }
 };
 

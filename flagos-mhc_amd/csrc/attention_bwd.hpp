@@ -30,7 +30,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot;
   int h, first;
-  att_item(slots, slot, h);
+  att_item(a.n, slots, slot, h);
   const AttSeq s = q_tile(a.n, slot, BM, first);
   if (first >= s.lq) return;
   const int hk = h / (a.n.H / a.n.Hk), d = a.n.d, dc = d * ES / 16;

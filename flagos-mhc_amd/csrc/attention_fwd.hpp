@@ -7,14 +7,16 @@
 
 namespace mhc {
 
-// Items (tile of queries, head): an XCD walks a contiguous run of heads, so
+// Items (tile of queries, head): an XCD walks a contiguous run of key heads, so
 // that the blocks it runs at a time read the same keys and values from its L2;
-// a head's tiles go from its last to its first, since under a causal mask the
-// last ones are the longest.
-__device__ __forceinline__ void att_item(int64_t slots, int64_t& slot, int& h) {
+// within a key head the tiles go from the last to the first, each for all heads
+// of the group, since under a causal mask the last ones are the longest.
+__device__ __forceinline__ void att_item(const AttDims& n, int64_t slots, int64_t& slot, int& h) {
   const int64_t item = xcd_contig(blockIdx.x, gridDim.x);
-  h = (int)(item / slots);
-  slot = slots - 1 - item % slots;
+  const int G = n.H / n.Hk;
+  const int64_t of = item / G;
+  h = (int)(of / slots) * G + (int)(item % G);
+  slot = slots - 1 - of % slots;
 }
 
 template <typename S, int DB>
@@ -36,7 +38,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int64_t slot;
   int h, first;
-  att_item(slots, slot, h);
+  att_item(a.n, slots, slot, h);
   const AttSeq s = q_tile(a.n, slot, BM, first);
   if (first >= s.lq) return;
   const int hk = h / (a.n.H / a.n.Hk), d = a.n.d, dc = d * ES / 16;

@@ -28,8 +28,12 @@ inline int64_t att_slots(bool packed, int64_t T, int B, int S, int R) {
 // tokens, 700 blocks: 10 % slower.
 inline bool att_big(const AttDims& n, int64_t slots, int cus) { return slots * n.H >= 8 * (int64_t)cus; }
 
-// Few queries: the rows of a group's heads share tiles, and the keys of a tile
-// are split into `splits` parts.
+// Few queries, or few blocks of 128 (less than one a compute unit): the rows of
+// a group's heads share tiles of 32, whose keys a block's waves split, and,
+// where even those are few, `splits` blocks.
+//   1024 tokens, 4 heads of 128 bf16 (36 blocks of 128): 30 -> 17 us; 777 in
+//   three, 16 heads of 80 (160): 16.1 -> 13.7 us; 2048 in four, 16 heads of 128
+//   (288): 27 us, split 32 us.
 struct AttSplit {
   bool use;
   int splits;
@@ -44,12 +48,12 @@ inline AttSplit att_split(const AttDims& n, int cus) {
   AttSplit s = {false, 1, 0};
   if (n.B == 0 || n.Tq == 0 || n.Tk == 0) return s;
   const int64_t rows = (n.Tq + n.B - 1) / n.B * G;  // of a sequence, on average
-  s.use = rows <= 64;
+  s.use = rows <= 64 || att_slots(n.cu_q != nullptr, n.Tq, n.B, n.Sq, 128) * n.H < cus;
   s.slots = n.cu_q ? n.Tq * G / 32 + n.B + 1 : (int64_t)n.B * (((int64_t)n.Sq * G + 31) / 32);
   const int64_t blocks = s.slots * n.Hk;
-  const int64_t longest = n.cu_k ? n.Tk : n.Sk;
-  int64_t want = (2 * (int64_t)cus + blocks - 1) / blocks;
-  const int64_t most = (longest + 127) / 128;  // a tile for each wave
+  const int64_t longest = n.cu_k ? (n.Tk + n.B - 1) / n.B : n.Sk;  // keys of a sequence, on average
+  int64_t want = 2 * (int64_t)cus / blocks;
+  const int64_t most = longest / 512;  // four tiles for each wave
   if (want > most) want = most;
   s.splits = want < 1 ? 1 : (int)want;
   return s;
@@ -61,15 +65,15 @@ struct AttBwdPlan {
   size_t delta_bytes, part_bytes;
 };
 
-inline AttBwdPlan att_bwd_plan(const AttDims& n, int cus) {
+inline AttBwdPlan att_bwd_plan(const AttDims& n, bool fp32, int cus) {
   AttBwdPlan p = {1, ((size_t)n.H * n.Tq * 4 + 255) / 256 * 256, 0};
   if (n.B == 0 || n.Tq == 0 || n.Tk == 0) return p;
   const int64_t blocks = att_slots(n.cu_k != nullptr, n.Tk, n.B, n.Sk, 128) * n.Hk;
   const int64_t rows = (n.Tq + n.B - 1) / n.B * (n.H / n.Hk);  // queries of a key head and sequence, on average
   int64_t want = (3 * (int64_t)cus + blocks - 1) / blocks;
-  const int64_t most = rows / 256;  // tiles of 32 worth the sums' way through memory
+  const int64_t most = rows / (fp32 ? 64 : 128);  // what is worth the sums' way through memory
   want = want < most ? want : most;
-  p.splits = want < 1 ? 1 : (want > 8 ? 8 : (int)want);
+  p.splits = want < 1 ? 1 : (want > 16 ? 16 : (int)want);
   if (p.splits > 1) p.part_bytes = (size_t)p.splits * 2 * n.Tk * n.Hk * n.d * 4;
   return p;
 }

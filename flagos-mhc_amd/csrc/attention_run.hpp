@@ -26,7 +26,8 @@ template <typename S, int DB> struct AttShape {
   static constexpr int kBytes = 32 * DB * (int)sizeof(S);
   static constexpr int kWPE = kBytes <= 256 ? 2 : 1;
   static constexpr int kFwdNB = sizeof(S) == 2 && DB <= 4 ? 2 : 1;
-  static constexpr bool kDkvLds = kBytes >= 256;
+  static constexpr int kBwdNB = sizeof(S) == 2 && DB <= 2 ? 2 : 1;
+  static constexpr bool kDkvLds = kBytes > 128;
   static constexpr bool kBig = kBytes == 256 && sizeof(S) == 2;  // 256 queries a block are a choice
 };
 
@@ -52,8 +53,9 @@ int att_fwd_run(const AttArgs& a, int64_t slots, hipStream_t st) {
 }
 template <typename S, int DB, int NW>
 int att_dq_run(const AttArgs& a, int64_t slots, hipStream_t st) {
-  return att_launch(att_dq_kernel<S, DB, NW, 1, AttShape<S, DB>::kWPE>, a, slots, a.n.H, 64 * NW,
-                    (size_t)4 * 32 * Tile<S, DB>::kPitch, st, "attention_backward");
+  constexpr int NB = AttShape<S, DB>::kBwdNB;
+  return att_launch(att_dq_kernel<S, DB, NW, NB, AttShape<S, DB>::kWPE>, a, slots, a.n.H, 64 * NW,
+                    (size_t)4 * 32 * NB * Tile<S, DB>::kPitch, st, "attention_backward");
 }
 
 template <typename S, int DB>
@@ -70,6 +72,10 @@ int att_fwd_width(const AttArgs& a, hipStream_t st) {
 
 template <typename S, int DB>
 int att_dq_width(const AttArgs& a, hipStream_t st) {
+  const AttSplit p = att_split(a.n, device_cu_count());
+  if (p.use)
+    return att_launch(att_dq_split_kernel<S, DB, AttShape<S, DB>::kBytes <= 128 ? 2 : 1>, a, p.slots, a.n.Hk, 64 * kSplitWaves,
+                      split_lds<S, DB>(), st, "attention_backward");
   if constexpr (AttShape<S, DB>::kBig) {
     const int64_t big = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 256);
     if (att_big(a.n, big, device_cu_count())) return att_dq_run<S, DB, 8>(a, big, st);
@@ -82,10 +88,10 @@ int att_bwd_width(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
   constexpr int kPitch = Tile<S, DB>::kPitch;
   if (const int rc = att_dq_width<S, DB>(a, st)) return rc;
-  const AttBwdPlan p = att_bwd_plan(a.n, device_cu_count());
+  const AttBwdPlan p = att_bwd_plan(a.n, sizeof(S) == 4, device_cu_count());
   const int64_t slots = att_slots(a.n.cu_k != nullptr, a.n.Tk, a.n.B, a.n.Sk, 128);
-  constexpr size_t lds = 2 * (2 * 32 * kPitch + 256) + (A::kDkvLds ? 128 * kPitch : 0);
-  if (const int rc = att_launch(att_dkv_kernel<S, DB, 4, 1, A::kWPE, A::kDkvLds>, a, slots, (int64_t)a.n.Hk * p.splits, 256,
+  constexpr size_t lds = 2 * (2 * 32 * A::kBwdNB * kPitch + 256 * A::kBwdNB) + (A::kDkvLds ? 128 * kPitch : 0);
+  if (const int rc = att_launch(att_dkv_kernel<S, DB, 4, A::kBwdNB, A::kWPE, A::kDkvLds>, a, slots, (int64_t)a.n.Hk * p.splits, 256,
                                 lds, st, "attention_backward", p.splits))
     return rc;
   if (p.splits == 1) return MHC_OK;
@@ -99,15 +105,17 @@ int att_bwd_width(const AttArgs& a, hipStream_t st) {
 template <typename S>
 int att_fwd(const AttArgs& a, hipStream_t st) {
   if (a.n.d <= 64) return att_fwd_width<S, 2>(a, st);
+  if (a.n.d <= 96) return att_fwd_width<S, 3>(a, st);
   if (a.n.d <= 128) return att_fwd_width<S, 4>(a, st);
-  if constexpr (sizeof(S) == 2) return att_fwd_width<S, 8>(a, st);
+  if constexpr (sizeof(S) == 2) return a.n.d <= 192 ? att_fwd_width<S, 6>(a, st) : att_fwd_width<S, 8>(a, st);
   return MHC_ERR_UNSUPPORTED;  // (refused before)
 }
 template <typename S>
 int att_bwd(const AttArgs& a, hipStream_t st) {
   if (a.n.d <= 64) return att_bwd_width<S, 2>(a, st);
+  if (a.n.d <= 96) return att_bwd_width<S, 3>(a, st);
   if (a.n.d <= 128) return att_bwd_width<S, 4>(a, st);
-  if constexpr (sizeof(S) == 2) return att_bwd_width<S, 8>(a, st);
+  if constexpr (sizeof(S) == 2) return a.n.d <= 192 ? att_bwd_width<S, 6>(a, st) : att_bwd_width<S, 8>(a, st);
   return MHC_ERR_UNSUPPORTED;
 }
 

@@ -26,6 +26,43 @@ constexpr size_t split_lds() {
   return kSplitWaves * ((tile > sums ? tile : sums) + 32 * 2 * 4);
 }
 
+// Tile of 32 rows (query * G + head of the group) that slot `slot` stands for:
+// its sequence and first row (lq * G or more: nothing to do).
+__device__ __forceinline__ AttSeq group_tile(const AttDims& n, int64_t slot, int64_t& first) {
+  const int G = n.H / n.Hk;
+  if (!n.cu_q) {
+    const int64_t per = ((int64_t)n.Sq * G + 31) / 32;
+    first = slot % per * 32;
+    return att_seq(n, (int)(slot / per));
+  }
+  // the slots of tiles of 32 of G rows a query, as slot_sequence's
+  const int lane = threadIdx.x & 63;
+  int lo = 0, m = n.B + 1;
+  while (m > 1) {
+    const int step = (m + 63) / 64, c = lane * step;
+    int hit = __popcll(__ballot(c < m && cu_at(n.cu_q, lo + c, n.Tq) * G / 32 + lo + c <= slot));
+    hit = hit < 1 ? 1 : hit;
+    const int skip = (hit - 1) * step;
+    lo += skip;
+    m = m - skip < step ? m - skip : step;
+  }
+  const int b = __builtin_amdgcn_readfirstlane(lo);
+  const AttSeq s = att_seq(n, b);
+  first = (slot - (s.row0 * G / 32 + b)) * 32;
+  return s;
+}
+
+// A lane's own row as fragments; zero if there is none.
+template <typename S, int DB>
+__device__ __forceinline__ void lane_row(const char* p, bool live, int d_chunks, int lane, u32x4 (&f)[Tile<S, DB>::kSteps]) {
+#pragma unroll
+  for (int t = 0; t < Tile<S, DB>::kSteps; ++t) {
+    const int c = 2 * t + (lane >> 5);
+    f[t] = u32x4{0u, 0u, 0u, 0u};
+    if (live && c < d_chunks) f[t] = ld16(p + c * 16);
+  }
+}
+
 template <typename S, int DB, int WPE>
 __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_split_kernel(AttArgs a, int64_t slots, int splits) {
   using T = Tile<S, DB>;
@@ -39,27 +76,8 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_split_kernel(AttArg
   const int hk = (int)(item / splits % a.n.Hk);
   const int64_t slot = item / splits / a.n.Hk;
   const int G = a.n.H / a.n.Hk, d = a.n.d, dc = d * ES / 16;
-  AttSeq s;
   int64_t first;  // first row (query * G + head)
-  if (a.n.cu_q) {
-    // rows are G a query: the slots of tiles of 32 of them
-    int lo = 0, n = a.n.B + 1;
-    while (n > 1) {
-      const int step = (n + 63) / 64, c = lane * step;
-      int hit = __popcll(__ballot(c < n && cu_at(a.n.cu_q, lo + c, a.n.Tq) * G / 32 + lo + c <= slot));
-      hit = hit < 1 ? 1 : hit;
-      const int skip = (hit - 1) * step;
-      lo += skip;
-      n = n - skip < step ? n - skip : step;
-    }
-    const int b = __builtin_amdgcn_readfirstlane(lo);
-    s = att_seq(a.n, b);
-    first = (slot - (s.row0 * G / 32 + b)) * 32;
-  } else {
-    const int64_t per = ((int64_t)a.n.Sq * G + 31) / 32;
-    s = att_seq(a.n, (int)(slot / per));
-    first = slot % per * 32;
-  }
+  const AttSeq s = group_tile(a.n, slot, first);
   if (first >= (int64_t)s.lq * G) return;
   const int64_t r = first + (lane & 31);
   const int i = (int)(r / G), g = (int)(r % G), h = hk * G + g;
@@ -75,15 +93,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_split_kernel(AttArg
   const int tiles = (to - from + 31) / 32;
 
   u32x4 q[T::kSteps];
-  {
-    const char* p = row_ptr(a.q, a.n.cu_q, s.row0, s.b, live ? i : 0, h, ES);
-#pragma unroll
-    for (int t = 0; t < T::kSteps; ++t) {
-      const int c = 2 * t + half;
-      q[t] = u32x4{0u, 0u, 0u, 0u};
-      if (live && !s.none && c < dc) q[t] = ld16(p + c * 16);
-    }
-  }
+  lane_row<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, live ? i : 0, h, ES), live && !s.none, dc, lane, q);
   const int k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES);
   const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, from, hk, ES);
   const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, from, hk, ES);
@@ -204,6 +214,137 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_split_kernel(AttArg
       store_rows<float, 1>(z, 1.f, a.part + ((int64_t)part * a.n.Tq * a.n.H + orow) * d + 32 * db, live, d - 32 * db, lane);
     else
       store_rows<S, 1>(z, inv, static_cast<S*>(a.out) + orow * d + 32 * db, live, d - 32 * db, lane);
+  }
+}
+
+// dq, and D, for the same rows: a backward of few queries, or of too few blocks
+// of 128.  Each of the four waves adds what its tiles of keys give; the four
+// sums meet in LDS.  k is turned through LDS, v comes as the operand it is.
+template <typename S, int DB, int WPE>
+__global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(AttArgs a, int64_t slots) {
+  using T = Tile<S, DB>;
+  constexpr int ES = (int)sizeof(S);
+  constexpr size_t kRegion = split_lds<S, DB>() / kSplitWaves - 256;
+  extern __shared__ __attribute__((aligned(256))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+  const int hk = (int)(blockIdx.x % a.n.Hk);
+  const int64_t slot = slots - 1 - blockIdx.x / a.n.Hk;
+  const int G = a.n.H / a.n.Hk, d = a.n.d, dc = d * ES / 16;
+  int64_t first;
+  const AttSeq s = group_tile(a.n, slot, first);
+  if (first >= (int64_t)s.lq * G) return;
+  const int64_t r = first + (lane & 31);
+  const int i = (int)(r / G), h = hk * G + (int)(r % G);
+  const bool live = i < s.lq;
+  const int64_t orow = (s.row0 + i) * a.n.H + h, stat = (int64_t)h * a.n.Tq + s.row0 + i;
+  const int shift = s.lk - s.lq;
+  const int lim = s.none || !live ? -1 : (a.n.causal ? min(s.lk - 1, i + shift) : s.lk - 1);
+  const int last = (int)min((int64_t)s.lq - 1, (first + 31) / G);
+  const int keys = s.none ? 0 : max(0, a.n.causal ? min(s.lk, last + shift + 1) : s.lk);
+  const int tiles = (keys + 31) / 32;
+
+  u32x4 q[T::kSteps], go[T::kSteps];
+  const bool load = live && !s.none;
+  const int at_row = live ? i : 0;
+  lane_row<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, at_row, h, ES), load, dc, lane, q);
+  lane_row<S, DB>(row_ptr(a.go, a.n.cu_q, s.row0, s.b, at_row, h, ES), load, dc, lane, go);
+  float delta = 0.f;
+  {
+    u32x4 o[T::kSteps];
+    lane_row<S, DB>(row_ptr(a.o, a.n.cu_q, s.row0, s.b, at_row, h, ES), load, dc, lane, o);
+#pragma unroll
+    for (int t = 0; t < T::kSteps; ++t) {
+      float x[Store<S>::VEC], y[Store<S>::VEC];
+      Store<S>::unpack(o[t], x);
+      Store<S>::unpack(go[t], y);
+#pragma unroll
+      for (int j = 0; j < Store<S>::VEC; ++j) delta = __builtin_fmaf(x[j], y[j], delta);
+    }
+    delta = add_xor32(delta);
+    if (live && wave == 0 && lane < 32) a.delta[stat] = delta;
+  }
+  const float lse = load ? a.lse[stat] : -__builtin_inff();
+  const float lse2 = lse == -__builtin_inff() ? __builtin_inff() : lse * kLog2e;
+
+  const int k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES);
+  const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const uint32_t tile = lds_addr(smem) + wave * kRegion;
+  const int zone = a.n.causal ? max(0, (int)(first / G) + shift + 1) : 0x7fffffff;
+  bool bad = false;
+  floatx16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[db][j] = 0.f;
+  const float c = a.scale2;
+  u32x4 v[T::kSteps];
+  TileStage<S, DB, 32, 64> sk;
+  const uint32_t k_off = sk.offset(k_ts, dc, lane);
+  T at(lane);
+  if (wave < tiles) {
+    sk.load(kp + (int64_t)wave * 32 * k_ts, k_ts, s.lk - wave * 32, k_off);
+    load_rows<S, DB>(vp + (int64_t)wave * 32 * v_ts, v_ts, s.lk - wave * 32, dc, lane, v);
+  }
+  for (int t = wave; t < tiles; t += kSplitWaves) {
+    const int next = t + kSplitWaves, k0 = t * 32;
+    at.keep();
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    if (k0 + 32 > zone) bad |= sk.clean();
+    sk.store(tile, ln & 63);
+    if (next < tiles) sk.load(kp + (int64_t)next * 32 * k_ts, k_ts, s.lk - next * 32, k_off);
+    floatx16 dp;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) dp[j] = 0.f;
+#pragma unroll
+    for (int u = 0; u < T::kSteps; ++u) dp = Mma32<S>::fma(v[u], go[u], dp);
+    if (next < tiles) load_rows<S, DB>(vp + (int64_t)next * 32 * v_ts, v_ts, s.lk - next * 32, dc, lane, v);
+    const floatx16 sc = row_products<S, DB>(at, tile, 0, q);
+    const int left = lim - k0 - 4 * half;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float x = hw_exp2(__builtin_fmaf(sc[j], c, -lse2)) * (dp[j] - delta);
+      dp[j] = acc_row(j, 0) <= left ? x : 0.f;
+    }
+    u32x4 p[1][T::kColSteps];
+#pragma unroll
+    for (int u = 0; u < T::kColSteps; ++u) p[0][u] = acc_frag<S>(dp, u);
+    add_columns<S, DB, 1>(acc, at, tile, p);
+  }
+
+  bad = __syncthreads_or(bad);
+  float* region = reinterpret_cast<float*>(smem + wave * kRegion);
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) region[(db * 16 + j) * 64 + lane] = acc[db][j];
+  __syncthreads();
+  for (int db = wave; db < DB; db += kSplitWaves) {
+    floatx16 z[1];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < kSplitWaves; ++w) x += reinterpret_cast<const float*>(smem + w * kRegion)[(db * 16 + j) * 64 + lane];
+      z[0][j] = x;
+    }
+    if (bad) {
+      // whole rows become NaN: every column of the row is looked at, this block of 32 written
+      const int z0 = zone / 32 * 32;
+      for (int row = 0; row < keys - z0; ++row) {
+        float any = 0.f;
+        for (int e = 0; e < d; ++e) {
+          const float x = load_elem<S>(reinterpret_cast<const S*>(kp + (int64_t)(z0 + row) * k_ts), e);
+          any = (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 1.f : any;
+        }
+        if (any != 0.f && z0 + row <= lim) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) z[0][j] = __builtin_nanf("");
+        }
+      }
+    }
+    store_rows<S, 1>(z, a.scale, static_cast<S*>(a.out) + orow * d + 32 * db, live, d - 32 * db, lane);
   }
 }
 
