@@ -244,3 +244,13 @@ def attention_fn(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None,
         return attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, lengths_k=lengths_k, causal=causal,
                          scale=scale)["out"]
     return AttentionFn.apply(q, k, v, cu_seqlens, cu_seqlens_k, lengths_k, causal, scale)
+
+
+def projected_width(what, heads, w_q, w_k, w_v):
+    """The head width of projections (heads * d, D), (heads_k * d, D) twice."""
+    if heads < 1 or w_q.dim() != 2 or w_q.shape[0] % heads or w_q.shape[0] < heads:
+        raise ValueError(f"{what}: w_q of shape {tuple(w_q.shape)} for {heads} heads")
+    d = w_q.shape[0] // heads
+    if w_k.dim() != 2 or w_k.shape[0] % d or w_k.shape[0] < d or w_v.shape != w_k.shape:
+        raise ValueError(f"{what}: w_k of shape {tuple(w_k.shape)} and w_v of {tuple(w_v.shape)} for heads of {d}")
+    return d

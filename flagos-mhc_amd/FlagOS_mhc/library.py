@@ -36,6 +36,12 @@ and the operators between pre and post (``FlagOS_mhc.sublayer``):
         -> (grad_x, grad_w_gate, grad_w_up, grad_w_down); the last three are empty with need_weights=False
     torch.ops.flagos_mhc.dropout(x, p, seed, offset, state) -> y, with seed and
         offset as signed 64-bit integers; its backward is the op on the gradient
+    torch.ops.flagos_mhc.rotary(q, k, freqs, positions, cu_seqlens, layout, amplitude, inverse)
+        -> (q, k), k's empty if it is None; its backward is the op with inverse the other way
+    torch.ops.flagos_mhc.attention(q, k, v, cu_seqlens, cu_seqlens_k, lengths_k, causal, scale, save)
+        -> (out, lse); lse is empty with save=False
+    torch.ops.flagos_mhc.attention_backward(grad_out, q, k, v, out, lse, cu_seqlens,
+        cu_seqlens_k, lengths_k, causal, scale) -> (grad_q, grad_k, grad_v)
 
 The forward pre op also returns the fp32 inv_rms, mixes and pre its backward
 needs; they are marked non-differentiable (likewise for the fused op).
@@ -43,8 +49,8 @@ needs; they are marked non-differentiable (likewise for the fused op).
 ``mhc_post_pre_clamp_sinkhorn_op`` are the autograd-aware entry points with
 the return conventions of ``mhc_post_fn`` / ``mhc_pre_clamp_sinkhorn_fn``
 (src/autograd.py:14-87) and ``mhc_post_pre_clamp_sinkhorn_fn``;
-``layer_norm_op``, ``gated_ffn_op``, ``dropout_op`` and ``mhc_ffn_layer_op``
-those of the same functions of ``FlagOS_mhc.sublayer``.  They refuse inputs
+``layer_norm_op``, ``gated_ffn_op``, ``dropout_op``, ``rotary_op``,
+``attention_op``, ``mhc_ffn_layer_op`` and ``mhc_attention_layer_op`` those of the same functions of ``FlagOS_mhc.sublayer``.  They refuse inputs
 with forward-mode derivatives, which the bare ops would drop without a word
 where no input requires a gradient.  The kernels allocate nothing outside
 torch's allocator and call no host synchronisation, so they can be captured in
@@ -60,6 +66,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from .attention import attention, attention_backward, projected_width
 from .dropout import dropout
 from .gated_ffn import gated_ffn, gated_ffn_backward, hidden_width
 from .layer_norm import layer_norm, layer_norm_backward
@@ -68,6 +75,7 @@ from .mhc_post_backward import mhc_post_backward, mhc_post_backward_sum, post_ba
 from .mhc_post_pre import mhc_post_pre_clamp_sinkhorn
 from .mhc_pre_clamp_sinkhorn import _pre_forward
 from .mhc_pre_clamp_sinkhorn_backward import _pre_backward, mhc_pre_clamp_sinkhorn_backward
+from .rotary import rotary, rotary_backward
 
 NAMESPACE = "flagos_mhc"
 
@@ -393,6 +401,90 @@ def _drop_grad(ctx, grad_y):
 _drop.register_autograd(_drop_grad, setup_context=_drop_setup)
 
 
+# ---- rotary positions ------------------------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::rotary", mutates_args=())
+def _rot(q: Tensor, k: Optional[Tensor], freqs: Tensor, positions: Optional[Tensor] = None,
+         cu_seqlens: Optional[Tensor] = None, layout: str = "half", amplitude: float = 1.0,
+         inverse: bool = False) -> Tuple[Tensor, Tensor]:
+    run = rotary_backward if inverse else rotary
+    qo, ko = run(q, k, freqs, positions, cu_seqlens=cu_seqlens, layout=layout, amplitude=amplitude)
+    return qo, q.new_empty((0,)) if ko is None else ko
+
+
+@_rot.register_fake
+def _rot_fake(q, k, freqs, positions=None, cu_seqlens=None, layout="half", amplitude=1.0, inverse=False):
+    return q.new_empty(q.shape), q.new_empty((0,) if k is None else k.shape)
+
+
+def _rot_setup(ctx, inputs, output):
+    q, k, freqs, *opt = inputs
+    positions, cu, layout, amplitude, inverse = (*opt, *(None, None, "half", 1.0, False)[len(opt):])
+    ctx.save_for_backward(freqs, positions, cu)
+    ctx.args = (layout, amplitude, not inverse)
+    ctx.one = k is None
+
+
+def _rot_grad(ctx, grad_q, grad_k):
+    freqs, positions, cu = ctx.saved_tensors
+    gq, gk = torch.ops.flagos_mhc.rotary(grad_q.contiguous(), None if ctx.one else grad_k.contiguous(), freqs, positions,
+                                         cu, *ctx.args)
+    return gq, None if ctx.one else gk, None, None, None, None, None, None
+
+
+_rot.register_autograd(_rot_grad, setup_context=_rot_setup)
+
+
+# ---- attention ---------------------------------------------------------------------------
+
+@torch.library.custom_op(f"{NAMESPACE}::attention", mutates_args=())
+def _att(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Optional[Tensor] = None, cu_seqlens_k: Optional[Tensor] = None,
+         lengths_k: Optional[Tensor] = None, causal: bool = True, scale: Optional[float] = None,
+         save: bool = True) -> Tuple[Tensor, Tensor]:
+    f = attention(q, k, v, cu_seqlens, cu_seqlens_k=cu_seqlens_k, lengths_k=lengths_k, causal=causal, scale=scale,
+                  need_backward=save)
+    return f["out"], f["lse"] if save else q.new_empty((0,), dtype=torch.float32)
+
+
+@_att.register_fake
+def _att_fake(q, k, v, cu_seqlens=None, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None, save=True):
+    rows = math.prod(q.shape[:-2])
+    return q.new_empty(q.shape), q.new_empty((q.shape[-2], rows) if save else (0,), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::attention_backward", mutates_args=())
+def _att_bwd(grad_out: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
+             cu_seqlens: Optional[Tensor] = None, cu_seqlens_k: Optional[Tensor] = None,
+             lengths_k: Optional[Tensor] = None, causal: bool = True,
+             scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    return attention_backward(grad_out, q, k, v, out, lse, cu_seqlens, cu_seqlens_k=cu_seqlens_k, lengths_k=lengths_k,
+                              causal=causal, scale=scale)
+
+
+@_att_bwd.register_fake
+def _att_bwd_fake(grad_out, q, k, v, out, lse, cu_seqlens=None, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None):
+    return tuple(t.new_empty(t.shape) for t in (q, k, v))
+
+
+def _att_setup(ctx, inputs, output):
+    q, k, v, *opt = inputs
+    cu, cu_k, lengths, causal, scale, save = (*opt, *(None, None, None, True, None, True)[len(opt):])
+    out, lse = output
+    ctx.mark_non_differentiable(lse)
+    ctx.save_for_backward(q, k, v, out, lse, cu, cu_k, lengths)
+    ctx.args, ctx.saved = (causal, scale), save
+
+
+def _att_grad(ctx, grad_out, _g_lse):
+    if not ctx.saved:
+        raise RuntimeError("attention: the forward ran with save=False")
+    return (*torch.ops.flagos_mhc.attention_backward(grad_out.contiguous(), *ctx.saved_tensors, *ctx.args),
+            *(None,) * 6)
+
+
+_att.register_autograd(_att_grad, setup_context=_att_setup)
+
+
 # ---- autograd-aware entry points ---------------------------------------------
 
 def _refuse_tangents(what, *tensors):
@@ -459,6 +551,38 @@ def mhc_ffn_layer_op(x, phi, alpha, base, norm_weight, norm_bias, w_gate, w_up, 
     """``mhc_ffn_layer_fn`` (``FlagOS_mhc.sublayer``) through the registered ops."""
     y, post, comb = mhc_pre_clamp_sinkhorn_op(x, phi, alpha, base, **mhc)
     h = gated_ffn_op(layer_norm_op(y, norm_weight, norm_bias, ln_eps), w_gate, w_up, w_down, activation)
+    if dropout_p != 0.0:
+        h = dropout_op(h, dropout_p, seed, offset, state)
+    return mhc_post_op(x, comb, h, post)
+
+
+def rotary_op(q, k, freqs, positions=None, *, cu_seqlens=None, layout="half", amplitude=1.0):
+    """``rotary_fn`` through the registered op."""
+    _refuse_tangents("rotary", q, k)
+    qo, ko = torch.ops.flagos_mhc.rotary(q, k, freqs, positions, cu_seqlens, layout, float(amplitude))
+    return qo, None if k is None else ko
+
+
+def attention_op(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None):
+    """``attention_fn`` through the registered op."""
+    _refuse_tangents("attention", q, k, v)
+    save = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v))
+    return torch.ops.flagos_mhc.attention(q, k, v, cu_seqlens, cu_seqlens_k, lengths_k, bool(causal),
+                                          None if scale is None else float(scale), save)[0]
+
+
+def mhc_attention_layer_op(x, phi, alpha, base, norm_weight, norm_bias, w_q, w_k, w_v, w_out, freqs=None, *, heads,
+                           cu_seqlens=None, positions=None, layout="half", amplitude=1.0, causal=True, scale=None,
+                           dropout_p=0.0, seed=0, offset=0, state=None, ln_eps=1e-5, **mhc):
+    """``mhc_attention_layer_fn`` (``FlagOS_mhc.sublayer``) through the registered ops."""
+    d = projected_width("mhc_attention_layer", heads, w_q, w_k, w_v)
+    y, post, comb = mhc_pre_clamp_sinkhorn_op(x, phi, alpha, base, **mhc)
+    h = layer_norm_op(y, norm_weight, norm_bias, ln_eps)
+    q, k, v = (torch.nn.functional.linear(h, w).unflatten(-1, (w.shape[0] // d, d)) for w in (w_q, w_k, w_v))
+    if freqs is not None:
+        at = None if positions is not None else cu_seqlens
+        q, k = rotary_op(q, k, freqs, positions, cu_seqlens=at, layout=layout, amplitude=amplitude)
+    h = torch.nn.functional.linear(attention_op(q, k, v, cu_seqlens, causal=causal, scale=scale).flatten(-2), w_out)
     if dropout_p != 0.0:
         h = dropout_op(h, dropout_p, seed, offset, state)
     return mhc_post_op(x, comb, h, post)
