@@ -13,6 +13,7 @@
 #pragma once
 
 #include "attention.hpp"
+#include "attention_bwd.hpp"
 #include "attention_fwd.hpp"
 
 namespace mhc {
@@ -248,8 +249,9 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(Att
   const int at_row = live ? i : 0;
   lane_row<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, at_row, h, ES), load, dc, lane, q);
   lane_row<S, DB>(row_ptr(a.go, a.n.cu_q, s.row0, s.b, at_row, h, ES), load, dc, lane, go);
+  const int sum = keys <= kSumKeys ? tiles : 0;  // as in att_dq_kernel
   float delta = 0.f;
-  {
+  if (sum == 0) {
     u32x4 o[T::kSteps];
     lane_row<S, DB>(row_ptr(a.o, a.n.cu_q, s.row0, s.b, at_row, h, ES), load, dc, lane, o);
 #pragma unroll
@@ -282,11 +284,13 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(Att
   TileStage<S, DB, 32, 64> sk;
   const uint32_t k_off = sk.offset(k_ts, dc, lane);
   T at(lane);
-  if (wave < tiles) {
+  // tile t's dS (P (go v^T) while delta is 0); the next tile's loads are begun on the way
+  const auto first_loads = [&]() {
+    if (wave >= tiles) return;
     sk.load(kp + (int64_t)wave * 32 * k_ts, k_ts, s.lk - wave * 32, k_off);
     load_rows<S, DB>(vp + (int64_t)wave * 32 * v_ts, v_ts, s.lk - wave * 32, dc, lane, v);
-  }
-  for (int t = wave; t < tiles; t += kSplitWaves) {
+  };
+  const auto scores = [&](int t) __attribute__((always_inline)) {
     const int next = t + kSplitWaves, k0 = t * 32;
     at.keep();
     int ln = lane;
@@ -307,6 +311,27 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(Att
       const float x = hw_exp2(__builtin_fmaf(sc[j], c, -lse2)) * (dp[j] - delta);
       dp[j] = acc_row(j, 0) <= left ? x : 0.f;
     }
+    return dp;
+  };
+  first_loads();
+  if (sum) {
+    float total = 0.f;
+    for (int t = wave; t < tiles; t += kSplitWaves) {
+      const floatx16 x = scores(t);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) total += x[j];
+    }
+    first_loads();
+    float* sums = reinterpret_cast<float*>(smem + kSplitWaves * kRegion);
+    total = add_xor32(total);
+    if (lane < 32) sums[wave * 32 + lane] = total;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kSplitWaves; ++w) delta += sums[w * 32 + (lane & 31)];
+    if (live && wave == 0 && lane < 32) a.delta[stat] = delta;
+  }
+  for (int t = wave; t < tiles; t += kSplitWaves) {
+    const floatx16 dp = scores(t);
     u32x4 p[1][T::kColSteps];
 #pragma unroll
     for (int u = 0; u < T::kColSteps; ++u) p[0][u] = acc_frag<S>(dp, u);
