@@ -77,8 +77,7 @@ _SIGNATURES = {
     "mhc_gated_ffn_bwd": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp,
                                      _vp, _vp, _sz, _i64, _i32, _i32, _i32, _vp]),
     "mhc_dropout": (_c.c_int, [_vp, _vp, _i64, _i32, _c.c_double, _c.c_uint64, _c.c_uint64, _vp, _vp]),
-    "mhc_rotary": (_c.c_int, [_vp, _vp, _i32, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _i32, _i64, _i32, _f32,
-                              _i32, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "mhc_rotary": (_c.c_int, [_c.c_char_p, _vp]),
     "mhc_attention_fwd_workspace_size": (_sz, [_c.c_char_p]),
     "mhc_attention_fwd": (_c.c_int, [_c.c_char_p, _vp, _vp, _vp, _sz, _vp]),
     "mhc_attention_bwd_workspace_size": (_sz, [_c.c_char_p]),
@@ -165,9 +164,10 @@ def operand(t: torch.Tensor, shape, dtype: torch.dtype) -> torch.Tensor:
 
 def cu_operand(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
     """Starts of packed sequences as the kernels take them: (B + 1,) int32."""
-    if t.dim() != 1 or t.numel() < 1 or t.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: {name} of shape {tuple(t.shape)} and {t.dtype}, expected (sequences + 1,) of int32")
-    return operand(t, t.shape, torch.int32)
+    dt = t.dtype
+    if t.dim() != 1 or t.shape[0] < 1 or (dt is not torch.int32 and dt is not torch.int64):
+        raise ValueError(f"{what}: {name} of shape {tuple(t.shape)} and {dt}, expected (sequences + 1,) of int32")
+    return t if dt is torch.int32 and t.is_contiguous() else operand(t, t.shape, torch.int32)
 
 
 @functools.lru_cache(maxsize=1024)

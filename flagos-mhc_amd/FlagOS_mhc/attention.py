@@ -24,6 +24,7 @@ runs PyTorch's.
 
 from __future__ import annotations
 
+import functools
 import math
 import struct
 
@@ -34,42 +35,55 @@ from . import _lib
 _ARGS = struct.Struct("3P9q3P2q6ifi")  # mhc_attention_args (include/mhc_amd.h)
 _STRIDES = struct.Struct("3q")
 _MAX_ROW_BYTES = 1 << 24
+_INTS = (torch.int32, torch.int64)
 
 
-def _rows(t, es):
-    """(t, (sequence, row, head) strides): t as the kernels take it, a copy
-    where its strides or address are not whole 16 bytes."""
-    shape, st = t.shape, t.stride()
-    H, d = shape[-2:]
-    n = len(shape)
-    row = st[-3] if shape[-3] > 1 else H * d
-    head = st[-2] if H > 1 else d
-    batch = st[0] if n == 4 and shape[0] > 1 else 0
-    mask = 16 // es - 1
-    if ((st[-1] != 1 and d > 1) or (row | head | batch) & mask or t.data_ptr() & 15 or row < d
-            or row * es > _MAX_ROW_BYTES):
-        t = t.clone(memory_format=torch.contiguous_format)
-        row, head = H * d, d
-        batch = shape[1] * row if n == 4 else 0
-    return t, (batch, row, head)
+def _rows(t, shape, es):
+    """(t, its address, (sequence, row, head) strides): t as the kernels take it,
+    a copy where its strides or address are not whole 16 bytes."""
+    H, d = shape[-2], shape[-1]
+    at = t.data_ptr()
+    if t.is_contiguous():
+        if not at & 15 and H * d * es <= _MAX_ROW_BYTES:
+            return t, at, (shape[1] * H * d if len(shape) == 4 else 0, H * d, d)
+    else:
+        st = t.stride()
+        row = st[-3] if shape[-3] > 1 else H * d
+        head = st[-2] if H > 1 else d
+        batch = st[0] if len(shape) == 4 and shape[0] > 1 else 0
+        if not ((st[-1] != 1 and d > 1) or (row | head | batch) & (16 // es - 1) or at & 15 or row < d
+                or row * es > _MAX_ROW_BYTES):
+            return t, at, (batch, row, head)
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), (shape[1] * H * d if len(shape) == 4 else 0, H * d, d)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(name, dev_index, packed_q, packed_k, *sizes):
+    """A *_workspace_size query: a function of the sizes and the device alone."""
+    rows_q, rows_k, B, H, Hk, wide, code = sizes
+    row = wide  # (the strides have to pass the checks, no more)
+    args = _ARGS.pack(16, 16, 16, 0, row, wide, 0, row, wide, 0, row, wide, 16 if packed_q else 0, 16 if packed_k else 0, 0,
+                      rows_q, rows_k, B, H, Hk, wide, code, 1, 1.0, 0)
+    with torch.cuda.device(dev_index):
+        return int(getattr(_lib.load(), name)(args))
 
 
 class _Call:
     """The checked operands of a call."""
 
-    __slots__ = ("q", "k", "v", "cu_q", "cu_k", "lengths", "B", "H", "Hk", "d", "wide", "es", "code", "rows_q", "rows_k",
-                 "args")
+    __slots__ = ("keep", "H", "Hk", "d", "wide", "es", "code", "rows_q", "rows_k", "args", "sizes")
 
     def __init__(self, what, q, k, v, cu_q, cu_k, lengths, causal, scale):
-        code = self.code = _lib.dtype_code(what, q.dtype)
-        if k.dtype is not q.dtype or v.dtype is not q.dtype:
-            raise ValueError(f"{what}: q is {q.dtype}, k {k.dtype} and v {v.dtype}, expected one type")
+        dt = q.dtype
+        code = self.code = _lib.dtype_code(what, dt)
+        if k.dtype is not dt or v.dtype is not dt:
+            raise ValueError(f"{what}: q is {dt}, k {k.dtype} and v {v.dtype}, expected one type")
         qs, ks = q.shape, k.shape
         nq, nk = len(qs), len(ks)
         if nq not in (3, 4) or nk not in (3, 4) or v.shape != ks or ks[-1] != qs[-1]:
             raise ValueError(f"{what}: q {tuple(qs)}, k {tuple(ks)} and v {tuple(v.shape)} do not fit")
-        H, d = self.H, self.d = qs[-2], qs[-1]
-        Hk = self.Hk = ks[-2]
+        H, d, Hk = qs[-2], qs[-1], ks[-2]
         if H < 1 or Hk < 1 or H % Hk or d < 1:
             raise ValueError(f"{what}: {H} query heads of {d} in groups of {Hk} key heads")
         if d > (128 if code == 0 else 256):
@@ -78,6 +92,7 @@ class _Call:
             scale = d ** -0.5
         elif not 0.0 < scale <= 3e38:
             raise ValueError(f"{what}: scale {scale}, expected a positive number")
+        at_q = at_k = at_n = 0
         if cu_q is not None:
             if nq != 3:
                 raise ValueError(f"{what}: cu_seqlens goes with packed rows (T, H, d), q is {tuple(qs)}")
@@ -87,9 +102,10 @@ class _Call:
                 cu_k = cu_q
             same = cu_k is cu_q
             cu_q = _lib.cu_operand(what, "cu_seqlens", cu_q)
-            B = cu_q.numel() - 1
             if same:
                 cu_k = cu_q
+            B = cu_q.shape[0] - 1
+            at_q = cu_q.data_ptr()
         else:
             B = qs[0] if nq == 4 else 1
         if cu_k is not None:
@@ -97,43 +113,51 @@ class _Call:
                 raise ValueError(f"{what}: cu_seqlens_k goes with packed keys (T, Hk, d) and no lengths_k, k is {tuple(ks)}")
             if cu_k is not cu_q:
                 cu_k = _lib.cu_operand(what, "cu_seqlens_k", cu_k)
-            Bk = cu_k.numel() - 1
+            Bk = cu_k.shape[0] - 1
+            at_k = cu_k.data_ptr()
         else:
             Bk = ks[0] if nk == 4 else 1
         if Bk != B:
             raise ValueError(f"{what}: {B} sequences of queries and {Bk} of keys")
         if lengths is not None:
-            if lengths.dim() != 1 or lengths.numel() != B or lengths.dtype not in (torch.int32, torch.int64):
+            if lengths.dim() != 1 or lengths.shape[0] != B or lengths.dtype not in _INTS:
                 raise ValueError(f"{what}: lengths_k of shape {tuple(lengths.shape)} and {lengths.dtype} for {B} sequences")
-            lengths = _lib.operand(lengths, (B,), torch.int32)
+            if lengths.dtype is not torch.int32 or not lengths.is_contiguous():
+                lengths = _lib.operand(lengths, (B,), torch.int32)
+            at_n = lengths.data_ptr()
         es = self.es = 4 if code == 0 else 2
-        self.wide = -(-d * es // 16) * 16 // es  # d in whole 16 bytes
-        q, qst = self.take(q)
-        k, kst = self.take(k)
-        v, vst = self.take(v)
-        self.q, self.k, self.v, self.cu_q, self.cu_k, self.lengths, self.B = q, k, v, cu_q, cu_k, lengths, B
-        self.rows_q = qs[0] if nq == 3 else qs[0] * qs[1]
-        self.rows_k = ks[0] if nk == 3 else ks[0] * ks[1]
-        self.args = _ARGS.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), *qst, *kst, *vst, cu_q.data_ptr() if cu_q is not None else 0,
-            cu_k.data_ptr() if cu_k is not None else 0, lengths.data_ptr() if lengths is not None else 0, self.rows_q,
-            self.rows_k, B, H, Hk, self.wide, code, 1 if causal else 0, scale, 0)
+        wide = self.wide = -(-d * es // 16) * 16 // es  # d in whole 16 bytes
+        self.H, self.Hk, self.d = H, Hk, d
+        if wide == d:
+            q, pq, qst = _rows(q, qs, es)
+            k, pk, kst = _rows(k, ks, es)
+            v, pv, vst = _rows(v, ks, es)
+        else:
+            (q, pq, qst), (k, pk, kst), (v, pv, vst) = self.take(q), self.take(k), self.take(v)
+        rows_q = self.rows_q = qs[0] if nq == 3 else qs[0] * qs[1]
+        rows_k = self.rows_k = ks[0] if nk == 3 else ks[0] * ks[1]
+        self.keep = (q, k, v, cu_q, cu_k, lengths)  # as long as their addresses are used
+        self.sizes = (at_q != 0, at_k != 0, rows_q, rows_k, B, H, Hk, wide, code)
+        self.args = _ARGS.pack(pq, pk, pv, *qst, *kst, *vst, at_q, at_k, at_n, rows_q, rows_k, B, H, Hk, wide, code,
+                               1 if causal else 0, scale, 0)
 
     def take(self, t):
+        """_rows of a tensor in the call's width."""
         if self.wide != self.d:
             t = torch.nn.functional.pad(t, (0, self.wide - self.d))
-        return _rows(t, self.es)
+        return _rows(t, t.shape, self.es)
 
     def empty(self, like):
-        return torch.empty(like.shape[:-1] + (self.wide,), dtype=like.dtype, device=like.device)
+        if self.wide == self.d:
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
+        return like.new_empty(like.shape[:-1] + (self.wide,))
 
     def trim(self, t):
         return t if self.wide == self.d else t[..., :self.d].contiguous()
 
-    def workspace(self, name, dev):
-        with _lib.on_device(dev):
-            n = getattr(_lib.load(), name)(self.args)
-        return (torch.empty(n, dtype=torch.uint8, device=dev), n) if n else (None, 0)
+    def workspace(self, name, dev_index, like):
+        n = _workspace_size(name, dev_index, *self.sizes)
+        return (like.new_empty(n, dtype=torch.uint8), n) if n else (None, 0)
 
 
 def attention(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None,
@@ -152,14 +176,16 @@ def attention(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, ca
     _lib.require_device(what, q, k, v, cu_seqlens, cu_seqlens_k, lengths_k)
     c = _Call(what, q, k, v, cu_seqlens, cu_seqlens_k, lengths_k, causal, scale)
     out = c.empty(q)
-    res = {}
+    res = {"out": out}
     lse = None
     if need_backward:
-        lse = res["lse"] = torch.empty((c.H, c.rows_q), dtype=torch.float32, device=q.device)
+        lse = res["lse"] = q.new_empty((c.H, c.rows_q), dtype=torch.float32)
     if c.rows_q > 0:
-        ws, n = c.workspace("mhc_attention_fwd_workspace_size", q.device)
-        _lib.call(what, _lib.load().mhc_attention_fwd, q.get_device(), c.args, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), n)
-    res["out"] = c.trim(out)
+        dev = q.get_device()
+        ws, n = c.workspace("mhc_attention_fwd_workspace_size", dev, q)
+        _lib.call(what, _lib.load().mhc_attention_fwd, dev, c.args, out.data_ptr(), _lib.ptr(lse), _lib.ptr(ws), n)
+    if c.wide != c.d:
+        res["out"] = c.trim(out)
     return res
 
 
@@ -178,16 +204,15 @@ def attention_backward(grad_out, q, k, v, out, lse, cu_seqlens=None, *, cu_seqle
         raise ValueError(f"{what}: lse of shape {tuple(lse.shape)} and {lse.dtype}, expected {(c.H, c.rows_q)} of float32")
     if not lse.is_contiguous():
         lse = lse.contiguous()
-    go, gst = c.take(grad_out if grad_out.dtype is q.dtype else grad_out.to(q.dtype))
-    o, ost = c.take(out)
-    if not o.is_contiguous():
-        o = o.contiguous()
+    go, at_go, gst = c.take(grad_out if grad_out.dtype is q.dtype else grad_out.to(q.dtype))
+    o, at_o, _ = c.take(out if out.is_contiguous() else out.contiguous())
     dq, dk, dv = c.empty(q), c.empty(k), c.empty(v)
     if c.rows_q > 0 or c.rows_k > 0:
-        ws, n = c.workspace("mhc_attention_bwd_workspace_size", q.device)
-        _lib.call(what, _lib.load().mhc_attention_bwd, q.get_device(), c.args, go.data_ptr(), _STRIDES.pack(*gst),
-                  o.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), n)
-    return c.trim(dq), c.trim(dk), c.trim(dv)
+        dev = q.get_device()
+        ws, n = c.workspace("mhc_attention_bwd_workspace_size", dev, q)
+        _lib.call(what, _lib.load().mhc_attention_bwd, dev, c.args, at_go, _STRIDES.pack(*gst), at_o, lse.data_ptr(),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), n)
+    return (dq, dk, dv) if c.wide == c.d else (c.trim(dq), c.trim(dk), c.trim(dv))
 
 
 def attention_ref(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None):

@@ -13,6 +13,7 @@ The reference has no such operator: its model code runs PyTorch's.
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
@@ -59,72 +60,85 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, or
     return torch.tensor(f, dtype=torch.float64, device=device), amplitude
 
 
-def _strided(t):
+_ARGS = struct.Struct("7P4q2qf8i")  # mhc_rotary_args (include/mhc_amd.h)
+
+
+def _strided(t, shape):
     """(t, row stride, head stride): t (..., H, d) with its rows one stride apart
     and a head's elements side by side; a copy where it is not so."""
-    if t.is_contiguous():
-        return t, t.shape[-2] * t.shape[-1], t.shape[-1]
-    shape, st = t.shape, t.stride()
-    if st[-1] == 1 or shape[-1] == 1:
-        row = 0
-        rows = 1  # of the dimensions seen so far
-        for n, s in zip(reversed(shape[:-2]), reversed(st[:-2])):
-            if n == 1:
-                continue
-            if rows == 1:
-                row = s
-            elif s != row * rows:
-                break
-            rows *= n
-        else:
-            return t, row, st[-2]
-    t = t.contiguous()
+    if not t.is_contiguous():
+        st = t.stride()
+        if st[-1] == 1 or shape[-1] == 1:
+            row = 0
+            rows = 1  # of the dimensions seen so far
+            for n, s in zip(reversed(shape[:-2]), reversed(st[:-2])):
+                if n == 1:
+                    continue
+                if rows == 1:
+                    row = s
+                elif s != row * rows:
+                    break
+                rows *= n
+            else:
+                return t, row, st[-2]
+        t = t.contiguous()
     return t, shape[-2] * shape[-1], shape[-1]
 
 
 def _run(what, q, k, freqs, positions, cu_seqlens, layout, amplitude, inverse):
     _lib.require_device(what, q, k, freqs, positions, cu_seqlens)
-    code = _lib.dtype_code(what, q.dtype)
+    dt = q.dtype
+    code = _lib.dtype_code(what, dt)
     if layout not in LAYOUTS:
         raise ValueError(f"{what}: layout {layout!r}, expected one of {tuple(LAYOUTS)}")
-    if q.dim() < 3:
-        raise ValueError(f"{what}: q of shape {tuple(q.shape)}, expected (..., heads, d) with a dimension of tokens")
-    lead, (H, d) = q.shape[:-2], q.shape[-2:]
-    T = math.prod(lead)
+    shape = q.shape
+    if len(shape) < 3:
+        raise ValueError(f"{what}: q of shape {tuple(shape)}, expected (..., heads, d) with a dimension of tokens")
+    H, d = shape[-2], shape[-1]
+    if H < 1 or d < 1:
+        raise ValueError(f"{what}: q of shape {tuple(shape)} has no heads")
+    T = q.numel() // (H * d)
     Hk = 0
     if k is not None:
-        if k.dim() != q.dim() or k.shape[:-2] != lead or k.shape[-1] != d or k.dtype is not q.dtype:
-            raise ValueError(f"{what}: k of shape {tuple(k.shape)} and {k.dtype} for q of {tuple(q.shape)} and {q.dtype}")
-        Hk = k.shape[-2]
-    if H < 1 or d < 1 or (k is not None and Hk < 1):
-        raise ValueError(f"{what}: q of shape {tuple(q.shape)} has no heads" if H < 1 or d < 1 else f"{what}: k has no heads")
-    r = 2 * freqs.numel()
-    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or r > d:
+        ks = k.shape
+        if len(ks) != len(shape) or ks[:-2] != shape[:-2] or ks[-1] != d or k.dtype is not dt:
+            raise ValueError(f"{what}: k of shape {tuple(ks)} and {k.dtype} for q of {tuple(shape)} and {dt}")
+        Hk = ks[-2]
+        if Hk < 1:
+            raise ValueError(f"{what}: k of shape {tuple(ks)} has no heads")
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or 2 * freqs.shape[0] > d:
         raise ValueError(f"{what}: freqs of shape {tuple(freqs.shape)} and {freqs.dtype}, expected float64 and at most {d // 2}")
     if not freqs.is_contiguous():
         freqs = freqs.contiguous()
+    at_p = at_cu = wide = B = 0
     if positions is not None:
         if cu_seqlens is not None:
             raise ValueError(f"{what}: positions and cu_seqlens")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.numel() != T:
+        wide = positions.dtype is torch.int64
+        if not (wide or positions.dtype is torch.int32) or positions.numel() != T:
             raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} and {positions.dtype}, expected "
                              f"{T} of int32 or int64")
         if not positions.is_contiguous():
             positions = positions.contiguous()
-    if cu_seqlens is not None:
-        if q.dim() != 3:
-            raise ValueError(f"{what}: cu_seqlens goes with packed rows (T, heads, d), q is {tuple(q.shape)}")
+        at_p = positions.data_ptr()
+    elif cu_seqlens is not None:
+        if len(shape) != 3:
+            raise ValueError(f"{what}: cu_seqlens goes with packed rows (T, heads, d), q is {tuple(shape)}")
         cu_seqlens = _lib.cu_operand(what, "cu_seqlens", cu_seqlens)
-    qs, q_row, q_head = _strided(q)
-    ks, k_row, k_head = (None, 0, 0) if k is None else _strided(k)
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        at_cu, B = cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1
+    qs, q_row, q_head = _strided(q, shape)
+    qo = torch.empty_like(qs, memory_format=torch.contiguous_format)
+    at_k = at_ko = k_row = k_head = 0
+    ko = None
+    if k is not None:
+        ks, k_row, k_head = _strided(k, ks)
+        ko = torch.empty_like(ks, memory_format=torch.contiguous_format)
+        at_k, at_ko = ks.data_ptr(), ko.data_ptr()
     if T > 0:
-        _lib.call(what, _lib.load().mhc_rotary, q.get_device(), qs.data_ptr(), _lib.ptr(ks), code, q_row, q_head, k_row,
-                  k_head, freqs.data_ptr(), _lib.ptr(positions),
-                  0 if positions is None else int(positions.dtype is torch.int64), _lib.ptr(cu_seqlens),
-                  0 if cu_seqlens is None else cu_seqlens.numel() - 1, lead[-1], LAYOUTS[layout], amplitude, inverse,
-                  qo.data_ptr(), _lib.ptr(ko), T, H, Hk, d, r)
+        args = _ARGS.pack(qs.data_ptr(), at_k, qo.data_ptr(), at_ko, freqs.data_ptr(), at_p, at_cu, q_row, q_head, k_row, k_head,
+                          T, shape[-3], amplitude, B, code, H, Hk, d, 2 * freqs.shape[0], LAYOUTS[layout],
+                          wide | inverse << 1)
+        _lib.call(what, _lib.load().mhc_rotary, q.get_device(), args)
     return qo, ko
 
 

@@ -148,30 +148,34 @@ int rotary_run(const RotArgs& a, bool half_layout, hipStream_t st) {
 
 using namespace mhc;
 
-extern "C" int mhc_rotary(const void* q, const void* k, int32_t dtype, int64_t q_row, int64_t q_head, int64_t k_row,
-                          int64_t k_head, const double* freqs, const void* positions, int32_t positions_wide,
-                          const int32_t* cu_seqlens, int32_t sequences, int64_t length, int32_t layout, float amplitude,
-                          int32_t inverse, void* q_out, void* k_out, int64_t T, int32_t heads, int32_t heads_k, int32_t d,
-                          int32_t r, void* stream) {
+extern "C" int mhc_rotary(const mhc_rotary_args* c, void* stream) {
   clear_error();
-  if (T < 0 || heads < 1 || heads_k < 0 || d < 1 || r < 0 || r > d || r % 2 || (layout != 0 && layout != 1))
-    return set_error(MHC_ERR_INVALID, "rotary: T=%lld heads=%d heads_k=%d d=%d r=%d layout=%d", (long long)T, heads, heads_k,
-                     d, r, layout);
-  if (dtype != MHC_DTYPE_F32 && dtype != MHC_DTYPE_BF16 && dtype != MHC_DTYPE_F16)
-    return set_error(MHC_ERR_UNSUPPORTED, "rotary: dtype %d not supported", dtype);
-  if (r > 2 * kTrig) return set_error(MHC_ERR_UNSUPPORTED, "rotary: r=%d above the supported %d", r, 2 * kTrig);
+  if (!c) return set_error(MHC_ERR_INVALID, "rotary: null arguments");
+  if (c->rows < 0 || c->heads < 1 || c->heads_k < 0 || c->d < 1 || c->r < 0 || c->r > c->d || c->r % 2 ||
+      (c->layout != MHC_ROTARY_HALF && c->layout != MHC_ROTARY_INTERLEAVED))
+    return set_error(MHC_ERR_INVALID, "rotary: rows=%lld heads=%d heads_k=%d d=%d r=%d layout=%d", (long long)c->rows, c->heads,
+                     c->heads_k, c->d, c->r, c->layout);
+  if (c->flags & ~(MHC_ROTARY_WIDE_POSITIONS | MHC_ROTARY_INVERSE))
+    return set_error(MHC_ERR_INVALID, "rotary: flags 0x%x", c->flags);
+  if (c->dtype != MHC_DTYPE_F32 && c->dtype != MHC_DTYPE_BF16 && c->dtype != MHC_DTYPE_F16)
+    return set_error(MHC_ERR_UNSUPPORTED, "rotary: dtype %d not supported", c->dtype);
+  if (c->r > 2 * kTrig) return set_error(MHC_ERR_UNSUPPORTED, "rotary: r=%d above the supported %d", c->r, 2 * kTrig);
   // a block's items are counted in 32 bits
-  if (((int64_t)heads + heads_k) * d > (1 << 28))
-    return set_error(MHC_ERR_UNSUPPORTED, "rotary: heads=%d heads_k=%d d=%d above the supported sizes", heads, heads_k, d);
-  if (q_row < 0 || q_head < 0 || k_row < 0 || k_head < 0) return set_error(MHC_ERR_INVALID, "rotary: negative stride");
-  if (!positions && !cu_seqlens && length < 1) return set_error(MHC_ERR_INVALID, "rotary: length %lld", (long long)length);
-  if (cu_seqlens && sequences < 0) return set_error(MHC_ERR_INVALID, "rotary: sequences %d", sequences);
-  if (T == 0) return MHC_OK;
-  if (!q || !q_out || (heads_k && (!k || !k_out)) || (r && !freqs)) return set_error(MHC_ERR_INVALID, "rotary: null pointer");
-  const RotArgs a = {{q, k}, {q_out, k_out}, {q_row, k_row}, {q_head, k_head}, {heads, heads_k}, freqs, positions, cu_seqlens,
-                     T, length, positions_wide, sequences, d, r, amplitude, inverse ? -1 : 1};
+  if (((int64_t)c->heads + c->heads_k) * c->d > (1 << 28))
+    return set_error(MHC_ERR_UNSUPPORTED, "rotary: heads=%d heads_k=%d d=%d above the supported sizes", c->heads, c->heads_k, c->d);
+  if (c->q_row < 0 || c->q_head < 0 || c->k_row < 0 || c->k_head < 0)
+    return set_error(MHC_ERR_INVALID, "rotary: negative stride");
+  if (!c->positions && !c->cu_seqlens && c->length < 1)
+    return set_error(MHC_ERR_INVALID, "rotary: length %lld", (long long)c->length);
+  if (c->cu_seqlens && c->sequences < 0) return set_error(MHC_ERR_INVALID, "rotary: sequences %d", c->sequences);
+  if (c->rows == 0) return MHC_OK;
+  if (!c->q || !c->q_out || (c->heads_k && (!c->k || !c->k_out)) || (c->r && !c->freqs))
+    return set_error(MHC_ERR_INVALID, "rotary: null pointer");
+  const RotArgs a = {{c->q, c->k}, {c->q_out, c->k_out}, {c->q_row, c->k_row}, {c->q_head, c->k_head}, {c->heads, c->heads_k},
+                     c->freqs, c->positions, c->cu_seqlens, c->rows, c->length, (c->flags & MHC_ROTARY_WIDE_POSITIONS) != 0,
+                     c->sequences, c->d, c->r, c->amplitude, c->flags & MHC_ROTARY_INVERSE ? -1 : 1};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == MHC_DTYPE_F32) return rotary_run<float>(a, layout == 0, st);
-  if (dtype == MHC_DTYPE_BF16) return rotary_run<bf16_t>(a, layout == 0, st);
-  return rotary_run<f16_t>(a, layout == 0, st);
+  if (c->dtype == MHC_DTYPE_F32) return rotary_run<float>(a, c->layout == MHC_ROTARY_HALF, st);
+  if (c->dtype == MHC_DTYPE_BF16) return rotary_run<bf16_t>(a, c->layout == MHC_ROTARY_HALF, st);
+  return rotary_run<f16_t>(a, c->layout == MHC_ROTARY_HALF, st);
 }

@@ -390,26 +390,35 @@ int mhc_dropout(const void* x, void* y, int64_t n, int32_t dtype, double p, uint
                 uint64_t offset, const uint64_t* state, void* stream);
 
 /*
- * Rotary positions of q (T, heads, d) and k (T, heads_k, d; heads_k == 0:
- * none), all `dtype`, any element alignment; rows and heads `*_row` and
+ * Rotary positions of q (rows, heads, d) and k (rows, heads_k, d; heads_k ==
+ * 0: none), all `dtype`, any element alignment; rows and heads `*_row` and
  * `*_head` elements apart, a head's elements side by side:
  *   (a, b) -> amplitude (a cos w - b sin w, a sin w + b cos w), w = position * freqs[i]
- * for the r / 2 pairs (i, i + r / 2) (layout 0) or (2 i, 2 i + 1) (layout 1)
- * of the first r elements; the others are copied.  inverse: by -w (the
+ * for the r / 2 pairs (i, i + r / 2) (MHC_ROTARY_HALF) or (2 i, 2 i + 1) of
+ * the first r elements; the others are copied.  MHC_ROTARY_INVERSE: by -w (the
  * backward).  freqs: (r / 2,) device doubles, radians a position; angles are
- * reduced in 64 bits.  A row's position: positions[t] (int32, or int64 with
- * positions_wide), else its place in its packed sequence (cu_seqlens:
- * (sequences + 1,) first rows, the first one 0; rows behind the last sequence
- * count from its end), else t % length.  q_out, k_out: contiguous, not q or k.
- * r <= 4096, (heads + heads_k) * d <= 2^28.
+ * reduced in 64 bits.  A row's position: positions[row] (int32, or int64 with
+ * MHC_ROTARY_WIDE_POSITIONS), else its place in its packed sequence
+ * (cu_seqlens: (sequences + 1,) first rows, the first one 0; rows behind the
+ * last sequence count from its end), else row % length.  q_out, k_out:
+ * contiguous, not q or k.  r <= 4096, (heads + heads_k) * d <= 2^28.
  */
 #define MHC_ROTARY_HALF 0
 #define MHC_ROTARY_INTERLEAVED 1
-int mhc_rotary(const void* q, const void* k, int32_t dtype, int64_t q_row, int64_t q_head, int64_t k_row,
-               int64_t k_head, const double* freqs, const void* positions, int32_t positions_wide,
-               const int32_t* cu_seqlens, int32_t sequences, int64_t length, int32_t layout, float amplitude,
-               int32_t inverse, void* q_out, void* k_out, int64_t T, int32_t heads, int32_t heads_k, int32_t d,
-               int32_t r, void* stream);
+#define MHC_ROTARY_WIDE_POSITIONS 1
+#define MHC_ROTARY_INVERSE 2
+typedef struct {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const double* freqs;
+  const void* positions;
+  const int32_t* cu_seqlens;
+  int64_t q_row, q_head, k_row, k_head; /* elements */
+  int64_t rows, length;
+  float amplitude;
+  int32_t sequences, dtype, heads, heads_k, d, r, layout, flags;
+} mhc_rotary_args;
+int mhc_rotary(const mhc_rotary_args* args, void* stream);
 
 /*
  * Attention of `heads` query heads over `heads_k` key heads (a divisor; head h

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import sys
 
 import pytest
 import torch
@@ -12,6 +13,7 @@ import torch
 import attention_ref as R
 from FlagOS_mhc import _lib, sublayer as S
 from FlagOS_mhc.attention import _ARGS, _STRIDES
+from FlagOS_mhc.rotary import _ARGS as _ROTARY
 
 P = 0x1000
 ODD = 0x1002
@@ -82,16 +84,17 @@ def test_nothing_to_do():
 
 def test_rotary_refusals():
     lib = _lib.load()
-    f = lambda q=P, k=P, dt=1, freqs=P, pos=P, cu=None, seqs=0, length=4, layout=0, qo=P, ko=P, T=4, H=2, Hk=1, d=64, r=64, \
-        row=128: lib.mhc_rotary(q, k, dt, row, 64, 64, 64, freqs, pos, 0, cu, seqs, length, layout, 1.0, 0, qo, ko, T, H, Hk, d, r, None)
+    f = lambda q=P, k=P, dt=1, freqs=P, pos=P, cu=0, seqs=0, length=4, layout=0, qo=P, ko=P, T=4, H=2, Hk=1, d=64, r=64, \
+        row=128, flags=0: lib.mhc_rotary(_ROTARY.pack(q, k, qo, ko, freqs, pos, cu, row, 64, 64, 64, T, length, 1.0, seqs, dt, H,
+                                                      Hk, d, r, layout, flags), None)
     assert f(T=-1) == -1 and f(H=0) == -1 and f(Hk=-1) == -1 and f(d=0) == -1 and f(r=66) == -1 and f(r=7) == -1
-    assert f(layout=2) == -1 and f(row=-1) == -1
+    assert f(layout=2) == -1 and f(row=-1) == -1 and f(flags=4) == -1
     assert f(dt=5) == -2 and b"dtype" in _err()
     assert f(d=8192, r=4098) == -2 and b"r=4098" in _err()
     assert f(H=1 << 20, d=1 << 12) == -2
-    assert f(pos=None, length=0) == -1 and f(pos=None, cu=P, seqs=-1) == -1
-    assert f(q=None) == -1 and f(qo=None) == -1 and f(k=None) == -1 and f(ko=None) == -1 and f(freqs=None) == -1
-    assert f(T=0) == 0
+    assert f(pos=0, length=0) == -1 and f(pos=0, cu=P, seqs=-1) == -1
+    assert f(q=0) == -1 and f(qo=0) == -1 and f(k=0) == -1 and f(ko=0) == -1 and f(freqs=0) == -1
+    assert f(T=0) == 0 and lib.mhc_rotary(None, None) == -1
 
 
 # ---- Python checks ------------------------------------------------------------------
@@ -100,6 +103,7 @@ def test_rotary_refusals():
 def on_cpu(monkeypatch):
     """The operators' own checks, without a device."""
     monkeypatch.setattr(_lib, "require_device", lambda *a: None)
+    monkeypatch.setattr(sys.modules["FlagOS_mhc.attention"], "_workspace_size", lambda *a: 0)
     monkeypatch.setattr(_lib, "call", lambda *a: None)
 
 
@@ -270,3 +274,16 @@ def test_struct_is_the_headers():
     assert ctypes.sizeof(Args) == _ARGS.size
     a = Args.from_buffer_copy(_args(B=7, H=6, Hk=3, d=40, scale=0.25, rows_k=99, vs=(1, 2, 3)))
     assert (a.seqs, a.heads, a.heads_k, a.d, a.scale, a.rk, list(a.vs), a.ck) == (7, 6, 3, 40, 0.25, 99, [1, 2, 3], P)
+
+
+def test_rotary_struct_is_the_headers():
+    class Args(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "qo", "ko", "freqs", "positions", "cu")]
+                    + [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "rows", "length")]
+                    + [("amplitude", ctypes.c_float)]
+                    + [(n, ctypes.c_int32) for n in ("sequences", "dtype", "heads", "heads_k", "d", "r", "layout", "flags")])
+    raw = _ROTARY.pack(*range(1, 8), *range(8, 14), 0.5, *range(14, 22))
+    # (the C struct ends on a multiple of 8 bytes: its last one is four whole ones here)
+    assert ctypes.sizeof(Args) - _ROTARY.size in (0, 4)
+    a = Args.from_buffer_copy(raw + bytes(ctypes.sizeof(Args) - _ROTARY.size))
+    assert (a.q, a.cu, a.q_row, a.length, a.amplitude, a.sequences, a.flags) == (1, 7, 8, 13, 0.5, 14, 21)
