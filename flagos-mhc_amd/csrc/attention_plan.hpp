@@ -52,10 +52,16 @@ inline AttSplit att_split(const AttDims& n, int cus) {
   s.slots = n.cu_q ? n.Tq * G / 32 + n.B + 1 : (int64_t)n.B * (((int64_t)n.Sq * G + 31) / 32);
   const int64_t blocks = s.slots * n.Hk;
   const int64_t longest = n.cu_k ? (n.Tk + n.B - 1) / n.B : n.Sk;  // keys of a sequence, on average
-  int64_t want = 2 * (int64_t)cus / blocks;
-  const int64_t most = longest / 512;  // four tiles for each wave
-  if (want > most) want = most;
-  s.splits = want < 1 ? 1 : (int)want;
+  // As many parts as there are compute units for, of a tile a wave at least
+  // (one token, 8 key heads, 32768 keys: 64 parts 30.2 us, 32 28.9 us, 8 54 us) ..
+  int64_t parts = cus / blocks;
+  if (parts > longest / 128) parts = longest / 128;
+  // .. or, for few queries of many sequences, about 1024 keys each, so that
+  // blocks end when others do (64 x 8192, one token, 8 key heads: 371 us whole,
+  // 320 us in 8 parts).  An odd number: the parts of a head then fall to
+  // different XCDs from head to head (7 parts 296 us, 9 parts 296 us).
+  if (parts < 4 && rows <= 64 && longest >= 2048 && parts < (longest / 1024 | 1)) parts = longest / 1024 | 1;
+  s.splits = parts < 1 ? 1 : (int)parts;
   return s;
 }
 
