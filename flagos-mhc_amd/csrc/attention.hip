@@ -96,10 +96,15 @@ extern "C" int mhc_attention_fwd(const mhc_attention_args* c, void* out, float* 
   return att_fwd<f16_t>(a, st);
 }
 
+static AttBwdPlan bwd_plan(const mhc_attention_args* c, const AttArgs& a) {
+  const bool fp32 = c->dtype == MHC_DTYPE_F32;
+  return att_bwd_plan(a.n, fp32, att_big_head(a.n, fp32), device_cu_count());
+}
+
 extern "C" size_t mhc_attention_bwd_workspace_size(const mhc_attention_args* c) {
   AttArgs a;
   if (check_att("", c, a)) return 0;
-  const AttBwdPlan p = att_bwd_plan(a.n, c->dtype == MHC_DTYPE_F32, device_cu_count());
+  const AttBwdPlan p = bwd_plan(c, a);
   return p.delta_bytes + p.part_bytes;
 }
 
@@ -128,7 +133,7 @@ extern "C" int mhc_attention_bwd(const mhc_attention_args* c, const void* grad_o
   a.dv = grad_v;
   a.lse = const_cast<float*>(lse);
   a.delta = static_cast<float*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + att_bwd_plan(a.n, c->dtype == MHC_DTYPE_F32, device_cu_count()).delta_bytes);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + bwd_plan(c, a).delta_bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (c->dtype == MHC_DTYPE_F32) return att_bwd<float>(a, st);
   if (c->dtype == MHC_DTYPE_BF16) return att_bwd<bf16_t>(a, st);

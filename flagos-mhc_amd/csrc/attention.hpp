@@ -301,6 +301,15 @@ struct Tile {
   }
 };
 
+// A pointer that is the same for the wave, known to be so: resources made of
+// one that the compiler cannot prove uniform are loaded with in a loop over
+// their values.
+__device__ __forceinline__ const char* uniform(const char* p) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  return reinterpret_cast<const char*>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
+
 // Rows of a head on their way from memory to a tile, through registers: NT
 // threads hold the next tile while this one is computed with.  `left` rows
 // exist (others read zero without touching memory), chunks past `d` too.  A

@@ -62,15 +62,16 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   const int q_ts = (int)(a.q.ts * ES), k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES);
   u32x4 q[T::kSteps];
   load_rows<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, wave_first, h, ES), q_ts, s.lq - wave_first, dc, lane, q);
-  const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES);
-  const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES);
+  const char* kp = uniform(row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES));
+  const char* vp = uniform(row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES));
+  const int lk = __builtin_amdgcn_readfirstlane(s.lk);
   const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
 
   TileStage<S, DB, BN, NT> sk, sv;
   uint32_t k_off = sk.offset(k_ts, dc, tid), v_off = sv.offset(v_ts, dc, tid);
   const uint32_t lds = lds_addr(smem);
-  sk.load(kp, k_ts, s.lk, k_off);
-  sv.load(vp, v_ts, s.lk, v_off);
+  sk.load(kp, k_ts, lk, k_off);
+  sv.load(vp, v_ts, lk, v_off);
   // tiles with keys from here on are hidden from some of the block's queries
   const int zone = a.n.causal ? max(0, first + shift + 1) : 0x7fffffff;
   bool bad = false;
@@ -97,8 +98,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
     at.keep();
     const int k0 = t * BN;
     if (t + 1 < tiles) {
-      sk.load(kp + (t + 1) * k_step, k_ts, s.lk - k0 - BN, k_off);
-      sv.load(vp + (t + 1) * v_step, v_ts, s.lk - k0 - BN, v_off);
+      sk.load(kp + (t + 1) * k_step, k_ts, lk - k0 - BN, k_off);
+      sv.load(vp + (t + 1) * v_step, v_ts, lk - k0 - BN, v_off);
     }
     if (k0 <= wave_hi) {
       floatx16 sc[NB];

@@ -65,23 +65,38 @@ inline AttSplit att_split(const AttDims& n, int cus) {
   return s;
 }
 
-// Backward: parts of the queries that a tile of 128 keys is shared over.
+// Backward, dk and dv: keys of a block, and parts of the queries that a block's
+// keys are shared over.
 struct AttBwdPlan {
-  int splits;
+  int keys, splits;
+  int64_t slots;
   size_t delta_bytes, part_bytes;
 };
 
-inline AttBwdPlan att_bwd_plan(const AttDims& n, bool fp32, int cus) {
-  AttBwdPlan p = {1, ((size_t)n.H * n.Tq * 4 + 255) / 256 * 256, 0};
+// big: heads of 128 16-bit elements, whose kernel has a form of 256 keys a
+// block (half the reads of q and the output's gradient; 16384 x 56 heads over 8:
+// 14.1 -> 13.5 ms for the whole backward in two parts).
+inline AttBwdPlan att_bwd_plan(const AttDims& n, bool fp32, bool big, int cus) {
+  AttBwdPlan p = {128, 1, att_slots(n.cu_k != nullptr, n.Tk, n.B, n.Sk, 128), ((size_t)n.H * n.Tq * 4 + 255) / 256 * 256, 0};
   if (n.B == 0 || n.Tq == 0 || n.Tk == 0) return p;
-  const int64_t blocks = att_slots(n.cu_k != nullptr, n.Tk, n.B, n.Sk, 128) * n.Hk;
+  const int64_t tall = att_slots(n.cu_k != nullptr, n.Tk, n.B, n.Sk, 256);
+  if (big && tall * n.Hk >= 2 * (int64_t)cus) {
+    p.keys = 256;
+    p.slots = tall;
+  }
+  const int64_t blocks = p.slots * n.Hk;
   const int64_t rows = (n.Tq + n.B - 1) / n.B * (n.H / n.Hk);  // queries of a key head and sequence, on average
+  // three blocks a compute unit, and enough queries to be worth the sums' way through memory
+  //   777 tokens in three, 16 heads over 4 of 80 (40 blocks): whole 110 us, 8 parts 46 us;
+  //   4099 in five, 32 over 8 of 128 (304 blocks): whole 417 us, 3 parts 249 us, 8 parts 299 us
   int64_t want = (3 * (int64_t)cus + blocks - 1) / blocks;
-  const int64_t most = rows / (fp32 ? 64 : 128);  // what is worth the sums' way through memory
+  const int64_t most = rows / (fp32 ? 64 : 128);
   want = want < most ? want : most;
   p.splits = want < 1 ? 1 : (want > 16 ? 16 : (int)want);
   if (p.splits > 1) p.part_bytes = (size_t)p.splits * 2 * n.Tk * n.Hk * n.d * 4;
   return p;
 }
+
+inline bool att_big_head(const AttDims& n, bool fp32) { return !fp32 && n.d > 96 && n.d <= 128; }
 
 }  // namespace mhc

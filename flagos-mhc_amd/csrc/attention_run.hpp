@@ -28,7 +28,7 @@ template <typename S, int DB> struct AttShape {
   static constexpr int kFwdNB = sizeof(S) == 2 && DB <= 4 ? 2 : 1;
   static constexpr int kBwdNB = sizeof(S) == 2 && DB <= 2 ? 2 : 1;
   static constexpr bool kDkvLds = kBytes > 128;
-  static constexpr bool kBig = kBytes == 256 && sizeof(S) == 2;  // 256 queries a block are a choice
+  static constexpr bool kBig = DB == 4 && sizeof(S) == 2;  // 256 rows a block are a choice (att_big_head)
 };
 
 template <typename S, int DB>
@@ -83,18 +83,23 @@ int att_dq_width(const AttArgs& a, hipStream_t st) {
   return att_dq_run<S, DB, 4>(a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 128), st);
 }
 
-template <typename S, int DB>
-int att_bwd_width(const AttArgs& a, hipStream_t st) {
+template <typename S, int DB, int NW>
+int att_dkv_run(const AttArgs& a, const AttBwdPlan& p, hipStream_t st) {
   using A = AttShape<S, DB>;
   constexpr int kPitch = Tile<S, DB>::kPitch;
+  constexpr size_t lds = 2 * (2 * 32 * A::kBwdNB * kPitch + 256 * A::kBwdNB) + (A::kDkvLds ? 32 * NW * kPitch : 0);
+  return att_launch(att_dkv_kernel<S, DB, NW, A::kBwdNB, A::kWPE, A::kDkvLds>, a, p.slots, (int64_t)a.n.Hk * p.splits, 64 * NW,
+                    lds, st, "attention_backward", p.splits);
+}
+
+template <typename S, int DB>
+int att_bwd_width(const AttArgs& a, hipStream_t st) {
   if (const int rc = att_dq_width<S, DB>(a, st)) return rc;
-  const AttBwdPlan p = att_bwd_plan(a.n, sizeof(S) == 4, device_cu_count());
-  const int64_t slots = att_slots(a.n.cu_k != nullptr, a.n.Tk, a.n.B, a.n.Sk, 128);
-  constexpr size_t lds = 2 * (2 * 32 * A::kBwdNB * kPitch + 256 * A::kBwdNB) + (A::kDkvLds ? 128 * kPitch : 0);
-  if (const int rc = att_launch(att_dkv_kernel<S, DB, 4, A::kBwdNB, A::kWPE, A::kDkvLds>, a, slots, (int64_t)a.n.Hk * p.splits, 256,
-                                lds, st, "attention_backward", p.splits))
-    return rc;
-  if (p.splits == 1) return MHC_OK;
+  const AttBwdPlan p = att_bwd_plan(a.n, sizeof(S) == 4, AttShape<S, DB>::kBig, device_cu_count());
+  int rc;
+  if constexpr (AttShape<S, DB>::kBig) rc = p.keys == 256 ? att_dkv_run<S, DB, 8>(a, p, st) : att_dkv_run<S, DB, 4>(a, p, st);
+  else rc = att_dkv_run<S, DB, 4>(a, p, st);
+  if (rc || p.splits == 1) return rc;
   const int64_t all = a.n.Tk * a.n.Hk * a.n.d, blocks = (2 * all + 1023) / 1024;
   if (blocks > 0xffffffffll / 256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention_backward: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);

@@ -26,10 +26,10 @@ int main() {
     AttDims n = {packed ? some : nullptr, packed ? some : nullptr, nullptr, Tq, Tk, (int)B, B ? (int)(Tq / B) : 0,
                  B ? (int)(Tk / B) : 0, (int)H, (int)Hk, (int)d, 1};
     const AttSplit s = att_split(n, 256);
-    const AttBwdPlan p = att_bwd_plan(n, fp32, 256);
-    printf("%lld %lld %lld %d %d %lld %zu %d %zu %zu\n", (long long)att_slots(packed, Tq, (int)B, n.Sq, 128),
+    const AttBwdPlan p = att_bwd_plan(n, fp32, att_big_head(n, fp32), 256);
+    printf("%lld %lld %lld %d %d %lld %zu %d %zu %zu %d %lld\n", (long long)att_slots(packed, Tq, (int)B, n.Sq, 128),
            (long long)att_slots(packed, Tq, (int)B, n.Sq, 256), (long long)att_slots(packed, Tk, (int)B, n.Sk, 128),
-           s.use, s.splits, (long long)s.slots, s.bytes(n), p.splits, p.delta_bytes, p.part_bytes);
+           s.use, s.splits, (long long)s.slots, s.bytes(n), p.splits, p.delta_bytes, p.part_bytes, p.keys, (long long)p.slots);
   }
 }
 """
@@ -48,7 +48,7 @@ def plan(tmp_path_factory):
     def run(rows):
         text = "\n".join(" ".join(str(int(v)) for v in r) for r in rows)
         out = subprocess.run([str(d / "plan")], input=text, capture_output=True, text=True, check=True).stdout
-        names = ("slots128", "slots256", "slots_k", "use", "splits", "split_slots", "bytes", "parts", "delta", "part_bytes")
+        names = ("slots128", "slots256", "slots_k", "use", "splits", "split_slots", "bytes", "parts", "delta", "part_bytes", "keys", "key_slots")
         return [dict(zip(names, map(int, line.split()))) for line in out.splitlines()]
 
     return run
@@ -84,6 +84,8 @@ def test_every_tile_has_a_slot_of_its_own(plan):
         G = rng.choice([1, 3, 4, 7, 40])
         cu = _starts(rng, B, T)
         got = plan([(1, T, T, B, G, 1, 64, 0)])[0]
+        tall = plan([(1, T, 100000, B, 128, 128, 128, 0)])[0]
+        assert tall["keys"] == 256 and got["keys"] == 128 and got["key_slots"] == got["slots_k"]
         for R, scale, slots in ((128, 1, got["slots128"]), (256, 1, got["slots256"]), (32, G, got["split_slots"])):
             seen = set()
             ends = cu[1:] + [T]
@@ -119,8 +121,8 @@ def test_parts_fit_their_workspace(plan):
         assert p["bytes"] == (p["splits"] * Tq * H * (d + 2) * 4 if p["use"] and p["splits"] > 1 else 0)
         assert p["delta"] >= H * Tq * 4 and p["delta"] % 256 == 0
         assert p["part_bytes"] == (p["parts"] * 2 * Tk * Hk * d * 4 if p["parts"] > 1 else 0)
-        # a part of the keys has four tiles for each wave, one of the queries 64 rows or more
-        assert p["splits"] <= max(1, -(-Tk // B) // 512) and p["parts"] <= max(1, -(-Tq // B) * (H // Hk) // 64)
+        # a part of the keys has a tile for each wave, one of the queries 64 rows or more
+        assert p["splits"] <= max(1, -(-Tk // B) // 128) and p["parts"] <= max(1, -(-Tq // B) * (H // Hk) // 64)
 
 
 def test_nothing_to_split(plan):
