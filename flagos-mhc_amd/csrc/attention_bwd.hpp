@@ -29,14 +29,15 @@ namespace mhc {
 
 constexpr int kSumKeys = 256;
 
-// dq, and D.
-template <typename S, int DB, int NW, int NB, int WPE>
+// dq, and D.  KS as in the forward.
+template <typename S, int DB, int NW, int KS, int NB, int WPE>
 __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t slots) {
   using T = Tile<S, DB>;
-  constexpr int BN = 32 * NB, BM = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
-  constexpr int kTileBytes = BN * T::kPitch;
-  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (K, V)
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int RW = NW / KS, BN = 32 * NB, BS = BN * KS, BM = 32 * RW, NT = 64 * NW, ES = (int)sizeof(S);
+  constexpr int kTileBytes = BS * T::kPitch;
+  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (K, V); at the end the sums of KS - 1 waves a row
+  const int tid = threadIdx.x, lane = tid & 63, id = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = id % RW, part = id / RW;
   int64_t slot;
   int h, first;
   att_item(a.n, slots, slot, h);
@@ -63,8 +64,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const int q_ts = (int)(a.q.ts * ES), k_ts = (int)(a.k.ts * ES), v_ts = (int)(a.v.ts * ES), go_ts = (int)(a.go.ts * ES);
   const char* kp = row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES);
   const char* vp = row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES);
-  const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
-  TileStage<S, DB, BN, NT> sk, sv;
+  const int64_t k_step = (int64_t)BS * k_ts, v_step = (int64_t)BS * v_ts;
+  TileStage<S, DB, BS, NT> sk, sv;
   const uint32_t k_off = sk.offset(k_ts, dc, tid), v_off = sv.offset(v_ts, dc, tid), lds = lds_addr(smem);
   sk.load(kp, k_ts, s.lk, k_off);
   sv.load(vp, v_ts, s.lk, v_off);
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const int left = s.lq - wave_first;
   load_rows<S, DB>(row_ptr(a.q, a.n.cu_q, s.row0, s.b, wave_first, h, ES), q_ts, left, dc, lane, q);
   load_rows<S, DB>(row_ptr(a.go, a.n.cu_q, s.row0, s.b, wave_first, h, ES), go_ts, left, dc, lane, go);
-  const int tiles = (keys + BN - 1) / BN, half = lane >> 5;
+  const int tiles = (keys + BS - 1) / BS, half = lane >> 5;
   const int sum = keys <= kSumKeys ? tiles : 0;  // a round over the tiles for D
   float delta = 0.f;
   if (sum == 0) {
@@ -96,7 +97,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const int zone = a.n.causal ? max(0, first + shift + 1) : 0x7fffffff;  // as in the forward, for the keys
   bool bad = false;
   auto stage = [&](int it, int t) {
-    if ((t + 1) * BN > zone) bad |= sk.clean();
+    if ((t + 1) * BS > zone) bad |= sk.clean();
     const uint32_t to = lds + (it & 1) * 2 * kTileBytes;
     sk.store(to, tid);
     sv.store(to + kTileBytes, tid);
@@ -113,13 +114,13 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   const float c = a.scale2;
   float total = 0.f;
   for (int it = 0; it < sum + tiles; ++it) {
-    const uint32_t tk = lds + (it & 1) * 2 * kTileBytes, tv = tk + kTileBytes;
+    const uint32_t tk = lds + (it & 1) * 2 * kTileBytes + part * BN * T::kPitch, tv = tk + kTileBytes;
     at.keep();
-    const int k0 = (it < sum ? it : it - sum) * BN;
+    const int k0 = (it < sum ? it : it - sum) * BS + part * BN;
     const int next = it + 1 < sum ? it + 1 : it + 1 - sum;
     if (it + 1 < sum + tiles) {
-      sk.load(kp + next * k_step, k_ts, s.lk - next * BN, k_off);
-      sv.load(vp + next * v_step, v_ts, s.lk - next * BN, v_off);
+      sk.load(kp + next * k_step, k_ts, s.lk - next * BS, k_off);
+      sv.load(vp + next * v_step, v_ts, s.lk - next * BS, v_off);
     }
     if (k0 <= wave_hi) {
       const bool masked = k0 + BN - 1 > wave_lo;
@@ -148,6 +149,12 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
     }
     if (it + 1 == sum) {
       delta = add_xor32(total);
+      if constexpr (KS == 2) {
+        __shared__ float sums[KS][BM];
+        sums[part][32 * wave + (lane & 31)] = delta;
+        __syncthreads();
+        delta = sums[0][32 * wave + (lane & 31)] + sums[1][32 * wave + (lane & 31)];
+      }
       if (live && lane < 32) a.delta[stat] = delta;
     }
     if (it + 1 < sum + tiles) {
@@ -155,9 +162,25 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
       __syncthreads();
     }
   }
-  if (__syncthreads_or(bad)) {
-    const int z = zone / BN;
-    add_nonfinite<S, DB, true>(acc, kp + z * k_step, k_ts, keys - z * BN, d, lane, [&](int r) { return z * BN + r <= lim; });
+  bad = __syncthreads_or(bad);
+  if constexpr (KS == 2) {
+    float* other = reinterpret_cast<float*>(smem) + wave * DB * 16 * 64 + lane;
+    if (part == 1) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) other[(db * 16 + i) * 64] = acc[db][i];
+    }
+    __syncthreads();
+    if (part == 1) return;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] += other[(db * 16 + i) * 64];
+  }
+  if (bad) {
+    const int z = zone / BS * BS;
+    add_nonfinite<S, DB, true>(acc, kp + (int64_t)z * k_ts, k_ts, keys - z, d, lane, [&](int r) { return z + r <= lim; });
   }
   store_rows<S, DB>(acc, a.scale, out, live, d, lane);
 }

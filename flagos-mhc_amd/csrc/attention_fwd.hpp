@@ -1,6 +1,8 @@
-// Attention forward: a block takes 32 NW queries of one head, a wave 32 of
+// Attention forward: a block takes 32 NW / KS queries of one head, a wave 32 of
 // them, and walks the keys they see in tiles of 32 NB, one pass with a running
-// maximum and sum.
+// maximum and sum.  KS = 2: two waves share 32 queries, each takes every other
+// tile, and their sums meet at the end: a long row is done in half the steps,
+// which is what a call of few blocks waits for.
 #pragma once
 
 #include "attention.hpp"
@@ -29,13 +31,14 @@ __device__ __forceinline__ void store_none(S* row, bool live, int d, int lane) {
   store_rows<S, DB>(z, 0.f, row, live, d, lane);
 }
 
-template <typename S, int DB, int NW, int NB, int WPE>
+template <typename S, int DB, int NW, int KS, int NB, int WPE>
 __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_t slots) {
   using T = Tile<S, DB>;
-  constexpr int BN = 32 * NB, BM = 32 * NW, NT = 64 * NW, ES = (int)sizeof(S);
-  constexpr int kTileBytes = BN * T::kPitch;
-  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (K, V)
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int RW = NW / KS, BN = 32 * NB, BS = BN * KS, BM = 32 * RW, NT = 64 * NW, ES = (int)sizeof(S);
+  constexpr int kTileBytes = BS * T::kPitch;  // KS tiles
+  extern __shared__ __attribute__((aligned(256))) char smem[];  // 2 x (K, V); at the end the sums of KS - 1 waves a row
+  const int tid = threadIdx.x, lane = tid & 63, id = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = id % RW, part = id / RW;
   int64_t slot;
   int h, first;
   att_item(a.n, slots, slot, h);
@@ -65,9 +68,9 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   const char* kp = uniform(row_ptr(a.k, a.n.cu_k, s.k0, s.b, 0, hk, ES));
   const char* vp = uniform(row_ptr(a.v, a.n.cu_k, s.k0, s.b, 0, hk, ES));
   const int lk = __builtin_amdgcn_readfirstlane(s.lk);
-  const int64_t k_step = (int64_t)BN * k_ts, v_step = (int64_t)BN * v_ts;
+  const int64_t k_step = (int64_t)BS * k_ts, v_step = (int64_t)BS * v_ts;
 
-  TileStage<S, DB, BN, NT> sk, sv;
+  TileStage<S, DB, BS, NT> sk, sv;
   uint32_t k_off = sk.offset(k_ts, dc, tid), v_off = sv.offset(v_ts, dc, tid);
   const uint32_t lds = lds_addr(smem);
   sk.load(kp, k_ts, lk, k_off);
@@ -76,7 +79,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
   const int zone = a.n.causal ? max(0, first + shift + 1) : 0x7fffffff;
   bool bad = false;
   auto stage = [&](int t) {
-    if ((t + 1) * BN > zone) bad |= sv.clean();
+    if ((t + 1) * BS > zone) bad |= sv.clean();
     const uint32_t to = lds + (t & 1) * 2 * kTileBytes;
     sk.store(to, tid);
     sv.store(to + kTileBytes, tid);
@@ -92,14 +95,14 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
     for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
   float m = -__builtin_inff(), l = 0.f;  // reference point (powers of two) and the lane's share of the sum
   const float c = a.scale2;
-  const int tiles = (keys + BN - 1) / BN, half = lane >> 5;
+  const int tiles = (keys + BS - 1) / BS, half = lane >> 5;
   for (int t = 0; t < tiles; ++t) {
-    const uint32_t tk = lds + (t & 1) * 2 * kTileBytes, tv = tk + kTileBytes;
+    const uint32_t tk = lds + (t & 1) * 2 * kTileBytes + part * BN * T::kPitch, tv = tk + kTileBytes;
     at.keep();
-    const int k0 = t * BN;
+    const int k0 = t * BS + part * BN;
     if (t + 1 < tiles) {
-      sk.load(kp + (t + 1) * k_step, k_ts, lk - k0 - BN, k_off);
-      sv.load(vp + (t + 1) * v_step, v_ts, lk - k0 - BN, v_off);
+      sk.load(kp + (t + 1) * k_step, k_ts, lk - (t + 1) * BS, k_off);
+      sv.load(vp + (t + 1) * v_step, v_ts, lk - (t + 1) * BS, v_off);
     }
     if (k0 <= wave_hi) {
       floatx16 sc[NB];
@@ -150,9 +153,32 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
       __syncthreads();
     }
   }
-  if (__syncthreads_or(bad)) {
-    const int z = zone / BN;
-    add_nonfinite<S, DB, false>(acc, vp + z * v_step, v_ts, keys - z * BN, d, lane, [&](int r) { return z * BN + r <= lim; });
+  bad = __syncthreads_or(bad);
+  if constexpr (KS == 2) {
+    // the second wave's sums to the first, both from the larger reference point
+    float* other = reinterpret_cast<float*>(smem) + wave * (DB * 16 + 2) * 64 + lane;
+    if (part == 1) {
+      other[0] = m;
+      other[64] = l;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) other[(2 + db * 16 + i) * 64] = acc[db][i];
+    }
+    __syncthreads();
+    if (part == 1) return;
+    const float m1 = other[0], top = fmaxf(m, m1), ref = top == -__builtin_inff() ? 0.f : top;
+    const float f0 = hw_exp2(m - ref), f1 = hw_exp2(m1 - ref);
+    m = top;
+    l = l * f0 + other[64] * f1;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] = acc[db][i] * f0 + other[(2 + db * 16 + i) * 64] * f1;
+  }
+  if (bad) {
+    const int z = zone / BS * BS;
+    add_nonfinite<S, DB, false>(acc, vp + (int64_t)z * v_ts, v_ts, keys - z, d, lane, [&](int r) { return z + r <= lim; });
   }
   l = add_xor32(l);
   // (a NaN among the scores leaves l NaN: not the empty row's zero)

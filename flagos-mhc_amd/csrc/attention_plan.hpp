@@ -22,11 +22,18 @@ inline int64_t att_slots(bool packed, int64_t T, int B, int S, int R) {
   return packed ? T / R + B + 1 : (int64_t)B * ((S + R - 1) / R);
 }
 
-// Blocks of 256 queries instead of 128: half the reads of k and v, but more
-// queries past the sequences' ends, and less to choose from when blocks end.
-// 32768 x 32 heads of 128 bf16: 3 to 5 % faster; documents of 400 to 1300
-// tokens, 700 blocks: 10 % slower.
-inline bool att_big(const AttDims& n, int64_t slots, int cus) { return slots * n.H >= 8 * (int64_t)cus; }
+// Blocks of 128 queries; or of 256, where there are many: half the reads of k
+// and v, but more queries past the sequences' ends, and less to choose from when
+// blocks end (32768 x 32 heads of 128 bf16: 3 to 5 % faster; documents of 400 to
+// 1300 tokens, 700 blocks: 10 % slower); or of 128 with two waves for every 32
+// of them, where there are few (4096 x 16 heads over 8, 544 blocks: 110 -> 92 us
+// forward, 368 -> 333 us backward; 4096 x 32, 1088 blocks: 172 -> 179 us).
+enum AttBlocks { kBlocks128, kBlocks256, kBlocksPairs };
+inline AttBlocks att_blocks(const AttDims& n, bool big, int cus) {
+  if (big && att_slots(n.cu_q != nullptr, n.Tq, n.B, n.Sq, 256) * n.H >= 8 * (int64_t)cus) return kBlocks256;
+  if (att_slots(n.cu_q != nullptr, n.Tq, n.B, n.Sq, 128) * n.H <= 3 * (int64_t)cus) return kBlocksPairs;
+  return kBlocks128;
+}
 
 // Few queries, or few blocks of 128 (less than one a compute unit): the rows of
 // a group's heads share tiles of 32, whose keys a block's waves split, and,

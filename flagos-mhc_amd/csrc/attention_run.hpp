@@ -32,7 +32,7 @@ template <typename S, int DB> struct AttShape {
 };
 
 template <typename S, int DB>
-int att_split_width(const AttArgs& a, const AttSplit& p, hipStream_t st) {
+int att_split_run(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   const int64_t blocks = p.slots * a.n.Hk * p.splits, rows = a.n.Tq * a.n.H;
   if (blocks > 0xffffffffll / 256 || rows > 0xffffffffll / 256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
@@ -45,42 +45,55 @@ int att_split_width(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   return check_launch("attention");
 }
 
-template <typename S, int DB, int NW>
-int att_fwd_run(const AttArgs& a, int64_t slots, hipStream_t st) {
-  using A = AttShape<S, DB>;
-  return att_launch(att_fwd_kernel<S, DB, NW, A::kFwdNB, A::kWPE>, a, slots, a.n.H, 64 * NW,
-                    (size_t)4 * 32 * A::kFwdNB * Tile<S, DB>::kPitch, st, "attention");
+// LDS of a kernel that holds two times `rows` rows of k and of v, and in the
+// end the sums of half of its waves.
+template <typename S, int DB, int NW, int KS>
+constexpr size_t att_lds(int rows) {
+  const size_t tiles = (size_t)4 * rows * Tile<S, DB>::kPitch, sums = KS == 2 ? (size_t)NW / 2 * (DB * 16 + 2) * 256 : 0;
+  return tiles > sums ? tiles : sums;
 }
-template <typename S, int DB, int NW>
-int att_dq_run(const AttArgs& a, int64_t slots, hipStream_t st) {
-  constexpr int NB = AttShape<S, DB>::kBwdNB;
-  return att_launch(att_dq_kernel<S, DB, NW, NB, AttShape<S, DB>::kWPE>, a, slots, a.n.H, 64 * NW,
-                    (size_t)4 * 32 * NB * Tile<S, DB>::kPitch, st, "attention_backward");
+
+template <typename S, int DB, int NW, int KS>
+int att_fwd_run(const AttArgs& a, hipStream_t st) {
+  using A = AttShape<S, DB>;
+  constexpr int BM = 32 * NW / KS;
+  return att_launch(att_fwd_kernel<S, DB, NW, KS, A::kFwdNB, A::kWPE>, a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, BM),
+                    a.n.H, 64 * NW, att_lds<S, DB, NW, KS>(32 * A::kFwdNB * KS), st, "attention");
+}
+template <typename S, int DB, int NW, int KS>
+int att_dq_run(const AttArgs& a, hipStream_t st) {
+  using A = AttShape<S, DB>;
+  constexpr int BM = 32 * NW / KS;
+  return att_launch(att_dq_kernel<S, DB, NW, KS, A::kBwdNB, A::kWPE>, a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, BM),
+                    a.n.H, 64 * NW, att_lds<S, DB, NW, KS>(32 * A::kBwdNB * KS), st, "attention_backward");
 }
 
 template <typename S, int DB>
 int att_fwd_width(const AttArgs& a, hipStream_t st) {
   const int cus = device_cu_count();
   const AttSplit p = att_split(a.n, cus);
-  if (p.use) return att_split_width<S, DB>(a, p, st);
-  if constexpr (AttShape<S, DB>::kBig) {
-    const int64_t big = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 256);
-    if (att_big(a.n, big, cus)) return att_fwd_run<S, DB, 8>(a, big, st);
-  }
-  return att_fwd_run<S, DB, 4>(a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 128), st);
+  if (p.use) return att_split_run<S, DB>(a, p, st);
+  const AttBlocks b = att_blocks(a.n, AttShape<S, DB>::kBig, cus);
+  if constexpr (AttShape<S, DB>::kBig)
+    if (b == kBlocks256) return att_fwd_run<S, DB, 8, 1>(a, st);
+  if constexpr (AttShape<S, DB>::kWPE == 2)
+    if (b == kBlocksPairs) return att_fwd_run<S, DB, 8, 2>(a, st);
+  return att_fwd_run<S, DB, 4, 1>(a, st);
 }
 
 template <typename S, int DB>
 int att_dq_width(const AttArgs& a, hipStream_t st) {
-  const AttSplit p = att_split(a.n, device_cu_count());
+  const int cus = device_cu_count();
+  const AttSplit p = att_split(a.n, cus);
   if (p.use)
     return att_launch(att_dq_split_kernel<S, DB, AttShape<S, DB>::kBytes <= 128 ? 2 : 1>, a, p.slots, a.n.Hk, 64 * kSplitWaves,
                       split_lds<S, DB>(), st, "attention_backward");
-  if constexpr (AttShape<S, DB>::kBig) {
-    const int64_t big = att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 256);
-    if (att_big(a.n, big, device_cu_count())) return att_dq_run<S, DB, 8>(a, big, st);
-  }
-  return att_dq_run<S, DB, 4>(a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, 128), st);
+  const AttBlocks b = att_blocks(a.n, AttShape<S, DB>::kBig, cus);
+  if constexpr (AttShape<S, DB>::kBig)
+    if (b == kBlocks256) return att_dq_run<S, DB, 8, 1>(a, st);
+  if constexpr (AttShape<S, DB>::kWPE == 2)
+    if (b == kBlocksPairs) return att_dq_run<S, DB, 8, 2>(a, st);
+  return att_dq_run<S, DB, 4, 1>(a, st);
 }
 
 template <typename S, int DB, int NW>

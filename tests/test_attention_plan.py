@@ -27,9 +27,9 @@ int main() {
                  B ? (int)(Tk / B) : 0, (int)H, (int)Hk, (int)d, 1};
     const AttSplit s = att_split(n, 256);
     const AttBwdPlan p = att_bwd_plan(n, fp32, att_big_head(n, fp32), 256);
-    printf("%lld %lld %lld %d %d %lld %zu %d %zu %zu %d %lld\n", (long long)att_slots(packed, Tq, (int)B, n.Sq, 128),
+    printf("%lld %lld %lld %d %d %lld %zu %d %zu %zu %d %lld %d\n", (long long)att_slots(packed, Tq, (int)B, n.Sq, 128),
            (long long)att_slots(packed, Tq, (int)B, n.Sq, 256), (long long)att_slots(packed, Tk, (int)B, n.Sk, 128),
-           s.use, s.splits, (long long)s.slots, s.bytes(n), p.splits, p.delta_bytes, p.part_bytes, p.keys, (long long)p.slots);
+           s.use, s.splits, (long long)s.slots, s.bytes(n), p.splits, p.delta_bytes, p.part_bytes, p.keys, (long long)p.slots, att_blocks(n, att_big_head(n, fp32), 256));
   }
 }
 """
@@ -48,7 +48,7 @@ def plan(tmp_path_factory):
     def run(rows):
         text = "\n".join(" ".join(str(int(v)) for v in r) for r in rows)
         out = subprocess.run([str(d / "plan")], input=text, capture_output=True, text=True, check=True).stdout
-        names = ("slots128", "slots256", "slots_k", "use", "splits", "split_slots", "bytes", "parts", "delta", "part_bytes", "keys", "key_slots")
+        names = ("slots128", "slots256", "slots_k", "use", "splits", "split_slots", "bytes", "parts", "delta", "part_bytes", "keys", "key_slots", "blocks")
         return [dict(zip(names, map(int, line.split()))) for line in out.splitlines()]
 
     return run
@@ -129,3 +129,19 @@ def test_nothing_to_split(plan):
     for r in ((1, 0, 0, 3, 4, 2, 64, 0), (0, 0, 0, 0, 4, 2, 64, 0), (1, 10, 10, 0, 4, 2, 64, 0)):
         p = plan([r])[0]
         assert p["use"] == 0 and p["splits"] == p["parts"] == 1 and p["bytes"] == p["part_bytes"] == 0
+
+
+def test_gpu_tests_reach_every_kernel(plan):
+    """The calls of the GPU tests choose the kernels that they are there for (256 compute units)."""
+    from test_gpu_attention_blocks import OF_128, OF_256, PAIRS, _lengths
+    for heads, kind, d, longest, fp32 in ((PAIRS, 2, 64, 700, 0), (PAIRS, 2, 128, 700, 1), (OF_128, 0, 128, 700, 0),
+                                          (OF_128, 0, 256, 700, 0), (OF_128, 0, 64, 700, 1), (OF_256, 1, 128, 1200, 0)):
+        for seed in (5, 9, 64, 72, 96, 128, 192, 256):
+            T = sum(_lengths(seed, 70, longest))
+            p = plan([(1, T, T, 70, *heads, d, fp32)])[0]
+            assert p["use"] == 0 and p["blocks"] == kind, (heads, seed, p)
+            assert p["keys"] == (256 if kind == 1 else 128)
+    # parts of the keys, and none; parts of the queries, and none
+    one = plan([(0, 1, 5000, 1, 8, 1, 64, 0), (0, 3, 6300, 3, 4, 4, 128, 1), (1, 5, 5, 1, 4, 2, 64, 0), (1, 1030, 1030, 1, 2, 1, 64, 0)])
+    assert [p["use"] for p in one] == [1, 1, 1, 1]
+    assert one[0]["splits"] > 1 and one[1]["splits"] > 1 and one[2]["splits"] == one[2]["parts"] == 1 and one[3]["parts"] > 1

@@ -29,23 +29,28 @@ def _inputs(lengths, H, Hk, d, dtype, pad=0, seed=0):
     return (*(_randn(g, T, n, d, dtype=DT[dtype]) for n in (H, Hk, Hk, H)), _cu(lengths))
 
 
-# 128 queries a block: at least 256 blocks, so 70 sequences of 4 heads
+# (heads, key heads) that choose a kernel for 70 sequences (tests/test_attention_plan.py checks that they do)
+PAIRS, OF_128, OF_256 = (4, 2), (12, 4), (32, 8)
+
+
+# 128 queries a block, with two waves for 32 of them or one
+@pytest.mark.parametrize("heads", [PAIRS, OF_128])
 @pytest.mark.parametrize("d", [64, 72, 96, 128, 192, 256])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("causal", [True, False])
-def test_blocks_of_128(d, dtype, causal):
+def test_blocks_of_128(heads, d, dtype, causal):
     if dtype == "f32" and d > 128:
         pytest.skip("fp32 heads wider than 128 are refused")
-    print(f"[attention] 128: d={d} {dtype} causal={causal}", flush=True)
-    q, k, v, go, cu = _inputs(_lengths(d, 70, 700), 4, 2, d, dtype, pad=5)
-    _check(q, k, v, go, cu, causal=causal, what=f"{d} {dtype}")
+    print(f"[attention] 128: {heads} d={d} {dtype} causal={causal}", flush=True)
+    q, k, v, go, cu = _inputs(_lengths(d, 70, 700), *heads, d, dtype, pad=5)
+    _check(q, k, v, go, cu, causal=causal, what=f"{heads} {d} {dtype}")
 
 
-# 256 queries a block: at least 2048 blocks
+# 256 queries, and keys, a block
 @pytest.mark.parametrize("dtype,d,causal", [("bf16", 128, True), ("f16", 112, True), ("bf16", 128, False)])
 def test_blocks_of_256(dtype, d, causal):
     print(f"[attention] 256: d={d} {dtype} causal={causal}", flush=True)
-    q, k, v, go, cu = _inputs(_lengths(5, 70, 1200), 32, 8, d, dtype, pad=2)
+    q, k, v, go, cu = _inputs(_lengths(5, 70, 1200), *OF_256, d, dtype, pad=2)
     _check(q, k, v, go, cu, causal=causal, what=f"{d} {dtype}")
 
 
@@ -126,7 +131,7 @@ def test_offsets_past_32_bits():
     assert not out[:4].any()
 
 
-@pytest.mark.parametrize("d,H,Hk", [(64, 4, 2), (128, 4, 2), (128, 32, 8)])
+@pytest.mark.parametrize("d,H,Hk", [(64, *PAIRS), (128, *PAIRS), (64, *OF_128), (128, *OF_128), (128, *OF_256)])
 def test_hidden_nans_in_blocks(d, H, Hk):
     """As for small calls: a token reaches no query before it and no key behind it."""
     lengths = _lengths(9, 70, 500)
