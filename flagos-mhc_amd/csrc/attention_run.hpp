@@ -25,6 +25,8 @@ int att_launch(K kernel, const AttArgs& a, int64_t slots, int64_t per_slot, int 
 template <typename S, int DB> struct AttShape {
   static constexpr int kBytes = 32 * DB * (int)sizeof(S);
   static constexpr int kWPE = kBytes <= 256 ? 2 : 1;
+  static constexpr int kFwdWPE = sizeof(S) == 2 || kBytes <= 256 ? 2 : 1;  // (fewer sums than the backward)
+  static constexpr int kFwdNW = DB == 8 ? 8 : 4;  // heads of 256: 8 waves 489 us, 4 waves 627 us, one a SIMD unit 882 us (8192 in 2, 20 heads)
   static constexpr int kFwdNB = sizeof(S) == 2 && DB <= 4 ? 2 : 1;
   static constexpr int kBwdNB = sizeof(S) == 2 && DB <= 2 ? 2 : 1;
   static constexpr bool kDkvLds = kBytes > 128;
@@ -57,7 +59,7 @@ template <typename S, int DB, int NW, int KS>
 int att_fwd_run(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
   constexpr int BM = 32 * NW / KS;
-  return att_launch(att_fwd_kernel<S, DB, NW, KS, A::kFwdNB, A::kWPE>, a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, BM),
+  return att_launch(att_fwd_kernel<S, DB, NW, KS, A::kFwdNB, A::kFwdWPE>, a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, BM),
                     a.n.H, 64 * NW, att_lds<S, DB, NW, KS>(32 * A::kFwdNB * KS), st, "attention");
 }
 template <typename S, int DB, int NW, int KS>
@@ -76,9 +78,9 @@ int att_fwd_width(const AttArgs& a, hipStream_t st) {
   const AttBlocks b = att_blocks(a.n, AttShape<S, DB>::kBig, cus);
   if constexpr (AttShape<S, DB>::kBig)
     if (b == kBlocks256) return att_fwd_run<S, DB, 8, 1>(a, st);
-  if constexpr (AttShape<S, DB>::kWPE == 2)
+  if constexpr (AttShape<S, DB>::kFwdWPE == 2 && DB < 8)
     if (b == kBlocksPairs) return att_fwd_run<S, DB, 8, 2>(a, st);
-  return att_fwd_run<S, DB, 4, 1>(a, st);
+  return att_fwd_run<S, DB, AttShape<S, DB>::kFwdNW, 1>(a, st);
 }
 
 template <typename S, int DB>
