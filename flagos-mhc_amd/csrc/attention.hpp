@@ -26,10 +26,10 @@ typedef _Float16 f16x8_att __attribute__((ext_vector_type(8)));
 typedef short s16x4_att __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Two scaled products per exp2: a new row maximum moves the reference point
-// only where it exceeds the old one by more than this (in powers of two), so
-// that sums are rescaled a few times a row and not once a tile.  p is then at
-// most 2^8, exact in every type's range, and the result does not depend on it.
+// A new row maximum moves the reference point only where it exceeds the old one
+// by more than this (in powers of two), so that sums are rescaled a few times a
+// row and not once a tile.  Weights are then at most 2^8 instead of 1: within
+// every type's range, and as many bits are left to them.
 constexpr float kLazyMax = 8.0f;
 
 // One of q, k, v or a gradient: element (sequence's row t, head h, i) at
@@ -54,11 +54,11 @@ struct AttArgs {
 // ---- sequences ---------------------------------------------------------------
 
 struct AttSeq {
-  int64_t row0;    // first row in the outputs' and lse's order
-  int64_t q0, k0;  // element offsets of row 0 of q and k: add AttRows.p
-  int lq, lk;      // rows; lq counts output rows of the sequence behind the last one too
+  int64_t row0;  // first row in the outputs' and lse's order
+  int64_t k0;    // first row of packed keys
+  int lq, lk;    // rows; lq counts output rows of the sequence behind the last one too
   int b;
-  bool none;       // rows behind the last sequence: zeros are written
+  bool none;     // rows behind the last sequence: zeros are written
 };
 
 __device__ __forceinline__ int64_t cu_at(const int32_t* cu, int b, int64_t T) {
@@ -121,7 +121,8 @@ __device__ __forceinline__ AttSeq att_seq(const AttDims& n, int b) {
 }
 
 // Tile of `R` query rows that slot `slot` stands for: its sequence and first
-// row (lq or more: nothing to do).
+// row (lq or more: nothing to do).  Starts that decrease can lead to a sequence
+// whose slots begin later: no tile of it.
 __device__ __forceinline__ AttSeq q_tile(const AttDims& n, int64_t slot, int R, int& first) {
   if (!n.cu_q) {
     const int per = (n.Sq + R - 1) / R;
@@ -132,7 +133,7 @@ __device__ __forceinline__ AttSeq q_tile(const AttDims& n, int64_t slot, int R, 
   const int b = slot_sequence(n.cu_q, n.B, n.Tq, R, slot);
   const int64_t t = slot - slot_start(n.cu_q, b, n.Tq, R);
   AttSeq s = att_seq(n, b);
-  first = t * R < s.lq ? (int)(t * R) : s.lq;
+  first = t >= 0 && t * R < s.lq ? (int)(t * R) : s.lq;
   return s;
 }
 
@@ -153,7 +154,7 @@ __device__ __forceinline__ AttSeq k_tile(const AttDims& n, int64_t slot, int R, 
   row0 = cu_at(n.cu_k, b, n.Tk);
   const int64_t e = s.none ? n.Tk : cu_at(n.cu_k, b + 1, n.Tk);
   rows = e > row0 ? (int)(e - row0) : 0;
-  first = t * R < rows ? (int)(t * R) : rows;
+  first = t >= 0 && t * R < rows ? (int)(t * R) : rows;
   return s;
 }
 

@@ -50,6 +50,7 @@ __device__ __forceinline__ AttSeq group_tile(const AttDims& n, int64_t slot, int
   const int b = __builtin_amdgcn_readfirstlane(lo);
   const AttSeq s = att_seq(n, b);
   first = (slot - (s.row0 * G / 32 + b)) * 32;
+  if (first < 0) first = (int64_t)s.lq * G;  // (decreasing starts)
   return s;
 }
 
