@@ -185,6 +185,12 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
   store_rows<S, DB>(acc, a.scale, out, live, d, lane);
 }
 
+// A float of the `bytes` at p; zero past them.
+__device__ __forceinline__ float buffer_f32(const float* p, int bytes, uint32_t off) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, max(bytes, 0), 0x00020000);
+  return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+}
+
 // dk and dv, or, of `splits` parts of the queries, a part's share of them in
 // fp32, for att_dkv_join_kernel.  VLDS: the block's own rows of v are in LDS, and read as they are
 // needed, instead of in registers: with those two waves fit a SIMD unit.
@@ -237,19 +243,27 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
     load_rows<S, DB>(row_ptr(a.v, a.n.cu_k, s.k0, s.b, wave_first, hk, ES), (int)(a.v.ts * ES), s.lk - wave_first, dc, lane, v);
   }
 
+  // Items: the tiles of queries of every head that shares the keys.  What is
+  // loaded next is kept as pointers: divisions and 64-bit products an item cost
+  // as many instructions as a tile of 64-wide heads.
+  const int items = tiles * G, it0 = (int)((int64_t)items * part / splits), it1 = (int)((int64_t)items * (part + 1) / splits);
+  const int h0 = hk * G + it0 / tiles, end = t0 + tiles;
+  int t = t0 + it0 % tiles;
+  const char* qp = uniform(row_ptr(a.q, a.n.cu_q, s.row0, s.b, (int64_t)t * BQ, h0, ES));
+  const char* gp = uniform(row_ptr(a.go, a.n.cu_q, s.row0, s.b, (int64_t)t * BQ, h0, ES));
+  int64_t sp = (int64_t)uniform(reinterpret_cast<const char*>((int64_t)h0 * a.n.Tq + s.row0 + (int64_t)t * BQ));
+  const int lq = __builtin_amdgcn_readfirstlane(s.lq);
   TileStage<S, DB, BQ, NT> sq, sg;
   const uint32_t q_off = sq.offset(q_ts, dc, tid), go_off = sg.offset(go_ts, dc, tid), lds = lds_addr(smem) + kOwn;
-  float st_lse = 0.f, st_delta = 0.f;
-  auto load = [&](int it) {
-    const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ;
-    sq.load(row_ptr(a.q, a.n.cu_q, s.row0, s.b, q0, h, ES), q_ts, s.lq - q0, q_off);
-    sg.load(row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, s.lq - q0, go_off);
-    if (tid < BQ) {
-      const bool in = q0 + tid < s.lq;
-      const int64_t i = (int64_t)h * a.n.Tq + s.row0 + q0 + tid;
-      const float l = in ? a.lse[i] : -__builtin_inff();
-      st_lse = l == -__builtin_inff() ? __builtin_inff() : l * kLog2e;  // no such row, or an empty one: P = 0
-      st_delta = in ? a.delta[i] : 0.f;
+  float st_lse = 0.f, st_delta = 0.f;  // of query `lane` of the tile, in wave 0
+  auto load = [&]() {
+    const int left = lq - t * BQ;
+    sq.load(qp, q_ts, left, q_off);
+    sg.load(gp, go_ts, left, go_off);
+    if (wave == 0) {
+      const int bytes = min(left, BQ) * 4;
+      st_lse = buffer_f32(a.lse + sp, bytes, lane * 4);
+      st_delta = buffer_f32(a.delta + sp, bytes, lane * 4);
     }
   };
   // queries before `zone` see not all of the block's keys: as in the forward,
@@ -258,7 +272,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   bool bad = false;
   auto store = [&](int it) {
     const int buf = it & 1;
-    if ((t0 + it % tiles) * BQ < zone) {
+    if (t * BQ < zone) {
       bad |= sq.clean();
       bad |= sg.clean();
     }
@@ -266,12 +280,24 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
     sg.store(lds + buf * kStage + kTileBytes, tid);
     if (tid < BQ) {
       float* to = reinterpret_cast<float*>(smem + kOwn + buf * kStage + 2 * kTileBytes);
-      to[tid] = st_lse;
+      // no such row, or an empty one: P = 0
+      to[tid] = t * BQ + tid >= lq || st_lse == -__builtin_inff() ? __builtin_inff() : st_lse * kLog2e;
       to[BQ + tid] = st_delta;
     }
   };
-  const int items = tiles * G, it0 = (int)((int64_t)items * part / splits), it1 = (int)((int64_t)items * (part + 1) / splits);
-  load(it0);
+  auto advance = [&]() {
+    ++t;
+    qp += (int64_t)BQ * q_ts;
+    gp += (int64_t)BQ * go_ts;
+    sp += BQ;
+    if (t == end) {
+      t = t0;
+      qp += a.q.hs * ES - (int64_t)tiles * BQ * q_ts;
+      gp += a.go.hs * ES - (int64_t)tiles * BQ * go_ts;
+      sp += a.n.Tq - (int64_t)tiles * BQ;
+    }
+  };
+  load();
   store(it0);
   __syncthreads();
   T at(lane);
@@ -288,8 +314,11 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
     const uint32_t tq = lds + (it & 1) * kStage, tg = tq + kTileBytes;
     const float* stats = reinterpret_cast<const float*>(smem + kOwn + (it & 1) * kStage + 2 * kTileBytes);
     at.keep();
-    const int q0 = (t0 + it % tiles) * BQ;
-    if (it + 1 < it1) load(it + 1);
+    const int q0 = t * BQ;
+    if (it + 1 < it1) {
+      advance();
+      load();
+    }
     // queries from here on see the lane's key; all of the wave's keys are seen by the tile or none
     const int lim = a.n.causal ? key - shift : 0;
     const bool any = wave_first < s.lk && (!a.n.causal || q0 + BQ - 1 >= wave_first - shift);
@@ -344,7 +373,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   }
   if (__syncthreads_or(bad)) {
     for (int it = it0; it < it1; ++it) {
-      const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ, n = min(BQ, s.lq - q0);
+      const int h = hk * G + it / tiles, q0 = (t0 + it % tiles) * BQ, n = min(BQ, lq - q0);
       if (q0 >= zone) continue;
       const auto seen = [&](int r) { return q0 + r >= key - shift; };
       add_nonfinite<S, DB, false>(av, row_ptr(a.go, a.n.cu_q, s.row0, s.b, q0, h, ES), go_ts, n, d, lane, seen);
