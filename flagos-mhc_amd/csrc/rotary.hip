@@ -47,12 +47,50 @@ __device__ __forceinline__ int64_t packed_position(const int32_t* cu, int B, int
 
 constexpr int kThreads = 256, kTrig = 2048;  // float2 of LDS: tokens * r / 2 at most
 
-// VEC: elements of an access; 1: any layout and alignment.
+// VEC elements at any alignment: 16 bytes, or 8.
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+template <typename S, bool WHOLE> struct Piece;
+template <typename S> struct Piece<S, true> {
+  using T = u32x4;
+  static __device__ __forceinline__ T load(const S* p) { return ld16nt_u(p); }
+  static __device__ __forceinline__ void store(S* p, T w) { st16nt_u(p, w); }
+  static __device__ __forceinline__ void unpack(T w, float (&v)[Store<S>::VEC]) { Store<S>::unpack(w, v); }
+  static __device__ __forceinline__ T pack(const float (&v)[Store<S>::VEC]) { return Store<S>::pack(v); }
+};
+template <typename S> struct Piece<S, false> {
+  static constexpr int N = Store<S>::VEC / 2;
+  using T = u32x2;
+  static __device__ __forceinline__ T load(const S* p) { return __builtin_nontemporal_load(reinterpret_cast<const u32x2_a2*>(p)); }
+  static __device__ __forceinline__ void store(S* p, T w) { __builtin_nontemporal_store(w, reinterpret_cast<u32x2_a2*>(p)); }
+  static __device__ __forceinline__ void unpack(T w, float (&v)[N]) {
+    float all[2 * N];
+    Store<S>::unpack(u32x4{w[0], w[1], 0u, 0u}, all);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = all[j];
+  }
+  static __device__ __forceinline__ T pack(const float (&v)[N]) {
+    float all[2 * N] = {};
+#pragma unroll
+    for (int j = 0; j < N; ++j) all[j] = v[j];
+    const u32x4 w = Store<S>::pack(all);
+    return u32x2{w[0], w[1]};
+  }
+};
+
+// VEC: elements of an access; 1: any sizes.
 template <typename S, int VEC, bool HALF>
 __global__ __launch_bounds__(kThreads) void rotary_kernel(RotArgs a, int tokens) {
   __shared__ float2 trig[kTrig];
   const int64_t t0 = xcd_contig(blockIdx.x, gridDim.x) * tokens;
   const int n = (int)(a.T - t0 < tokens ? a.T - t0 : tokens), half = a.r / 2, wave = threadIdx.x >> 6;
+  // a head's items: pairs of vectors (HALF), vectors of pairs, or single pairs;
+  // then what is copied, as many elements an item
+  const int rot = VEC > 1 && !HALF ? a.r / VEC : half / VEC;
+  const int wide = VEC > 1 && !HALF ? VEC : 2 * VEC;  // elements of an item
+  const int per = rot + (a.d - a.r + wide - 1) / wide, heads = a.heads[0] + a.heads[1];
+  // item `at` of head `th` of token `tok`; the next one is kThreads items on
+  const int step_th = kThreads / per, step_at = kThreads % per, step_i = step_th / heads, step_h = step_th % heads;
+  int at = threadIdx.x % per, th = threadIdx.x / per % heads, tok = threadIdx.x / per / heads;
   for (int i = wave; i < n; i += kThreads / 64) {
     const int64_t t = t0 + i;
     int64_t p;
@@ -68,67 +106,66 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotArgs a, int tokens)
     }
   }
   __syncthreads();
-  // a head's items: pairs of vectors (HALF) or vectors of pairs, then what is copied
-  const int rot = HALF ? half / VEC : (VEC == 1 ? half : a.r / VEC), copies = (a.d - a.r) / VEC, per = rot + copies;
-  const int heads = a.heads[0] + a.heads[1], all = n * heads * per;
-  for (int id = threadIdx.x; id < all; id += kThreads) {
-    const int item = id % per, th = id / per;
-    int h = th % heads;
-    const int i = th / heads;
-    const int64_t t = t0 + i;
-    const int w = h >= a.heads[0];
-    h -= w ? a.heads[0] : 0;
+  while (tok < n) {
+    const int w = th >= a.heads[0], h = th - (w ? a.heads[0] : 0);
+    const int64_t t = t0 + tok;
     const S* x = static_cast<const S*>(a.x[w]) + t * a.ts[w] + (int64_t)h * a.hs[w];
     S* y = static_cast<S*>(a.y[w]) + (t * a.heads[w] + h) * (int64_t)a.d;
-    const float2* cs = trig + i * half;
-    if (item >= rot) {
-      const int e = a.r + (item - rot) * VEC;
-      if constexpr (VEC == 1) store_elem<S>(y, e, load_elem<S>(x, e));
-      else st16nt(y + e, ld16nt(x + e));
-    } else if constexpr (VEC == 1) {
-      const int i0 = HALF ? item : 2 * item, i1 = HALF ? item + half : i0 + 1;
-      const float u = load_elem<S>(x, i0), v = load_elem<S>(x, i1);
-      const float2 q = cs[item];
-      store_elem<S>(y, i0, u * q.x - v * q.y);
-      store_elem<S>(y, i1, u * q.y + v * q.x);
+    // Turned or copied, an item is loaded and stored by the same instructions:
+    // apart, a wave with both waits for memory twice (16384 x 64 heads of 80, 40
+    // turned, bf16: 155 -> 75 us in pairs of neighbours, 4.5 TB/s).
+    const bool copy = at >= rot;
+    const float2* cs = trig + tok * half;
+    const int e = copy ? a.r + (at - rot) * wide : at * (HALF ? VEC : (VEC > 1 ? VEC : 2));
+    if constexpr (VEC == 1) {
+      const int e1 = HALF && !copy ? e + half : e + 1;
+      const bool two = e1 < a.d;
+      const float2 z = copy ? make_float2(1.f, 0.f) : cs[at];
+      const float u = load_elem<S>(x, e), v = two ? load_elem<S>(x, e1) : 0.f;
+      store_elem<S>(y, e, copy ? u : u * z.x - v * z.y);
+      if (two) store_elem<S>(y, e1, copy ? v : u * z.y + v * z.x);
     } else if constexpr (HALF) {
-      const int e = item * VEC;
-      float u[VEC], v[VEC];
-      Store<S>::unpack(ld16nt(x + e), u);
-      Store<S>::unpack(ld16nt(x + half + e), v);
-      float p[VEC], q[VEC];
+      using P = Piece<S, VEC == Store<S>::VEC>;
+      const int e1 = copy ? e + VEC : e + half;
+      const bool two = e1 < a.d;
+      const typename P::T wu = P::load(x + e), wv = P::load(x + (two ? e1 : e));
+      float u[VEC], v[VEC], p[VEC], q[VEC];
+      P::unpack(wu, u);
+      P::unpack(wv, v);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float2 z = cs[e + j];
+        const float2 z = cs[copy ? 0 : e + j];
         p[j] = u[j] * z.x - v[j] * z.y;
         q[j] = u[j] * z.y + v[j] * z.x;
       }
-      st16nt(y + e, Store<S>::pack(p));
-      st16nt(y + half + e, Store<S>::pack(q));
+      P::store(y + e, copy ? wu : P::pack(p));
+      if (two) P::store(y + e1, copy ? wv : P::pack(q));
     } else {
-      const int e = item * VEC;
-      float u[VEC];
-      Store<S>::unpack(ld16nt(x + e), u);
+      using P = Piece<S, VEC == Store<S>::VEC>;
+      const typename P::T wu = P::load(x + e);
+      float u[VEC], p[VEC];
+      P::unpack(wu, u);
 #pragma unroll
       for (int j = 0; j < VEC; j += 2) {
-        const float2 z = cs[(e + j) / 2];
-        const float p = u[j] * z.x - u[j + 1] * z.y;
-        u[j + 1] = u[j] * z.y + u[j + 1] * z.x;
-        u[j] = p;
+        const float2 z = cs[copy ? 0 : (e + j) / 2];
+        p[j] = u[j] * z.x - u[j + 1] * z.y;
+        p[j + 1] = u[j] * z.y + u[j + 1] * z.x;
       }
-      st16nt(y + e, Store<S>::pack(u));
+      P::store(y + e, copy ? wu : P::pack(p));
     }
+    at += step_at;
+    const int more = at >= per;
+    at -= more ? per : 0;
+    th += step_h + more;
+    const int wrap = th >= heads;
+    th -= wrap ? heads : 0;
+    tok += step_i + wrap;
   }
 }
 
-template <typename S>
-int rotary_run(const RotArgs& a, bool half_layout, hipStream_t st) {
-  constexpr int VEC = Store<S>::VEC;
+template <typename S, int VEC>
+int rotary_launch(const RotArgs& a, bool half_layout, hipStream_t st) {
   const int half = a.r / 2;
-  bool vec = a.d % VEC == 0 && a.r % VEC == 0 && (!half_layout || half % VEC == 0);
-  for (int w = 0; w < 2; ++w)
-    if (a.heads[w])
-      vec = vec && aligned16(a.x[w]) && aligned16(a.y[w]) && a.ts[w] % VEC == 0 && a.hs[w] % VEC == 0;
   // four tokens a block (a wave a token's angles) where there are blocks enough
   int tokens = a.T >= (int64_t)device_cu_count() * 16 ? 4 : 1;
   while (tokens > 1 && tokens * half > kTrig) tokens /= 2;
@@ -136,11 +173,22 @@ int rotary_run(const RotArgs& a, bool half_layout, hipStream_t st) {
   if (blocks > 0xffffffffll / kThreads)
     return set_error(MHC_ERR_UNSUPPORTED, "rotary: %lld rows exceed a dispatch", (long long)a.T);
   const dim3 g((unsigned)blocks), b(kThreads);
-  if (vec && half_layout) hipLaunchKernelGGL((rotary_kernel<S, VEC, true>), g, b, 0, st, a, tokens);
-  else if (vec) hipLaunchKernelGGL((rotary_kernel<S, VEC, false>), g, b, 0, st, a, tokens);
-  else if (half_layout) hipLaunchKernelGGL((rotary_kernel<S, 1, true>), g, b, 0, st, a, tokens);
-  else hipLaunchKernelGGL((rotary_kernel<S, 1, false>), g, b, 0, st, a, tokens);
+  if (half_layout) hipLaunchKernelGGL((rotary_kernel<S, VEC, true>), g, b, 0, st, a, tokens);
+  else hipLaunchKernelGGL((rotary_kernel<S, VEC, false>), g, b, 0, st, a, tokens);
   return check_launch("rotary");
+}
+
+// 16 bytes an access where a head's parts are whole ones, else 8 (heads of 80
+// with 40 turned in halves, 16384 x 64, bf16: 105 us, single elements 243 us),
+// else single elements.  Addresses need no alignment (16384 x 64 heads of 128
+// from an odd address: 119 us, 109 us from a whole 16 bytes, 4.9 TB/s).
+template <typename S>
+int rotary_run(const RotArgs& a, bool half_layout, hipStream_t st) {
+  constexpr int VEC = Store<S>::VEC;
+  const int part = half_layout ? a.r / 2 : a.r, rest = a.d - a.r;
+  if (part % VEC == 0 && rest % VEC == 0) return rotary_launch<S, VEC>(a, half_layout, st);
+  if (part % (VEC / 2) == 0 && rest % (VEC / 2) == 0) return rotary_launch<S, VEC / 2>(a, half_layout, st);
+  return rotary_launch<S, 1>(a, half_layout, st);
 }
 
 }  // namespace

@@ -130,3 +130,22 @@ def test_rotation_by_a_difference():
         vals.append(float((a.double() * b.double()).sum()))
     size = float(q.norm() * k.norm())
     assert max(vals) - min(vals) <= 2 * 24 * 2 ** -24 * size
+
+
+@pytest.mark.parametrize("off,pad", [(1, 0), (0, 1), (3, 5), (4, 4)])
+@pytest.mark.parametrize("d,r", [(80, 40), (64, 64), (48, 24), (36, 20)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_any_alignment_and_stride(off, pad, d, r, layout, dtype):
+    """Views that begin and step at any element: the same bits as of copies."""
+    g = _gen(off + pad)
+    T, H = 37, 3
+    buf = _randn(g, off + T * H * (d + pad) + 8, dtype=DT[dtype])
+    q = buf[off:off + T * H * (d + pad)].view(T, H, d + pad)[..., :d]
+    k = buf[off:off + T * (H * (d + pad))].view(T, H, d + pad)[:, :2, :d]
+    freqs, _ = S.rotary_frequencies(r)
+    pos = torch.randint(0, 1 << 17, (T,), device=DEV, generator=g)
+    for got, want in zip(S.rotary(q, k, freqs, pos, layout=layout),
+                         S.rotary(q.contiguous(), k.contiguous(), freqs, pos, layout=layout)):
+        assert torch.equal(got, want)
+    R.within(S.rotary(q, k, freqs, pos, layout=layout)[0], _want(q, freqs, pos, layout, 1.0), "q")
