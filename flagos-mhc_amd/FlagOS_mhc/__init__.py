@@ -20,8 +20,9 @@ single-pass pre forward gave up one of its bounded waits (the pre backward
 and every later pre forward check that too).
 
 The operators between the two, with their own names, are in
-``FlagOS_mhc.sublayer``: layer norm, gated feed-forward block, dropout and the
-mHC feed-forward layer made of them.
+``FlagOS_mhc.sublayer``: layer norm, gated feed-forward block, dropout, rotary
+positions, attention, and the mHC feed-forward and attention layers made of
+them.
 
 Importing the package also registers the operators as torch.ops.flagos_mhc.*
 (``FlagOS_mhc.library``) for torch.compile and HIP-graph capture.

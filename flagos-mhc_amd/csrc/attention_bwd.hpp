@@ -20,6 +20,9 @@
 // P and dS are rounded to the operands' type for the products that sum them,
 // in fp16 with its limits: P below 2^-14 and dS outside 2^-14 .. 65504 lose
 // bits, as values of that type do.
+//
+// Both are bound as the forward is.  16384 tokens, 56 heads of 128 over 8,
+// causal, bf16: dq 5.6 ms, dk and dv 7.5 ms, 1.03 PFLOP/s each.
 #pragma once
 
 #include "attention.hpp"
@@ -192,8 +195,11 @@ __device__ __forceinline__ float buffer_f32(const float* p, int bytes, uint32_t 
 }
 
 // dk and dv, or, of `splits` parts of the queries, a part's share of them in
-// fp32, for att_dkv_join_kernel.  VLDS: the block's own rows of v are in LDS, and read as they are
-// needed, instead of in registers: with those two waves fit a SIMD unit.
+// fp32, for att_dkv_join_kernel.  VLDS: the block's own rows of v are in LDS,
+// and read as they are needed, instead of in registers: with those two waves
+// fit a SIMD unit (16384 x 56 heads, forward and backward: 24.6 -> 18.6 ms).
+// Heads of 64 keep them in registers: 64 queries a step fit as well (three waves
+// a SIMD unit, 32 queries a step: 2.53 -> 2.98 ms the whole backward of 16384 in two, 32 heads).
 template <typename S, int DB, int NW, int NB, int WPE, bool VLDS>
 __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_t slots, int splits) {
   using T = Tile<S, DB>;
@@ -398,7 +404,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
   }
 }
 
-// dk, dv: the parts' shares added in their order, four elements a thread.
+// dk, dv: the parts' shares added in their order, four elements a thread: 3
+// parts of 4099 keys, 8 heads of 128: 118 MB in 18 us (some from the caches).
 template <typename S>
 __global__ __launch_bounds__(256) void att_dkv_join_kernel(AttArgs a, int64_t all, int splits) {
   const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;  // of 2 `all`: dk, then dv

@@ -1,6 +1,17 @@
 // Attention forward: a block takes 32 NW / KS queries of one head, a wave 32 of
 // them, and walks the keys they see in tiles of 32 NB, one pass with a running
-// maximum and sum.  KS = 2: two waves share 32 queries, each takes every other
+// maximum and sum.
+//
+// Keys and values go through registers to LDS one tile ahead, in the rows they
+// have in memory: k is read back as rows (first operand of K Q^T), v as columns
+// (of V^T P^T) with the transposing read, so nothing is turned in memory.  What
+// bounds it is the matrix instructions together with the exponentials between
+// them (16 a product of 32 x 32, at a quarter of the others' rate): two waves a
+// SIMD unit take turns.  32768 tokens, 32 heads of 128 over 8, causal, bf16:
+// 8.6 ms, 1.03 PFLOP/s (a large library product reaches 1.42 on this card); with
+// the loads of keys and values left out it is 17 % faster.
+//
+// KS = 2: two waves share 32 queries, each takes every other
 // tile, and their sums meet at the end: a long row is done in half the steps,
 // which is what a call of few blocks waits for.
 #pragma once

@@ -10,6 +10,10 @@
 // registers, loaded as the operand it is, and turns the values through 8 KB
 // of LDS of its own: no wave waits for another, and 16 KB a wave are in
 // flight while it computes.
+//
+// Reading the cache bounds it: 64 sequences of up to 8192 keys, 32 heads of 128
+// over 8, bf16: 290 us, 5.5 TB/s; one of 32768: 26 us, 5.2 TB/s, and 4 us for
+// the join (a copy of large tensors moves 4.96 TB/s, read and written).
 #pragma once
 
 #include "attention.hpp"
