@@ -61,6 +61,14 @@ struct AttSeq {
   bool none;     // rows behind the last sequence: zeros are written
 };
 
+// A value that is the same for the wave, known to be so: what a scalar register
+// holds costs no vector instruction, and a branch on it no mask.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 __device__ __forceinline__ int64_t cu_at(const int32_t* cu, int b, int64_t T) {
   const int64_t c = b == 0 ? 0 : (int64_t)cu[b];
   return c < 0 ? 0 : (c > T ? T : c);
@@ -117,6 +125,10 @@ __device__ __forceinline__ AttSeq att_seq(const AttDims& n, int b) {
       }
     }
   }
+  s.row0 = uniform(s.row0);
+  s.k0 = uniform(s.k0);
+  s.lq = uniform(s.lq);
+  s.lk = uniform(s.lk);
   return s;
 }
 
@@ -133,7 +145,7 @@ __device__ __forceinline__ AttSeq q_tile(const AttDims& n, int64_t slot, int R, 
   const int b = slot_sequence(n.cu_q, n.B, n.Tq, R, slot);
   const int64_t t = slot - slot_start(n.cu_q, b, n.Tq, R);
   AttSeq s = att_seq(n, b);
-  first = t >= 0 && t * R < s.lq ? (int)(t * R) : s.lq;
+  first = uniform(t >= 0 && t * R < s.lq ? (int)(t * R) : s.lq);
   return s;
 }
 
@@ -154,7 +166,9 @@ __device__ __forceinline__ AttSeq k_tile(const AttDims& n, int64_t slot, int R, 
   row0 = cu_at(n.cu_k, b, n.Tk);
   const int64_t e = s.none ? n.Tk : cu_at(n.cu_k, b + 1, n.Tk);
   rows = e > row0 ? (int)(e - row0) : 0;
-  first = t >= 0 && t * R < rows ? (int)(t * R) : rows;
+  rows = uniform(rows);
+  row0 = uniform(row0);
+  first = uniform(t >= 0 && t * R < rows ? (int)(t * R) : rows);
   return s;
 }
 
@@ -330,7 +344,8 @@ struct TileStage {
   __device__ __forceinline__ void load(const char* base, int ts_bytes, int left, uint32_t off) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int rows = min(max(left - i * kRows, 0), kRows);
+      // (uniform: the minimum of a maximum is a vector instruction)
+      const int rows = uniform(min(max(left - i * kRows, 0), kRows));
       const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<char*>(base + (int64_t)(i * kRows) * ts_bytes), 0, rows * ts_bytes, 0x00020000);
       v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
@@ -361,7 +376,7 @@ struct TileStage {
 template <typename S, int DB>
 __device__ __forceinline__ void load_rows(const char* base, int ts_bytes, int left, int d_chunks, int lane,
                                           u32x4 (&f)[Tile<S, DB>::kSteps]) {
-  const int rows = min(max(left, 0), 32);
+  const int rows = uniform(min(max(left, 0), 32));
   const __amdgpu_buffer_rsrc_t rs =
       __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, rows * ts_bytes, 0x00020000);
   const uint32_t off = (uint32_t)((lane & 31) * ts_bytes + (lane >> 5) * 16);

@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
 
 // A float of the `bytes` at p; zero past them.
 __device__ __forceinline__ float buffer_f32(const float* p, int bytes, uint32_t off) {
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, max(bytes, 0), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, uniform(max(bytes, 0)), 0x00020000);
   return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
 }
 
