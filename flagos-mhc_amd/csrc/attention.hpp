@@ -51,6 +51,15 @@ struct AttArgs {
   float scale, scale2;     // scale, scale * log2(e)
 };
 
+// The kernel's arguments (its first parameter) read once more: what only the
+// end of a kernel uses is not to hold scalar registers over its loop, which are
+// otherwise kept in lanes of vector registers and read back in every step.
+__device__ __forceinline__ AttArgs args_again() {
+  auto p = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttArgs*)p;
+}
+
 // ---- sequences ---------------------------------------------------------------
 
 struct AttSeq {
