@@ -22,7 +22,7 @@
 // bits, as values of that type do.
 //
 // Both are bound as the forward is.  16384 tokens, 56 heads of 128 over 8,
-// causal, bf16: dq 5.6 ms, dk and dv 7.5 ms, 1.03 PFLOP/s each.
+// causal, bf16: dq 5.5 ms, dk and dv 7.4 ms, 1.04 PFLOP/s each.
 #pragma once
 
 #include "attention.hpp"

@@ -8,7 +8,7 @@
 // bounds it is the matrix instructions together with the exponentials between
 // them (16 a product of 32 x 32, at a quarter of the others' rate): two waves a
 // SIMD unit take turns.  32768 tokens, 32 heads of 128 over 8, causal, bf16:
-// 8.6 ms, 1.03 PFLOP/s (a large library product reaches 1.42 on this card); with
+// 8.4 ms, 1.04 PFLOP/s (a large library product reaches 1.42 on this card); with
 // the loads of keys and values left out it is 17 % faster.
 //
 // KS = 2: two waves share 32 queries, each takes every other

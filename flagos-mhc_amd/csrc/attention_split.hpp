@@ -12,7 +12,7 @@
 // flight while it computes.
 //
 // Reading the cache bounds it: 64 sequences of up to 8192 keys, 32 heads of 128
-// over 8, bf16: 290 us, 5.5 TB/s; one of 32768: 26 us, 5.2 TB/s, and 4 us for
+// over 8, bf16: 283 us, 5.7 TB/s; one of 32768: 25 us, 5.3 TB/s, and 4 us for
 // the join (a copy of large tensors moves 4.96 TB/s, read and written).
 #pragma once
 
