@@ -149,3 +149,17 @@ def test_any_alignment_and_stride(off, pad, d, r, layout, dtype):
                          S.rotary(q.contiguous(), k.contiguous(), freqs, pos, layout=layout)):
         assert torch.equal(got, want)
     R.within(S.rotary(q, k, freqs, pos, layout=layout)[0], _want(q, freqs, pos, layout, 1.0), "q")
+
+
+@pytest.mark.parametrize("d,r", [(36, 18), (38, 6), (46, 22), (40, 4), (44, 40), (20, 0)])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_parts_of_every_width(d, r, layout, dtype):
+    """Turned and copied parts that are whole accesses of 16 bytes, of 8, or of neither; r = 0 copies."""
+    g = _gen(d + r)
+    q, k = _randn(g, 1031, 3, d, dtype=DT[dtype]), _randn(g, 1031, 1, d, dtype=DT[dtype])
+    freqs = S.rotary_frequencies(r)[0] if r else torch.empty(0, dtype=torch.float64, device=DEV)
+    pos = torch.arange(1031, device=DEV)
+    for x, y in zip((q, k), S.rotary(q, k, freqs, layout=layout)):
+        R.within(y, _want(x, freqs, pos, layout, 1.0), f"{d} {r}")
+        assert torch.equal(y[..., r:], x[..., r:])
