@@ -35,6 +35,7 @@ from . import _lib
 _ARGS = struct.Struct("3P9q3P2q6ifi")  # mhc_attention_args (include/mhc_amd.h)
 _STRIDES = struct.Struct("3q")
 _MAX_ROW_BYTES = 1 << 24
+_MAX_SCALE = torch.finfo(torch.float32).max * math.log(2.0)  # scale * log2(e) is a fp32 number
 _INTS = (torch.int32, torch.int64)
 
 
@@ -90,8 +91,8 @@ class _Call:
             raise NotImplementedError(f"{what}: head width {d} not supported (at most 256, in fp32 128)")
         if scale is None:
             scale = d ** -0.5
-        elif not 0.0 < scale <= 3e38:
-            raise ValueError(f"{what}: scale {scale}, expected a positive number")
+        elif not 0.0 < scale <= _MAX_SCALE:
+            raise ValueError(f"{what}: scale {scale}, expected a positive number of at most {_MAX_SCALE:.4g}")
         at_q = at_k = at_n = 0
         if cu_q is not None:
             if nq != 3:

@@ -44,7 +44,9 @@ int check_att(const char* who, const mhc_attention_args* c, AttArgs& a) {
   if (c->rows_q > kMaxRows || c->rows_k > kMaxRows || c->heads > 65535 || c->sequences > kMaxRows)
     return set_error(MHC_ERR_UNSUPPORTED, "%s: rows_q=%lld rows_k=%lld heads=%d sequences=%d above the supported sizes", who,
                      (long long)c->rows_q, (long long)c->rows_k, c->heads, c->sequences);
-  if (!(c->scale > 0.f) || c->scale > 3e38f) return set_error(MHC_ERR_INVALID, "%s: scale %g", who, (double)c->scale);
+  // (the kernels take scale * log2(e), which has to be a number too: an infinite one makes NaN of scores of 0)
+  if (!(c->scale > 0.f) || !(c->scale * kLog2e <= __FLT_MAX__))
+    return set_error(MHC_ERR_INVALID, "%s: scale %g", who, (double)c->scale);
   if (c->cu_seqlens_k && c->lengths_k) return set_error(MHC_ERR_INVALID, "%s: cu_seqlens_k and lengths_k", who);
   if ((!c->cu_seqlens_q && c->sequences == 0 && c->rows_q) || (!c->cu_seqlens_k && c->sequences == 0 && c->rows_k) ||
       (!c->cu_seqlens_q && c->sequences && c->rows_q % c->sequences) || (!c->cu_seqlens_k && c->sequences && c->rows_k % c->sequences))

@@ -446,7 +446,7 @@ typedef struct {
   const int32_t *cu_seqlens_q, *cu_seqlens_k, *lengths_k;
   int64_t rows_q, rows_k;
   int32_t sequences, heads, heads_k, d, dtype, causal;
-  float scale; /* > 0 */
+  float scale; /* > 0, scale * log2(e) finite */
   int32_t reserved; /* 0 */
 } mhc_attention_args;
 

@@ -1,0 +1,40 @@
+"""Arguments of attention and rotary positions that are refused, or taken, at
+the edges of what is documented (no GPU: nothing is launched)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from FlagOS_mhc import _lib, sublayer as S
+from FlagOS_mhc.attention import _STRIDES
+from test_attention_cpu import P, _args, _err, on_cpu, t  # noqa: F401 (on_cpu is a fixture)
+
+LIMIT = 2.3586e38  # the largest fp32 number by log2(e)
+
+
+def _c_calls(a):
+    """Return codes of the C entry points."""
+    lib, st = _lib.load(), _STRIDES.pack(0, 128, 64)
+    yield lib.mhc_attention_fwd(a, P, None, P, 1 << 40, None)
+    yield lib.mhc_attention_bwd(a, P, st, P, P, P, P, P, P, 1 << 40, None)
+
+
+@pytest.mark.parametrize("scale", [LIMIT * 1.001, 2.4e38, 3e38])
+def test_scale_times_log2e_is_a_number(on_cpu, scale):  # noqa: F811
+    a = _args(scale=scale)
+    for rc in _c_calls(a):
+        assert rc == -1 and b"scale" in _err()
+    assert _lib.load().mhc_attention_bwd_workspace_size(a) == 0
+    q, k = t(6, 4, 64), t(6, 2, 64)
+    with pytest.raises(ValueError, match="scale"):
+        S.attention(q, k, k, scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        S.attention_backward(q, q, k, k, q, t(4, 6, dtype=torch.float32), scale=scale)
+
+
+@pytest.mark.parametrize("scale", [1e-38, 1.0, LIMIT * 0.999])
+def test_scales_up_to_the_limit_are_taken(on_cpu, scale):  # noqa: F811
+    assert _lib.load().mhc_attention_bwd_workspace_size(_args(scale=scale)) > 0
+    q, k = t(6, 4, 64), t(6, 2, 64)
+    assert S.attention(q, k, k, scale=scale)["out"].shape == q.shape
