@@ -47,6 +47,7 @@ int check_att(const char* who, const mhc_attention_args* c, AttArgs& a) {
   // (the kernels take scale * log2(e), which has to be a number too: an infinite one makes NaN of scores of 0)
   if (!(c->scale > 0.f) || !(c->scale * kLog2e <= __FLT_MAX__))
     return set_error(MHC_ERR_INVALID, "%s: scale %g", who, (double)c->scale);
+  if (c->reserved) return set_error(MHC_ERR_INVALID, "%s: reserved=%d, expected 0", who, c->reserved);
   if (c->cu_seqlens_k && c->lengths_k) return set_error(MHC_ERR_INVALID, "%s: cu_seqlens_k and lengths_k", who);
   if ((!c->cu_seqlens_q && c->sequences == 0 && c->rows_q) || (!c->cu_seqlens_k && c->sequences == 0 && c->rows_k) ||
       (!c->cu_seqlens_q && c->sequences && c->rows_q % c->sequences) || (!c->cu_seqlens_k && c->sequences && c->rows_k % c->sequences))

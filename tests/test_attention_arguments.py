@@ -38,3 +38,11 @@ def test_scales_up_to_the_limit_are_taken(on_cpu, scale):  # noqa: F811
     assert _lib.load().mhc_attention_bwd_workspace_size(_args(scale=scale)) > 0
     q, k = t(6, 4, 64), t(6, 2, 64)
     assert S.attention(q, k, k, scale=scale)["out"].shape == q.shape
+
+
+def test_reserved_is_zero():
+    for word in (1, -1, 1 << 30):
+        a = _args()[:-4] + word.to_bytes(4, "little", signed=True)
+        assert _lib.load().mhc_attention_fwd_workspace_size(a) == _lib.load().mhc_attention_bwd_workspace_size(a) == 0
+        for rc in _c_calls(a):
+            assert rc == -1 and b"reserved" in _err()
