@@ -33,17 +33,21 @@ template <typename S, int DB> struct AttShape {
   static constexpr bool kBig = DB == 4 && sizeof(S) == 2;  // 256 rows a block are a choice (att_big_head)
 };
 
+// Blocks of 256 threads that a dispatch holds.
+constexpr int64_t kMaxBlocks256 = 0xffffffffll / 256;
+
 template <typename S, int DB>
 int att_split_run(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   const int64_t blocks = p.slots * a.n.Hk * p.splits, rows = a.n.Tq * a.n.H;
-  if (blocks > 0xffffffffll / 256 || rows > 0xffffffffll / 256)
+  if (blocks > kMaxBlocks256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
   constexpr int WPE = AttShape<S, DB>::kWPE;
   hipLaunchKernelGGL((att_split_kernel<S, DB, WPE>), dim3((unsigned)blocks), dim3(64 * kSplitWaves), (split_lds<S, DB>()), st, a,
                      p.slots, p.splits);
   if (const int rc = check_launch("attention")) return rc;
   if (p.splits == 1) return MHC_OK;
-  hipLaunchKernelGGL(att_join_kernel<S>, dim3((unsigned)rows), dim3(256), 0, st, a, rows, p.splits);
+  const int64_t joins = rows < kMaxBlocks256 ? rows : kMaxBlocks256;
+  hipLaunchKernelGGL(att_join_kernel<S>, dim3((unsigned)joins), dim3(256), 0, st, a, rows, p.splits);
   return check_launch("attention");
 }
 
@@ -116,7 +120,7 @@ int att_bwd_width(const AttArgs& a, hipStream_t st) {
   else rc = att_dkv_run<S, DB, 4>(a, p, st);
   if (rc || p.splits == 1) return rc;
   const int64_t all = a.n.Tk * a.n.Hk * a.n.d, blocks = (2 * all + 1023) / 1024;
-  if (blocks > 0xffffffffll / 256)
+  if (blocks > kMaxBlocks256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention_backward: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
   hipLaunchKernelGGL(att_dkv_join_kernel<S>, dim3((unsigned)blocks), dim3(256), 0, st, a, all, p.splits);
   return check_launch("attention_backward");

@@ -379,63 +379,67 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(Att
 }
 
 // out = sum over parts of 2^(m - M) O / sum of 2^(m - M) l: a block a row and
-// head, 16, 32 or 64 lanes a part (four elements each), so that 4 to 16 parts
-// are read at a time; their sums meet in LDS, always in the same order.
+// head (or every so many of them, where a dispatch holds fewer blocks), 16, 32
+// or 64 lanes a part (four elements each), so that 4 to 16 parts are read at a
+// time; their sums meet in LDS, always in the same order.
 template <typename S>
 __global__ __launch_bounds__(256) void att_join_kernel(AttArgs a, int64_t rows, int splits) {
   __shared__ float sums[256 * 5];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int64_t row = blockIdx.x;  // (row of q, head)
   const int d = a.n.d, per = d <= 64 ? 16 : (d <= 128 ? 32 : 64), groups = 256 / per;
   const int mine = tid / per, e = tid % per * 4;
   const float* ml = a.part + (int64_t)splits * rows * d;
-  float top = -__builtin_inff();
-  for (int p = lane; p < splits; p += 64) top = fmaxf(top, ml[2 * ((int64_t)p * rows + row)]);
-  top = group_max<63>(top);
-  const float ref = top == -__builtin_inff() ? 0.f : top;
-  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  constexpr int kAhead = 4;
-  for (int p0 = mine; p0 < splits; p0 += groups * kAhead) {
-    float m[kAhead], l[kAhead];
-    floatx4 o[kAhead];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {  // (row of q, head)
+    float top = -__builtin_inff();
+    for (int p = lane; p < splits; p += 64) top = fmaxf(top, ml[2 * ((int64_t)p * rows + row)]);
+    top = group_max<63>(top);
+    const float ref = top == -__builtin_inff() ? 0.f : top;
+    float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kAhead = 4;
+    for (int p0 = mine; p0 < splits; p0 += groups * kAhead) {
+      float m[kAhead], l[kAhead];
+      floatx4 o[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int p = p0 + u * groups;
-      const int64_t at = (int64_t)(p < splits ? p : p0) * rows + row;
-      m[u] = ml[2 * at];
-      l[u] = p < splits ? ml[2 * at + 1] : 0.f;
-      o[u] = e < d ? *reinterpret_cast<const floatx4*>(a.part + at * d + e) : floatx4{0.f, 0.f, 0.f, 0.f};
+      for (int u = 0; u < kAhead; ++u) {
+        const int p = p0 + u * groups;
+        const int64_t at = (int64_t)(p < splits ? p : p0) * rows + row;
+        m[u] = ml[2 * at];
+        l[u] = p < splits ? ml[2 * at + 1] : 0.f;
+        o[u] = e < d ? *reinterpret_cast<const floatx4*>(a.part + at * d + e) : floatx4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (l[u] == 0.f) continue;  // no keys in this part: it left its sums as they were
+        const float f = hw_exp2(m[u] - ref);
+        sum += l[u] * f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += o[u][j] * f;
+      }
     }
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (l[u] == 0.f) continue;  // no keys in this part: it left its sums as they were
-      const float f = hw_exp2(m[u] - ref);
-      sum += l[u] * f;
+    for (int j = 0; j < 4; ++j) sums[j * 256 + tid] = v[j];
+    sums[1024 + tid] = sum;
+    __syncthreads();
+    if (tid < per) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += o[u][j] * f;
+      for (int j = 0; j < 4; ++j) v[j] = 0.f;
+      sum = 0.f;
+      for (int g = 0; g < groups; ++g) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += sums[j * 256 + g * per + tid];
+        sum += sums[1024 + g * per + tid];
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      S* out = static_cast<S*>(a.out) + row * d + e;
+      if (e < d) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) store_elem<S>(out, j, v[j] * inv);
+      }
+      if (a.lse && tid == 0)
+        a.lse[row % a.n.H * a.n.Tq + row / a.n.H] = sum == 0.f ? -__builtin_inff() : top * kLn2 + logf(sum);
     }
+    __syncthreads();  // the sums are read before the next row's are written
   }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) sums[j * 256 + tid] = v[j];
-  sums[1024 + tid] = sum;
-  __syncthreads();
-  if (tid >= per) return;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = 0.f;
-  sum = 0.f;
-  for (int g = 0; g < groups; ++g) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += sums[j * 256 + g * per + tid];
-    sum += sums[1024 + g * per + tid];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  S* out = static_cast<S*>(a.out) + row * d + e;
-  if (e < d) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) store_elem<S>(out, j, v[j] * inv);
-  }
-  if (a.lse && tid == 0)
-    a.lse[row % a.n.H * a.n.Tq + row / a.n.H] = sum == 0.f ? -__builtin_inff() : top * kLn2 + logf(sum);
 }
 
 }  // namespace mhc
