@@ -267,9 +267,8 @@ template <typename S, int DB>
 struct Tile {
   static constexpr int kEs = (int)sizeof(S);
   static constexpr int kE = Mma32<S>::E;
-  static constexpr int kD = 32 * DB;                                   // columns held
-  static constexpr int kWide = DB <= 2 ? 64 : (DB <= 4 ? 128 : 256);   // columns of a row's place
-  static constexpr int kPitch = kWide * kEs;                           // bytes
+  static constexpr int kD = 32 * DB;                 // columns held
+  static constexpr int kPitch = att_pitch(kEs, DB);  // bytes from row to row
   static constexpr int kChunks = kPitch / 16;
   static constexpr int kUsed = kD * kEs / 16;    // chunks that are read
   static constexpr int kSteps = kUsed / 2;       // row fragments

@@ -104,6 +104,27 @@ inline AttBwdPlan att_bwd_plan(const AttDims& n, bool fp32, bool big, int cus) {
   return p;
 }
 
+// ---- LDS --------------------------------------------------------------------
+
+// Bytes of a tile's row: DB blocks of 32 columns of `es` bytes, at a power of two.
+constexpr int att_pitch(int es, int db) { return (db <= 2 ? 64 : (db <= 4 ? 128 : 256)) * es; }
+
+// A block that asks for more than a compute unit has does not run, and nothing
+// but the launch's error says so: every launch's bytes go through here, with
+// room for what a kernel declares itself.
+constexpr size_t kCuLds = 160 * 1024, kOwnLds = 2048;
+template <size_t BYTES>
+constexpr size_t att_fits() {
+  static_assert(BYTES + kOwnLds <= kCuLds, "a block's LDS exceeds a compute unit's");
+  return BYTES;
+}
+
+// dk and dv: two stages of `rows` rows of q and of the output's gradient, with
+// lse and D, and the block's own rows of v if they are held there.
+constexpr size_t att_dkv_lds(int es, int db, int waves, int rows, bool own) {
+  return (size_t)2 * (2 * rows * att_pitch(es, db) + (2 * rows * 4 + 255) / 256 * 256) + (own ? 32 * waves * att_pitch(es, db) : 0);
+}
+
 inline bool att_big_head(const AttDims& n, bool fp32) { return !fp32 && n.d > 96 && n.d <= 128; }
 
 }  // namespace mhc

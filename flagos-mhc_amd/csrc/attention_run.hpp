@@ -42,7 +42,7 @@ int att_split_run(const AttArgs& a, const AttSplit& p, hipStream_t st) {
   if (blocks > kMaxBlocks256)
     return set_error(MHC_ERR_UNSUPPORTED, "attention: %lld blocks exceed the 2^32 work-items of a dispatch", (long long)blocks);
   constexpr int WPE = AttShape<S, DB>::kWPE;
-  hipLaunchKernelGGL((att_split_kernel<S, DB, WPE>), dim3((unsigned)blocks), dim3(64 * kSplitWaves), (split_lds<S, DB>()), st, a,
+  hipLaunchKernelGGL((att_split_kernel<S, DB, WPE>), dim3((unsigned)blocks), dim3(64 * kSplitWaves), (att_fits<split_lds<S, DB>()>()), st, a,
                      p.slots, p.splits);
   if (const int rc = check_launch("attention")) return rc;
   if (p.splits == 1) return MHC_OK;
@@ -64,14 +64,14 @@ int att_fwd_run(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
   constexpr int BM = 32 * NW / KS;
   return att_launch(att_fwd_kernel<S, DB, NW, KS, A::kFwdNB, A::kFwdWPE>, a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, BM),
-                    a.n.H, 64 * NW, att_lds<S, DB, NW, KS>(32 * A::kFwdNB * KS), st, "attention");
+                    a.n.H, 64 * NW, att_fits<att_lds<S, DB, NW, KS>(32 * A::kFwdNB * KS)>(), st, "attention");
 }
 template <typename S, int DB, int NW, int KS>
 int att_dq_run(const AttArgs& a, hipStream_t st) {
   using A = AttShape<S, DB>;
   constexpr int BM = 32 * NW / KS;
   return att_launch(att_dq_kernel<S, DB, NW, KS, A::kBwdNB, A::kWPE>, a, att_slots(a.n.cu_q != nullptr, a.n.Tq, a.n.B, a.n.Sq, BM),
-                    a.n.H, 64 * NW, att_lds<S, DB, NW, KS>(32 * A::kBwdNB * KS), st, "attention_backward");
+                    a.n.H, 64 * NW, att_fits<att_lds<S, DB, NW, KS>(32 * A::kBwdNB * KS)>(), st, "attention_backward");
 }
 
 template <typename S, int DB>
@@ -93,7 +93,7 @@ int att_dq_width(const AttArgs& a, hipStream_t st) {
   const AttSplit p = att_split(a.n, cus);
   if (p.use)
     return att_launch(att_dq_split_kernel<S, DB, AttShape<S, DB>::kBytes <= 128 ? 2 : 1>, a, p.slots, a.n.Hk, 64 * kSplitWaves,
-                      split_lds<S, DB>(), st, "attention_backward");
+                      att_fits<split_lds<S, DB>()>(), st, "attention_backward");
   const AttBlocks b = att_blocks(a.n, AttShape<S, DB>::kBig, cus);
   if constexpr (AttShape<S, DB>::kBig)
     if (b == kBlocks256) return att_dq_run<S, DB, 8, 1>(a, st);
@@ -105,8 +105,7 @@ int att_dq_width(const AttArgs& a, hipStream_t st) {
 template <typename S, int DB, int NW>
 int att_dkv_run(const AttArgs& a, const AttBwdPlan& p, hipStream_t st) {
   using A = AttShape<S, DB>;
-  constexpr int kPitch = Tile<S, DB>::kPitch;
-  constexpr size_t lds = 2 * (2 * 32 * A::kBwdNB * kPitch + 256 * A::kBwdNB) + (A::kDkvLds ? 32 * NW * kPitch : 0);
+  constexpr size_t lds = att_fits<att_dkv_lds(sizeof(S), DB, NW, 32 * A::kBwdNB, A::kDkvLds)>();
   return att_launch(att_dkv_kernel<S, DB, NW, A::kBwdNB, A::kWPE, A::kDkvLds>, a, p.slots, (int64_t)a.n.Hk * p.splits, 64 * NW,
                     lds, st, "attention_backward", p.splits);
 }
