@@ -31,6 +31,13 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // row and not once a tile.  Weights are then at most 2^8 instead of 1: within
 // every type's range, and as many bits are left to them.
 constexpr float kLazyMax = 8.0f;
+// fp16 weights lose bits below 2^-14 and are 0 below 2^-25, though many of them
+// may make a result.  Its numbers reach 65504, so its reference point lies this
+// far below the row's maximum: weights are at most 2^15, and keep all bits down
+// to 2^-21 of the row's largest (1024 keys of 2^-18.4, the largest's value 0:
+// off by 1.1 % before).  bf16 and fp32 have fp32's range.
+template <typename S> inline constexpr float kBelowMax = 0.0f;
+template <> inline constexpr float kBelowMax<f16_t> = 7.0f;
 
 // One of q, k, v or a gradient: element (sequence's row t, head h, i) at
 // p[b * bs + t * ts + h * hs + i]; packed sequences have bs = 0 and rows

@@ -133,7 +133,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_fwd_kernel(AttArgs a, int64_
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[b][i]);
-      top = max_xor32(top) * c;
+      top = max_xor32(top) * c - kBelowMax<S>;
       if (__any(top > m + kLazyMax || m == -__builtin_inff())) {
         const float mn = fmaxf(m, top);
         const float f = mn == -__builtin_inff() ? 1.f : hw_exp2(m - mn);

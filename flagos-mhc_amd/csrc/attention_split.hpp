@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_split_kernel(AttArg
       sc[j] = acc_row(j, 0) <= left ? sc[j] : -__builtin_inff();
       top = fmaxf(top, sc[j]);
     }
-    top = max_xor32(top) * c;
+    top = max_xor32(top) * c - kBelowMax<S>;
     if (__any(top > m + kLazyMax || m == -__builtin_inff())) {
       const float mn = fmaxf(m, top);
       const float f = mn == -__builtin_inff() ? 1.f : hw_exp2(m - mn);
