@@ -408,6 +408,59 @@ __device__ __forceinline__ void load_rows(const char* base, int ts_bytes, int le
   }
 }
 
+// The backward's P and dS = P (dP - D) in fp16, whose full precision is that of
+// 2^-14 .. 65504: a row's weights are 2^-14 at 16384 keys, and dS is as small,
+// or large, as these times the output's gradient, whatever dq and dk come to
+// (8192 keys, gradients of 1e-4: dq was off by 10 %; two keys, gradients of
+// 1.2e4: infinite).  So P is taken 2^14 times as large (at most 2^14, for the sum
+// over queries that is dv), and dS times a power of two of the lane's own, 2^e:
+// the lane's query in dq, its key in dk, for which its products add up.  e is
+// found as the forward's reference point is: where the largest of a tile's dS
+// comes past 2^15, it moves to put that at 2^8, and the lane's sums with it.  Both
+// are taken back from the fp32 sums at the end.  It costs a maximum and a product
+// an element (backward of 4096 in two, 16 heads over 4, fp16: of 64 158 -> 174 us,
+// of 128 262 -> 276, of 256 608 -> 681).  bf16 and fp32 have fp32's range.
+template <typename S> struct Lift {
+  static constexpr bool kOn = false;
+  static constexpr float kWeights = 0.0f;  // log2 of P's factor
+  template <bool ACC, int DB> __device__ __forceinline__ void fit(floatx16&, floatx16 (&)[DB]) {}
+  __device__ __forceinline__ float back() const { return 1.0f; }
+};
+template <> struct Lift<f16_t> {
+  static constexpr bool kOn = true;
+  static constexpr float kWeights = 14.0f;
+  float f = 0x1p126f;  // 2^e
+
+  // x: a tile's dS of the lane, in place; acc: the lane's sums of the tiles before.
+  // ACC: they fill accumulation registers (kernels of one wave a SIMD unit) and
+  // are to stay there but for the factor.
+  template <bool ACC, int DB>
+  __device__ __forceinline__ void fit(floatx16& x, floatx16 (&acc)[DB]) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));  // (passes over NaN)
+    top = max_xor32(top);
+    const bool over = top * f > 0x1p15f;
+    if (__any(over)) {
+      // (an infinite dS has exponent 0 here, and stays infinite)
+      const int e = __builtin_amdgcn_frexp_expf(f) - 1, to = over ? min(e, 9 - __builtin_amdgcn_frexp_expf(top)) : e;
+      const float r = ldexpf(1.0f, to - e);
+      f = ldexpf(1.0f, to);
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        if constexpr (ACC) asm volatile("" : "+a"(acc[db]));
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] *= r;
+        if constexpr (ACC) asm volatile("" : "+a"(acc[db]));
+        __builtin_amdgcn_sched_barrier(0);  // rare: not to cost the kernel registers
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] *= f;
+  }
+  __device__ __forceinline__ float back() const { return ldexpf(1.0f, 1 - __builtin_amdgcn_frexp_expf(f)); }
+};
+
 // The transposed 32 x 32 DB result of a wave (lane: row l % 32 of the output,
 // its columns 32 db + 8 (i / 4) + 4 (l / 32) + i % 4) to rows of `ts` elements.
 template <typename S, int DB>

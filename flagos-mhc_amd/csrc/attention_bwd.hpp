@@ -17,9 +17,8 @@
 // dk of short sequences: errors of 0.0036 -> 0.0024 relative in bf16, where
 // rounding the exact result gives 0.0017).
 //
-// P and dS are rounded to the operands' type for the products that sum them,
-// in fp16 with its limits: P below 2^-14 and dS outside 2^-14 .. 65504 lose
-// bits, as values of that type do.
+// P and dS are rounded to the operands' type for the products that sum them, in
+// fp16 times powers of two that keep them within its range (Lift).
 //
 // Both are bound as the forward is.  16384 tokens, 56 heads of 128 over 8,
 // causal, bf16: dq 5.5 ms, dk and dv 7.4 ms, 1.04 PFLOP/s each.
@@ -116,6 +115,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
     for (int i = 0; i < 16; ++i) acc[db][i] = 0.f;
   const float c = a.scale2;
   float total = 0.f;
+  Lift<S> lift;
   for (int it = 0; it < sum + tiles; ++it) {
     const uint32_t tk = lds + (it & 1) * 2 * kTileBytes + part * BN * T::kPitch, tv = tk + kTileBytes;
     at.keep();
@@ -145,10 +145,21 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
 #pragma unroll
           for (int i = 0; i < 16; ++i) total += dp[i];
         }
+        if constexpr (Lift<S>::kOn) {
+          // (a block of 32 keys at a time: the next one may move the sums)
+          if (it < sum) continue;
+          lift.template fit<WPE == 1>(dp, acc);
+          u32x4 one[1][T::kColSteps];
 #pragma unroll
-        for (int u = 0; u < T::kColSteps; ++u) p[b][u] = acc_frag<S>(dp, u);
+          for (int u = 0; u < T::kColSteps; ++u) one[0][u] = acc_frag<S>(dp, u);
+          add_columns<S, DB, 1>(acc, at, tk + b * 32 * T::kPitch, one);
+        } else {
+#pragma unroll
+          for (int u = 0; u < T::kColSteps; ++u) p[b][u] = acc_frag<S>(dp, u);
+        }
       }
-      if (it >= sum) add_columns<S, DB, NB>(acc, at, tk, p);
+      if constexpr (!Lift<S>::kOn)
+        if (it >= sum) add_columns<S, DB, NB>(acc, at, tk, p);
     }
     if (it + 1 == sum) {
       delta = add_xor32(total);
@@ -164,6 +175,13 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dq_kernel(AttArgs a, int64_t
       stage(it + 1, next);
       __syncthreads();
     }
+  }
+  if constexpr (Lift<S>::kOn) {
+    const float back = lift.back();
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[db][i] *= back;
   }
   bad = __syncthreads_or(bad);
   if constexpr (KS == 2) {
@@ -287,7 +305,8 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
     if (tid < BQ) {
       float* to = reinterpret_cast<float*>(smem + kOwn + buf * kStage + 2 * kTileBytes);
       // no such row, or an empty one: P = 0
-      to[tid] = t * BQ + tid >= lq || st_lse == -__builtin_inff() ? __builtin_inff() : st_lse * kLog2e;
+      to[tid] = t * BQ + tid >= lq || st_lse == -__builtin_inff() ? __builtin_inff()
+                                                                  : __builtin_fmaf(st_lse, kLog2e, -Lift<S>::kWeights);
       to[BQ + tid] = st_delta;
     }
   };
@@ -314,6 +333,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
 #pragma unroll
     for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
   const float c = a.scale2;
+  Lift<S> lift;
   const int half = lane >> 5;
   const uint32_t own_v = lds_addr(smem) + wave * 32 * T::kPitch;
   for (int it = it0; it < it1; ++it) {
@@ -362,6 +382,7 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
             dp[i] = in ? dp[i] : 0.f;
           }
         }
+        lift.template fit<WPE == 1>(dp, ak);
         u32x4 p[1][T::kColSteps], ds[1][T::kColSteps];
 #pragma unroll
         for (int u = 0; u < T::kColSteps; ++u) {
@@ -396,14 +417,18 @@ __global__ __launch_bounds__(64 * NW, WPE) void att_dkv_kernel(AttArgs a, int64_
 #pragma unroll
       for (int i = 0; i < 16; ++i) ak[db][i] = av[db][i] = 0.f;
   }
+  // (P's factor is in dS too)
+  constexpr float kBack = Lift<S>::kOn ? 0x1p-14f : 1.0f;
+  static_assert(!Lift<S>::kOn || Lift<S>::kWeights == 14.0f, "P's factor");
+  const float ak_f = e.scale * (lift.back() * kBack);
   const int d_end = e.n.d;
   const int64_t place = ((row0 + key) * e.n.Hk + hk) * (int64_t)d_end, all = e.n.Tk * e.n.Hk * d_end;
   if (splits > 1) {
-    store_rows<float, DB>(ak, e.scale, e.part + 2 * part * all + place, live, d_end, lane);
-    store_rows<float, DB>(av, 1.f, e.part + (2 * part + 1) * all + place, live, d_end, lane);
+    store_rows<float, DB>(ak, ak_f, e.part + 2 * part * all + place, live, d_end, lane);
+    store_rows<float, DB>(av, kBack, e.part + (2 * part + 1) * all + place, live, d_end, lane);
   } else {
-    store_rows<S, DB>(ak, e.scale, static_cast<S*>(e.dk) + place, live, d_end, lane);
-    store_rows<S, DB>(av, 1.f, static_cast<S*>(e.dv) + place, live, d_end, lane);
+    store_rows<S, DB>(ak, ak_f, static_cast<S*>(e.dk) + place, live, d_end, lane);
+    store_rows<S, DB>(av, kBack, static_cast<S*>(e.dv) + place, live, d_end, lane);
   }
 }
 

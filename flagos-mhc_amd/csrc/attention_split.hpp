@@ -335,8 +335,10 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(Att
     for (int w = 0; w < kSplitWaves; ++w) delta += sums[w * 32 + (lane & 31)];
     if (live && wave == 0 && lane < 32) a.delta[stat] = delta;
   }
+  Lift<S> lift;
   for (int t = wave; t < tiles; t += kSplitWaves) {
-    const floatx16 dp = scores(t);
+    floatx16 dp = scores(t);
+    lift.template fit<WPE == 1>(dp, acc);
     u32x4 p[1][T::kColSteps];
 #pragma unroll
     for (int u = 0; u < T::kColSteps; ++u) p[0][u] = acc_frag<S>(dp, u);
@@ -345,10 +347,11 @@ __global__ __launch_bounds__(64 * kSplitWaves, WPE) void att_dq_split_kernel(Att
 
   bad = __syncthreads_or(bad);
   float* region = reinterpret_cast<float*>(smem + wave * kRegion);
+  const float back = lift.back();
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) region[(db * 16 + j) * 64 + lane] = acc[db][j];
+    for (int j = 0; j < 16; ++j) region[(db * 16 + j) * 64 + lane] = acc[db][j] * back;
   __syncthreads();
   for (int db = wave; db < DB; db += kSplitWaves) {
     floatx16 z[1];
