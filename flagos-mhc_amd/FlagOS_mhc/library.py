@@ -75,7 +75,7 @@ from .mhc_post_backward import mhc_post_backward, mhc_post_backward_sum, post_ba
 from .mhc_post_pre import mhc_post_pre_clamp_sinkhorn
 from .mhc_pre_clamp_sinkhorn import _pre_forward
 from .mhc_pre_clamp_sinkhorn_backward import _pre_backward, mhc_pre_clamp_sinkhorn_backward
-from .rotary import rotary, rotary_backward
+from .rotary import refuse_trained, rotary, rotary_backward
 
 NAMESPACE = "flagos_mhc"
 
@@ -419,6 +419,7 @@ def _rot_fake(q, k, freqs, positions=None, cu_seqlens=None, layout="half", ampli
 
 def _rot_setup(ctx, inputs, output):
     q, k, freqs, *opt = inputs
+    refuse_trained(ctx.needs_input_grad[2])
     positions, cu, layout, amplitude, inverse = (*opt, *(None, None, "half", 1.0, False)[len(opt):])
     ctx.save_for_backward(freqs, positions, cu)
     ctx.args = (layout, amplitude, not inverse)
@@ -558,7 +559,7 @@ def mhc_ffn_layer_op(x, phi, alpha, base, norm_weight, norm_bias, w_gate, w_up, 
 
 def rotary_op(q, k, freqs, positions=None, *, cu_seqlens=None, layout="half", amplitude=1.0):
     """``rotary_fn`` through the registered op."""
-    _refuse_tangents("rotary", q, k)
+    _refuse_tangents("rotary", q, k, freqs)
     qo, ko = torch.ops.flagos_mhc.rotary(q, k, freqs, positions, cu_seqlens, layout, float(amplitude))
     return qo, None if k is None else ko
 

@@ -217,9 +217,16 @@ def _back(gq, gk, *args):
     return _pair(_RotaryBackFn.apply, gq, gk, *args)
 
 
+def refuse_trained(asked):
+    """freqs' own gradient is not computed: asked for, it is an error, not None."""
+    if asked:
+        raise NotImplementedError("rotary: freqs requires a gradient, which is not computed (freqs.detach() needs none)")
+
+
 def rotary_fn(q, k, freqs, positions=None, *, cu_seqlens=None, layout="half", amplitude=1.0):
-    """Autograd-aware rotary: (q, k)."""
-    if not _lib.needs_autograd(q, k):
+    """Autograd-aware rotary: (q, k).  freqs that require a gradient are refused."""
+    refuse_trained(freqs.requires_grad and torch.is_grad_enabled())
+    if not _lib.needs_autograd(q, k, freqs):
         return rotary(q, k, freqs, positions, cu_seqlens=cu_seqlens, layout=layout, amplitude=amplitude)
     out = RotaryFn.apply(q, k, freqs, positions, cu_seqlens, layout, amplitude)
     return (out, None) if k is None else out
