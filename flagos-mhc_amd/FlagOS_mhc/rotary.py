@@ -118,6 +118,10 @@ def _run(what, q, k, freqs, positions, cu_seqlens, layout, amplitude, inverse):
         if not (wide or positions.dtype is torch.int32) or positions.numel() != T:
             raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} and {positions.dtype}, expected "
                              f"{T} of int32 or int64")
+        if positions.dim() > 1:
+            at = [n for n in positions.shape if n != 1]
+            if len(at) > 1 and at != [n for n in shape[:-2] if n != 1]:
+                raise ValueError(f"{what}: positions of shape {tuple(positions.shape)} for rows {tuple(shape[:-2])}")
         if not positions.is_contiguous():
             positions = positions.contiguous()
         at_p = positions.data_ptr()
@@ -146,9 +150,10 @@ def rotary(q, k, freqs, positions=None, *, cu_seqlens=None, layout="half", ampli
     """Rotary positions on the HIP device, for q (..., H, d) and k (..., Hk, d)
     (or None) of one call: new tensors (q, k), k's None if it is.
 
-    A row's position is positions[t] (int32 or int64, one a row; any sign),
-    else, with cu_seqlens (B + 1,) of packed rows (T, H, d), its place in its
-    sequence, else its place along the dimension before the heads."""
+    A row's position is positions[t] (int32 or int64, any sign; one a row, flat
+    or in the shape of the dimensions before the heads), else, with cu_seqlens
+    (B + 1,) of packed rows (T, H, d), its place in its sequence, else its place
+    along the dimension before the heads."""
     return _run("rotary", q, k, freqs, positions, cu_seqlens, layout, amplitude, 0)
 
 

@@ -46,3 +46,18 @@ def test_reserved_is_zero():
         assert _lib.load().mhc_attention_fwd_workspace_size(a) == _lib.load().mhc_attention_bwd_workspace_size(a) == 0
         for rc in _c_calls(a):
             assert rc == -1 and b"reserved" in _err()
+
+
+def test_positions_have_the_rows_order(on_cpu):  # noqa: F811
+    """One a row, flat or in the shape of the dimensions before the heads: another shape of as
+    many (a transposed one) would be taken in its own order."""
+    f, _ = S.rotary_frequencies(64, device="cpu")
+    q, k = t(2, 3, 4, 64), t(2, 3, 1, 64)
+    for shape in ((3, 2), (3, 1, 2), (1, 3, 2)):
+        for call in (S.rotary, S.rotary_backward, S.rotary_fn):
+            with pytest.raises(ValueError, match="positions"):
+                call(q, k, f, torch.zeros(shape, dtype=torch.int64))
+    for shape in ((6,), (6, 1), (2, 3), (1, 2, 3), (2, 3, 1)):
+        assert S.rotary(q, k, f, torch.zeros(shape, dtype=torch.int32))[0].shape == q.shape
+    assert S.rotary(t(6, 4, 64), None, f, torch.zeros(1, 6, dtype=torch.int32))[0].shape == (6, 4, 64)
+    assert S.rotary(t(1, 1, 4, 64), None, f, torch.tensor(7))[0].shape == (1, 1, 4, 64)
