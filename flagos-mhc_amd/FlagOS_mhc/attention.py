@@ -193,10 +193,10 @@ def attention(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, ca
 
 
 def attention_backward(grad_out, q, k, v, out, lse, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, causal=True,
-                       scale=None):
+                       scale=None, need_kv=True):
     """(grad_q, grad_k, grad_v) from the forward's out and lse, in the shapes
-    and dtype of q, k and v; rows of no sequence, and of a cache past its
-    lengths, get 0.  Deterministic."""
+    and dtype of q, k and v; the last two are None with ``need_kv=False``.  Rows
+    of no sequence, and of a cache past its lengths, get 0.  Deterministic."""
     what = "attention_backward"
     _lib.require_device(what, grad_out, q, k, v, out, lse, cu_seqlens, cu_seqlens_k, lengths_k)
     c = _Call(what, q, k, v, cu_seqlens, cu_seqlens_k, lengths_k, causal, scale)
@@ -209,13 +209,19 @@ def attention_backward(grad_out, q, k, v, out, lse, cu_seqlens=None, *, cu_seqle
         lse = lse.contiguous()
     go, at_go, gst = c.take(grad_out if grad_out.dtype is q.dtype else grad_out.to(q.dtype))
     o, at_o, _ = c.take(out if out.is_contiguous() else out.contiguous())
-    dq, dk, dv = c.empty(q), c.empty(k), c.empty(v)
-    if c.rows_q > 0 or c.rows_k > 0:
+    dq, dk, dv = c.empty(q), c.empty(k) if need_kv else None, c.empty(v) if need_kv else None
+    if c.rows_q > 0 or (need_kv and c.rows_k > 0):
         dev = q.get_device()
-        ws, n = c.workspace("mhc_attention_bwd_workspace_size", dev, q)
+        if need_kv:
+            ws, n = c.workspace("mhc_attention_bwd_workspace_size", dev, q)
+        else:
+            n = -(-c.H * c.rows_q * 4 // 256) * 256
+            ws = q.new_empty(n, dtype=torch.uint8)
         _lib.call(what, _lib.load().mhc_attention_bwd, dev, c.args, at_go, _STRIDES.pack(*gst), at_o, lse.data_ptr(),
-                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _lib.ptr(ws), n)
-    return (dq, dk, dv) if c.wide == c.d else (c.trim(dq), c.trim(dk), c.trim(dv))
+                  dq.data_ptr(), _lib.ptr(dk), _lib.ptr(dv), _lib.ptr(ws), n)
+    if c.wide != c.d:
+        dq, dk, dv = (None if t is None else c.trim(t) for t in (dq, dk, dv))
+    return dq, dk, dv
 
 
 def attention_ref(q, k, v, cu_seqlens=None, *, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None):
@@ -261,7 +267,8 @@ class AttentionFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_out):
         q, k, v, out, lse, cu, cu_k, lengths = ctx.saved_tensors
-        grads = attention_backward(grad_out, q, k, v, out, lse, cu, cu_seqlens_k=cu_k, lengths_k=lengths, **ctx.args)
+        grads = attention_backward(grad_out, q, k, v, out, lse, cu, cu_seqlens_k=cu_k, lengths_k=lengths, **ctx.args,
+                                   need_kv=any(ctx.needs_input_grad[1:3]))
         return (*_lib.first_order("attention", grads, grad_out, q, k, v), None, None, None, None, None)
 
 

@@ -41,7 +41,8 @@ and the operators between pre and post (``FlagOS_mhc.sublayer``):
     torch.ops.flagos_mhc.attention(q, k, v, cu_seqlens, cu_seqlens_k, lengths_k, causal, scale, save)
         -> (out, lse); lse is empty with save=False
     torch.ops.flagos_mhc.attention_backward(grad_out, q, k, v, out, lse, cu_seqlens,
-        cu_seqlens_k, lengths_k, causal, scale) -> (grad_q, grad_k, grad_v)
+        cu_seqlens_k, lengths_k, causal, scale, need_kv=True) -> (grad_q, grad_k, grad_v); the last two are
+        empty with need_kv=False
 
 The forward pre op also returns the fp32 inv_rms, mixes and pre its backward
 needs; they are marked non-differentiable (likewise for the fused op).
@@ -457,14 +458,16 @@ def _att_fake(q, k, v, cu_seqlens=None, cu_seqlens_k=None, lengths_k=None, causa
 def _att_bwd(grad_out: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor,
              cu_seqlens: Optional[Tensor] = None, cu_seqlens_k: Optional[Tensor] = None,
              lengths_k: Optional[Tensor] = None, causal: bool = True,
-             scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
-    return attention_backward(grad_out, q, k, v, out, lse, cu_seqlens, cu_seqlens_k=cu_seqlens_k, lengths_k=lengths_k,
-                              causal=causal, scale=scale)
+             scale: Optional[float] = None, need_kv: bool = True) -> Tuple[Tensor, Tensor, Tensor]:
+    grads = attention_backward(grad_out, q, k, v, out, lse, cu_seqlens, cu_seqlens_k=cu_seqlens_k, lengths_k=lengths_k,
+                               causal=causal, scale=scale, need_kv=need_kv)
+    return tuple(q.new_empty((0,)) if g is None else g for g in grads)
 
 
 @_att_bwd.register_fake
-def _att_bwd_fake(grad_out, q, k, v, out, lse, cu_seqlens=None, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None):
-    return tuple(t.new_empty(t.shape) for t in (q, k, v))
+def _att_bwd_fake(grad_out, q, k, v, out, lse, cu_seqlens=None, cu_seqlens_k=None, lengths_k=None, causal=True, scale=None,
+                  need_kv=True):
+    return q.new_empty(q.shape), *(t.new_empty(t.shape if need_kv else (0,)) for t in (k, v))
 
 
 def _att_setup(ctx, inputs, output):
@@ -479,8 +482,9 @@ def _att_setup(ctx, inputs, output):
 def _att_grad(ctx, grad_out, _g_lse):
     if not ctx.saved:
         raise RuntimeError("attention: the forward ran with save=False")
-    return (*torch.ops.flagos_mhc.attention_backward(grad_out.contiguous(), *ctx.saved_tensors, *ctx.args),
-            *(None,) * 6)
+    need = any(ctx.needs_input_grad[1:3])
+    gq, gk, gv = torch.ops.flagos_mhc.attention_backward(grad_out.contiguous(), *ctx.saved_tensors, *ctx.args, need)
+    return gq, gk if need else None, gv if need else None, *(None,) * 6
 
 
 _att.register_autograd(_att_grad, setup_context=_att_setup)

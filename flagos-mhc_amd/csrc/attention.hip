@@ -122,9 +122,11 @@ extern "C" int mhc_attention_bwd(const mhc_attention_args* c, const void* grad_o
   if (const int rc = check_rows("attention_backward", "grad_out", grad_out, grad_stride, c->rows_q, es, c->d)) return rc;
   if (c->rows_q && (!out || !lse || !grad_q || !aligned16(out) || !aligned16(grad_q)))
     return set_error(MHC_ERR_INVALID, "attention_backward: out, lse or grad_q is null or not 16-byte aligned");
-  if (c->rows_k && (!grad_k || !grad_v || !aligned16(grad_k) || !aligned16(grad_v)))
+  const bool keys = grad_k || grad_v;
+  if (c->rows_k && keys && (!grad_k || !grad_v || !aligned16(grad_k) || !aligned16(grad_v)))
     return set_error(MHC_ERR_INVALID, "attention_backward: grad_k or grad_v is null or not 16-byte aligned");
-  const size_t need = mhc_attention_bwd_workspace_size(c);
+  const AttBwdPlan plan = bwd_plan(c, a);
+  const size_t need = keys ? plan.delta_bytes + plan.part_bytes : plan.delta_bytes;
   if (need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
     return set_error(MHC_ERR_INVALID, "attention_backward: workspace too small or not 16-byte aligned (%zu < %zu bytes)",
                      workspace ? workspace_bytes : (size_t)0, need);
@@ -136,7 +138,7 @@ extern "C" int mhc_attention_bwd(const mhc_attention_args* c, const void* grad_o
   a.dv = grad_v;
   a.lse = const_cast<float*>(lse);
   a.delta = static_cast<float*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + bwd_plan(c, a).delta_bytes);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.delta_bytes);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (c->dtype == MHC_DTYPE_F32) return att_bwd<float>(a, st);
   if (c->dtype == MHC_DTYPE_BF16) return att_bwd<bf16_t>(a, st);

@@ -113,6 +113,7 @@ int att_dkv_run(const AttArgs& a, const AttBwdPlan& p, hipStream_t st) {
 template <typename S, int DB>
 int att_bwd_width(const AttArgs& a, hipStream_t st) {
   if (const int rc = att_dq_width<S, DB>(a, st)) return rc;
+  if (!a.dk) return MHC_OK;  // (keys' gradients that nobody takes)
   const AttBwdPlan p = att_bwd_plan(a.n, sizeof(S) == 4, AttShape<S, DB>::kBig, device_cu_count());
   int rc;
   if constexpr (AttShape<S, DB>::kBig) rc = p.keys == 256 ? att_dkv_run<S, DB, 8>(a, p, st) : att_dkv_run<S, DB, 4>(a, p, st);

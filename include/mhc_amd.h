@@ -464,7 +464,9 @@ int mhc_attention_fwd(const mhc_attention_args* args, void* out, float* lse, voi
  * and grad_v (rows_k, heads_k, d), `dtype`, 16-byte aligned; grad_out has
  * strides grad_stride[3] as q.  Deterministic.  The gradients of the scores
  * and the weights are rounded to `dtype` between the products, in fp16 times
- * powers of two that keep them within its range.
+ * powers of two that keep them within its range.  grad_k and grad_v may both be
+ * NULL: they are not computed then, and a workspace of heads * rows_q * 4 bytes,
+ * rounded up to 256, is enough.
  */
 size_t mhc_attention_bwd_workspace_size(const mhc_attention_args* args);
 int mhc_attention_bwd(const mhc_attention_args* args, const void* grad_out, const int64_t* grad_stride, const void* out,
