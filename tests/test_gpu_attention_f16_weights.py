@@ -22,7 +22,7 @@ def _gen(seed):
     return g
 
 
-@pytest.mark.parametrize("S_,H,Hk", [(1, 4, 1), (40, 2, 1), (1100, 4, 4), (3500, 8, 8), (3500, 32, 8), (4200, 64, 8)])
+@pytest.mark.parametrize("S_,H,Hk", [(1, 4, 1), (40, 2, 1), (1100, 4, 4), (3500, 16, 16), (3500, 32, 8), (4200, 128, 8)])
 @pytest.mark.parametrize("d", [64, 128])
 def test_small_weights(S_, H, Hk, d):
     """Keys whose weights are 48.5 * 2^-24 of the row's largest, which lies in the same tile
