@@ -13,15 +13,15 @@ sequence); keys and values likewise, a batch of them with lengths_k: a cache
 of which each sequence uses its first rows.  Prompts, training batches and
 single tokens over a cache are all this call.
 
-fp32 with d up to 128, bf16 and fp16 up to 256.  Scores, maxima and sums are fp32; the
-weights exp(..), and in the backward the gradients of the scores, are rounded
-to the operands' type for the product that follows, in fp16 times powers of two
-that leave them all bits: a forward's weights down to 2^-21 of their query's
-largest, a backward's to 2^-28, and the scores' gradients to 2^-22 of the largest
-of their query (grad_q) or key (grad_k).  q, k, v may be views with any strides of their rows and heads;
-rows that are not at multiples of 16 bytes, or d that is not whole 16 bytes,
-are copied in every call.  The reference has no such operator: its model code
-runs PyTorch's.
+fp32 with d up to 128, bf16 and fp16 up to 256.  Scores, maxima and sums are
+fp32; the weights exp(..), and in the backward the gradients of the scores, are
+rounded to the operands' type for the product that follows, in fp16 times powers
+of two that leave them all bits: a forward's weights down to 2^-21 of their
+query's largest, a backward's to 2^-28, and the scores' gradients to 2^-22 of the
+largest of their query (grad_q) or key (grad_k).  q, k, v may be views with any
+strides of their rows and heads; rows that are not at multiples of 16 bytes, or
+d that is not whole 16 bytes, are copied in every call.  The reference has no
+such operator: its model code runs PyTorch's.
 """
 
 from __future__ import annotations

@@ -34,7 +34,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, or
       "ntk"     base * factor^(r / (r - 2)): the slowest pair is stretched by factor, the fastest stays
       "yarn"    pairs that turn less than turns[0] times over original_length positions are stretched by
                 factor, those above turns[1] stay, in between by a linear share of their turns;
-                amplitude 0.1 ln(factor) + 1 (factor > 1)
+                amplitude 0.1 ln(factor) + 1 (factor > 1).  (Some model code shares linearly in the
+                pair's index: weights trained so need such freqs, which ``rotary`` takes as well)
     """
     what = "rotary_frequencies"
     r = int(rotary_dim)

@@ -21,7 +21,8 @@
 // fp16 times powers of two that keep them within its range (Lift).
 //
 // Both are bound as the forward is.  16384 tokens, 56 heads of 128 over 8,
-// causal, bf16: dq 5.5 ms, dk and dv 7.4 ms, 1.04 PFLOP/s each.
+// causal, bf16: dq 5.4 and 5.6 ms, dk and dv 7.2 and 7.4 ms (medians on two
+// cards), 1.02 to 1.07 PFLOP/s each.
 #pragma once
 
 #include "attention.hpp"

@@ -8,8 +8,9 @@
 // bounds it is the matrix instructions together with the exponentials between
 // them (16 a product of 32 x 32, at a quarter of the others' rate): two waves a
 // SIMD unit take turns.  32768 tokens, 32 heads of 128 over 8, causal, bf16:
-// 8.4 ms, 1.04 PFLOP/s (a large library product reaches 1.42 on this card); with
-// the loads of keys and values left out it is 17 % faster.
+// 8.2 and 8.5 ms (medians on two cards), 1.07 and 1.03 PFLOP/s (a large library
+// product reaches 1.42); with the loads of keys and values left out it is 17 %
+// faster.
 //
 // KS = 2: two waves share 32 queries, each takes every other
 // tile, and their sums meet at the end: a long row is done in half the steps,

@@ -12,8 +12,8 @@
 // flight while it computes.
 //
 // Reading the cache bounds it: 64 sequences of up to 8192 keys, 32 heads of 128
-// over 8, bf16: 283 us, 5.7 TB/s; one of 32768: 25 us, 5.3 TB/s, and 4 us for
-// the join (a copy of large tensors moves 4.96 TB/s, read and written).
+// over 8, bf16: 286 us, 5.6 TB/s; one of 32768: 26 us, 5.2 TB/s, and 4 us for
+// the join (medians; a copy of large tensors moves 4.96 TB/s, read and written).
 #pragma once
 
 #include "attention.hpp"

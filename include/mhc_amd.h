@@ -425,8 +425,8 @@ int mhc_rotary(const mhc_rotary_args* args, void* stream);
  * goes with key head h / (heads / heads_k)):
  *   out_i = sum_j exp(scale q_i . k_j - lse_i) v_j, lse_i = ln sum_j exp(scale q_i . k_j)
  * over the keys j < Lk of i's sequence and, if causal, j <= i + Lk - Lq: the
- * Lq queries are the last of the Lk positions.  A query that sees no key has
- * out 0 and lse -infinity.
+ * Lq queries are the last of the Lk positions.  A query that sees no key, or
+ * none whose score is above -infinity, has out 0 and lse -infinity.
  *
  * Element (sequence b, row t, head h, i) of q is q[b * q_stride[0] + t *
  * q_stride[1] + h * q_stride[2] + i], strides in elements; k and v likewise.
